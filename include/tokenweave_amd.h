@@ -314,6 +314,92 @@ TW_API int tw_gemm_bf16_nt_partials_bias(void* const* outs, const void* const* a
                                   int num_partials, int64_t M, int64_t N, int64_t K,
                                   int64_t ldc, int max_cus, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Between a decoder layer's projections: rotation of queries and keys by their
+ * positions, a paged cache of keys and values in 4 bits, attention over it.  (No
+ * counterpart on the reference's path; head counts and lengths are the caller's.)
+ *
+ * tw_heads: a tensor [num_tokens, heads, head_size] whose channels are contiguous; the
+ * strides are in elements (views of a wider projection output are fine).
+ * ------------------------------------------------------------------------- */
+typedef struct tw_heads {
+  void* data;
+  int64_t heads;
+  int64_t token_stride;
+  int64_t head_stride;
+} tw_heads;
+
+#define TW_ROTARY_INTERLEAVED 1 /* pairs are neighbours (2j, 2j+1), not (j, j + rotary_dim/2) */
+#define TW_ROTARY_INVERSE 2     /* turn back: the gradient of a rotation, or a key's move     */
+
+/* For every pair (x1, x2) of the first rotary_dim channels of every head:
+ *   y1 = x1 * cos - x2 * sin ;  y2 = x2 * cos + x1 * sin      (fp32, rounded once)
+ * cos_sin: [max_positions, rotary_dim] fp32, a row holding the cosines of its
+ * rotary_dim/2 pairs and then the sines; row positions[t] serves token t.  The channels
+ * behind rotary_dim are copied.  out may be the input.  A position outside
+ * [0, max_positions) makes the turned channels NaN.  k_out / k may both be NULL.
+ * dtype: TW_DTYPE_*; any head_size, rotary_dim even, 2 <= rotary_dim <= head_size. */
+TW_API int tw_rotary_positions(const tw_heads* q_out, const tw_heads* q, const tw_heads* k_out,
+                               const tw_heads* k, const int64_t* positions, const float* cos_sin,
+                               int64_t max_positions, int64_t num_tokens, int head_size,
+                               int rotary_dim, int flags, int dtype, void* stream);
+
+/* The cache: num_pages pages, [num_pages][kv_heads][page_size * (D + D/16)] bytes, 16-byte
+ * aligned; D = head_size in {64, 128, 256}, page_size a power of two, 16 to 256.  A value is
+ * 4 bits (sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6: e2m1) times 2^e, one e for 32
+ * channels of a token: 4.25 bits a value.  e is the smallest with |x| <= 7 * 2^e for all
+ * 32, in [-23, 13] (so that every value is exact in fp16; larger magnitudes saturate at
+ * 6 * 2^13); ties go to the even code; a block with an infinity or a NaN reads as NaN.
+ * Of one head in one page, P = page_size:
+ *   keys    [P][D/2]              two channels a byte, the lower in the low nibble
+ *   values  [P/4][16][4][D/32]    of four tokens each sixteenth of the channels together
+ *   scales  [D/32][P] of the keys, then [D/32][P] of the values: e + 127, or 255 for NaN */
+#define TW_KV4_MIN_PAGE 16
+#define TW_KV4_MAX_PAGE 256
+
+/* Writes the tokens' keys and values to their slots (slot = page * page_size + place;
+ * int64; a slot outside the cache, -1 for instance, is skipped; two tokens of a call with
+ * one slot are an error that is not found).  With cos_sin the keys are turned on the way, as
+ * tw_rotary_positions does and rounded to `dtype` before they are coded, and the queries
+ * (q -> q_out; both may be NULL) are turned in the same launch.  Without cos_sin
+ * (NULL; positions is not read) the keys are coded as they are and q must be NULL. */
+TW_API int tw_kv4_append(void* pages, int64_t num_pages, int page_size, const tw_heads* k,
+                         const tw_heads* v, const int64_t* slots, const tw_heads* q_out,
+                         const tw_heads* q, const int64_t* positions, const float* cos_sin,
+                         int64_t max_positions, int64_t num_tokens, int head_size, int rotary_dim,
+                         int flags, int dtype, void* stream);
+
+/* k_out, v_out <- the values that the slots hold; zeros where a slot is outside the cache. */
+TW_API int tw_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void* pages,
+                       int64_t num_pages, int page_size, const int64_t* slots, int64_t num_tokens,
+                       int head_size, int dtype, void* stream);
+
+/* out = softmax(scale * q k^T) v over a sequence's cached tokens, for every query head; query
+ * heads g * G .. g * G + G - 1 share key head g (G = q->heads / kv_heads).
+ *   block_table  [num_seqs][table_stride] int32, the first table_width of a row are read:
+ *                page of tokens 0 .. P-1, P .. 2P-1, ... of the sequence; tokens of a page
+ *                outside [0, num_pages) are as if masked
+ *   seq_lens     [num_seqs] int32: cached tokens, the new ones among them (appended before)
+ *   query_starts [num_seqs + 1] int32: sequence s has the tokens query_starts[s] ..
+ *                query_starts[s+1] - 1 of q and out, the last of its cached tokens; NULL:
+ *                num_tokens / num_seqs tokens each
+ * Query i of n sees the tokens up to its own, seq_len - n + i, and of these the last
+ * `window` where window > 0.  A query that sees none gives zeros.  max_queries: at least the
+ * largest number of new tokens of a sequence (more than that are not computed).
+ * bf16 or fp16; scores and sums in fp32.  seq_lens may change between the replays of a
+ * captured call.
+ * workspace: tw_kv4_attention_workspace() bytes, 16-byte aligned, contents of no meaning
+ * before and after; calls that may run at the same time need one each. */
+TW_API int64_t tw_kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs,
+                                          int64_t max_queries, int64_t table_width, int page_size);
+TW_API int tw_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
+                            int64_t num_pages, int page_size, int kv_heads,
+                            const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                            const int32_t* seq_lens, const int32_t* query_starts, int64_t num_seqs,
+                            int64_t num_tokens, int64_t max_queries, int head_size, float scale,
+                            int64_t window, int dtype, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

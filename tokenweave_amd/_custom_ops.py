@@ -768,6 +768,195 @@ def bind_gemm_bf16_nt_partials(outs: Sequence[torch.Tensor], a: Sequence[torch.T
     return BoundOp(*_prepare_gemm_bf16_nt_partials(outs, a, b, max_cus, biases))
 
 
+# ---------------------------------------------------------------------------
+# between a layer's projections: rotation, the paged 4-bit cache, attention
+# (no counterpart in vllm/_custom_ops.py)
+# ---------------------------------------------------------------------------
+def _check_heads(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, tokens: Optional[int] = None,
+                 heads: Optional[int] = None, head_size: Optional[int] = None) -> None:
+    """[tokens, heads, head_size] on the GPU, channels contiguous; a view of a wider tensor is fine."""
+    _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}: tokenweave_amd ops run on the GPU only "
+                           "(there is no CPU implementation)")
+    _require(t.device == device, f"{name} is on {t.device}, expected {device}")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    want = tuple(w if w is not None else g for w, g in zip((tokens, heads, head_size), t.shape))
+    if t.dim() != 3 or tuple(t.shape) != want:
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected [tokens, heads, head_size]"
+                           + (f" = {want}" if t.dim() == 3 else ""))
+    _require(t.stride(2) == 1 or t.size(2) == 1, f"the channels of {name} must be contiguous; got stride {t.stride()}")
+
+
+def _check_index(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, numel: int) -> None:
+    _require(isinstance(t, torch.Tensor) and t.is_cuda and t.device == device and t.dtype == dtype
+             and t.is_contiguous() and t.dim() == 1, f"{name} must be a contiguous 1-D {dtype} tensor on {device}")
+    _require(t.numel() == numel, f"{name} holds {t.numel()} values, expected {numel}")
+
+
+def _heads(t: Optional[torch.Tensor]):
+    """The tensor as the C ABI takes it, or None."""
+    return None if t is None else ctypes.byref(_lib.Heads(t.data_ptr(), t.size(1), t.stride(0), t.stride(1)))
+
+
+def _check_table(cos_sin: torch.Tensor, device: torch.device, head_size: int) -> Tuple[int, int]:
+    """(positions, turned channels) of a table of cosines and sines."""
+    _check_tensor("cos_sin", cos_sin, torch.float32, device)
+    _require(cos_sin.dim() == 2 and cos_sin.size(1) % 2 == 0 and 2 <= cos_sin.size(1) <= head_size,
+             f"cos_sin has shape {tuple(cos_sin.shape)}, expected [positions, rotary_dim], rotary_dim even and at most "
+             f"head_size {head_size}")
+    return cos_sin.size(0), cos_sin.size(1)
+
+
+def _rotary_flags(interleaved: bool, inverse: bool = False) -> int:
+    return (_lib.TW_ROTARY_INTERLEAVED if interleaved else 0) | (_lib.TW_ROTARY_INVERSE if inverse else 0)
+
+
+def rotary_positions(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, cos_sin: torch.Tensor,
+                     interleaved: bool = False, inverse: bool = False, q_out: Optional[torch.Tensor] = None,
+                     k_out: Optional[torch.Tensor] = None) -> None:
+    """Turns q and k ([tokens, heads, head_size], views of a wider tensor are fine) by their tokens'
+    positions, in place or into q_out / k_out: every pair (x1, x2) of the first rotary_dim channels
+    becomes (x1 cos - x2 sin, x2 cos + x1 sin), computed in fp32 and rounded once.  `cos_sin`
+    [positions, rotary_dim] fp32 holds a position's cosines and then its sines
+    (`RotaryPositions.cos_sin`).  `interleaved`: pairs are neighbours, else (j, j + rotary_dim / 2).
+    `inverse` turns back: the gradient of the rotation."""
+    if _fast is not None and not _tracing() and _fast.rotary_positions(q, k, positions, cos_sin, interleaved, inverse,
+                                                                       q_out, k_out):
+        return
+    code = _dtype_code("rotary_positions_kernel", q)
+    dev = q.device
+    _check_heads("q", q, q.dtype, dev)
+    T, _, D = q.shape
+    if q_out is not None:
+        _check_heads("q_out", q_out, q.dtype, dev, *q.shape)
+    if k is not None:
+        _check_heads("k", k, q.dtype, dev, T, None, D)
+    _require(k is not None or k_out is None, "k_out without k")
+    if k_out is not None:
+        _check_heads("k_out", k_out, q.dtype, dev, *k.shape)
+    _check_index("positions", positions, torch.int64, dev, T)
+    length, dim = _check_table(cos_sin, dev, D)
+    with _on_device(q):
+        _lib.check(_lib.lib().tw_rotary_positions(
+            _heads(q if q_out is None else q_out), _heads(q), _heads(k if k_out is None else k_out), _heads(k),
+            positions.data_ptr(), cos_sin.data_ptr(), length, T, D, dim, _rotary_flags(interleaved, inverse), code,
+            _stream_ptr(q)))
+
+
+def _check_pages(pages: torch.Tensor, device: torch.device, heads: int, head_size: int) -> Tuple[int, int]:
+    """(pages, tokens of a page) of a 4-bit cache."""
+    _check_tensor("pages", pages, torch.uint8, device)
+    token = head_size + head_size // 16
+    _require(pages.dim() == 3 and pages.size(1) == heads and pages.size(2) % token == 0 and pages.size(2) > 0,
+             f"pages has shape {tuple(pages.shape)}, expected [pages, kv_heads, page_size * {token}] with {heads} heads "
+             f"of {head_size}")
+    return pages.size(0), pages.size(2) // token
+
+
+def kv4_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
+               positions: Optional[torch.Tensor] = None, cos_sin: Optional[torch.Tensor] = None,
+               interleaved: bool = False, q: Optional[torch.Tensor] = None,
+               q_out: Optional[torch.Tensor] = None) -> None:
+    """Writes the tokens' keys and values ([tokens, kv_heads, head_size]) in 4 bits to their slots
+    (page * page_size + place; int64) of `pages` [pages, kv_heads, page_size * (D + D/16)] uint8; a slot
+    outside the cache (-1 for padding) is skipped.  With `cos_sin` the keys are turned on the way as
+    `rotary_positions` does, and `q`, where given, is turned in the same launch (into q_out, or in
+    place).  k and v are not modified."""
+    if _fast is not None and not _tracing() and _fast.kv4_append(pages, k, v, slots, positions, cos_sin, interleaved,
+                                                                 q, q_out):
+        return
+    code = _dtype_code("kv4_append_kernel", k)
+    dev = k.device
+    _check_heads("k", k, k.dtype, dev)
+    _check_heads("v", v, k.dtype, dev, *k.shape)
+    T, H, D = k.shape
+    num_pages, page = _check_pages(pages, dev, H, D)
+    _check_index("slots", slots, torch.int64, dev, T)
+    length = dim = 0
+    if cos_sin is not None:
+        length, dim = _check_table(cos_sin, dev, D)
+        _require(positions is not None, "cos_sin without positions")
+        _check_index("positions", positions, torch.int64, dev, T)
+    _require(q is None or cos_sin is not None, "q is only turned: it needs cos_sin and positions")
+    _require(q is not None or q_out is None, "q_out without q")
+    if q is not None:
+        _check_heads("q", q, k.dtype, dev, T, None, D)
+        if q_out is not None:
+            _check_heads("q_out", q_out, k.dtype, dev, *q.shape)
+    with _on_device(k):
+        _lib.check(_lib.lib().tw_kv4_append(
+            pages.data_ptr(), num_pages, page, _heads(k), _heads(v), slots.data_ptr(),
+            _heads(q if q_out is None else q_out), _heads(q), None if positions is None else positions.data_ptr(),
+            None if cos_sin is None else cos_sin.data_ptr(), length, T, D, dim, _rotary_flags(interleaved), code,
+            _stream_ptr(k)))
+
+
+def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor) -> None:
+    """k_out, v_out ([tokens, kv_heads, head_size]) <- the values that the slots of `pages` hold; zeros
+    where a slot is outside the cache.  Values up to 6 * 2^13 are exact in every type."""
+    if _fast is not None and not _tracing() and _fast.kv4_read(k_out, v_out, pages, slots):
+        return
+    code = _dtype_code("kv4_read_kernel", k_out)
+    dev = k_out.device
+    _check_heads("k_out", k_out, k_out.dtype, dev)
+    _check_heads("v_out", v_out, k_out.dtype, dev, *k_out.shape)
+    T, H, D = k_out.shape
+    num_pages, page = _check_pages(pages, dev, H, D)
+    _check_index("slots", slots, torch.int64, dev, T)
+    with _on_device(k_out):
+        _lib.check(_lib.lib().tw_kv4_read(_heads(k_out), _heads(v_out), pages.data_ptr(), num_pages, page,
+                                          slots.data_ptr(), T, D, code, _stream_ptr(k_out)))
+
+
+def kv4_attention(out: torch.Tensor, q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, scale: float, query_starts: Optional[torch.Tensor] = None,
+                  max_queries: Optional[int] = None, window: int = 0) -> None:
+    """out <- softmax(scale * q k^T) v over each sequence's cached tokens (`kv4_append` has put the new
+    ones there), q and out [tokens, heads, head_size] in bf16 or fp16; heads g*G .. g*G + G-1 share key
+    head g.  `block_table` [sequences, pages] int32 names a sequence's pages, `seq_lens` its cached
+    tokens, `query_starts` [sequences + 1] int32 its first token in q (None: the same number of tokens
+    for each sequence).  A token sees the cached tokens up to its own, of these the last `window` where
+    that is above 0; one that sees none gives zeros.  `max_queries`: the most new tokens of a sequence
+    (needed with query_starts, where it defaults to all of q's)."""
+    if _fast is not None and not _tracing() and _fast.kv4_attention(out, q, pages, block_table, seq_lens, scale,
+                                                                    query_starts, max_queries, window):
+        return
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f'"kv4_attention_kernel" not implemented for \'{q.dtype}\'')
+    code = _DTYPE_CODE[q.dtype]
+    dev = q.device
+    _check_heads("q", q, q.dtype, dev)
+    _check_heads("out", out, q.dtype, dev, *q.shape)
+    T, H, D = q.shape
+    _require(pages.dim() == 3, f"pages has shape {tuple(pages.shape)}, expected [pages, kv_heads, bytes]")
+    kv_heads = pages.size(1)
+    num_pages, page = _check_pages(pages, dev, kv_heads, D)
+    _require(H % kv_heads == 0, f"{H} query heads over {kv_heads} key heads")
+    _require(block_table.is_cuda and block_table.device == dev and block_table.dtype == torch.int32
+             and block_table.dim() == 2 and (block_table.stride(1) == 1 or block_table.size(1) <= 1),
+             f"block_table must be a 2-D torch.int32 tensor on {dev} with contiguous rows")
+    B, width = block_table.shape
+    _check_index("seq_lens", seq_lens, torch.int32, dev, B)
+    if query_starts is not None:
+        _check_index("query_starts", query_starts, torch.int32, dev, B + 1)
+    else:
+        _require(T % B == 0 if B else T == 0,
+                 f"{T} tokens are not the same number for each of {B} sequences: pass query_starts")
+    most = int(max_queries) if max_queries is not None else T if query_starts is not None or not B else T // B
+    _require(most >= 0 and window >= 0, "max_queries and window must not be negative")
+    L = _lib.lib()
+    with _on_device(q):
+        need = L.tw_kv4_attention_workspace(H, kv_heads, D, B, most, width, page)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(L.tw_kv4_attention(
+            _heads(out), _heads(q), pages.data_ptr(), num_pages, page, kv_heads, block_table.data_ptr(),
+            block_table.stride(0), width, seq_lens.data_ptr(),
+            None if query_starts is None else query_starts.data_ptr(), B, T, most, D, scale, window, code,
+            None if ws is None else ws.data_ptr(), need, _stream_ptr(q)))
+
+
 def num_compute_units(device=None) -> int:
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(dev):

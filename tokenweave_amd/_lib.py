@@ -24,9 +24,18 @@ TW_DTYPE_F32 = 2
 TW_MAX_PARTIALS = 16
 TW_SPLIT_MAX_TOKENS = 256
 TW_SPLIT_WORKSPACE_BYTES = TW_SPLIT_MAX_TOKENS * 384
+TW_ROTARY_INTERLEAVED = 1
+TW_ROTARY_INVERSE = 2
 
 _vp, _i64, _u64, _f32, _ci = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint64,
                               ctypes.c_float, ctypes.c_int)
+
+class Heads(ctypes.Structure):
+    """tw_heads: [tokens, heads, head_size] with contiguous channels, strides in elements."""
+    _fields_ = [("data", _vp), ("heads", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+_hp = ctypes.POINTER(Heads)
 
 # name -> argtypes; the order is the order of include/tokenweave_amd.h
 PROTOTYPES = {
@@ -58,7 +67,15 @@ PROTOTYPES = {
                                                        _i64, _i64, _ci, _f32, _ci, _vp],
     "tw_gemm_bf16_nt_partials_bias": [ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_vp),
                                       ctypes.POINTER(_vp), _ci, _i64, _i64, _i64, _i64, _ci, _vp],
+    "tw_rotary_positions": [_hp, _hp, _hp, _hp, _vp, _vp, _i64, _i64, _ci, _ci, _ci, _ci, _vp],
+    "tw_kv4_append": [_vp, _i64, _ci, _hp, _hp, _vp, _hp, _hp, _vp, _vp, _i64, _i64, _ci, _ci, _ci, _ci, _vp],
+    "tw_kv4_read": [_hp, _hp, _vp, _i64, _ci, _vp, _i64, _ci, _ci, _vp],
+    "tw_kv4_attention_workspace": [_ci, _ci, _ci, _i64, _i64, _i64, _ci],
+    "tw_kv4_attention": [_hp, _hp, _vp, _i64, _ci, _ci, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _ci, _f32, _i64,
+                         _ci, _vp, _i64, _vp],
 }
+# what an entry point returns where it is no status code
+RETURNS = {"tw_last_error": ctypes.c_char_p, "tw_kv4_attention_workspace": _i64}
 
 _lib = None
 
@@ -87,7 +104,7 @@ def lib() -> ctypes.CDLL:
         for name, argtypes in PROTOTYPES.items():
             fn = getattr(L, name)
             fn.argtypes = argtypes
-            fn.restype = ctypes.c_char_p if name == "tw_last_error" else _ci
+            fn.restype = RETURNS.get(name, _ci)
         _lib = L
     return _lib
 

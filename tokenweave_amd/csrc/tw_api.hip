@@ -1,6 +1,7 @@
 // extern "C" surface of libtokenweave_amd.so (declared in
 // include/tokenweave_amd.h): argument mapping only, kernels live in
-// tw_norm.hip and tw_gemm.hip.
+// tw_norm.hip and tw_gemm.hip.  The entry points of tw_rotary.hip and tw_attention.hip
+// are in tw_api_attention.hip.
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>

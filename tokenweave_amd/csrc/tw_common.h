@@ -76,6 +76,32 @@ int run_gemm_bf16_nt_partials(void* const* outs, const void* const* as, const vo
                               const void* const* biases, int count, int64_t M, int64_t N, int64_t K,
                               int64_t ldc, int max_cus, void* stream);
 
+struct Kv4Pages;
+
+int check_kv4_pages(const char* what, const void* pages, int64_t num_pages, int page_size, int64_t heads, int head_size,
+                    Kv4Pages* out);
+
+int run_rotary_positions(const tw_heads* q_out, const tw_heads* q, const tw_heads* k_out, const tw_heads* k,
+                         const int64_t* positions, const float* cos_sin, int64_t max_positions, int64_t T, int head_size,
+                         int rotary_dim, int flags, int dtype, void* stream);
+
+int run_kv4_append(void* pages, int64_t num_pages, int page_size, const tw_heads* k, const tw_heads* v,
+                   const int64_t* slots, const tw_heads* q_out, const tw_heads* q, const int64_t* positions,
+                   const float* cos_sin, int64_t max_positions, int64_t T, int head_size, int rotary_dim, int flags,
+                   int dtype, void* stream);
+
+int run_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void* pages, int64_t num_pages, int page_size,
+                 const int64_t* slots, int64_t T, int head_size, int dtype, void* stream);
+
+int64_t kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs, int64_t max_queries,
+                                int64_t table_width, int page_size);
+
+int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages, int64_t num_pages, int page_size,
+                      int kv_heads, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                      const int32_t* seq_lens, const int32_t* query_starts, int64_t num_seqs, int64_t T,
+                      int64_t max_queries, int head_size, float scale, int64_t window, int dtype, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 }  // namespace tw
 
 #endif

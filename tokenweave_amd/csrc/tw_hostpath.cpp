@@ -261,6 +261,63 @@ PyObject* gemm_bf16_nt_partials(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return yes_no(ok);
 }
 
+// None or a tensor; false for anything else.
+bool optional_plain(PyObject* o, const Tensor** t, bool data = true) {
+  *t = o == Py_None ? nullptr : plain(o, data);
+  return *t || o == Py_None;
+}
+
+bool as_bool(PyObject* o, bool* v) {
+  *v = o == Py_True;
+  return o == Py_True || o == Py_False;
+}
+
+// (q, k | None, positions, cos_sin, interleaved, inverse, q_out | None, k_out | None)
+PyObject* rotary_positions(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  bool interleaved, inverse;
+  const Tensor *k, *qo, *ko;
+  if (n != 8 || !direct_allowed()) Py_RETURN_FALSE;
+  const Tensor *q = plain(a[0]), *pos = plain(a[2]), *table = plain(a[3]);
+  if (!q || !pos || !table || !optional_plain(a[1], &k) || !as_bool(a[4], &interleaved) || !as_bool(a[5], &inverse) ||
+      !optional_plain(a[6], &qo) || !optional_plain(a[7], &ko))
+    Py_RETURN_FALSE;
+  return yes_no(enqueue([&] { tw_torch::rotary_positions(*q, k, *pos, *table, interleaved, inverse, qo, ko); }));
+}
+
+// (pages, k, v, slots, positions | None, cos_sin | None, interleaved, q | None, q_out | None)
+PyObject* kv4_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  bool interleaved;
+  const Tensor *pos, *table, *q, *qo;
+  if (n != 9 || !direct_allowed()) Py_RETURN_FALSE;
+  const Tensor *pages = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *slots = plain(a[3]);
+  if (!pages || !k || !v || !slots || !optional_plain(a[4], &pos) || !optional_plain(a[5], &table) ||
+      !as_bool(a[6], &interleaved) || !optional_plain(a[7], &q) || !optional_plain(a[8], &qo))
+    Py_RETURN_FALSE;
+  return yes_no(enqueue([&] { tw_torch::kv4_append(*pages, *k, *v, *slots, pos, table, interleaved, q, qo); }));
+}
+
+// (k_out, v_out, pages, slots)
+PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4 || !direct_allowed()) Py_RETURN_FALSE;
+  const Tensor *k = plain(a[0]), *v = plain(a[1]), *pages = plain(a[2]), *slots = plain(a[3]);
+  if (!k || !v || !pages || !slots) Py_RETURN_FALSE;
+  return yes_no(enqueue([&] { tw_torch::kv4_read(*k, *v, *pages, *slots); }));
+}
+
+// (out, q, pages, block_table, seq_lens, scale, query_starts | None, max_queries | None, window)
+PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  double scale;
+  int64_t most = -1, window;
+  const Tensor* starts;
+  if (n != 9 || !direct_allowed()) Py_RETURN_FALSE;
+  const Tensor *out = plain(a[0]), *q = plain(a[1]), *pages = plain(a[2]), *table = plain(a[3]), *lens = plain(a[4]);
+  if (!out || !q || !pages || !table || !lens || !as_double(a[5], &scale) || !optional_plain(a[6], &starts) ||
+      (a[7] != Py_None && (!as_int(a[7], &most) || most < 0)) || !as_int(a[8], &window))
+    Py_RETURN_FALSE;
+  return yes_no(
+      enqueue([&] { tw_torch::kv4_attention(*out, *q, *pages, *table, *lens, scale, starts, most, window); }));
+}
+
 // ---------------------------------------------------------------------------
 // layers.  An nn.Module whose __call__ would do more than call the class's forward (hooks, a
 // compiled or replaced forward) is not handled here.
@@ -465,6 +522,10 @@ PyMethodDef g_methods[] = {
     TW_FAST_RESULT("rms_norm_dynamic_per_token_quant", rms_norm_dynamic_per_token_quant),
     TW_FAST("gemm_bf16_nt", gemm_bf16_nt),
     TW_FAST("gemm_bf16_nt_partials", gemm_bf16_nt_partials),
+    TW_FAST("rotary_positions", rotary_positions),
+    TW_FAST("kv4_append", kv4_append),
+    TW_FAST("kv4_read", kv4_read),
+    TW_FAST("kv4_attention", kv4_attention),
     TW_FAST_RESULT("rms_norm_forward", rms_norm_forward),
     TW_FAST_RESULT("rms_norm_call", rms_norm_call),
     TW_FAST("fused_allreduce_layernorm", fused_allreduce_layernorm),

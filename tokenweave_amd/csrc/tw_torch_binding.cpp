@@ -9,6 +9,7 @@
 // shapes); their messages follow the reference's where it has one.  CPU tensors reach
 // the CPU registration, which only raises: there is no CPU implementation.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <hip/hip_runtime_api.h>
@@ -445,6 +446,150 @@ void gemm_bf16_nt_partials(const std::vector<const Tensor*>& outs, const std::ve
                                            l.stream));
   else
     check_rc(tw_gemm_bf16_nt_partials(o, pa, pb, (int)P, shape.M, shape.N, shape.K, shape.ldc, (int)max_cus, l.stream));
+}
+
+// ---------------------------------------------------------------------------
+// rotation, the paged 4-bit cache, attention
+// ---------------------------------------------------------------------------
+namespace {
+
+// [tokens, heads, head_size] with contiguous channels; `like`: of that shape.
+tw_heads check_heads(const char* name, const Tensor& t, at::ScalarType dtype, const c10::Device& device,
+                     const Tensor* like = nullptr) {
+  TORCH_CHECK(t.is_cuda() && t.device() == device, name, " is on ", t.device(), ", expected ", device);
+  TORCH_CHECK(t.scalar_type() == dtype, name, " has dtype ", dtype_name(t.scalar_type()), ", expected ", dtype_name(dtype));
+  TORCH_CHECK(t.dim() == 3 && (!like || t.sizes() == like->sizes()), name, " has shape ", t.sizes(),
+              ", expected [tokens, heads, head_size]");
+  TORCH_CHECK(t.stride(2) == 1 || t.size(2) == 1, "the channels of ", name, " must be contiguous");
+  return {t.data_ptr(), t.size(1), t.stride(0), t.stride(1)};
+}
+
+void check_same_rows(const char* name, const Tensor& t, const Tensor& like) {
+  TORCH_CHECK(t.size(0) == like.size(0) && t.size(2) == like.size(2), name, " has shape ", t.sizes());
+}
+
+void check_index(const char* name, const Tensor& t, at::ScalarType dtype, const c10::Device& device, int64_t numel) {
+  TORCH_CHECK(t.is_cuda() && t.device() == device && t.scalar_type() == dtype && t.dim() == 1 && t.is_contiguous() &&
+                  t.numel() == numel,
+              name, " must be a contiguous 1-D tensor of ", numel, " ", dtype_name(dtype), " on ", device);
+}
+
+void check_table(const Tensor& cos_sin, const c10::Device& device, int64_t head_size) {
+  check_tensor("cos_sin", cos_sin, at::kFloat, device);
+  TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.size(1) % 2 == 0 && cos_sin.size(1) >= 2 && cos_sin.size(1) <= head_size,
+              "cos_sin has shape ", cos_sin.sizes(), ", expected [positions, rotary_dim]");
+}
+
+int rotary_flags(bool interleaved, bool inverse) {
+  return (interleaved ? TW_ROTARY_INTERLEAVED : 0) | (inverse ? TW_ROTARY_INVERSE : 0);
+}
+
+// Tokens of a page.
+int64_t check_pages(const Tensor& pages, const c10::Device& device, int64_t heads, int64_t head_size) {
+  check_tensor("pages", pages, at::kByte, device);
+  const int64_t token = head_size + head_size / 16;
+  TORCH_CHECK(pages.dim() == 3 && pages.size(1) == heads && token > 0 && pages.size(2) % token == 0, "pages has shape ",
+              pages.sizes(), ", expected [pages, kv_heads, page_size * ", token, "]");
+  const int64_t page = pages.size(2) / token;
+  TORCH_CHECK(page >= TW_KV4_MIN_PAGE && page <= TW_KV4_MAX_PAGE, "pages of ", page, " tokens");
+  return page;
+}
+
+}  // namespace
+
+void rotary_positions(const Tensor& q, const Tensor* k, const Tensor& positions, const Tensor& cos_sin, bool interleaved,
+                      bool inverse, const Tensor* q_out, const Tensor* k_out) {
+  const int code = dtype_code("rotary_positions_kernel", q);
+  const auto dt = q.scalar_type();
+  const auto dev = q.device();
+  const tw_heads hq = check_heads("q", q, dt, dev);
+  const tw_heads hqo = q_out ? check_heads("q_out", *q_out, dt, dev, &q) : hq;
+  tw_heads hk{}, hko{};
+  TORCH_CHECK(k || !k_out, "k_out without k");
+  if (k) {
+    hk = check_heads("k", *k, dt, dev);
+    check_same_rows("k", *k, q);
+    hko = k_out ? check_heads("k_out", *k_out, dt, dev, k) : hk;
+  }
+  check_index("positions", positions, at::kLong, dev, q.size(0));
+  check_table(cos_sin, dev, q.size(2));
+  Launch l(q);
+  check_rc(tw_rotary_positions(&hqo, &hq, k ? &hko : nullptr, k ? &hk : nullptr, positions.data_ptr<int64_t>(),
+                               cos_sin.data_ptr<float>(), cos_sin.size(0), q.size(0), (int)q.size(2),
+                               (int)cos_sin.size(1), rotary_flags(interleaved, inverse), code, l.stream));
+}
+
+void kv4_append(const Tensor& pages, const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor* positions,
+                const Tensor* cos_sin, bool interleaved, const Tensor* q, const Tensor* q_out) {
+  const int code = dtype_code("kv4_append_kernel", k);
+  const auto dt = k.scalar_type();
+  const auto dev = k.device();
+  const tw_heads hk = check_heads("k", k, dt, dev), hv = check_heads("v", v, dt, dev, &k);
+  const int64_t page = check_pages(pages, dev, k.size(1), k.size(2));
+  check_index("slots", slots, at::kLong, dev, k.size(0));
+  if (cos_sin) {
+    check_table(*cos_sin, dev, k.size(2));
+    TORCH_CHECK(positions, "cos_sin without positions");
+    check_index("positions", *positions, at::kLong, dev, k.size(0));
+  }
+  TORCH_CHECK((!q || cos_sin) && (q || !q_out), "q needs cos_sin, q_out needs q");
+  tw_heads hq{}, hqo{};
+  if (q) {
+    hq = check_heads("q", *q, dt, dev);
+    check_same_rows("q", *q, k);
+    hqo = q_out ? check_heads("q_out", *q_out, dt, dev, q) : hq;
+  }
+  Launch l(k);
+  check_rc(tw_kv4_append(pages.data_ptr(), pages.size(0), (int)page, &hk, &hv, slots.data_ptr<int64_t>(),
+                         q ? &hqo : nullptr, q ? &hq : nullptr, cos_sin ? positions->data_ptr<int64_t>() : nullptr,
+                         cos_sin ? cos_sin->data_ptr<float>() : nullptr, cos_sin ? cos_sin->size(0) : 0, k.size(0),
+                         (int)k.size(2), cos_sin ? (int)cos_sin->size(1) : 0, rotary_flags(interleaved, false), code,
+                         l.stream));
+}
+
+void kv4_read(const Tensor& k_out, const Tensor& v_out, const Tensor& pages, const Tensor& slots) {
+  const int code = dtype_code("kv4_read_kernel", k_out);
+  const auto dt = k_out.scalar_type();
+  const auto dev = k_out.device();
+  const tw_heads hk = check_heads("k_out", k_out, dt, dev), hv = check_heads("v_out", v_out, dt, dev, &k_out);
+  const int64_t page = check_pages(pages, dev, k_out.size(1), k_out.size(2));
+  check_index("slots", slots, at::kLong, dev, k_out.size(0));
+  Launch l(k_out);
+  check_rc(tw_kv4_read(&hk, &hv, pages.data_ptr(), pages.size(0), (int)page, slots.data_ptr<int64_t>(), k_out.size(0),
+                       (int)k_out.size(2), code, l.stream));
+}
+
+void kv4_attention(const Tensor& out, const Tensor& q, const Tensor& pages, const Tensor& block_table,
+                   const Tensor& seq_lens, double scale, const Tensor* query_starts, int64_t max_queries, int64_t window) {
+  const auto dt = q.scalar_type();
+  TORCH_CHECK_NOT_IMPLEMENTED(dt == at::kBFloat16 || dt == at::kHalf, "\"kv4_attention_kernel\" not implemented for '",
+                              dtype_name(dt), "'");
+  const auto dev = q.device();
+  const tw_heads hq = check_heads("q", q, dt, dev), ho = check_heads("out", out, dt, dev, &q);
+  TORCH_CHECK(pages.dim() == 3, "pages has shape ", pages.sizes(), ", expected [pages, kv_heads, bytes]");
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2), kv_heads = pages.size(1);
+  const int64_t page = check_pages(pages, dev, kv_heads, D);
+  TORCH_CHECK(kv_heads > 0 && H % kv_heads == 0, H, " query heads over ", kv_heads, " key heads");
+  TORCH_CHECK(block_table.is_cuda() && block_table.device() == dev && block_table.scalar_type() == at::kInt &&
+                  block_table.dim() == 2 && (block_table.stride(1) == 1 || block_table.size(1) <= 1),
+              "block_table must be a 2-D torch.int32 tensor with contiguous rows");
+  const int64_t B = block_table.size(0), width = block_table.size(1);
+  check_index("seq_lens", seq_lens, at::kInt, dev, B);
+  if (query_starts) check_index("query_starts", *query_starts, at::kInt, dev, B + 1);
+  else TORCH_CHECK(B ? T % B == 0 : T == 0, T, " tokens are not the same number for each of ", B, " sequences");
+  const int64_t most = max_queries >= 0 ? max_queries : query_starts || !B ? T : T / B;
+  TORCH_CHECK(window >= 0, "window must not be negative");
+  Launch l(q);
+  const int64_t need = tw_kv4_attention_workspace((int)H, (int)kv_heads, (int)D, B, most, width, (int)page);
+  // from the allocator's pool: a block that a captured graph keeps, or that later work of this
+  // stream may be given again
+  Tensor ws;
+  if (need > 0) ws = at::detail::empty_cuda({need}, at::kByte, dev, std::nullopt);
+  check_rc(tw_kv4_attention(&ho, &hq, pages.data_ptr(), pages.size(0), (int)page, (int)kv_heads,
+                            block_table.data_ptr<int>(), block_table.stride(0), width, seq_lens.data_ptr<int>(),
+                            query_starts ? query_starts->data_ptr<int>() : nullptr, B, T, most, (int)D, (float)scale,
+                            window, dt == at::kBFloat16 ? TW_DTYPE_BF16 : TW_DTYPE_F16, need > 0 ? ws.data_ptr() : nullptr,
+                            need, l.stream));
 }
 
 }  // namespace tw_torch

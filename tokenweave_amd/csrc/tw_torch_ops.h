@@ -41,6 +41,20 @@ TW_TORCH_API void gemm_bf16_nt_partials(const std::vector<const Tensor*>& outs, 
                                         const std::vector<const Tensor*>& b, int64_t max_cus,
                                         const std::vector<const Tensor*>& biases);
 
+
+// Rotation, the paged 4-bit cache and attention over it; optional tensors may be null.  Not
+// registered: no reference schema.
+TW_TORCH_API void rotary_positions(const Tensor& q, const Tensor* k, const Tensor& positions, const Tensor& cos_sin,
+                                   bool interleaved, bool inverse, const Tensor* q_out, const Tensor* k_out);
+TW_TORCH_API void kv4_append(const Tensor& pages, const Tensor& k, const Tensor& v, const Tensor& slots,
+                             const Tensor* positions, const Tensor* cos_sin, bool interleaved, const Tensor* q,
+                             const Tensor* q_out);
+TW_TORCH_API void kv4_read(const Tensor& k_out, const Tensor& v_out, const Tensor& pages, const Tensor& slots);
+// max_queries < 0: not given.
+TW_TORCH_API void kv4_attention(const Tensor& out, const Tensor& q, const Tensor& pages, const Tensor& block_table,
+                                const Tensor& seq_lens, double scale, const Tensor* query_starts, int64_t max_queries,
+                                int64_t window);
+
 }  // namespace tw_torch
 
 #endif
