@@ -391,7 +391,8 @@ TW_API int tw_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void*
  * workspace: tw_kv4_attention_workspace() bytes, 16-byte aligned, contents of no meaning
  * before and after; calls that may run at the same time need one each. */
 TW_API int64_t tw_kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs,
-                                          int64_t max_queries, int64_t table_width, int page_size);
+                                          int64_t num_tokens, int64_t max_queries, int64_t table_width,
+                                          int page_size);
 TW_API int tw_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
                             int64_t num_pages, int page_size, int kv_heads,
                             const int32_t* block_table, int64_t table_stride, int64_t table_width,

@@ -164,7 +164,7 @@ def test_attention_entry_point_checks_before_it_launches():
                dict(width=-1), dict(width=1 << 40), dict(q=heads(4, AT, -2)), dict(pages=None)):
         assert attend(**kw) == bad, kw
     assert attend(dtype=_lib.TW_DTYPE_F32) == _lib.TW_ERR_DTYPE and attend(pages=AT + 4) == _lib.TW_ERR_ALIGNMENT
-    need = L.tw_kv4_attention_workspace(4, 2, 128, 2, 1, 8, 16)
+    need = L.tw_kv4_attention_workspace(4, 2, 128, 2, 2, 1, 8, 16)
     assert need >= 0
     if need:
         assert attend(ws=None) == bad and attend(ws_bytes=need - 1) == bad and attend(ws=AT + 4) == bad

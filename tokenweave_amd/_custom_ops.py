@@ -948,7 +948,7 @@ def kv4_attention(out: torch.Tensor, q: torch.Tensor, pages: torch.Tensor, block
     _require(most >= 0 and window >= 0, "max_queries and window must not be negative")
     L = _lib.lib()
     with _on_device(q):
-        need = L.tw_kv4_attention_workspace(H, kv_heads, D, B, most, width, page)
+        need = L.tw_kv4_attention_workspace(H, kv_heads, D, B, T, most, width, page)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(L.tw_kv4_attention(
             _heads(out), _heads(q), pages.data_ptr(), num_pages, page, kv_heads, block_table.data_ptr(),

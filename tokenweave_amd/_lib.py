@@ -70,7 +70,7 @@ PROTOTYPES = {
     "tw_rotary_positions": [_hp, _hp, _hp, _hp, _vp, _vp, _i64, _i64, _ci, _ci, _ci, _ci, _vp],
     "tw_kv4_append": [_vp, _i64, _ci, _hp, _hp, _vp, _hp, _hp, _vp, _vp, _i64, _i64, _ci, _ci, _ci, _ci, _vp],
     "tw_kv4_read": [_hp, _hp, _vp, _i64, _ci, _vp, _i64, _ci, _ci, _vp],
-    "tw_kv4_attention_workspace": [_ci, _ci, _ci, _i64, _i64, _i64, _ci],
+    "tw_kv4_attention_workspace": [_ci, _ci, _ci, _i64, _i64, _i64, _i64, _ci],
     "tw_kv4_attention": [_hp, _hp, _vp, _i64, _ci, _ci, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _ci, _f32, _i64,
                          _ci, _vp, _i64, _vp],
 }

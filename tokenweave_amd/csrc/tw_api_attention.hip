@@ -25,9 +25,10 @@ int tw_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void* pages,
   return tw::run_kv4_read(k_out, v_out, pages, num_pages, page_size, slots, num_tokens, head_size, dtype, stream);
 }
 
-int64_t tw_kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs, int64_t max_queries,
-                                   int64_t table_width, int page_size) {
-  return tw::kv4_attention_workspace(q_heads, kv_heads, head_size, num_seqs, max_queries, table_width, page_size);
+int64_t tw_kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs, int64_t num_tokens,
+                                   int64_t max_queries, int64_t table_width, int page_size) {
+  return tw::kv4_attention_workspace(q_heads, kv_heads, head_size, num_seqs, num_tokens, max_queries, table_width,
+                                     page_size);
 }
 
 int tw_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages, int64_t num_pages, int page_size,

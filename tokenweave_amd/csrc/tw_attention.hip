@@ -56,82 +56,10 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int64_t s) 
   return q;
 }
 
-__device__ __forceinline__ const uint8_t* page_of(const AttentionArgs& a, int64_t s, int64_t token, int head) {
-  const int64_t page = a.block_table[s * a.table_stride + (token >> a.pages.page_log2)];
-  return page < 0 || page >= a.pages.num_pages ? nullptr
-                                               : a.pages.data + (page * a.pages.heads + head) * a.pages.head_bytes;
-}
-
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
   for (int i = 1; i < 64; i <<= 1) x = fmaxf(x, __shfl_xor(x, i));
   return x;
-}
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) x += __shfl_xor(x, i);
-  return x;
-}
-
-// One wave for one query head of one new token: a lane scores a token, then holds D / 64 channels.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void attention_row_kernel(AttentionArgs a) {
-  using L = Kv4<D>;
-  __shared__ float q_row[D];
-  const int P = 1 << a.pages.page_log2, lane = threadIdx.x;
-  const int64_t s = blockIdx.z;
-  const int head = blockIdx.y, kv_head = head / a.group;
-  const Sequence seq = sequence(a, s);
-  for (int64_t i = blockIdx.x; i < seq.count && i < a.max_queries; i += gridDim.x) {
-    const T* q = static_cast<const T*>(a.q) + (seq.first + i) * a.q_token + head * a.q_head;
-    __syncthreads();
-    for (int c = lane; c < D; c += 64) q_row[c] = (float)q[c];
-    __syncthreads();
-    const int64_t end = seq.length - seq.count + i + 1;  // tokens before it are seen
-    const int64_t begin = a.window > 0 ? max(end - a.window, (int64_t)0) : 0;
-    float m = -__builtin_inff(), l = 0.0f, o[D / 64] = {};
-    for (int64_t base = begin & ~(int64_t)63; base < end; base += 64) {
-      const int64_t t = base + lane;
-      const int at = (int)t & (P - 1);
-      const uint8_t* page = t >= begin && t < end ? page_of(a, s, t, kv_head) : nullptr;
-      float score = -__builtin_inff();
-      if (page) {
-        score = 0.0f;
-        for (int g = 0; g < L::kGroups; ++g) {
-          float sum = 0.0f;
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(page + L::key(at) + g * 16 + w * 4);
-            for (int c = 0; c < 8; ++c) sum += q_row[g * 32 + w * 8 + c] * e2m1_value(word >> (4 * c));
-          }
-          score += sum * scale_of(page[L::key_scale(P, at, g)]);
-        }
-        score *= a.scale;
-      }
-      const float most = fmaxf(m, wave_max(score));
-      const float base_score = most == -__builtin_inff() ? 0.0f : most;
-      const float p = __builtin_amdgcn_exp2f(score - base_score), old = __builtin_amdgcn_exp2f(m - base_score);
-      l = l * old + wave_sum(p);
-      m = most;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) o[c] *= old;
-      for (int j = 0; j < 64; ++j) {
-        const float pj = __shfl(p, j);
-        const uint8_t* pg = reinterpret_cast<const uint8_t*>(__shfl((unsigned long long)page, j));
-        if (!pg) continue;
-        const int tj = (int)(base + j) & (P - 1);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const int ch = c * 64 + lane, sixteenth = ch / (D / 16), in = ch % (D / 16);
-          const uint32_t byte = pg[L::value(P, tj, sixteenth) + in / 2];
-          o[c] += pj * e2m1_value(byte >> (4 * (in & 1))) * scale_of(pg[L::value_scale(P, tj, ch / 32)]);
-        }
-      }
-    }
-    T* out = static_cast<T*>(a.out) + (seq.first + i) * a.out_token + head * a.out_head;
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) out[c * 64 + lane] = (T)(l > 0.0f || l != l ? o[c] / l : 0.0f);
-  }
 }
 
 // ---------------------------------------------------------------------------
@@ -660,21 +588,421 @@ int launch_split(const SplitArgs& args, int D, int grid, void* stream) {
   return launch_split<T, 256>(args, grid, stream);
 }
 
-template <typename T>
-int launch_rows(const AttentionArgs& a, int D, int q_heads, void* stream) {
-  const dim3 grid((unsigned)min(a.max_queries, (int64_t)65535), (unsigned)q_heads, (unsigned)a.num_seqs);
-  auto kernel = D == 64 ? attention_row_kernel<T, 64> : D == 128 ? attention_row_kernel<T, 128> : attention_row_kernel<T, 256>;
-  launch_kernel(kernel, grid, dim3(64), 0, static_cast<hipStream_t>(stream), a);
+// ---------------------------------------------------------------------------
+// Many rows: a tile of 32 rows a wave, all of one key head.
+//
+// The workgroup turns 64 tokens at a time into fp16 in LDS, once for all its rows, double-buffered: the
+// codes of the tile after next are on their way and the next tile is written while the present one is
+// multiplied.  32 x 32 x 16 products; as above the scores of a row stay in the two lanes that hold
+// the row, and go into the second product without moving.  Values lie in LDS by channel, their
+// tokens in the order in which the scores' registers hold them: of 16 tokens 0-3, 8-11, 4-7, 12-15.
+// ---------------------------------------------------------------------------
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+constexpr int kTileTokens = 64;
+
+struct TileArgs {
+  AttentionArgs a;
+  float* parts;  // of `splits` pieces of every tile's tokens: [tile][head][split][rows][D + 2]; null: one piece
+  int tiles, splits;
+};
+
+// Sequence and place in it of tile `tile` (uniform); a tile behind the last: seq < 0.
+template <int THREADS>
+__device__ __forceinline__ void find_tile(const AttentionArgs& a, int tile, int rows_of_tile, int* seq, int* place,
+                                          int* lds) {
+  constexpr int kW = THREADS / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) lds[kW] = -1;
+  int base = 0;
+  for (int64_t s0 = 0; s0 < a.num_seqs; s0 += THREADS) {
+    const int64_t s = s0 + threadIdx.x;
+    int count = 0;
+    if (s < a.num_seqs) {
+      const int64_t rows = min(sequence(a, s).count, a.max_queries) * a.group;
+      count = (int)((rows + rows_of_tile - 1) / rows_of_tile);
+    }
+    int sum = count;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+      const int y = __shfl_up(sum, i);
+      if (lane >= i) sum += y;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = sum;
+    __syncthreads();
+    int before = base + sum - count;
+    for (int w = 0; w < kW; ++w) {
+      before += w < wave ? lds[w] : 0;
+      base += lds[w];
+    }
+    if (tile >= before && tile < before + count) {
+      lds[kW] = (int)s;
+      lds[kW + 1] = tile - before;
+    }
+    if (base > tile) break;
+  }
+  __syncthreads();
+  *seq = uniform(lds[kW]);
+  *place = uniform(lds[kW + 1]);
+}
+
+template <int D, int WAVES>
+struct TileShape {
+  static constexpr int kThreads = 64 * WAVES, kRows = 32 * WAVES;
+  static constexpr int kKeyRow = D * 2 + 16, kValueRow = kTileTokens * 2 + 16;  // 16 bytes more: no two lanes' rows in one bank
+  static constexpr int kKeyChunks = kTileTokens * (D / 32);                     // 32 channels of a token
+  static constexpr int kValueChunks = (kTileTokens / 4) * 16;                   // 4 tokens of a sixteenth
+  static constexpr int kKeyTurns = (kKeyChunks + kThreads - 1) / kThreads;
+  static constexpr int kValueTurns = (kValueChunks + kThreads - 1) / kThreads;
+  // keys by the first threads and values by the last ones where there are threads for both
+  static constexpr int kValueThread = kKeyChunks + kValueChunks <= kThreads ? kThreads - kValueChunks : 0;
+};
+
+template <int D, int WAVES>
+struct __align__(16) TileBuffer {
+  using S = TileShape<D, WAVES>;
+  uint8_t k[kTileTokens * S::kKeyRow];
+  uint8_t v[D * S::kValueRow];
+};
+
+// What a thread fetches of a tile.
+template <int D, int WAVES>
+struct Fetched {
+  using S = TileShape<D, WAVES>;
+  uint32_t k[S::kKeyTurns][4], ks[S::kKeyTurns];
+  uint32_t v[S::kValueTurns][D / 32], vs[S::kValueTurns];
+};
+
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(TileArgs args) {
+  using S = TileShape<D, WAVES>;
+  using L = Kv4<D>;
+  const AttentionArgs& a = args.a;
+  __shared__ TileBuffer<D, WAVES> buffers[2];
+  __shared__ int found[WAVES + 2];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int P = 1 << a.pages.page_log2, heads = a.pages.heads;
+  const int tile = args.tiles - 1 - (int)blockIdx.x;  // a prompt's last tiles see the most: they go first
+  const int head = blockIdx.y, split = blockIdx.z;
+
+  int s, place;
+  find_tile<S::kThreads>(a, tile, S::kRows, &s, &place, found);
+  if (s < 0) return;
+  const Sequence seq = sequence(a, s);
+  const int queries = (int)min(seq.count, a.max_queries), rows = queries * a.group, length = (int)seq.length;
+  const int new_from = length - (int)seq.count;
+  const int row0 = place * S::kRows, last_row = min(row0 + S::kRows, rows) - 1;
+
+  // ---- tokens that the tile's rows see, and this piece of them
+  const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
+  auto end_of = [&](int row) { return min(new_from + row / a.group + 1, length); };
+  auto begin_of = [&](int row) { return (int)max((int64_t)new_from + row / a.group + 1 - window, (int64_t)0); };
+  const int some_from = begin_of(row0), some_to = end_of(last_row);
+  int tile_from = some_from / kTileTokens, tile_to = max((some_to + kTileTokens - 1) / kTileTokens, tile_from);
+  if (args.splits > 1) {
+    const int each = (tile_to - tile_from + args.splits - 1) / args.splits;
+    tile_from = min(tile_from + split * each, tile_to);
+    tile_to = min(tile_from + each, tile_to);
+  }
+
+  // ---- this wave's rows
+  const int row = row0 + wave * 32 + n, query = row / a.group, q_head = head * a.group + row - query * a.group;
+  const int row_end = row < rows ? end_of(row) : 0, row_begin = row < rows ? begin_of(row) : 0;
+  const int wave_row = row0 + wave * 32, wave_last = min(wave_row + 31, rows - 1);
+  const bool idle = wave_row >= rows;
+  const int wave_to = idle ? 0 : end_of(wave_last), wave_from = idle ? 0 : begin_of(wave_row);
+  const int all_to = idle ? 0 : end_of(wave_row), all_from = idle ? 0 : begin_of(wave_last);
+  half8_t q[D / 16];
+  float scale;
+  {
+    const T* from = static_cast<const T*>(a.q) + (seq.first + query) * a.q_token + (int64_t)q_head * a.q_head + h * 8;
+    float x[D / 2], most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[c * 8 + j] = row < rows ? (float)from[c * 16 + j] : 0.0f;
+        most = fmaxf(most, __builtin_fabsf(x[c * 8 + j]));
+      }
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
+    const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < D / 2; ++i) q[i / 8][i % 8] = (_Float16)(x[i] * up);
+    scale = __uint_as_float((uint32_t)(127 - 14 + e) << 23) * a.scale;
+  }
+  float m = -__builtin_inff(), l = 0.0f;
+  float16_t o[D / 32];
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
+
+  const int32_t* table = a.block_table + (int64_t)s * a.table_stride;
+  // Base of the block that holds token t; tokens of a missing page are read from page 0 and masked.
+  auto block_of = [&](int t, bool* there) {
+    const int id = t < length ? table[t >> a.pages.page_log2] : -1;
+    *there = id >= 0 && id < a.pages.num_pages;
+    return a.pages.data + ((int64_t)(*there ? id : 0) * heads + head) * a.pages.head_bytes;
+  };
+  auto fetch = [&](Fetched<D, WAVES>& f, int t0) {
+#pragma unroll
+    for (int i = 0; i < S::kKeyTurns; ++i) {
+      const int chunk = (int)threadIdx.x + i * S::kThreads;
+      if (S::kKeyChunks % S::kThreads == 0 || chunk < S::kKeyChunks) {
+        const int t = t0 + chunk / (D / 32), g = chunk % (D / 32), at = t & (P - 1);
+        bool there;
+        const uint8_t* b = block_of(t, &there);
+        load_words(f.k[i], b + (L::key(at) + g * 16));
+        f.ks[i] = b[L::key_scale(P, at, g)];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::kValueTurns; ++i) {
+      const int chunk = (int)threadIdx.x - S::kValueThread + i * S::kThreads;
+      if (S::kValueChunks % S::kThreads == 0 || (chunk >= 0 && chunk < S::kValueChunks)) {
+        // of 32 neighbouring lanes two sixteenths and all 16 fours of tokens: their LDS writes cover all banks
+        const int sixteenth = (chunk & 1) | (chunk >> 5 << 1), t = t0 + (chunk >> 1 & 15) * 4, at = t & (P - 1);
+        bool there;
+        const uint8_t* b = block_of(t, &there);
+        load_words(f.v[i], b + L::value(P, at, sixteenth));
+        uint32_t vs = *reinterpret_cast<const uint32_t*>(b + L::value_scale(P, at, sixteenth * (D / 16) / 32));
+        // what no row sees may hold anything, and nothing times zero has to be zero
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!there || t + j >= length || t + j < some_from) vs = (vs & ~(255u << (8 * j))) | 127u << (8 * j);
+        f.vs[i] = vs;
+      }
+    }
+  };
+  auto spread = [&](const Fetched<D, WAVES>& f, TileBuffer<D, WAVES>& to) {
+#pragma unroll
+    for (int i = 0; i < S::kKeyTurns; ++i) {
+      const int chunk = (int)threadIdx.x + i * S::kThreads;
+      if (S::kKeyChunks % S::kThreads == 0 || chunk < S::kKeyChunks) {
+        uint8_t* at = to.k + chunk / (D / 32) * S::kKeyRow + chunk % (D / 32) * 64;
+        const float ks = __uint_as_float(f.ks[i] << 23);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) *reinterpret_cast<half8_t*>(at + w * 16) = eight_values(f.k[i][w], ks);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::kValueTurns; ++i) {
+      const int chunk = (int)threadIdx.x - S::kValueThread + i * S::kThreads;
+      if (S::kValueChunks % S::kThreads == 0 || (chunk >= 0 && chunk < S::kValueChunks)) {
+        const int sixteenth = (chunk & 1) | (chunk >> 5 << 1), four = chunk >> 1 & 15;
+        // fours 0, 1, 2, 3 of 16 tokens lie in the order 0, 2, 1, 3
+        uint8_t* at = to.v + sixteenth * (D / 16) * S::kValueRow +
+                      ((four & ~3) | (four & 1) << 1 | (four >> 1 & 1)) * 8;
+        float vs[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vs[j] = __uint_as_float((f.vs[i] >> (8 * j) & 255) << 23);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {  // byte b of each token: two channels
+          half2_t x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int byte = j * (D / 32) + b;
+            const uint32_t w = f.v[i][byte / 4];
+            x[j] = byte % 4 == 0 ? two_values<0>(w, vs[j]) : byte % 4 == 1 ? two_values<1>(w, vs[j])
+                 : byte % 4 == 2 ? two_values<2>(w, vs[j]) : two_values<3>(w, vs[j]);
+          }
+          typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            *reinterpret_cast<half4_t*>(at + (2 * b + c) * S::kValueRow) = half4_t{x[0][c], x[1][c], x[2][c], x[3][c]};
+        }
+      }
+    }
+  };
+
+  Fetched<D, WAVES> next;
+  if (tile_from < tile_to) {
+    fetch(next, tile_from * kTileTokens);
+    spread(next, buffers[0]);
+    if (tile_from + 1 < tile_to) fetch(next, (tile_from + 1) * kTileTokens);
+  }
+  __syncthreads();
+  for (int at = tile_from; at < tile_to; ++at) {
+    const TileBuffer<D, WAVES>& now = buffers[(at - tile_from) & 1];
+    const int t0 = at * kTileTokens;
+    if (at + 1 < tile_to) spread(next, buffers[(at - tile_from + 1) & 1]);
+    if (at + 2 < tile_to) fetch(next, t0 + 2 * kTileTokens);
+    if (t0 < wave_to && t0 + kTileTokens > wave_from) {
+      float16_t sc[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[i][j] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const half8_t k = *reinterpret_cast<const half8_t*>(now.k + (i * 32 + n) * S::kKeyRow + c * 32 + h * 16);
+          sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[c], sc[i], 0, 0, 0);
+        }
+      bool whole = t0 >= all_from && t0 + kTileTokens <= all_to;
+      // pages of the tile's four sixteens
+      bool there[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i * 16, id = t < length ? table[t >> a.pages.page_log2] : -1;
+        there[i] = id >= 0 && id < a.pages.num_pages;
+        whole = whole && there[i];
+      }
+      float most = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float x = sc[i][j] * scale;
+          if (!whole) {
+            const int t = t0 + i * 32 + (j / 4) * 8 + h * 4 + j % 4;
+            if (t >= row_end || t < row_begin || !there[i * 2 + j / 8]) x = -__builtin_inff();
+          }
+          sc[i][j] = x;
+          most = fmaxf(most, x);
+        }
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if (__builtin_amdgcn_ballot_w64(most > m)) {
+        const float higher = fmaxf(m, most);
+        const float old = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
+        m = higher;
+        l *= old;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) o[c] *= old;
+      }
+      const float sub = (m == -__builtin_inff() ? 0.0f : m) - kLift;
+      half8_t p[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float x = __builtin_amdgcn_exp2f(sc[i][j] - sub);
+          l += x;
+          p[i * 2 + j / 8][j % 8] = (_Float16)x;
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const half8_t v = *reinterpret_cast<const half8_t*>(now.v + (c * 32 + n) * S::kValueRow + k * 32 + h * 16);
+          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[k], o[c], 0, 0, 0);
+        }
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32);
+  if (row >= rows) return;
+  if (args.splits == 1) {
+    T* out = static_cast<T*>(a.out) + (seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) out[c * 32 + (i / 4) * 8 + h * 4 + i % 4] = (T)(o[c][i] * inv);
+  } else {
+    float* part = args.parts + ((((int64_t)tile * heads + head) * args.splits + split) * S::kRows + row - row0) * (D + 2);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[c * 32 + (i / 4) * 8 + h * 4 + i % 4] = o[c][i];
+    if (h == 0) {
+      part[D] = m;
+      part[D + 1] = l;
+    }
+  }
+}
+
+// Joins the pieces of a tile's rows: a wave takes one row.
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args) {
+  using S = TileShape<D, WAVES>;
+  const AttentionArgs& a = args.a;
+  __shared__ int found[4 + 2];
+  const int tile = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63;
+  int s, place;
+  find_tile<256>(a, tile, S::kRows, &s, &place, found);
+  if (s < 0) return;
+  const Sequence seq = sequence(a, s);
+  const int rows = (int)min(seq.count, a.max_queries) * a.group;
+  const int in_tile = blockIdx.z * 4 + (threadIdx.x >> 6), row = place * S::kRows + in_tile;
+  if (row >= rows) return;
+  const float* part = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows + in_tile) * (D + 2);
+  const int64_t stride = (int64_t)S::kRows * (D + 2);
+  float m = -__builtin_inff(), l = 0.0f, o[D / 64] = {};
+  for (int c = 0; c < args.splits; ++c) m = fmaxf(m, part[c * stride + D]);
+#pragma unroll 4
+  for (int c = 0; c < args.splits; ++c) {
+    const float* p = part + c * stride;
+    const float weight = p[D] == m ? 1.0f : __builtin_amdgcn_exp2f(p[D] - m);
+    l += p[D + 1] * weight;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) o[k] += p[k * 64 + lane] * weight;
+  }
+  const int query = row / a.group;
+  T* out = static_cast<T*>(a.out) + (seq.first + query) * a.out_token +
+           (int64_t)(head * a.group + row - query * a.group) * a.out_head;
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) out[k * 64 + lane] = (T)(l > 0.0f || l != l ? o[k] / l : 0.0f);
+}
+
+// Tiles and pieces of a call.
+struct TilePlan {
+  int waves, tiles, splits;
+  int64_t bytes;
+};
+
+// Eight waves, two a SIMD unit, share a tile's keys and values; heads of 256 channels leave registers for one.
+int tile_waves(int head_size) { return head_size == 256 ? 4 : 8; }
+
+TilePlan plan_tiles(int64_t T, int group, int kv_heads, int head_size, int64_t num_seqs, int64_t max_queries,
+                    int64_t table_width, int page_size) {
+  TilePlan plan;
+  plan.waves = tile_waves(head_size);
+  const int64_t rows = 32 * plan.waves;
+  // every sequence may leave one tile that is not full
+  const int64_t tiles = min((T * group + rows - 1) / rows + num_seqs, num_seqs * ((max_queries * group + rows - 1) / rows));
+  const int cus = device_compute_units();
+  // too few tiles for the compute units: their tokens are cut into pieces of 256 and more
+  const int64_t units = tiles * kv_heads, most = max(table_width * page_size / 256, (int64_t)1);
+  plan.splits = (int)min(max((cus > 0 ? cus : 256) / units, (int64_t)1), most);
+  plan.tiles = (int)min(tiles, (int64_t)0x7fffffff);
+  plan.bytes = plan.splits == 1 ? 0 : tiles * kv_heads * plan.splits * rows * (head_size + 2) * (int64_t)sizeof(float);
+  return plan;
+}
+
+template <typename T, int D, int WAVES>
+int launch_tiles(const TileArgs& args, void* stream) {
+  const unsigned heads = (unsigned)args.a.pages.heads;
+  launch_kernel(attention_tile_kernel<T, D, WAVES>, dim3((unsigned)args.tiles, heads, (unsigned)args.splits),
+                dim3(64 * WAVES), 0, static_cast<hipStream_t>(stream), args);
+  int rc = finish_launch("kv4_attention");
+  if (rc != TW_OK || args.splits == 1) return rc;
+  launch_kernel(attention_join_tile_kernel<T, D, WAVES>, dim3((unsigned)args.tiles, heads, 32 * WAVES / 4), dim3(256), 0,
+                static_cast<hipStream_t>(stream), args);
   return finish_launch("kv4_attention");
+}
+
+template <typename T>
+int launch_tiles(const TileArgs& args, int D, void* stream) {
+  if (D == 64) return launch_tiles<T, 64, 8>(args, stream);
+  if (D == 128) return launch_tiles<T, 128, 8>(args, stream);
+  return launch_tiles<T, 256, 4>(args, stream);
 }
 
 }  // namespace
 
-int64_t kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs, int64_t max_queries,
-                                int64_t table_width, int page_size) {
-  if (q_heads < 1 || kv_heads < 1 || num_seqs < 1 || max_queries < 1) return 0;
-  const int64_t rows = max_queries * (q_heads / kv_heads);
-  return rows > kMostRows ? 0 : split_bytes(split_grid(num_seqs, kv_heads, table_width, page_size), (int)rows, head_size);
+int64_t kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs, int64_t num_tokens,
+                                int64_t max_queries, int64_t table_width, int page_size) {
+  if (q_heads < 1 || kv_heads < 1 || num_seqs < 1 || num_tokens < 1 || max_queries < 1) return 0;
+  const int group = q_heads / kv_heads;
+  max_queries = min(max_queries, num_tokens);
+  if (max_queries * group <= kMostRows)
+    return split_bytes(split_grid(num_seqs, kv_heads, table_width, page_size), (int)max_queries * group, head_size);
+  return plan_tiles(num_tokens, group, kv_heads, head_size, num_seqs, max_queries, table_width, page_size).bytes;
 }
 
 int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages, int64_t num_pages, int page_size,
@@ -703,7 +1031,8 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   if (!query_starts && T % num_seqs != 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld tokens are not the same number for each of %lld sequences", what,
                      (long long)T, (long long)num_seqs);
-  const int64_t need = kv4_attention_workspace((int)q->heads, kv_heads, head_size, num_seqs, max_queries, table_width, page_size);
+  const int64_t need = kv4_attention_workspace((int)q->heads, kv_heads, head_size, num_seqs, T, max_queries,
+                                               table_width, page_size);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, need %lld, 16-byte aligned", what,
                      (long long)workspace_bytes, (long long)need);
@@ -725,7 +1054,8 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   a.max_queries = min(max_queries, T);
   a.scale = scale * kLog2e;
   a.window = window;
-  if (need > 0) {
+  max_queries = a.max_queries;
+  if (max_queries * a.group <= kMostRows) {
     const int grid = split_grid(num_seqs, kv_heads, table_width, page_size);
     // steps are counted in 32 bits
     if ((double)num_seqs * kv_heads * (double)((table_width * page_size + kStep - 1) / kStep + 1) > 2e9)
@@ -736,8 +1066,12 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
     return dtype == TW_DTYPE_BF16 ? launch_split<__bf16>(args, head_size, grid, stream)
                                   : launch_split<_Float16>(args, head_size, grid, stream);
   }
-  return dtype == TW_DTYPE_BF16 ? launch_rows<__bf16>(a, head_size, (int)q->heads, stream)
-                                : launch_rows<_Float16>(a, head_size, (int)q->heads, stream);
+  const TilePlan plan = plan_tiles(T, a.group, kv_heads, head_size, num_seqs, max_queries, table_width, page_size);
+  if ((double)T * a.group + (double)num_seqs * 256 > 2e9 || kv_heads > 65535)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too many rows", what);
+  const TileArgs args{a, static_cast<float*>(workspace), plan.tiles, plan.splits};
+  return dtype == TW_DTYPE_BF16 ? launch_tiles<__bf16>(args, head_size, stream)
+                                : launch_tiles<_Float16>(args, head_size, stream);
 }
 
 }  // namespace tw

@@ -93,8 +93,8 @@ int run_kv4_append(void* pages, int64_t num_pages, int page_size, const tw_heads
 int run_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void* pages, int64_t num_pages, int page_size,
                  const int64_t* slots, int64_t T, int head_size, int dtype, void* stream);
 
-int64_t kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs, int64_t max_queries,
-                                int64_t table_width, int page_size);
+int64_t kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_t num_seqs, int64_t num_tokens,
+                                int64_t max_queries, int64_t table_width, int page_size);
 
 int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages, int64_t num_pages, int page_size,
                       int kv_heads, const int32_t* block_table, int64_t table_stride, int64_t table_width,

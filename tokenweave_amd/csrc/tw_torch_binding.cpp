@@ -580,7 +580,7 @@ void kv4_attention(const Tensor& out, const Tensor& q, const Tensor& pages, cons
   const int64_t most = max_queries >= 0 ? max_queries : query_starts || !B ? T : T / B;
   TORCH_CHECK(window >= 0, "window must not be negative");
   Launch l(q);
-  const int64_t need = tw_kv4_attention_workspace((int)H, (int)kv_heads, (int)D, B, most, width, (int)page);
+  const int64_t need = tw_kv4_attention_workspace((int)H, (int)kv_heads, (int)D, B, T, most, width, (int)page);
   // from the allocator's pool: a block that a captured graph keeps, or that later work of this
   // stream may be given again
   Tensor ws;
