@@ -32,6 +32,7 @@ struct AttentionArgs {
   int64_t num_seqs, num_tokens, max_queries;
   float scale;  // with log2(e)
   int64_t window;
+  bool q_wide, out_wide;  // every row is 16-byte aligned
 };
 
 // Sequence `s`: its new tokens [first, first + count) and its cached ones.
@@ -93,7 +94,7 @@ struct SplitHeader {
 struct SplitArgs {
   AttentionArgs a;
   SplitHeader* headers;  // one a workgroup
-  float* parts;          // two a workgroup: [rows][D + 2], m and l behind the D channels
+  float* parts;          // two a workgroup: [rows][D + 4], m and l behind the D channels
   int rows;              // of a part
 };
 
@@ -107,27 +108,17 @@ __device__ __forceinline__ void steps_of(const AttentionArgs& a, const Sequence&
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Sum over the workgroup's threads before this one, and over all.
-__device__ __forceinline__ int block_scan(int x, int* total, int* lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int sum = x;
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) {
-    const int y = __shfl_up(sum, i);
-    if (lane >= i) sum += y;
-  }
-  __syncthreads();
-  if (lane == 63) lds[wave] = sum;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const int y = lds[w];
-    before += w < wave ? y : 0;
-    all += y;
-  }
-  *total = all;
-  return before + sum - x;
+// Sum over the wave's lanes up to this one.
+__device__ __forceinline__ int wave_scan(int x) {
+#define TW_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
+  TW_SCAN_STEP(0x111, 0xf);  // from 1, 2, 4, 8 lanes before, within 16
+  TW_SCAN_STEP(0x112, 0xf);
+  TW_SCAN_STEP(0x114, 0xf);
+  TW_SCAN_STEP(0x118, 0xf);
+  TW_SCAN_STEP(0x142, 0xa);  // the 16 before, into the second and the fourth 16
+  TW_SCAN_STEP(0x143, 0xc);  // the first half, into the second
+#undef TW_SCAN_STEP
+  return x;
 }
 
 // One wave's 32 tokens of the cache.
@@ -197,21 +188,54 @@ __device__ __forceinline__ half8_t eight_values(uint32_t word, float scale) {
 // The rows' queries as the right operand: lane (n, h) holds row n's channels h * D/4 .. in steps of 8.
 // A row is multiplied by the power of two that brings its largest magnitude to [2^14, 2^15), where
 // every bf16 and fp16 value down to 2^-28 of it is exact; the score is multiplied back.
-template <typename T, int D>
-__device__ __forceinline__ float load_queries(half8_t (&q)[D / 32], const T* row) {
-  float x[D / 4], most = 0.0f;
+template <typename T, int N>
+__device__ __forceinline__ void load_row(float (&x)[N], const T* row, bool wide) {
+  if (wide) {
+    typedef T vec_t __attribute__((ext_vector_type(8)));
 #pragma unroll
-  for (int i = 0; i < D / 4; ++i) {
-    x[i] = row ? (float)row[i] : 0.0f;
-    most = fmaxf(most, __builtin_fabsf(x[i]));
+    for (int i = 0; i < N; i += 8) {
+      const vec_t v = *reinterpret_cast<const vec_t*>(row + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i + j] = (float)v[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = (float)row[i];
   }
+}
+
+// The power of two that brings the largest magnitude to [2^14, 2^15), and its inverse.
+__device__ __forceinline__ float lift_of(float most, float* back) {
+  const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
+  *back = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+  return __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+}
+
+template <typename T, int D>
+__device__ __forceinline__ float load_queries(half8_t (&q)[D / 32], const T* row, bool wide) {
+  float x[D / 4] = {}, most = 0.0f, back;
+  if (row) load_row(x, row, wide);
+#pragma unroll
+  for (int i = 0; i < D / 4; ++i) most = fmaxf(most, __builtin_fabsf(x[i]));
   most = fmaxf(most, __shfl_xor(most, 16));
   most = fmaxf(most, __shfl_xor(most, 32));
-  const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
-  const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+  const float up = lift_of(most, &back);
 #pragma unroll
   for (int i = 0; i < D / 4; ++i) q[i / 8][i % 8] = (_Float16)(x[i] * up);
-  return __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+  return back;
+}
+
+// Four neighbouring channels of an output row.
+template <typename T>
+__device__ __forceinline__ void store4(T* out, const float4_t& x, bool wide) {
+  typedef T vec_t __attribute__((ext_vector_type(4)));
+  const vec_t v = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+  if (wide) {
+    *reinterpret_cast<vec_t*>(out) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = v[i];
+  }
 }
 
 constexpr float kLift = 14.0f;  // probabilities are held times 2^14: fp16's normal range reaches down to 2^-28 of the largest
@@ -220,52 +244,54 @@ template <typename T, int D, int NT>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split_kernel(SplitArgs args) {
   const AttentionArgs& a = args.a;
   constexpr int kTiles = D / 16;          // of channels
-  constexpr int kRegs = kTiles * 4 + 2;   // what a lane holds of a row: O, m, l
-  __shared__ int scan_lds[kWaves];
-  __shared__ int found[4];
-  __shared__ float merge[2][NT][kRegs][64];
+  __shared__ __align__(16) float merge[kWaves][NT * 16][D + 4];  // a wave's O; four words more: no two rows in one bank
+  __shared__ float merge_m[kWaves][NT * 16], merge_l[kWaves][NT * 16];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 15, h4 = lane >> 4;
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads, w = blockIdx.x;
 
-  // ---- this workgroup's steps
-  int total = 0, first_steps = 0, before = 0;
-  const int rounds = (int)((a.num_seqs + 64 * kWaves - 1) / (64 * kWaves));
-  for (int r = 0; r < rounds; ++r) {
-    const int s = r * 64 * kWaves + threadIdx.x;
-    int first, count = 0, sum;
+  // ---- this workgroup's steps: every wave counts all sequences', 64 at a time, the first 256 kept
+  constexpr int kKept = 4;
+  int kept[kKept] = {}, total = 0;
+  const int rounds = (int)((a.num_seqs + 63) / 64);
+  auto count_of = [&](int r) {
+    const int64_t s = (int64_t)r * 64 + lane;
+    int first, count = 0;
     if (s < a.num_seqs) steps_of(a, sequence(a, s), &first, &count);
-    const int at = block_scan(count, &sum, scan_lds);
-    if (r == 0) {
-      first_steps = count;
-      before = at;
-    }
-    total += sum;
-  }
-  total *= heads;
+    return count;
+  };
+#pragma unroll
+  for (int r = 0; r < kKept; ++r) kept[r] = count_of(r);
+#pragma unroll
+  for (int r = 0; r < kKept; ++r) total += kept[r];
+  for (int r = kKept; r < rounds; ++r) total += count_of(r);
+  total = __builtin_amdgcn_readlane(wave_scan(total), 63) * heads;
   const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
   int pos = w * share;
   const int end = min(pos + share, total);
   if (threadIdx.x == 0) args.headers[w].seq = -1;
   if (pos >= end) return;
   // the sequence that the first step belongs to
-  int base = 0;
-  for (int r = 0; r < rounds; ++r) {
-    const int s = r * 64 * kWaves + threadIdx.x;
-    int first, count = first_steps, sum = 0, at = before;
-    if (rounds > 1) {
-      count = 0;
-      if (s < a.num_seqs) steps_of(a, sequence(a, s), &first, &count);
-      at = base + block_scan(count, &sum, scan_lds);
-    }
-    if (count > 0 && at * heads <= pos && pos < (at + count) * heads) {
-      found[0] = s;
-      found[1] = at * heads;
-    }
-    base += sum;
+  int s = 0, seq_base = 0;
+  {
+    bool found = false;
+    int base = 0;
+    auto look = [&](int r, int count) {
+      const int upto = base + wave_scan(count);
+      const uint64_t here = __builtin_amdgcn_ballot_w64(pos < upto * heads);
+      if (here) {
+        const int at = __builtin_ctzll(here);
+        s = r * 64 + at;
+        seq_base = __builtin_amdgcn_readlane(upto - count, at) * heads;
+        found = true;
+      }
+      base = __builtin_amdgcn_readlane(upto, 63);
+    };
+#pragma unroll
+    for (int r = 0; r < kKept; ++r)
+      if (!found) look(r, kept[r]);
+    for (int r = kKept; r < rounds && !found; ++r) look(r, count_of(r));
   }
-  __syncthreads();
-  int s = uniform(found[0]), seq_base = uniform(found[1]);
 
   const LaneOffsets<D> offsets(P, lane);
   while (pos < end) {
@@ -294,7 +320,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
       const T* from = row < rows ? static_cast<const T*>(a.q) + (seq.first + i) * a.q_token +
                                        (int64_t)(head * a.group + row - i * a.group) * a.q_head + h4 * (D / 4)
                                  : nullptr;
-      scale[t] = load_queries<T, D>(q[t], from) * a.scale;
+      scale[t] = load_queries<T, D>(q[t], from, a.q_wide) * a.scale;
       row_end[t] = row < rows ? new_from + i + 1 : 0;
       row_begin[t] = a.window > 0 ? (int)max((int64_t)new_from + i + 1 - a.window, (int64_t)0) : 0;
       m[t] = -__builtin_inff();
@@ -434,66 +460,53 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
       l[t] += __shfl_xor(l[t], 32);
     }
 
-    // ---- the waves' parts become one: 2 and 3 into 0 and 1, then 1 into 0
+    // ---- the waves' parts become one
+    __syncthreads();
 #pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-      __syncthreads();
-      if (wave >= half && wave < 2 * half) {
+    for (int t = 0; t < NT; ++t) {
+      const int row = t * 16 + n;
+      if (row >= rows) continue;
+      // lane (n, h): channels (4h + r) * D/16 + c of row n
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float(*to)[64] = merge[wave - half][t];
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[c * 4 + i][lane] = o[t][c][i];
-          to[kTiles * 4][lane] = m[t];
-          to[kTiles * 4 + 1][lane] = l[t];
-        }
+        for (int c = 0; c < kTiles; c += 4)
+          *reinterpret_cast<float4_t*>(&merge[wave][row][h4 * (D / 4) + r * kTiles + c]) =
+              float4_t{o[t][c][r], o[t][c + 1][r], o[t][c + 2][r], o[t][c + 3][r]};
+      if (h4 == 0) {
+        merge_m[wave][row] = m[t];
+        merge_l[wave][row] = l[t];
       }
-      __syncthreads();
-      if (wave < half) {
+    }
+    __syncthreads();
+    for (int item = threadIdx.x; item < rows * (D / 4); item += 64 * kWaves) {
+      const int row = item / (D / 4), ch = item % (D / 4) * 4, i = row / a.group;
+      float most = merge_m[0][row];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float(*from)[64] = merge[wave][t];
-          const float m2 = from[kTiles * 4][lane], now = fmaxf(m[t], m2);
-          const float w1 = m[t] == now ? 1.0f : __builtin_amdgcn_exp2f(m[t] - now);
-          const float w2 = m2 == now ? 1.0f : __builtin_amdgcn_exp2f(m2 - now);
-          m[t] = now;
-          l[t] = l[t] * w1 + from[kTiles * 4 + 1][lane] * w2;
+      for (int k = 1; k < kWaves; ++k) most = fmaxf(most, merge_m[k][row]);
+      float4_t sum = {0, 0, 0, 0};
+      float all = 0.0f;
 #pragma unroll
-          for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[t][c][i] = o[t][c][i] * w1 + from[c * 4 + i][lane] * w2;
+      for (int k = 0; k < kWaves; ++k) {
+        const float mk = merge_m[k][row], weight = mk == most ? 1.0f : __builtin_amdgcn_exp2f(mk - most);
+        all += merge_l[k][row] * weight;
+        sum += *reinterpret_cast<const float4_t*>(&merge[k][row][ch]) * weight;
+      }
+      if (starts && ends) {
+        T* out = static_cast<T*>(a.out) + (seq.first + i) * a.out_token +
+                 (int64_t)(head * a.group + row - i * a.group) * a.out_head + ch;
+        store4(out, sum * (all > 0.0f || all != all ? 1.0f / all : 0.0f), a.out_wide);
+      } else {
+        float* part = args.parts + ((int64_t)(2 * w + (starts ? 1 : 0)) * args.rows + row) * (D + 4);
+        *reinterpret_cast<float4_t*>(part + ch) = sum;
+        if (ch == 0) {
+          part[D] = most;
+          part[D + 1] = all;
         }
       }
     }
-    if (wave == 0) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int row = t * 16 + n, i = row / a.group;
-        if (row >= rows) continue;
-        // lane (n, h): channels (4h + i) * D/16 + c of row n
-        if (starts && ends) {
-          T* out = static_cast<T*>(a.out) + (seq.first + i) * a.out_token +
-                   (int64_t)(head * a.group + row - i * a.group) * a.out_head + h4 * (D / 4);
-          const float inv = l[t] > 0.0f || l[t] != l[t] ? 1.0f / l[t] : 0.0f;
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int c = 0; c < kTiles; ++c) out[r * kTiles + c] = (T)(o[t][c][r] * inv);
-        } else {
-          float* part = args.parts + ((int64_t)(2 * w + (starts ? 1 : 0)) * args.rows + row) * (D + 2);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int c = 0; c < kTiles; ++c) part[h4 * (D / 4) + r * kTiles + c] = o[t][c][r];
-          if (h4 == 0) {
-            part[D] = m[t];
-            part[D + 1] = l[t];
-          }
-        }
-      }
-      if (lane == 0 && starts && !ends) {
+    {
+      if (threadIdx.x == 0 && starts && !ends) {
         args.headers[w].head = head;
         args.headers[w].last = (pos - inside + count - 1) / share;
         args.headers[w].seq = s;
@@ -523,7 +536,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
   const int parts = header.last - w + 1;
   // part 0 is the workgroup's own second place, the others the first place of those behind it
   auto part = [&](int c) {
-    return args.parts + ((int64_t)(c == 0 ? 2 * w + 1 : 2 * (w + c)) * args.rows + row) * (D + 2);
+    return args.parts + ((int64_t)(c == 0 ? 2 * w + 1 : 2 * (w + c)) * args.rows + row) * (D + 4);
   };
   float m = -__builtin_inff();
   for (int c = threadIdx.x; c < parts; c += kJoinThreads) m = fmaxf(m, part(c)[D]);
@@ -532,14 +545,14 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
   __syncthreads();
   for (int k = 0; k < kJoinThreads / 64; ++k) m = fmaxf(m, most_of[k]);
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  float o[4] = {}, l = 0.0f;
+  float4_t o = {0, 0, 0, 0};
+  float l = 0.0f;
 #pragma unroll 4
   for (int c = group; c < parts; c += kGroups) {
     const float* p = part(c);
     const float mc = p[D], weight = mc == m ? 1.0f : __builtin_amdgcn_exp2f(mc - m);
     l += p[D + 1] * weight;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] += p[lane * 4 + k] * weight;
+    o += *reinterpret_cast<const float4_t*>(p + lane * 4) * weight;
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) lds[group][lane * 4 + k] = o[k];
@@ -568,7 +581,7 @@ int split_grid(int64_t num_seqs, int kv_heads, int64_t table_width, int page_siz
 constexpr int kMostRows = 32;  // of the split kernel
 
 int64_t split_bytes(int grid, int rows, int head_size) {
-  return grid * ((int64_t)sizeof(SplitHeader) + 2 * rows * (head_size + 2) * (int64_t)sizeof(float));
+  return grid * ((int64_t)sizeof(SplitHeader) + 2 * rows * (head_size + 4) * (int64_t)sizeof(float));
 }
 
 template <typename T, int D>
@@ -603,7 +616,7 @@ constexpr int kTileTokens = 64;
 
 struct TileArgs {
   AttentionArgs a;
-  float* parts;  // of `splits` pieces of every tile's tokens: [tile][head][split][rows][D + 2]; null: one piece
+  float* parts;  // of `splits` pieces of every tile's tokens: [tile][head][split][rows][D + 4]; null: one piece
   int tiles, splits;
 };
 
@@ -718,20 +731,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   float scale;
   {
     const T* from = static_cast<const T*>(a.q) + (seq.first + query) * a.q_token + (int64_t)q_head * a.q_head + h * 8;
-    float x[D / 2], most = 0.0f;
+    float most = 0.0f, back;
+    float x[D / 16][8] = {};
+    if (row < rows) {
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) load_row(x[c], from + c * 16, a.q_wide);
+    }
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[c * 8 + j] = row < rows ? (float)from[c * 16 + j] : 0.0f;
-        most = fmaxf(most, __builtin_fabsf(x[c * 8 + j]));
-      }
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(x[c][j]));
     most = fmaxf(most, __shfl_xor(most, 32));
-    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
-    const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+    const float up = lift_of(most, &back);
 #pragma unroll
-    for (int i = 0; i < D / 2; ++i) q[i / 8][i % 8] = (_Float16)(x[i] * up);
-    scale = __uint_as_float((uint32_t)(127 - 14 + e) << 23) * a.scale;
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[c][j] = (_Float16)(x[c][j] * up);
+    scale = back * a.scale;
   }
   float m = -__builtin_inff(), l = 0.0f;
   float16_t o[D / 32];
@@ -902,13 +918,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) out[c * 32 + (i / 4) * 8 + h * 4 + i % 4] = (T)(o[c][i] * inv);
+      for (int i = 0; i < 16; i += 4)
+        store4(out + c * 32 + i * 2 + h * 4, float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv, a.out_wide);
   } else {
-    float* part = args.parts + ((((int64_t)tile * heads + head) * args.splits + split) * S::kRows + row - row0) * (D + 2);
+    float* part = args.parts + ((((int64_t)tile * heads + head) * args.splits + split) * S::kRows + row - row0) * (D + 4);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) part[c * 32 + (i / 4) * 8 + h * 4 + i % 4] = o[c][i];
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4_t*>(part + c * 32 + i * 2 + h * 4) = float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]};
     if (h == 0) {
       part[D] = m;
       part[D + 1] = l;
@@ -930,8 +948,8 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
   const int rows = (int)min(seq.count, a.max_queries) * a.group;
   const int in_tile = blockIdx.z * 4 + (threadIdx.x >> 6), row = place * S::kRows + in_tile;
   if (row >= rows) return;
-  const float* part = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows + in_tile) * (D + 2);
-  const int64_t stride = (int64_t)S::kRows * (D + 2);
+  const float* part = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows + in_tile) * (D + 4);
+  const int64_t stride = (int64_t)S::kRows * (D + 4);
   float m = -__builtin_inff(), l = 0.0f, o[D / 64] = {};
   for (int c = 0; c < args.splits; ++c) m = fmaxf(m, part[c * stride + D]);
 #pragma unroll 4
@@ -970,7 +988,7 @@ TilePlan plan_tiles(int64_t T, int group, int kv_heads, int head_size, int64_t n
   const int64_t units = tiles * kv_heads, most = max(table_width * page_size / 256, (int64_t)1);
   plan.splits = (int)min(max((cus > 0 ? cus : 256) / units, (int64_t)1), most);
   plan.tiles = (int)min(tiles, (int64_t)0x7fffffff);
-  plan.bytes = plan.splits == 1 ? 0 : tiles * kv_heads * plan.splits * rows * (head_size + 2) * (int64_t)sizeof(float);
+  plan.bytes = plan.splits == 1 ? 0 : tiles * kv_heads * plan.splits * rows * (head_size + 4) * (int64_t)sizeof(float);
   return plan;
 }
 
@@ -991,6 +1009,10 @@ int launch_tiles(const TileArgs& args, int D, void* stream) {
   if (D == 64) return launch_tiles<T, 64, 8>(args, stream);
   if (D == 128) return launch_tiles<T, 128, 8>(args, stream);
   return launch_tiles<T, 256, 4>(args, stream);
+}
+
+bool wide_rows(const tw_heads* h) {
+  return reinterpret_cast<uintptr_t>(h->data) % 16 == 0 && h->token_stride % 8 == 0 && h->head_stride % 8 == 0;
 }
 
 }  // namespace
@@ -1054,6 +1076,8 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   a.max_queries = min(max_queries, T);
   a.scale = scale * kLog2e;
   a.window = window;
+  a.q_wide = wide_rows(q);
+  a.out_wide = wide_rows(out);
   max_queries = a.max_queries;
   if (max_queries * a.group <= kMostRows) {
     const int grid = split_grid(num_seqs, kv_heads, table_width, page_size);
