@@ -40,12 +40,18 @@ struct Sequence {
   int64_t first, count, length;
 };
 
+// Reads of what no kernel here writes, at addresses that a wave's lanes share: through the scalar cache.
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;
+__device__ __forceinline__ ConstInts constant(const int32_t* p) { return (ConstInts)(uintptr_t)p; }
+
+// UNIFORM: s is the same in all lanes.
+template <bool UNIFORM = false>
 __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int64_t s) {
   Sequence q;
   int64_t end;
   if (a.query_starts) {
-    q.first = a.query_starts[s];
-    end = a.query_starts[s + 1];
+    q.first = UNIFORM ? constant(a.query_starts)[s] : a.query_starts[s];
+    end = UNIFORM ? constant(a.query_starts)[s + 1] : a.query_starts[s + 1];
   } else {
     q.first = s * a.per_seq;
     end = q.first + a.per_seq;
@@ -53,14 +59,8 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int64_t s) 
   // whatever the arrays hold, only tokens of q and tokens that the table has places for are touched
   q.first = min(max(q.first, (int64_t)0), a.num_tokens);
   q.count = max(min(end, a.num_tokens) - q.first, (int64_t)0);
-  q.length = min(max((int64_t)a.seq_lens[s], (int64_t)0), a.table_width << a.pages.page_log2);
+  q.length = min(max((int64_t)(UNIFORM ? constant(a.seq_lens)[s] : a.seq_lens[s]), (int64_t)0), a.table_width << a.pages.page_log2);
   return q;
-}
-
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) x = fmaxf(x, __shfl_xor(x, i));
-  return x;
 }
 
 // ---------------------------------------------------------------------------
@@ -85,10 +85,11 @@ typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4, kWaveTokens = 32, kStep = kWaves * kWaveTokens, kJoinThreads = 256;
 
-// Which unfinished sequence a workgroup began, for the join.
+// The unfinished piece that a workgroup began, for the join: `rows` rows of key head `head`, of the new
+// tokens from `first` on, ended by workgroup `last`.
 struct SplitHeader {
-  int32_t seq, head, last;  // seq < 0: none; last: the workgroup that holds its end
-  int32_t unused;
+  int32_t rows;  // 0: none
+  int32_t first, head, last;
 };
 
 struct SplitArgs {
@@ -159,18 +160,31 @@ struct LaneOffsets {
   }
 };
 
+// Where a wave's 32 tokens are: two sixteens, each in one page.
+struct Place {
+  const uint8_t* block[2];
+  int at[2];
+  bool there[2];
+};
+
 template <int D>
-__device__ __forceinline__ void load_tile(Tile<D>& tile, const uint8_t* const (&page)[2], const int (&at)[2],
-                                          const LaneOffsets<D>& lane, int P) {
-  using L = Kv4<D>;
+__device__ __forceinline__ void load_keys(Tile<D>& tile, const Place& place, const LaneOffsets<D>& lane, int P) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint8_t* p = page[i];
-    load_words(tile.k[i], p + (at[i] * L::kRow + lane.k));
-    load_words(tile.v[i], p + (at[i] * L::kRow + lane.v));
+    const uint8_t* p = place.block[i];
+    load_words(tile.k[i], p + (place.at[i] * Kv4<D>::kRow + lane.k));
 #pragma unroll
-    for (int g = 0; g < (D + 127) / 128; ++g) tile.ks[i][g] = p[at[i] + lane.ks + g * P];
-    tile.vs[i] = *reinterpret_cast<const uint32_t*>(p + (at[i] + lane.vs));
+    for (int g = 0; g < (D + 127) / 128; ++g) tile.ks[i][g] = p[place.at[i] + lane.ks + g * P];
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_values(Tile<D>& tile, const Place& place, const LaneOffsets<D>& lane) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint8_t* p = place.block[i];
+    load_words(tile.v[i], p + (place.at[i] * Kv4<D>::kRow + lane.v));
+    tile.vs[i] = *reinterpret_cast<const uint32_t*>(p + (place.at[i] + lane.vs));
   }
 }
 
@@ -269,7 +283,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
   const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
   int pos = w * share;
   const int end = min(pos + share, total);
-  if (threadIdx.x == 0) args.headers[w].seq = -1;
+  if (threadIdx.x == 0) args.headers[w] = SplitHeader{0, 0, 0, 0};
   if (pos >= end) return;
   // the sequence that the first step belongs to
   int s = 0, seq_base = 0;
@@ -296,7 +310,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
   const LaneOffsets<D> offsets(P, lane);
   while (pos < end) {
     // ---- the next piece: steps [step, step + steps) of key head `head` of sequence s
-    const Sequence seq = sequence(a, s);
+    const Sequence seq = sequence<true>(a, s);
     int first_step, count;
     steps_of(a, seq, &first_step, &count);
     if (count == 0) {
@@ -332,33 +346,34 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
     const int all_from = a.window > 0 ? (int)max((int64_t)new_from + queries - a.window, (int64_t)0) : 0;
     const int all_to = new_from + 1;
     const int some_from = a.window > 0 ? (int)max((int64_t)new_from + 1 - a.window, (int64_t)0) : 0;
-    const int32_t* table = a.block_table + (int64_t)s * a.table_stride;
+    const ConstInts table = constant(a.block_table) + (int64_t)s * a.table_stride;
 
-    const int step0 = first_step + inside;
-    auto locate = [&](int step, const uint8_t* (&page)[2], int (&at)[2], bool (&there)[2]) {
+    // Two tiles in registers, worked on in turn: the keys of the tile after next are fetched over those just
+    // used, and so are the values; the pages' numbers are fetched one tile earlier still.
+    const int step0 = first_step + inside, step_end = step0 + steps;
+    int ids[2];
+    auto ids_of = [&](int step) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int t = step * kStep + wave * kWaveTokens + i * 16;
-        const int id = t < length ? table[t >> a.pages.page_log2] : -1;
-        there[i] = id >= 0 && id < a.pages.num_pages;
-        page[i] = a.pages.data + ((int64_t)(there[i] ? id : 0) * heads + head) * a.pages.head_bytes;
-        at[i] = t & (P - 1);
+        ids[i] = step < step_end && t < length ? table[t >> a.pages.page_log2] : -1;
       }
     };
-
-    Tile<D> tile;
-    const uint8_t* page[2];
-    int at[2];
-    bool there[2], next_there[2];
-    locate(step0, page, at, there);
-    load_tile<D>(tile, page, at, offsets, P);
-    for (int step = step0; step < step0 + steps; ++step) {
-      Tile<D> next = tile;
-      next_there[0] = next_there[1] = false;
-      if (step + 1 < step0 + steps) {
-        locate(step + 1, page, at, next_there);
-        load_tile<D>(next, page, at, offsets, P);
+    auto place_of = [&](int step) {
+      Place place;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        place.there[i] = ids[i] >= 0 && ids[i] < a.pages.num_pages;
+        // tokens of a missing page are read from page 0 and masked
+        place.block[i] = a.pages.data + ((int64_t)(place.there[i] ? ids[i] : 0) * heads + head) * a.pages.head_bytes;
+        place.at[i] = (step * kStep + wave * kWaveTokens + i * 16) & (P - 1);
       }
+      return place;
+    };
+
+    auto work_on = [&](Tile<D>& tile, Place& place, int step) {
+      const bool there[2] = {place.there[0], place.there[1]};
+      const bool more = step + 2 < step_end;
       const int t0 = step * kStep + wave * kWaveTokens;
       const bool whole = t0 >= all_from && t0 + kWaveTokens <= all_to && there[0] && there[1];
 
@@ -374,6 +389,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
 #pragma unroll
           for (int t = 0; t < NT; ++t) sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[t][c], sc[t][i], 0, 0, 0);
         }
+      }
+      if (more) {
+        place = place_of(step + 2);
+        load_keys<D>(tile, place, offsets, P);
+        ids_of(step + 3);
       }
       // ---- probabilities
       half8_t p[NT];
@@ -450,9 +470,25 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
           channels(std::integral_constant<int, 3>{}, word);
         }
       }
-      tile = next;
-      there[0] = next_there[0];
-      there[1] = next_there[1];
+      if (more) load_values<D>(tile, place, offsets);
+    };
+
+    Tile<D> even, odd;
+    Place even_place, odd_place;
+    ids_of(step0);
+    even_place = place_of(step0);
+    load_keys<D>(even, even_place, offsets, P);
+    load_values<D>(even, even_place, offsets);
+    ids_of(step0 + 1);
+    odd_place = place_of(step0 + 1);
+    if (steps > 1) {
+      load_keys<D>(odd, odd_place, offsets, P);
+      load_values<D>(odd, odd_place, offsets);
+    }
+    ids_of(step0 + 2);
+    for (int step = step0; step < step_end; step += 2) {
+      work_on(even, even_place, step);
+      if (step + 1 < step_end) work_on(odd, odd_place, step + 1);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -505,13 +541,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
         }
       }
     }
-    {
-      if (threadIdx.x == 0 && starts && !ends) {
-        args.headers[w].head = head;
-        args.headers[w].last = (pos - inside + count - 1) / share;
-        args.headers[w].seq = s;
-      }
-    }
+    if (threadIdx.x == 0 && starts && !ends)
+      args.headers[w] = SplitHeader{rows, (int32_t)seq.first, head, (pos + count - 1) / share};
     pos += steps;
     if (pos == seq_base + heads * count) {
       seq_base = pos;
@@ -520,55 +551,72 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
   }
 }
 
-// Joins the parts of one row of a sequence that several workgroups shared: block (w, row).
+// Joins the parts of one row of a piece that several workgroups shared: block (w, row).  A thread has four
+// channels of every kGroups-th part, kAtOnce of them under way at once.
 template <typename T, int D>
 __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs args) {
   const AttentionArgs& a = args.a;
   const int w = blockIdx.x, row = blockIdx.y;
   const SplitHeader header = args.headers[w];
-  if (header.seq < 0) return;
-  const Sequence seq = sequence(a, header.seq);
-  const int i = row / a.group;
-  if (i >= seq.count || i >= a.max_queries) return;
-  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
-  __shared__ float lds[kGroups][D + 1];
-  __shared__ float most_of[kJoinThreads / 64];
-  const int parts = header.last - w + 1;
-  // part 0 is the workgroup's own second place, the others the first place of those behind it
-  auto part = [&](int c) {
-    return args.parts + ((int64_t)(c == 0 ? 2 * w + 1 : 2 * (w + c)) * args.rows + row) * (D + 4);
-  };
-  float m = -__builtin_inff();
-  for (int c = threadIdx.x; c < parts; c += kJoinThreads) m = fmaxf(m, part(c)[D]);
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) most_of[threadIdx.x >> 6] = m;
-  __syncthreads();
-  for (int k = 0; k < kJoinThreads / 64; ++k) m = fmaxf(m, most_of[k]);
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  if (row >= header.rows) return;
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAtOnce = 8;
+  __shared__ __align__(16) float lds[kGroups][D];
+  __shared__ float lds_m[kGroups], lds_l[kGroups];
+  const int parts = header.last - w + 1, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int64_t part_size = (int64_t)args.rows * (D + 4);
+  const float* base = args.parts + (int64_t)row * (D + 4);
   float4_t o = {0, 0, 0, 0};
-  float l = 0.0f;
-#pragma unroll 4
-  for (int c = group; c < parts; c += kGroups) {
-    const float* p = part(c);
-    const float mc = p[D], weight = mc == m ? 1.0f : __builtin_amdgcn_exp2f(mc - m);
-    l += p[D + 1] * weight;
-    o += *reinterpret_cast<const float4_t*>(p + lane * 4) * weight;
-  }
+  float m = -__builtin_inff(), l = 0.0f;
+  for (int c0 = group; c0 < parts; c0 += kGroups * kAtOnce) {
+    float4_t x[kAtOnce];
+    float2 ml[kAtOnce];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) lds[group][lane * 4 + k] = o[k];
-  if (lane == 0) lds[group][D] = l;
-  __syncthreads();
-  T* out = static_cast<T*>(a.out) + (seq.first + i) * a.out_token +
-           (int64_t)(header.head * a.group + row - i * a.group) * a.out_head;
-  for (int ch = threadIdx.x; ch < D; ch += kJoinThreads) {
-    float sum = 0.0f, all = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      sum += lds[k][ch];
-      all += lds[k][D];
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int c = c0 + k * kGroups;
+      ml[k] = make_float2(-__builtin_inff(), 0.0f);
+      x[k] = float4_t{0, 0, 0, 0};
+      if (c < parts) {
+        // part 0 is the workgroup's own second place, the others the first place of those behind it
+        const float* p = base + (c == 0 ? 2 * w + 1 : 2 * (w + c)) * part_size;
+        x[k] = *reinterpret_cast<const float4_t*>(p + lane * 4);
+        ml[k] = *reinterpret_cast<const float2*>(p + D);
+      }
     }
-    out[ch] = (T)(all > 0.0f || all != all ? sum / all : 0.0f);
+    float most = m;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) most = fmaxf(most, ml[k].x);
+    const float old = m == most ? 1.0f : __builtin_amdgcn_exp2f(m - most);
+    m = most;
+    l *= old;
+    o *= old;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float weight = ml[k].x == most ? 1.0f : __builtin_amdgcn_exp2f(ml[k].x - most);
+      l += ml[k].y * weight;
+      o += x[k] * weight;
+    }
   }
+  *reinterpret_cast<float4_t*>(&lds[group][lane * 4]) = o;
+  if (lane == 0) {
+    lds_m[group] = m;
+    lds_l[group] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kLanes) return;
+  float most = lds_m[0], all = 0.0f;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) most = fmaxf(most, lds_m[k]);
+  float4_t sum = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) {
+    const float weight = lds_m[k] == most ? 1.0f : __builtin_amdgcn_exp2f(lds_m[k] - most);
+    all += lds_l[k] * weight;
+    sum += *reinterpret_cast<const float4_t*>(&lds[k][lane * 4]) * weight;
+  }
+  const int i = row / a.group;
+  T* out = static_cast<T*>(a.out) + ((int64_t)header.first + i) * a.out_token +
+           (int64_t)(header.head * a.group + row - i * a.group) * a.out_head + lane * 4;
+  store4(out, sum * (all > 0.0f || all != all ? 1.0f / all : 0.0f), a.out_wide);
 }
 
 // Workgroups of the split kernel: two a compute unit, and no more than there are steps.
@@ -1049,7 +1097,8 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table or seq_lens is null", what);
   if (table_width > ((int64_t)1 << 31) / page_size)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table has room for more than 2^31 tokens", what);
-  if (num_seqs > 65535) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: more than 65535 sequences", what);
+  if (num_seqs > 65535 || T > 0x7fffffff)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: more than 65535 sequences or 2^31 tokens", what);
   if (!query_starts && T % num_seqs != 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld tokens are not the same number for each of %lld sequences", what,
                      (long long)T, (long long)num_seqs);
