@@ -25,42 +25,41 @@ struct AttentionArgs {
   Kv4Pages pages;
   int group;  // query heads of a key head
   const int32_t* block_table;
-  int64_t table_stride, table_width;
+  int64_t table_stride;
+  int capacity;  // tokens that a row of the table has places for, at most 2^30
   const int32_t* seq_lens;
   const int32_t* query_starts;  // or null: per_seq each
-  int64_t per_seq;
-  int64_t num_seqs, num_tokens, max_queries;
+  int per_seq;
+  int num_seqs, num_tokens, max_queries;
   float scale;  // with log2(e)
-  int64_t window;
+  int window;   // 0: none
   bool q_wide, out_wide;  // every row is 16-byte aligned
 };
 
-// Sequence `s`: its new tokens [first, first + count) and its cached ones.
+// A sequence's new tokens [first, first + count) and how many are cached.
 struct Sequence {
-  int64_t first, count, length;
+  int first, count, length;
 };
 
 // Reads of what no kernel here writes, at addresses that a wave's lanes share: through the scalar cache.
 typedef const __attribute__((address_space(4))) int32_t* ConstInts;
 __device__ __forceinline__ ConstInts constant(const int32_t* p) { return (ConstInts)(uintptr_t)p; }
 
-// UNIFORM: s is the same in all lanes.
+// UNIFORM: s is the same in all lanes.  Whatever the arrays hold, only tokens of q and tokens that the table has
+// places for are touched.
 template <bool UNIFORM = false>
-__device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int64_t s) {
-  Sequence q;
-  int64_t end;
+__device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int s) {
+  int first, end;
   if (a.query_starts) {
-    q.first = UNIFORM ? constant(a.query_starts)[s] : a.query_starts[s];
+    first = UNIFORM ? constant(a.query_starts)[s] : a.query_starts[s];
     end = UNIFORM ? constant(a.query_starts)[s + 1] : a.query_starts[s + 1];
   } else {
-    q.first = s * a.per_seq;
-    end = q.first + a.per_seq;
+    first = s * a.per_seq;
+    end = first + a.per_seq;
   }
-  // whatever the arrays hold, only tokens of q and tokens that the table has places for are touched
-  q.first = min(max(q.first, (int64_t)0), a.num_tokens);
-  q.count = max(min(end, a.num_tokens) - q.first, (int64_t)0);
-  q.length = min(max((int64_t)(UNIFORM ? constant(a.seq_lens)[s] : a.seq_lens[s]), (int64_t)0), a.table_width << a.pages.page_log2);
-  return q;
+  const int length = UNIFORM ? constant(a.seq_lens)[s] : a.seq_lens[s];
+  first = min(max(first, 0), a.num_tokens);
+  return {first, max(min(end, a.num_tokens) - first, 0), min(max(length, 0), a.capacity)};
 }
 
 // ---------------------------------------------------------------------------
@@ -74,9 +73,9 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int64_t s) 
 // as 8 tokens of one channel; a lane loads 4 tokens x D/16 channels at once (the layout of tw_kv4.h)
 // and pairs tokens in registers.
 //
-// Work is shared by even numbers of 128-token steps over a fixed grid, whatever the sequences'
-// lengths: a workgroup finds its steps from the lengths on the device.  What a workgroup holds of a
-// sequence that others share goes to the workspace as (m, l, O), and attention_join_kernel joins.
+// A sequence's 128-token steps are cut into even pieces, as many in all as the grid holds workgroups,
+// whatever the lengths: a workgroup finds its pieces from the lengths on the device.  The pieces of a
+// sequence that has several go to the workspace as (m, l, O), and attention_join_kernel joins them.
 // ---------------------------------------------------------------------------
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -85,26 +84,27 @@ typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4, kWaveTokens = 32, kStep = kWaves * kWaveTokens, kJoinThreads = 256;
 
-// The unfinished piece that a workgroup began, for the join: `rows` rows of key head `head`, of the new
-// tokens from `first` on, ended by workgroup `last`.
-struct SplitHeader {
-  int32_t rows;  // 0: none
-  int32_t first, head, last;
+// Of a sequence and key head: in how many pieces its steps are, and the first one's part in the workspace
+// where they are several (the others' follow).
+struct PieceHeader {
+  int32_t count, slot;
 };
 
 struct SplitArgs {
   AttentionArgs a;
-  SplitHeader* headers;  // one a workgroup
-  float* parts;          // two a workgroup: [rows][D + 4], m and l behind the D channels
-  int rows;              // of a part
+  PieceHeader* headers;  // [num_seqs][kv_heads]
+  float* parts;    // [slots][rows][D + 4], m and l behind the D channels
+  int rows;        // of a part
+  int budget;      // pieces that the steps are cut into; at most one more for each sequence and key head
+  int group_inv;   // 65536 / group + 1
 };
 
 // First token that any new token of the sequence sees, and the 128-token steps from there to its end; a
 // sequence with new tokens has one step at least, in which its outputs are written.
 __device__ __forceinline__ void steps_of(const AttentionArgs& a, const Sequence& q, int* first, int* count) {
-  const int64_t seen = a.window > 0 ? max(q.length - q.count + 1 - a.window, (int64_t)0) : 0;
-  *first = (int)(seen / kStep);
-  *count = q.count == 0 ? 0 : max((int)((q.length + kStep - 1) / kStep) - *first, 1);
+  const int seen = a.window > 0 ? max(q.length - q.count + 1 - a.window, 0) : 0;
+  *first = seen / kStep;
+  *count = q.count == 0 ? 0 : max((q.length + kStep - 1) / kStep - *first, 1);
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -226,17 +226,41 @@ __device__ __forceinline__ float lift_of(float most, float* back) {
 }
 
 template <typename T, int D>
-__device__ __forceinline__ float load_queries(half8_t (&q)[D / 32], const T* row, bool wide) {
-  float x[D / 4] = {}, most = 0.0f, back;
-  if (row) load_row(x, row, wide);
+struct RawQueries {
+  typedef T vec_t __attribute__((ext_vector_type(8)));
+  vec_t x[D / 32];
+  __device__ __forceinline__ void load(const T* row, bool wide) {
 #pragma unroll
-  for (int i = 0; i < D / 4; ++i) most = fmaxf(most, __builtin_fabsf(x[i]));
-  most = fmaxf(most, __shfl_xor(most, 16));
-  most = fmaxf(most, __shfl_xor(most, 32));
-  const float up = lift_of(most, &back);
+    for (int i = 0; i < D / 32; ++i) {
+      x[i] = vec_t{};
+      if (row && wide) x[i] = *reinterpret_cast<const vec_t*>(row + i * 8);
+      if (row && !wide) {
 #pragma unroll
-  for (int i = 0; i < D / 4; ++i) q[i / 8][i % 8] = (_Float16)(x[i] * up);
-  return back;
+        for (int j = 0; j < 8; ++j) x[i][j] = row[i * 8 + j];
+      }
+    }
+  }
+  // Returns what the scores are multiplied back by.
+  __device__ __forceinline__ float lift(half8_t (&q)[D / 32]) const {
+    float most = 0.0f, back;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) most = fmaxf(most, __builtin_fabsf((float)x[i / 8][i % 8]));
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const float up = lift_of(most, &back);
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) q[i / 8][i % 8] = (_Float16)((float)x[i / 8][i % 8] * up);
+    return back;
+  }
+};
+
+// x / d for 0 <= x < 2^24 and d's reciprocal.
+__device__ __forceinline__ int divide(int x, int d, float inv) {
+  int q = (int)((float)x * inv);
+  const int r = x - q * d;
+  q += r >= d ? 1 : 0;
+  q -= r < 0 ? 1 : 0;
+  return q;
 }
 
 // Four neighbouring channels of an output row.
@@ -264,102 +288,97 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
   const int n = lane & 15, h4 = lane >> 4;
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads, w = blockIdx.x;
 
-  // ---- this workgroup's steps: every wave counts all sequences', 64 at a time, the first 256 kept
+  // ---- every wave counts all sequences' steps and pieces, 64 sequences at a time; the first 256 are kept
   constexpr int kKept = 4;
-  int kept[kKept] = {}, total = 0;
-  const int rounds = (int)((a.num_seqs + 63) / 64);
-  auto count_of = [&](int r) {
-    const int64_t s = (int64_t)r * 64 + lane;
-    int first, count = 0;
-    if (s < a.num_seqs) steps_of(a, sequence(a, s), &first, &count);
+  Sequence kept[kKept];
+  int pieces[kKept];
+  const int rounds = (a.num_seqs + 63) / 64;
+  auto read = [&](int r) {
+    const int s = r * 64 + lane;
+    return s < a.num_seqs ? sequence(a, s) : Sequence{0, 0, 0};
+  };
+  auto steps_in = [&](const Sequence& seq) {
+    int first, count;
+    steps_of(a, seq, &first, &count);
     return count;
   };
+  int total = 0;
 #pragma unroll
-  for (int r = 0; r < kKept; ++r) kept[r] = count_of(r);
+  for (int r = 0; r < kKept; ++r) kept[r] = read(r);
 #pragma unroll
-  for (int r = 0; r < kKept; ++r) total += kept[r];
-  for (int r = kKept; r < rounds; ++r) total += count_of(r);
-  total = __builtin_amdgcn_readlane(wave_scan(total), 63) * heads;
-  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
-  int pos = w * share;
-  const int end = min(pos + share, total);
-  if (threadIdx.x == 0) args.headers[w] = SplitHeader{0, 0, 0, 0};
-  if (pos >= end) return;
-  // the sequence that the first step belongs to
-  int s = 0, seq_base = 0;
-  {
-    bool found = false;
-    int base = 0;
-    auto look = [&](int r, int count) {
-      const int upto = base + wave_scan(count);
-      const uint64_t here = __builtin_amdgcn_ballot_w64(pos < upto * heads);
-      if (here) {
-        const int at = __builtin_ctzll(here);
-        s = r * 64 + at;
-        seq_base = __builtin_amdgcn_readlane(upto - count, at) * heads;
-        found = true;
-      }
-      base = __builtin_amdgcn_readlane(upto, 63);
-    };
-#pragma unroll
-    for (int r = 0; r < kKept; ++r)
-      if (!found) look(r, kept[r]);
-    for (int r = kKept; r < rounds && !found; ++r) look(r, count_of(r));
+  for (int r = 0; r < kKept; ++r) {
+    pieces[r] = steps_in(kept[r]);
+    total += pieces[r];
   }
+  for (int r = kKept; r < rounds; ++r) total += steps_in(read(r));
+  total = __builtin_amdgcn_readlane(wave_scan(total), 63) * heads;
+  const int share = max((total + args.budget - 1) / args.budget, 1);
+  const float share_inv = 1.0f / (float)share;
+  auto pieces_in = [&](int steps) { return divide(steps + share - 1, share, share_inv); };
+  auto several = [](int count) { return count > 1 ? count : 0; };
+  int all = 0;
+#pragma unroll
+  for (int r = 0; r < kKept; ++r) {
+    pieces[r] = pieces_in(pieces[r]);
+    all += pieces[r];
+  }
+  for (int r = kKept; r < rounds; ++r) {
+    all += pieces_in(steps_in(read(r)));
+  }
+  all = __builtin_amdgcn_readlane(wave_scan(all), 63) * heads;
 
   const LaneOffsets<D> offsets(P, lane);
-  while (pos < end) {
-    // ---- the next piece: steps [step, step + steps) of key head `head` of sequence s
-    const Sequence seq = sequence<true>(a, s);
-    int first_step, count;
-    steps_of(a, seq, &first_step, &count);
-    if (count == 0) {
-      ++s;
-      continue;
-    }
-    const int head = (pos - seq_base) / count, inside = (pos - seq_base) - head * count;
-    const int steps = min(count - inside, end - pos);
-    const int queries = (int)min(seq.count, a.max_queries), rows = queries * a.group;
-    const int length = (int)seq.length;
-    const int new_from = length - (int)seq.count;  // position of the first new token
-    const bool starts = inside == 0, ends = inside + steps == count;
-
-    half8_t q[NT][D / 32];
-    float scale[NT], m[NT], l[NT];
-    int row_end[NT], row_begin[NT];
-    float4_t o[NT][kTiles];
+  for (int piece = w; piece < all; piece += gridDim.x) {
+    // ---- whose piece it is
+    int s = 0, inside = 0, count = 1, slot = 0;
+    Sequence seq{0, 0, 0};
+    {
+      bool found = false;
+      int base = 0, slot_base = 0;
+      auto look = [&](int r, int own, const Sequence& from) {
+        const int upto = base + wave_scan(own), slots_upto = slot_base + wave_scan(several(own));
+        const uint64_t here = __builtin_amdgcn_ballot_w64(piece < upto * heads);
+        if (here) {
+          const int at = __builtin_ctzll(here);
+          s = r * 64 + at;
+          count = __builtin_amdgcn_readlane(own, at);
+          inside = piece - (__builtin_amdgcn_readlane(upto, at) - count) * heads;
+          slot = (__builtin_amdgcn_readlane(slots_upto, at) - several(count)) * heads + inside;
+          seq.first = __builtin_amdgcn_readlane(from.first, at);
+          seq.count = __builtin_amdgcn_readlane(from.count, at);
+          seq.length = __builtin_amdgcn_readlane(from.length, at);
+          found = true;
+        }
+        base = __builtin_amdgcn_readlane(upto, 63);
+        slot_base = __builtin_amdgcn_readlane(slots_upto, 63);
+      };
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int row = t * 16 + n, i = row / a.group;
-      const T* from = row < rows ? static_cast<const T*>(a.q) + (seq.first + i) * a.q_token +
-                                       (int64_t)(head * a.group + row - i * a.group) * a.q_head + h4 * (D / 4)
-                                 : nullptr;
-      scale[t] = load_queries<T, D>(q[t], from, a.q_wide) * a.scale;
-      row_end[t] = row < rows ? new_from + i + 1 : 0;
-      row_begin[t] = a.window > 0 ? (int)max((int64_t)new_from + i + 1 - a.window, (int64_t)0) : 0;
-      m[t] = -__builtin_inff();
-      l[t] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < kTiles; ++c) o[t][c] = float4_t{0, 0, 0, 0};
+      for (int r = 0; r < kKept; ++r)
+        if (!found) look(r, pieces[r], kept[r]);
+      for (int r = kKept; r < rounds && !found; ++r) {
+        const Sequence from = read(r);
+        look(r, pieces_in(steps_in(from)), from);
+      }
     }
-    // tokens that every row sees need no mask
-    const int all_from = a.window > 0 ? (int)max((int64_t)new_from + queries - a.window, (int64_t)0) : 0;
-    const int all_to = new_from + 1;
-    const int some_from = a.window > 0 ? (int)max((int64_t)new_from + 1 - a.window, (int64_t)0) : 0;
-    const ConstInts table = constant(a.block_table) + (int64_t)s * a.table_stride;
+    const int head = inside / count, part = inside - head * count;
+    int first_step, seq_steps;
+    steps_of(a, seq, &first_step, &seq_steps);
+    const int each = seq_steps / count, longer = seq_steps - each * count;
+    const int step0 = first_step + part * each + min(part, longer), step_end = step0 + each + (part < longer ? 1 : 0);
+    const int queries = min(seq.count, a.max_queries), rows = queries * a.group;
+    const int length = seq.length, new_from = length - seq.count;  // position of the first new token
 
     // Two tiles in registers, worked on in turn: the keys of the tile after next are fetched over those just
     // used, and so are the values; the pages' numbers are fetched one tile earlier still.
-    const int step0 = first_step + inside, step_end = step0 + steps;
-    int ids[2];
-    auto ids_of = [&](int step) {
+    const ConstInts table = constant(a.block_table) + (int64_t)s * a.table_stride;
+    auto ids_of = [&](int step, int (&ids)[2]) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int t = step * kStep + wave * kWaveTokens + i * 16;
         ids[i] = step < step_end && t < length ? table[t >> a.pages.page_log2] : -1;
       }
     };
-    auto place_of = [&](int step) {
+    auto place_of = [&](int step, const int (&ids)[2]) {
       Place place;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -370,6 +389,47 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
       }
       return place;
     };
+    int ids[2], first_ids[2];
+    ids_of(step0, first_ids);
+    ids_of(step0 + 1, ids);
+
+    RawQueries<T, D> raw[NT];
+    int row_end[NT], row_begin[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row = t * 16 + n, i = row * args.group_inv >> 16;
+      raw[t].load(row < rows ? static_cast<const T*>(a.q) + (int64_t)(seq.first + i) * a.q_token +
+                                   (int64_t)(head * a.group + row - i * a.group) * a.q_head + h4 * (D / 4)
+                             : nullptr,
+                  a.q_wide);
+      row_end[t] = row < rows ? new_from + i + 1 : 0;
+      row_begin[t] = a.window > 0 ? max(new_from + i + 1 - a.window, 0) : 0;
+    }
+    Tile<D> even, odd;
+    Place even_place = place_of(step0, first_ids), odd_place = place_of(step0 + 1, ids);
+    load_keys<D>(even, even_place, offsets, P);
+    load_values<D>(even, even_place, offsets);
+    if (step0 + 1 < step_end) {
+      load_keys<D>(odd, odd_place, offsets, P);
+      load_values<D>(odd, odd_place, offsets);
+    }
+    ids_of(step0 + 2, ids);
+
+    half8_t q[NT][D / 32];
+    float scale[NT], m[NT], l[NT];
+    float4_t o[NT][kTiles];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      scale[t] = raw[t].lift(q[t]) * a.scale;
+      m[t] = -__builtin_inff();
+      l[t] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c) o[t][c] = float4_t{0, 0, 0, 0};
+    }
+    // tokens that every row sees need no mask
+    const int all_from = a.window > 0 ? max(new_from + queries - a.window, 0) : 0;
+    const int all_to = new_from + 1;
+    const int some_from = a.window > 0 ? max(new_from + 1 - a.window, 0) : 0;
 
     auto work_on = [&](Tile<D>& tile, Place& place, int step) {
       const bool there[2] = {place.there[0], place.there[1]};
@@ -391,9 +451,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
         }
       }
       if (more) {
-        place = place_of(step + 2);
+        place = place_of(step + 2, ids);
         load_keys<D>(tile, place, offsets, P);
-        ids_of(step + 3);
+        ids_of(step + 3, ids);
       }
       // ---- probabilities
       half8_t p[NT];
@@ -473,19 +533,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
       if (more) load_values<D>(tile, place, offsets);
     };
 
-    Tile<D> even, odd;
-    Place even_place, odd_place;
-    ids_of(step0);
-    even_place = place_of(step0);
-    load_keys<D>(even, even_place, offsets, P);
-    load_values<D>(even, even_place, offsets);
-    ids_of(step0 + 1);
-    odd_place = place_of(step0 + 1);
-    if (steps > 1) {
-      load_keys<D>(odd, odd_place, offsets, P);
-      load_values<D>(odd, odd_place, offsets);
-    }
-    ids_of(step0 + 2);
     for (int step = step0; step < step_end; step += 2) {
       work_on(even, even_place, step);
       if (step + 1 < step_end) work_on(odd, odd_place, step + 1);
@@ -516,7 +563,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
     }
     __syncthreads();
     for (int item = threadIdx.x; item < rows * (D / 4); item += 64 * kWaves) {
-      const int row = item / (D / 4), ch = item % (D / 4) * 4, i = row / a.group;
+      const int row = item / (D / 4), ch = item % (D / 4) * 4, i = row * args.group_inv >> 16;
       float most = merge_m[0][row];
 #pragma unroll
       for (int k = 1; k < kWaves; ++k) most = fmaxf(most, merge_m[k][row]);
@@ -528,12 +575,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
         all += merge_l[k][row] * weight;
         sum += *reinterpret_cast<const float4_t*>(&merge[k][row][ch]) * weight;
       }
-      if (starts && ends) {
-        T* out = static_cast<T*>(a.out) + (seq.first + i) * a.out_token +
+      if (count == 1) {
+        T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + i) * a.out_token +
                  (int64_t)(head * a.group + row - i * a.group) * a.out_head + ch;
         store4(out, sum * (all > 0.0f || all != all ? 1.0f / all : 0.0f), a.out_wide);
       } else {
-        float* part = args.parts + ((int64_t)(2 * w + (starts ? 1 : 0)) * args.rows + row) * (D + 4);
+        float* part = args.parts + ((int64_t)slot * args.rows + row) * (D + 4);
         *reinterpret_cast<float4_t*>(part + ch) = sum;
         if (ch == 0) {
           part[D] = most;
@@ -541,30 +588,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
         }
       }
     }
-    if (threadIdx.x == 0 && starts && !ends)
-      args.headers[w] = SplitHeader{rows, (int32_t)seq.first, head, (pos + count - 1) / share};
-    pos += steps;
-    if (pos == seq_base + heads * count) {
-      seq_base = pos;
-      ++s;
-    }
+    if (threadIdx.x == 0 && part == 0) args.headers[s * heads + head] = PieceHeader{count, slot};
   }
 }
 
-// Joins the parts of one row of a piece that several workgroups shared: block (w, row).  A thread has four
-// channels of every kGroups-th part, kAtOnce of them under way at once.
-template <typename T, int D>
+// Joins the parts of one row: block (sequence and key head, row, CH channels).  A thread has four channels of
+// every kGroups-th part, kAtOnce of them under way at once.
+template <typename T, int D, int CH>
 __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs args) {
   const AttentionArgs& a = args.a;
-  const int w = blockIdx.x, row = blockIdx.y;
-  const SplitHeader header = args.headers[w];
-  if (row >= header.rows) return;
-  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAtOnce = 8;
-  __shared__ __align__(16) float lds[kGroups][D];
+  const int s = blockIdx.x / a.pages.heads, head = blockIdx.x - s * a.pages.heads, row = blockIdx.y, ch0 = blockIdx.z * CH;
+  const PieceHeader header = args.headers[blockIdx.x];
+  const Sequence seq = sequence<true>(a, s);
+  // (a sequence without new tokens has no piece and leaves its header as it was)
+  if (row >= min(seq.count, a.max_queries) * a.group || header.count < 2) return;
+  constexpr int kLanes = CH / 4, kGroups = kJoinThreads / kLanes, kAtOnce = 8;
+  __shared__ __align__(16) float lds[kGroups][CH];
   __shared__ float lds_m[kGroups], lds_l[kGroups];
-  const int parts = header.last - w + 1, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int parts = header.count, lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int64_t part_size = (int64_t)args.rows * (D + 4);
-  const float* base = args.parts + (int64_t)row * (D + 4);
+  const float* base = args.parts + header.slot * part_size + (int64_t)row * (D + 4);
   float4_t o = {0, 0, 0, 0};
   float m = -__builtin_inff(), l = 0.0f;
   for (int c0 = group; c0 < parts; c0 += kGroups * kAtOnce) {
@@ -572,16 +615,14 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
     float2 ml[kAtOnce];
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      const int c = c0 + k * kGroups;
-      ml[k] = make_float2(-__builtin_inff(), 0.0f);
-      x[k] = float4_t{0, 0, 0, 0};
-      if (c < parts) {
-        // part 0 is the workgroup's own second place, the others the first place of those behind it
-        const float* p = base + (c == 0 ? 2 * w + 1 : 2 * (w + c)) * part_size;
-        x[k] = *reinterpret_cast<const float4_t*>(p + lane * 4);
-        ml[k] = *reinterpret_cast<const float2*>(p + D);
-      }
+      // (a part behind the last is the last one again, with no weight)
+      const float* p = base + min(c0 + k * kGroups, parts - 1) * part_size;
+      x[k] = *reinterpret_cast<const float4_t*>(p + ch0 + lane * 4);
+      ml[k] = *reinterpret_cast<const float2*>(p + D);
     }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (c0 + k * kGroups >= parts) ml[k] = make_float2(-__builtin_inff(), 0.0f);
     float most = m;
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) most = fmaxf(most, ml[k].x);
@@ -591,7 +632,9 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
     o *= old;
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      const float weight = ml[k].x == most ? 1.0f : __builtin_amdgcn_exp2f(ml[k].x - most);
+      const float weight = c0 + k * kGroups >= parts ? 0.0f
+                           : ml[k].x == most        ? 1.0f
+                                                    : __builtin_amdgcn_exp2f(ml[k].x - most);
       l += ml[k].y * weight;
       o += x[k] * weight;
     }
@@ -613,23 +656,34 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
     all += lds_l[k] * weight;
     sum += *reinterpret_cast<const float4_t*>(&lds[k][lane * 4]) * weight;
   }
-  const int i = row / a.group;
-  T* out = static_cast<T*>(a.out) + ((int64_t)header.first + i) * a.out_token +
-           (int64_t)(header.head * a.group + row - i * a.group) * a.out_head + lane * 4;
+  const int i = row * args.group_inv >> 16;
+  T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + i) * a.out_token +
+           (int64_t)(head * a.group + row - i * a.group) * a.out_head + ch0 + lane * 4;
   store4(out, sum * (all > 0.0f || all != all ? 1.0f / all : 0.0f), a.out_wide);
-}
-
-// Workgroups of the split kernel: two a compute unit, and no more than there are steps.
-int split_grid(int64_t num_seqs, int kv_heads, int64_t table_width, int page_size) {
-  const int64_t steps = (table_width * page_size + kStep - 1) / kStep;
-  const int cus = device_compute_units();
-  return (int)min((int64_t)2 * (cus > 0 ? cus : 256), num_seqs * kv_heads * max(steps, (int64_t)1));
 }
 
 constexpr int kMostRows = 32;  // of the split kernel
 
-int64_t split_bytes(int grid, int rows, int head_size) {
-  return grid * ((int64_t)sizeof(SplitHeader) + 2 * rows * (head_size + 4) * (int64_t)sizeof(float));
+// Cut of a call's steps.  While there is room, every piece has a workgroup of its own and all run at once, two a
+// compute unit (their registers allow no third); sequences and key heads beyond half of that are cut in four
+// pieces a compute unit on top, which the workgroups take in turn.
+struct SplitPlan {
+  int grid, budget;
+  int64_t header_bytes, bytes;
+};
+
+SplitPlan plan_split(int64_t num_seqs, int kv_heads, int64_t table_width, int page_size, int rows, int head_size) {
+  const int cus = device_compute_units();
+  const int64_t room = 2 * (int64_t)(cus > 0 ? cus : 256), units = num_seqs * kv_heads;
+  const int64_t steps = units * max((table_width * page_size + kStep - 1) / kStep, (int64_t)1);
+  SplitPlan plan;
+  plan.grid = (int)min(room, steps);
+  plan.budget = (int)(units <= room / 2 ? room - units : 2 * room);
+  // of n > share steps come ceil(n / share) < 2 n / share pieces
+  const int64_t parts = min((int64_t)2 * plan.budget, steps);
+  plan.header_bytes = (units * (int64_t)sizeof(PieceHeader) + 15) / 16 * 16;
+  plan.bytes = plan.header_bytes + parts * rows * (head_size + 4) * (int64_t)sizeof(float);
+  return plan;
 }
 
 template <typename T, int D>
@@ -637,7 +691,10 @@ int launch_split(const SplitArgs& args, int grid, void* stream) {
   auto kernel = args.rows <= 16 ? attention_split_kernel<T, D, 1> : attention_split_kernel<T, D, 2>;
   launch_kernel(kernel, dim3((unsigned)grid), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), args);
   if (int rc = finish_launch("kv4_attention")) return rc;
-  launch_kernel(attention_join_kernel<T, D>, dim3((unsigned)grid, (unsigned)args.rows), dim3(kJoinThreads), 0,
+  // few sequences may be in very many pieces: more workgroups then share a row's channels
+  const bool few = (int64_t)args.a.num_seqs * args.a.pages.heads <= 16;
+  launch_kernel(few ? attention_join_kernel<T, D, 32> : attention_join_kernel<T, D, D>,
+                dim3((unsigned)(args.a.num_seqs * args.a.pages.heads), (unsigned)args.rows, few ? D / 32 : 1), dim3(kJoinThreads), 0,
                 static_cast<hipStream_t>(stream), args);
   return finish_launch("kv4_attention");
 }
@@ -676,13 +733,10 @@ __device__ __forceinline__ void find_tile(const AttentionArgs& a, int tile, int 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) lds[kW] = -1;
   int base = 0;
-  for (int64_t s0 = 0; s0 < a.num_seqs; s0 += THREADS) {
-    const int64_t s = s0 + threadIdx.x;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += THREADS) {
+    const int s = s0 + threadIdx.x;
     int count = 0;
-    if (s < a.num_seqs) {
-      const int64_t rows = min(sequence(a, s).count, a.max_queries) * a.group;
-      count = (int)((rows + rows_of_tile - 1) / rows_of_tile);
-    }
+    if (s < a.num_seqs) count = (min(sequence(a, s).count, a.max_queries) * a.group + rows_of_tile - 1) / rows_of_tile;
     int sum = count;
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) {
@@ -698,7 +752,7 @@ __device__ __forceinline__ void find_tile(const AttentionArgs& a, int tile, int 
       base += lds[w];
     }
     if (tile >= before && tile < before + count) {
-      lds[kW] = (int)s;
+      lds[kW] = s;
       lds[kW + 1] = tile - before;
     }
     if (base > tile) break;
@@ -751,15 +805,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   int s, place;
   find_tile<S::kThreads>(a, tile, S::kRows, &s, &place, found);
   if (s < 0) return;
-  const Sequence seq = sequence(a, s);
-  const int queries = (int)min(seq.count, a.max_queries), rows = queries * a.group, length = (int)seq.length;
-  const int new_from = length - (int)seq.count;
+  const Sequence seq = sequence<true>(a, s);
+  const int queries = min(seq.count, a.max_queries), rows = queries * a.group, length = seq.length;
+  const int new_from = length - seq.count;
   const int row0 = place * S::kRows, last_row = min(row0 + S::kRows, rows) - 1;
 
   // ---- tokens that the tile's rows see, and this piece of them
-  const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
+  const int window = a.window > 0 ? a.window : 1 << 30;
   auto end_of = [&](int row) { return min(new_from + row / a.group + 1, length); };
-  auto begin_of = [&](int row) { return (int)max((int64_t)new_from + row / a.group + 1 - window, (int64_t)0); };
+  auto begin_of = [&](int row) { return max(new_from + row / a.group + 1 - window, 0); };
   const int some_from = begin_of(row0), some_to = end_of(last_row);
   int tile_from = some_from / kTileTokens, tile_to = max((some_to + kTileTokens - 1) / kTileTokens, tile_from);
   if (args.splits > 1) {
@@ -778,7 +832,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   half8_t q[D / 16];
   float scale;
   {
-    const T* from = static_cast<const T*>(a.q) + (seq.first + query) * a.q_token + (int64_t)q_head * a.q_head + h * 8;
+    const T* from = static_cast<const T*>(a.q) + (int64_t)(seq.first + query) * a.q_token + (int64_t)q_head * a.q_head + h * 8;
     float most = 0.0f, back;
     float x[D / 16][8] = {};
     if (row < rows) {
@@ -804,7 +858,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
 
-  const int32_t* table = a.block_table + (int64_t)s * a.table_stride;
+  const int32_t* table = a.block_table + s * a.table_stride;
   // Base of the block that holds token t; tokens of a missing page are read from page 0 and masked.
   auto block_of = [&](int t, bool* there) {
     const int id = t < length ? table[t >> a.pages.page_log2] : -1;
@@ -961,7 +1015,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   l += __shfl_xor(l, 32);
   if (row >= rows) return;
   if (args.splits == 1) {
-    T* out = static_cast<T*>(a.out) + (seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
+    T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
@@ -992,8 +1046,8 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
   int s, place;
   find_tile<256>(a, tile, S::kRows, &s, &place, found);
   if (s < 0) return;
-  const Sequence seq = sequence(a, s);
-  const int rows = (int)min(seq.count, a.max_queries) * a.group;
+  const Sequence seq = sequence<true>(a, s);
+  const int rows = min(seq.count, a.max_queries) * a.group;
   const int in_tile = blockIdx.z * 4 + (threadIdx.x >> 6), row = place * S::kRows + in_tile;
   if (row >= rows) return;
   const float* part = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows + in_tile) * (D + 4);
@@ -1009,7 +1063,7 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
     for (int k = 0; k < D / 64; ++k) o[k] += p[k * 64 + lane] * weight;
   }
   const int query = row / a.group;
-  T* out = static_cast<T*>(a.out) + (seq.first + query) * a.out_token +
+  T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token +
            (int64_t)(head * a.group + row - query * a.group) * a.out_head;
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) out[k * 64 + lane] = (T)(l > 0.0f || l != l ? o[k] / l : 0.0f);
@@ -1071,7 +1125,7 @@ int64_t kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_
   const int group = q_heads / kv_heads;
   max_queries = min(max_queries, num_tokens);
   if (max_queries * group <= kMostRows)
-    return split_bytes(split_grid(num_seqs, kv_heads, table_width, page_size), (int)max_queries * group, head_size);
+    return plan_split(num_seqs, kv_heads, table_width, page_size, (int)max_queries * group, head_size).bytes;
   return plan_tiles(num_tokens, group, kv_heads, head_size, num_seqs, max_queries, table_width, page_size).bytes;
 }
 
@@ -1095,10 +1149,10 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: a stride is negative", what);
   if (!seq_lens || (!block_table && table_width > 0))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table or seq_lens is null", what);
-  if (table_width > ((int64_t)1 << 31) / page_size)
-    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table has room for more than 2^31 tokens", what);
-  if (num_seqs > 65535 || T > 0x7fffffff)
-    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: more than 65535 sequences or 2^31 tokens", what);
+  if (table_width > ((int64_t)1 << 30) / page_size)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table has room for more than 2^30 tokens", what);
+  if (num_seqs > 65535 || T > (1 << 30))
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: more than 65535 sequences or 2^30 tokens", what);
   if (!query_starts && T % num_seqs != 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld tokens are not the same number for each of %lld sequences", what,
                      (long long)T, (long long)num_seqs);
@@ -1116,28 +1170,29 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   a.group = (int)(q->heads / kv_heads);
   a.block_table = block_table;
   a.table_stride = table_stride;
-  a.table_width = table_width;
+  a.capacity = (int)(table_width * page_size);
   a.seq_lens = seq_lens;
   a.query_starts = query_starts;
-  a.per_seq = query_starts ? 0 : T / num_seqs;
-  a.num_seqs = num_seqs;
-  a.num_tokens = T;
-  a.max_queries = min(max_queries, T);
+  a.per_seq = query_starts ? 0 : (int)(T / num_seqs);
+  a.num_seqs = (int)num_seqs;
+  a.num_tokens = (int)T;
+  a.max_queries = (int)min(max_queries, T);
   a.scale = scale * kLog2e;
-  a.window = window;
+  a.window = (int)min(window, (int64_t)1 << 30);
   a.q_wide = wide_rows(q);
   a.out_wide = wide_rows(out);
   max_queries = a.max_queries;
   if (max_queries * a.group <= kMostRows) {
-    const int grid = split_grid(num_seqs, kv_heads, table_width, page_size);
     // steps are counted in 32 bits
     if ((double)num_seqs * kv_heads * (double)((table_width * page_size + kStep - 1) / kStep + 1) > 2e9)
       return set_error(TW_ERR_INVALID_ARGUMENT, "%s: the sequences have room for too many tokens", what);
-    SplitArgs args{a, static_cast<SplitHeader*>(workspace),
-                   reinterpret_cast<float*>(static_cast<char*>(workspace) + grid * sizeof(SplitHeader)),
-                   (int)(max_queries * a.group)};
-    return dtype == TW_DTYPE_BF16 ? launch_split<__bf16>(args, head_size, grid, stream)
-                                  : launch_split<_Float16>(args, head_size, grid, stream);
+    const int rows = (int)(max_queries * a.group);
+    const SplitPlan plan = plan_split(num_seqs, kv_heads, table_width, page_size, rows, head_size);
+    const SplitArgs args{a, static_cast<PieceHeader*>(workspace),
+                         reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.header_bytes), rows, plan.budget,
+                         65536 / a.group + 1};
+    return dtype == TW_DTYPE_BF16 ? launch_split<__bf16>(args, head_size, plan.grid, stream)
+                                  : launch_split<_Float16>(args, head_size, plan.grid, stream);
   }
   const TilePlan plan = plan_tiles(T, a.group, kv_heads, head_size, num_seqs, max_queries, table_width, page_size);
   if ((double)T * a.group + (double)num_seqs * 256 > 2e9 || kv_heads > 65535)
