@@ -218,11 +218,14 @@ __device__ __forceinline__ void load_row(float (&x)[N], const T* row, bool wide)
   }
 }
 
-// The power of two that brings the largest magnitude to [2^14, 2^15), and its inverse.
-__device__ __forceinline__ float lift_of(float most, float* back) {
+// What a row is multiplied by before its products, the power of two that brings its largest magnitude to [2^14,
+// 2^15) and the sign of `scale`, and what the products are multiplied by: more than zero, so that the largest
+// product is the largest score and a product of minus infinity a score of minus infinity.
+__device__ __forceinline__ float lift_of(float most, float scale, float* back) {
   const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
-  *back = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-  return __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+  const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+  *back = scale == 0.0f ? 1.0f : fmaxf(__uint_as_float((uint32_t)(127 - 14 + e) << 23) * __builtin_fabsf(scale), 0x1p-126f);
+  return scale == 0.0f ? 0.0f : __builtin_copysignf(up, scale);
 }
 
 template <typename T, int D>
@@ -240,14 +243,14 @@ struct RawQueries {
       }
     }
   }
-  // Returns what the scores are multiplied back by.
-  __device__ __forceinline__ float lift(half8_t (&q)[D / 32]) const {
+  // Returns what the products are multiplied by to be scores.
+  __device__ __forceinline__ float lift(half8_t (&q)[D / 32], float scale) const {
     float most = 0.0f, back;
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) most = fmaxf(most, __builtin_fabsf((float)x[i / 8][i % 8]));
     most = fmaxf(most, __shfl_xor(most, 16));
     most = fmaxf(most, __shfl_xor(most, 32));
-    const float up = lift_of(most, &back);
+    const float up = lift_of(most, scale, &back);
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) q[i / 8][i % 8] = (_Float16)((float)x[i / 8][i % 8] * up);
     return back;
@@ -420,7 +423,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
     float4_t o[NT][kTiles];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      scale[t] = raw[t].lift(q[t]) * a.scale;
+      scale[t] = raw[t].lift(q[t], a.scale);
       m[t] = -__builtin_inff();
       l[t] = 0.0f;
 #pragma unroll
@@ -462,7 +465,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
         float x[8], most = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[i] = sc[t][i / 4][i % 4] * scale[t];
+          x[i] = sc[t][i / 4][i % 4];
           if (!whole) {
             const int token = t0 + (i / 4) * 16 + h4 * 4 + i % 4;
             if (token >= row_end[t] || token < row_begin[t] || !there[i / 4]) x[i] = -__builtin_inff();
@@ -470,7 +473,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
           most = fmaxf(most, x[i]);
         }
         most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
+        most = fmaxf(most, __shfl_xor(most, 32)) * scale[t];
         if (__builtin_amdgcn_ballot_w64(most > m[t])) {
           const float now = fmaxf(m[t], most);
           const float old = m[t] == now ? 1.0f : __builtin_amdgcn_exp2f(m[t] - now);
@@ -479,11 +482,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
 #pragma unroll
           for (int c = 0; c < kTiles; ++c) o[t][c] *= old;
         }
-        const float sub = (m[t] == -__builtin_inff() ? 0.0f : m[t]) - kLift;
+        const float add = kLift - (m[t] == -__builtin_inff() ? 0.0f : m[t]);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[i] = __builtin_amdgcn_exp2f(x[i] - sub);
+          x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale[t], add));
           sum += x[i];
           p[t][i] = (_Float16)x[i];
         }
@@ -721,45 +724,74 @@ constexpr int kTileTokens = 64;
 
 struct TileArgs {
   AttentionArgs a;
-  float* parts;  // of `splits` pieces of every tile's tokens: [tile][head][split][rows][D + 4]; null: one piece
-  int tiles, splits;
+  float* parts;  // of up to `splits` pieces of every tile's tokens: [tile][head][split][rows][D + 4]
+  int tiles, splits, budget;
 };
 
-// Sequence and place in it of tile `tile` (uniform); a tile behind the last: seq < 0.
+// Tokens that the rows [row, last] of a sequence see, in tiles of 64: [from, to).
+struct Span {
+  int from, to;
+};
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, const Sequence& q, int row, int last) {
+  const int new_from = q.length - q.count, window = a.window > 0 ? a.window : 1 << 30;
+  const int from = max(new_from + row / a.group + 1 - window, 0) / kTileTokens;
+  return {from, max((min(new_from + last / a.group + 1, q.length) + kTileTokens - 1) / kTileTokens, from)};
+}
+
+// Pieces of a tile of `count` spans: none longer than an even share of all tiles' spans over the budget, none
+// shorter than 256 tokens.
+__device__ __forceinline__ int pieces_of_tile(const TileArgs& args, int count, int64_t total) {
+  const int share = max((int)((total + args.budget - 1) / args.budget), 256 / kTileTokens);
+  return min(max((count + share - 1) / share, 1), args.splits);
+}
+
+// Sequence and place in it of tile `tile` (uniform); a tile behind the last: seq < 0.  `total`, where it is asked
+// for: the spans of all tiles of all key heads, a sequence's taken to grow evenly from its first tile to its last.
 template <int THREADS>
 __device__ __forceinline__ void find_tile(const AttentionArgs& a, int tile, int rows_of_tile, int* seq, int* place,
-                                          int* lds) {
+                                          int64_t* total, int* lds) {
   constexpr int kW = THREADS / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) lds[kW] = -1;
   int base = 0;
+  int64_t spans = 0;
   for (int s0 = 0; s0 < a.num_seqs; s0 += THREADS) {
     const int s = s0 + threadIdx.x;
-    int count = 0;
-    if (s < a.num_seqs) count = (min(sequence(a, s).count, a.max_queries) * a.group + rows_of_tile - 1) / rows_of_tile;
-    int sum = count;
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) {
-      const int y = __shfl_up(sum, i);
-      if (lane >= i) sum += y;
+    int count = 0, span = 0;
+    if (s < a.num_seqs) {
+      const Sequence q = sequence(a, s);
+      const int rows = min(q.count, a.max_queries) * a.group;
+      count = (rows + rows_of_tile - 1) / rows_of_tile;
+      if (total && count > 0) {
+        const Span first = span_of(a, q, 0, min(rows_of_tile, rows) - 1);
+        const Span last = span_of(a, q, (count - 1) * rows_of_tile, rows - 1);
+        span = (int)min((int64_t)count * (first.to - first.from + last.to - last.from) / 2, (int64_t)1 << 24);
+      }
     }
+    const int sum = wave_scan(count);
+    if (total) span = wave_scan(span);
     __syncthreads();
-    if (lane == 63) lds[wave] = sum;
+    if (lane == 63) {
+      lds[wave] = sum;
+      lds[kW + 2 + wave] = span;
+    }
     __syncthreads();
     int before = base + sum - count;
     for (int w = 0; w < kW; ++w) {
       before += w < wave ? lds[w] : 0;
       base += lds[w];
+      spans += total ? lds[kW + 2 + w] : 0;
     }
     if (tile >= before && tile < before + count) {
       lds[kW] = s;
       lds[kW + 1] = tile - before;
     }
-    if (base > tile) break;
+    if (base > tile && !total) break;
   }
   __syncthreads();
   *seq = uniform(lds[kW]);
   *place = uniform(lds[kW + 1]);
+  if (total) *total = spans * a.pages.heads;
 }
 
 template <int D, int WAVES>
@@ -795,7 +827,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   using L = Kv4<D>;
   const AttentionArgs& a = args.a;
   __shared__ TileBuffer<D, WAVES> buffers[2];
-  __shared__ int found[WAVES + 2];
+  __shared__ int found[2 * WAVES + 2];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads;
@@ -803,7 +835,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   const int head = blockIdx.y, split = blockIdx.z;
 
   int s, place;
-  find_tile<S::kThreads>(a, tile, S::kRows, &s, &place, found);
+  int64_t total = 0;
+  find_tile<S::kThreads>(a, tile, S::kRows, &s, &place, args.splits > 1 ? &total : nullptr, found);
   if (s < 0) return;
   const Sequence seq = sequence<true>(a, s);
   const int queries = min(seq.count, a.max_queries), rows = queries * a.group, length = seq.length;
@@ -814,13 +847,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   const int window = a.window > 0 ? a.window : 1 << 30;
   auto end_of = [&](int row) { return min(new_from + row / a.group + 1, length); };
   auto begin_of = [&](int row) { return max(new_from + row / a.group + 1 - window, 0); };
-  const int some_from = begin_of(row0), some_to = end_of(last_row);
-  int tile_from = some_from / kTileTokens, tile_to = max((some_to + kTileTokens - 1) / kTileTokens, tile_from);
-  if (args.splits > 1) {
-    const int each = (tile_to - tile_from + args.splits - 1) / args.splits;
-    tile_from = min(tile_from + split * each, tile_to);
-    tile_to = min(tile_from + each, tile_to);
-  }
+  const int some_from = begin_of(row0);
+  const Span span = span_of(a, seq, row0, last_row);
+  const int pieces = args.splits > 1 ? pieces_of_tile(args, span.to - span.from, total) : 1;
+  if (split >= pieces) return;
+  const int each = (span.to - span.from) / pieces, longer = (span.to - span.from) - each * pieces;
+  const int tile_from = span.from + split * each + min(split, longer), tile_to = tile_from + each + (split < longer ? 1 : 0);
 
   // ---- this wave's rows
   const int row = row0 + wave * 32 + n, query = row / a.group, q_head = head * a.group + row - query * a.group;
@@ -844,12 +876,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
 #pragma unroll
       for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(x[c][j]));
     most = fmaxf(most, __shfl_xor(most, 32));
-    const float up = lift_of(most, &back);
+    const float up = lift_of(most, a.scale, &back);
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[c][j] = (_Float16)(x[c][j] * up);
-    scale = back * a.scale;
+    scale = back;
   }
   float m = -__builtin_inff(), l = 0.0f;
   float16_t o[D / 32];
@@ -858,21 +890,36 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
 
-  const int32_t* table = a.block_table + s * a.table_stride;
-  // Base of the block that holds token t; tokens of a missing page are read from page 0 and masked.
-  auto block_of = [&](int t, bool* there) {
-    const int id = t < length ? table[t >> a.pages.page_log2] : -1;
-    *there = id >= 0 && id < a.pages.num_pages;
+  const ConstInts table = constant(a.block_table) + s * a.table_stride;
+  // The pages of a tile's four sixteens, fetched a tile before they are used; a missing one is -1.
+  struct Pages {
+    int a, b, c, d;
+  };
+  auto page_of = [&](int at, int i) {
+    const int t = at * kTileTokens + i * 16;
+    return uniform(at < tile_to && t < length ? table[t >> a.pages.page_log2] : -1);
+  };
+  auto pages_of = [&](int at) { return Pages{page_of(at, 0), page_of(at, 1), page_of(at, 2), page_of(at, 3)}; };
+  auto missing_of = [&](const Pages& p) {  // a bit for each sixteen
+    auto bit = [&](int id, int b) { return id < 0 || id >= a.pages.num_pages ? b : 0; };
+    return bit(p.a, 1) | bit(p.b, 2) | bit(p.c, 4) | bit(p.d, 8);
+  };
+  // Base of the block that holds the tile's token `t`; tokens of a missing page are read from page 0 and masked.
+  auto block_of = [&](Pages pages, int missing, int t, bool* there) {
+    const int i = t >> 4;
+    const int a01 = i & 1 ? uniform(pages.b) : uniform(pages.a), a23 = i & 1 ? uniform(pages.d) : uniform(pages.c);
+    const int id = i & 2 ? a23 : a01;
+    *there = !(missing >> i & 1);
     return a.pages.data + ((int64_t)(*there ? id : 0) * heads + head) * a.pages.head_bytes;
   };
-  auto fetch = [&](Fetched<D, WAVES>& f, int t0) {
+  auto fetch = [&](Fetched<D, WAVES>& f, const Pages& pages, int missing, int t0) {
 #pragma unroll
     for (int i = 0; i < S::kKeyTurns; ++i) {
       const int chunk = (int)threadIdx.x + i * S::kThreads;
       if (S::kKeyChunks % S::kThreads == 0 || chunk < S::kKeyChunks) {
-        const int t = t0 + chunk / (D / 32), g = chunk % (D / 32), at = t & (P - 1);
+        const int t = chunk / (D / 32), g = chunk % (D / 32), at = (t0 + t) & (P - 1);
         bool there;
-        const uint8_t* b = block_of(t, &there);
+        const uint8_t* b = block_of(pages, missing, t, &there);
         load_words(f.k[i], b + (L::key(at) + g * 16));
         f.ks[i] = b[L::key_scale(P, at, g)];
       }
@@ -882,15 +929,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
       const int chunk = (int)threadIdx.x - S::kValueThread + i * S::kThreads;
       if (S::kValueChunks % S::kThreads == 0 || (chunk >= 0 && chunk < S::kValueChunks)) {
         // of 32 neighbouring lanes two sixteenths and all 16 fours of tokens: their LDS writes cover all banks
-        const int sixteenth = (chunk & 1) | (chunk >> 5 << 1), t = t0 + (chunk >> 1 & 15) * 4, at = t & (P - 1);
+        const int sixteenth = (chunk & 1) | (chunk >> 5 << 1), t = (chunk >> 1 & 15) * 4, at = (t0 + t) & (P - 1);
         bool there;
-        const uint8_t* b = block_of(t, &there);
+        const uint8_t* b = block_of(pages, missing, t, &there);
         load_words(f.v[i], b + L::value(P, at, sixteenth));
         uint32_t vs = *reinterpret_cast<const uint32_t*>(b + L::value_scale(P, at, sixteenth * (D / 16) / 32));
         // what no row sees may hold anything, and nothing times zero has to be zero
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (!there || t + j >= length || t + j < some_from) vs = (vs & ~(255u << (8 * j))) | 127u << (8 * j);
+          if (!there || t0 + t + j >= length || t0 + t + j < some_from) vs = (vs & ~(255u << (8 * j))) | 127u << (8 * j);
         f.vs[i] = vs;
       }
     }
@@ -937,17 +984,24 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   };
 
   Fetched<D, WAVES> next;
+  Pages pages = pages_of(tile_from);
+  int missing = missing_of(pages), missing_next = 0, missing_after = 0;  // of this tile, the next, the one after
   if (tile_from < tile_to) {
-    fetch(next, tile_from * kTileTokens);
+    fetch(next, pages, missing, tile_from * kTileTokens);
+    pages = pages_of(tile_from + 1);
     spread(next, buffers[0]);
-    if (tile_from + 1 < tile_to) fetch(next, (tile_from + 1) * kTileTokens);
+    missing_next = missing_of(pages);
+    if (tile_from + 1 < tile_to) fetch(next, pages, missing_next, (tile_from + 1) * kTileTokens);
+    pages = pages_of(tile_from + 2);
   }
   __syncthreads();
   for (int at = tile_from; at < tile_to; ++at) {
     const TileBuffer<D, WAVES>& now = buffers[(at - tile_from) & 1];
     const int t0 = at * kTileTokens;
     if (at + 1 < tile_to) spread(next, buffers[(at - tile_from + 1) & 1]);
-    if (at + 2 < tile_to) fetch(next, t0 + 2 * kTileTokens);
+    missing_after = missing_of(pages);
+    if (at + 2 < tile_to) fetch(next, pages, missing_after, t0 + 2 * kTileTokens);
+    pages = pages_of(at + 3);
     if (t0 < wave_to && t0 + kTileTokens > wave_from) {
       float16_t sc[2];
 #pragma unroll
@@ -961,29 +1015,22 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
           const half8_t k = *reinterpret_cast<const half8_t*>(now.k + (i * 32 + n) * S::kKeyRow + c * 32 + h * 16);
           sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[c], sc[i], 0, 0, 0);
         }
-      bool whole = t0 >= all_from && t0 + kTileTokens <= all_to;
-      // pages of the tile's four sixteens
-      bool there[4];
+      const bool whole = t0 >= all_from && t0 + kTileTokens <= all_to && missing == 0;
+      if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = t0 + i * 16, id = t < length ? table[t >> a.pages.page_log2] : -1;
-        there[i] = id >= 0 && id < a.pages.num_pages;
-        whole = whole && there[i];
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int t = t0 + i * 32 + (j / 4) * 8 + h * 4 + j % 4;
+            if (t >= row_end || t < row_begin || missing >> (i * 2 + j / 8) & 1) sc[i][j] = -__builtin_inff();
+          }
       }
       float most = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float x = sc[i][j] * scale;
-          if (!whole) {
-            const int t = t0 + i * 32 + (j / 4) * 8 + h * 4 + j % 4;
-            if (t >= row_end || t < row_begin || !there[i * 2 + j / 8]) x = -__builtin_inff();
-          }
-          sc[i][j] = x;
-          most = fmaxf(most, x);
-        }
-      most = fmaxf(most, __shfl_xor(most, 32));
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, sc[i][j]);
+      most = fmaxf(most, __shfl_xor(most, 32)) * scale;
       if (__builtin_amdgcn_ballot_w64(most > m)) {
         const float higher = fmaxf(m, most);
         const float old = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
@@ -992,13 +1039,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) o[c] *= old;
       }
-      const float sub = (m == -__builtin_inff() ? 0.0f : m) - kLift;
+      const float add = kLift - (m == -__builtin_inff() ? 0.0f : m);
       half8_t p[4];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float x = __builtin_amdgcn_exp2f(sc[i][j] - sub);
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][j], scale, add));
           l += x;
           p[i * 2 + j / 8][j % 8] = (_Float16)x;
         }
@@ -1010,11 +1057,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
           o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[k], o[c], 0, 0, 0);
         }
     }
+    missing = missing_next;
+    missing_next = missing_after;
     __syncthreads();
   }
   l += __shfl_xor(l, 32);
   if (row >= rows) return;
-  if (args.splits == 1) {
+  if (pieces == 1) {
     T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
@@ -1041,21 +1090,24 @@ template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args) {
   using S = TileShape<D, WAVES>;
   const AttentionArgs& a = args.a;
-  __shared__ int found[4 + 2];
+  __shared__ int found[2 * 4 + 2];
   const int tile = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63;
   int s, place;
-  find_tile<256>(a, tile, S::kRows, &s, &place, found);
+  int64_t total;
+  find_tile<256>(a, tile, S::kRows, &s, &place, &total, found);
   if (s < 0) return;
   const Sequence seq = sequence<true>(a, s);
   const int rows = min(seq.count, a.max_queries) * a.group;
   const int in_tile = blockIdx.z * 4 + (threadIdx.x >> 6), row = place * S::kRows + in_tile;
-  if (row >= rows) return;
+  const Span span = span_of(a, seq, place * S::kRows, min((place + 1) * S::kRows, rows) - 1);
+  const int pieces = pieces_of_tile(args, span.to - span.from, total);
+  if (row >= rows || pieces == 1) return;
   const float* part = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows + in_tile) * (D + 4);
   const int64_t stride = (int64_t)S::kRows * (D + 4);
   float m = -__builtin_inff(), l = 0.0f, o[D / 64] = {};
-  for (int c = 0; c < args.splits; ++c) m = fmaxf(m, part[c * stride + D]);
+  for (int c = 0; c < pieces; ++c) m = fmaxf(m, part[c * stride + D]);
 #pragma unroll 4
-  for (int c = 0; c < args.splits; ++c) {
+  for (int c = 0; c < pieces; ++c) {
     const float* p = part + c * stride;
     const float weight = p[D] == m ? 1.0f : __builtin_amdgcn_exp2f(p[D] - m);
     l += p[D + 1] * weight;
@@ -1071,7 +1123,7 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
 
 // Tiles and pieces of a call.
 struct TilePlan {
-  int waves, tiles, splits;
+  int waves, tiles, splits, budget;
   int64_t bytes;
 };
 
@@ -1086,9 +1138,11 @@ TilePlan plan_tiles(int64_t T, int group, int kv_heads, int head_size, int64_t n
   // every sequence may leave one tile that is not full
   const int64_t tiles = min((T * group + rows - 1) / rows + num_seqs, num_seqs * ((max_queries * group + rows - 1) / rows));
   const int cus = device_compute_units();
-  // too few tiles for the compute units: their tokens are cut into pieces of 256 and more
+  // Two tiles and more a compute unit even out among themselves, the longest first.  Fewer are cut so that no
+  // piece is longer than an even share.
   const int64_t units = tiles * kv_heads, most = max(table_width * page_size / 256, (int64_t)1);
-  plan.splits = (int)min(max((cus > 0 ? cus : 256) / units, (int64_t)1), most);
+  plan.budget = cus > 0 ? cus : 256;
+  plan.splits = units >= 2 * plan.budget ? 1 : (int)min((2 * plan.budget + units - 1) / units, most);
   plan.tiles = (int)min(tiles, (int64_t)0x7fffffff);
   plan.bytes = plan.splits == 1 ? 0 : tiles * kv_heads * plan.splits * rows * (head_size + 4) * (int64_t)sizeof(float);
   return plan;
@@ -1197,7 +1251,7 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   const TilePlan plan = plan_tiles(T, a.group, kv_heads, head_size, num_seqs, max_queries, table_width, page_size);
   if ((double)T * a.group + (double)num_seqs * 256 > 2e9 || kv_heads > 65535)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too many rows", what);
-  const TileArgs args{a, static_cast<float*>(workspace), plan.tiles, plan.splits};
+  const TileArgs args{a, static_cast<float*>(workspace), plan.tiles, plan.splits, plan.budget};
   return dtype == TW_DTYPE_BF16 ? launch_tiles<__bf16>(args, head_size, stream)
                                 : launch_tiles<_Float16>(args, head_size, stream);
 }
