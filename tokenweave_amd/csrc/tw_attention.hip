@@ -109,6 +109,27 @@ __device__ __forceinline__ void steps_of(const AttentionArgs& a, const Sequence&
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// The value of this lane and of the one 32 (16) lanes across, in two registers in either order.
+struct Both {
+  float a, b;
+};
+__device__ __forceinline__ Both across32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ Both across16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ float max32(float x) {
+  const Both y = across32(x);
+  return fmaxf(y.a, y.b);
+}
+__device__ __forceinline__ float max16(float x) {
+  const Both y = across16(x);
+  return fmaxf(y.a, y.b);
+}
+
 // Sum over the wave's lanes up to this one.
 __device__ __forceinline__ int wave_scan(int x) {
 #define TW_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
@@ -248,8 +269,7 @@ struct RawQueries {
     float most = 0.0f, back;
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) most = fmaxf(most, __builtin_fabsf((float)x[i / 8][i % 8]));
-    most = fmaxf(most, __shfl_xor(most, 16));
-    most = fmaxf(most, __shfl_xor(most, 32));
+    most = max32(max16(most));
     const float up = lift_of(most, scale, &back);
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) q[i / 8][i % 8] = (_Float16)((float)x[i / 8][i % 8] * up);
@@ -472,8 +492,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
           }
           most = fmaxf(most, x[i]);
         }
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32)) * scale[t];
+        most = max32(max16(most)) * scale[t];
         if (__builtin_amdgcn_ballot_w64(most > m[t])) {
           const float now = fmaxf(m[t], most);
           const float old = m[t] == now ? 1.0f : __builtin_amdgcn_exp2f(m[t] - now);
@@ -542,8 +561,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      l[t] += __shfl_xor(l[t], 16);
-      l[t] += __shfl_xor(l[t], 32);
+      const Both x = across16(l[t]), y = across32(x.a + x.b);
+      l[t] = y.a + y.b;
     }
 
     // ---- the waves' parts become one
@@ -712,15 +731,17 @@ int launch_split(const SplitArgs& args, int D, int grid, void* stream) {
 // ---------------------------------------------------------------------------
 // Many rows: a tile of 32 rows a wave, all of one key head.
 //
-// The workgroup turns 64 tokens at a time into fp16 in LDS, once for all its rows, double-buffered: the
-// codes of the tile after next are on their way and the next tile is written while the present one is
-// multiplied.  32 x 32 x 16 products; as above the scores of a row stay in the two lanes that hold
-// the row, and go into the second product without moving.  Values lie in LDS by channel, their
+// The workgroup turns 64 tokens at a time (32 where heads have 256 channels) into fp16 in LDS, once for all its
+// rows.  A wave works on 32 tokens at once with 32 x 32 x 16 products; as above the scores of a row stay in the
+// two lanes that hold the row and go into the second product without moving.  Values lie in LDS by channel, their
 // tokens in the order in which the scores' registers hold them: of 16 tokens 0-3, 8-11, 4-7, 12-15.
+//
+// The matrix and the vector units work side by side: the scores of the next 32 tokens are computed between the
+// exponentials of the present ones, and their maximum is found between the present products with the values.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
-constexpr int kTileTokens = 64;
+constexpr int kSpan = 64;  // tokens in which tiles are measured and cut
 
 struct TileArgs {
   AttentionArgs a;
@@ -728,28 +749,31 @@ struct TileArgs {
   int tiles, splits, budget;
 };
 
-// Tokens that the rows [row, last] of a sequence see, in tiles of 64: [from, to).
+// Tokens that the rows [row, last] of a sequence see, in spans: [from, to).
 struct Span {
   int from, to;
 };
 __device__ __forceinline__ Span span_of(const AttentionArgs& a, const Sequence& q, int row, int last) {
   const int new_from = q.length - q.count, window = a.window > 0 ? a.window : 1 << 30;
-  const int from = max(new_from + row / a.group + 1 - window, 0) / kTileTokens;
-  return {from, max((min(new_from + last / a.group + 1, q.length) + kTileTokens - 1) / kTileTokens, from)};
+  const int from = max(new_from + row / a.group + 1 - window, 0) / kSpan;
+  return {from, max((min(new_from + last / a.group + 1, q.length) + kSpan - 1) / kSpan, from)};
 }
 
 // Pieces of a tile of `count` spans: none longer than an even share of all tiles' spans over the budget, none
 // shorter than 256 tokens.
 __device__ __forceinline__ int pieces_of_tile(const TileArgs& args, int count, int64_t total) {
-  const int share = max((int)((total + args.budget - 1) / args.budget), 256 / kTileTokens);
+  const int share = max((int)((total + args.budget - 1) / args.budget), 256 / kSpan);
   return min(max((count + share - 1) / share, 1), args.splits);
 }
 
-// Sequence and place in it of tile `tile` (uniform); a tile behind the last: seq < 0.  `total`, where it is asked
-// for: the spans of all tiles of all key heads, a sequence's taken to grow evenly from its first tile to its last.
+// Whose tile it is and its place there (uniform); a tile behind the last: seq < 0.  `total`, where it is asked for:
+// the spans of all tiles of all key heads, a sequence's taken to grow evenly from its first tile to its last.
+struct FoundTile {
+  int seq, place;
+  int64_t total;
+};
 template <int THREADS>
-__device__ __forceinline__ void find_tile(const AttentionArgs& a, int tile, int rows_of_tile, int* seq, int* place,
-                                          int64_t* total, int* lds) {
+__device__ __forceinline__ FoundTile find_tile(const AttentionArgs& a, int tile, int rows_of_tile, bool total, int* lds) {
   constexpr int kW = THREADS / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) lds[kW] = -1;
@@ -789,59 +813,69 @@ __device__ __forceinline__ void find_tile(const AttentionArgs& a, int tile, int 
     if (base > tile && !total) break;
   }
   __syncthreads();
-  *seq = uniform(lds[kW]);
-  *place = uniform(lds[kW + 1]);
-  if (total) *total = spans * a.pages.heads;
+  return {uniform(lds[kW]), uniform(lds[kW + 1]), spans * a.pages.heads};
 }
 
-template <int D, int WAVES>
+template <int D>
 struct TileShape {
-  static constexpr int kThreads = 64 * WAVES, kRows = 32 * WAVES;
-  static constexpr int kKeyRow = D * 2 + 16, kValueRow = kTileTokens * 2 + 16;  // 16 bytes more: no two lanes' rows in one bank
-  static constexpr int kKeyChunks = kTileTokens * (D / 32);                     // 32 channels of a token
-  static constexpr int kValueChunks = (kTileTokens / 4) * 16;                   // 4 tokens of a sixteenth
-  static constexpr int kKeyTurns = (kKeyChunks + kThreads - 1) / kThreads;
-  static constexpr int kValueTurns = (kValueChunks + kThreads - 1) / kThreads;
-  // keys by the first threads and values by the last ones where there are threads for both
-  static constexpr int kValueThread = kKeyChunks + kValueChunks <= kThreads ? kThreads - kValueChunks : 0;
-};
-
-template <int D, int WAVES>
-struct __align__(16) TileBuffer {
-  using S = TileShape<D, WAVES>;
-  uint8_t k[kTileTokens * S::kKeyRow];
-  uint8_t v[D * S::kValueRow];
+  // eight waves, two a SIMD unit, share a tile's keys and values; heads of 256 channels leave registers for one
+  static constexpr int kWaves = D == 256 ? 4 : 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
+  static constexpr int kTokens = D == 256 ? 32 : 64, kUnits = kTokens / 32;
+  static constexpr int kKeyRow = D * 2 + 16, kValueRow = kTokens * 2 + 16;  // 16 bytes more: no two lanes' rows in one bank
+  static constexpr int kKeyBytes = kTokens * kKeyRow, kValueBytes = D * kValueRow;
+  static constexpr int kKeyBuffers = kUnits + 1;            // of the tiles whose scores are being computed, and the one written
+  static constexpr int kKeyChunks = kTokens * (D / 32);     // 32 channels of a token
+  static constexpr int kValueChunks = (kTokens / 4) * 16;   // 4 tokens of a sixteenth
+  // keys by the first threads, values by the last ones; where there are not threads for both, some do both
+  static constexpr bool kApart = kKeyChunks + kValueChunks <= kThreads;
+  static constexpr int kValueThread = kThreads - kValueChunks;
+  static_assert(kKeyChunks <= kThreads && kValueChunks <= kThreads, "one chunk a thread");
 };
 
 // What a thread fetches of a tile.
-template <int D, int WAVES>
+template <int D>
 struct Fetched {
-  using S = TileShape<D, WAVES>;
-  uint32_t k[S::kKeyTurns][4], ks[S::kKeyTurns];
-  uint32_t v[S::kValueTurns][D / 32], vs[S::kValueTurns];
+  using S = TileShape<D>;
+  uint32_t first[D / 32 > 4 ? D / 32 : 4], first_scale;
+  uint32_t second[S::kApart ? 1 : D / 32], second_scale;
+  __device__ __forceinline__ uint32_t (&keys())[4] { return reinterpret_cast<uint32_t(&)[4]>(first); }
+  __device__ __forceinline__ uint32_t (&values())[D / 32] {
+    if constexpr (S::kApart) return reinterpret_cast<uint32_t(&)[D / 32]>(first);
+    else return second;
+  }
+  __device__ __forceinline__ uint32_t& value_scale() {
+    if constexpr (S::kApart) return first_scale;
+    else return second_scale;
+  }
 };
 
-template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(TileArgs args) {
-  using S = TileShape<D, WAVES>;
+// A barrier for what is in LDS alone: loads from memory stay under way.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) void attention_tile_kernel(TileArgs args) {
+  using S = TileShape<D>;
   using L = Kv4<D>;
   const AttentionArgs& a = args.a;
-  __shared__ TileBuffer<D, WAVES> buffers[2];
-  __shared__ int found[2 * WAVES + 2];
+  __shared__ __align__(16) uint8_t key_buffers[S::kKeyBuffers][S::kKeyBytes];
+  __shared__ __align__(16) uint8_t value_buffers[2][S::kValueBytes];
+  __shared__ int found[2 * S::kWaves + 2];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads;
   const int tile = args.tiles - 1 - (int)blockIdx.x;  // a prompt's last tiles see the most: they go first
   const int head = blockIdx.y, split = blockIdx.z;
 
-  int s, place;
-  int64_t total = 0;
-  find_tile<S::kThreads>(a, tile, S::kRows, &s, &place, args.splits > 1 ? &total : nullptr, found);
-  if (s < 0) return;
-  const Sequence seq = sequence<true>(a, s);
+  const FoundTile own = find_tile<S::kThreads>(a, tile, S::kRows, args.splits > 1, found);
+  if (own.seq < 0) return;
+  const Sequence seq = sequence<true>(a, own.seq);
   const int queries = min(seq.count, a.max_queries), rows = queries * a.group, length = seq.length;
   const int new_from = length - seq.count;
-  const int row0 = place * S::kRows, last_row = min(row0 + S::kRows, rows) - 1;
+  const int row0 = own.place * S::kRows, last_row = min(row0 + S::kRows, rows) - 1;
 
   // ---- tokens that the tile's rows see, and this piece of them
   const int window = a.window > 0 ? a.window : 1 << 30;
@@ -849,23 +883,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
   auto begin_of = [&](int row) { return max(new_from + row / a.group + 1 - window, 0); };
   const int some_from = begin_of(row0);
   const Span span = span_of(a, seq, row0, last_row);
-  const int pieces = args.splits > 1 ? pieces_of_tile(args, span.to - span.from, total) : 1;
+  const int pieces = args.splits > 1 ? pieces_of_tile(args, span.to - span.from, own.total) : 1;
   if (split >= pieces) return;
   const int each = (span.to - span.from) / pieces, longer = (span.to - span.from) - each * pieces;
-  const int tile_from = span.from + split * each + min(split, longer), tile_to = tile_from + each + (split < longer ? 1 : 0);
+  const int span_from = span.from + split * each + min(split, longer);
+  const int tile_from = span_from * (kSpan / S::kTokens);
+  const int tile_to = (span_from + each + (split < longer ? 1 : 0)) * (kSpan / S::kTokens);
 
   // ---- this wave's rows
   const int row = row0 + wave * 32 + n, query = row / a.group, q_head = head * a.group + row - query * a.group;
   const int row_end = row < rows ? end_of(row) : 0, row_begin = row < rows ? begin_of(row) : 0;
   const int wave_row = row0 + wave * 32, wave_last = min(wave_row + 31, rows - 1);
   const bool idle = wave_row >= rows;
-  const int wave_to = idle ? 0 : end_of(wave_last), wave_from = idle ? 0 : begin_of(wave_row);
-  const int all_to = idle ? 0 : end_of(wave_row), all_from = idle ? 0 : begin_of(wave_last);
+  const int wave_to = uniform(idle ? 0 : end_of(wave_last)), wave_from = uniform(idle ? 0 : begin_of(wave_row));
+  const int all_to = uniform(idle ? 0 : end_of(wave_row)), all_from = uniform(idle ? 0 : begin_of(wave_last));
   half8_t q[D / 16];
   float scale;
   {
     const T* from = static_cast<const T*>(a.q) + (int64_t)(seq.first + query) * a.q_token + (int64_t)q_head * a.q_head + h * 8;
-    float most = 0.0f, back;
+    float most = 0.0f;
     float x[D / 16][8] = {};
     if (row < rows) {
 #pragma unroll
@@ -875,197 +911,311 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
     for (int c = 0; c < D / 16; ++c)
 #pragma unroll
       for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(x[c][j]));
-    most = fmaxf(most, __shfl_xor(most, 32));
-    const float up = lift_of(most, a.scale, &back);
+    const float up = lift_of(max32(most), a.scale, &scale);
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[c][j] = (_Float16)(x[c][j] * up);
-    scale = back;
   }
-  float m = -__builtin_inff(), l = 0.0f;
+  float m = -__builtin_inff(), l[4] = {};  // l: in four strands, so that no addition waits for the last
   float16_t o[D / 32];
 #pragma unroll
   for (int c = 0; c < D / 32; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
 
-  const ConstInts table = constant(a.block_table) + s * a.table_stride;
-  // The pages of a tile's four sixteens, fetched a tile before they are used; a missing one is -1.
+  // ---- Pages.  A lane holds the number of one sixteen's page, 1024 tokens in a wave; they are asked for tile by
+  // tile.  A missing page is -1, its tokens are read from page 0 and masked.
+  const int32_t* table = a.block_table + own.seq * a.table_stride;
+  constexpr int kSixteens = S::kTokens / 16, kTilesHeld = 64 / kSixteens;
   struct Pages {
     int a, b, c, d;
   };
-  auto page_of = [&](int at, int i) {
-    const int t = at * kTileTokens + i * 16;
-    return uniform(at < tile_to && t < length ? table[t >> a.pages.page_log2] : -1);
+  int held = -1;
+  auto pages_of = [&](int at) {
+    if (at % kTilesHeld == 0 || at == tile_from) {
+      const int64_t t = ((int64_t)(at / kTilesHeld) * 64 + lane) * 16;
+      const int id = t < length && t < (int64_t)tile_to * S::kTokens ? table[t >> a.pages.page_log2] : -1;
+      held = id < a.pages.num_pages ? max(id, -1) : -1;  // (used here, so that the wait for it is here too)
+    }
+    const int i = at % kTilesHeld * kSixteens;
+    auto one = [&](int j) { return j < kSixteens ? __builtin_amdgcn_readlane(held, i + j) : -1; };
+    return Pages{one(0), one(1), one(2), one(3)};
   };
-  auto pages_of = [&](int at) { return Pages{page_of(at, 0), page_of(at, 1), page_of(at, 2), page_of(at, 3)}; };
   auto missing_of = [&](const Pages& p) {  // a bit for each sixteen
-    auto bit = [&](int id, int b) { return id < 0 || id >= a.pages.num_pages ? b : 0; };
-    return bit(p.a, 1) | bit(p.b, 2) | bit(p.c, 4) | bit(p.d, 8);
+    const int first = (p.a < 0 ? 1 : 0) | (p.b < 0 ? 2 : 0);
+    return S::kTokens == 32 ? first : first | (p.c < 0 ? 4 : 0) | (p.d < 0 ? 8 : 0);
   };
-  // Base of the block that holds the tile's token `t`; tokens of a missing page are read from page 0 and masked.
-  auto block_of = [&](Pages pages, int missing, int t, bool* there) {
-    const int i = t >> 4;
-    const int a01 = i & 1 ? uniform(pages.b) : uniform(pages.a), a23 = i & 1 ? uniform(pages.d) : uniform(pages.c);
-    const int id = i & 2 ? a23 : a01;
-    *there = !(missing >> i & 1);
-    return a.pages.data + ((int64_t)(*there ? id : 0) * heads + head) * a.pages.head_bytes;
+  auto block_of = [&](int id) { return a.pages.data + ((int64_t)max(id, 0) * heads + head) * a.pages.head_bytes; };
+  // Base of the block that holds a thread's sixteen `i` of the tile: the same for all where a page holds the tile.
+  auto block_at = [&](const Pages& p, int i) {
+    const uint8_t* block = block_of(p.a);
+    if (P < S::kTokens) {
+      const uint8_t *b = block_of(p.b), *c = block_of(p.c), *d = block_of(p.d);
+      block = i == 1 ? b : block;
+      block = i == 2 ? c : block;
+      block = i == 3 ? d : block;
+    }
+    return block;
   };
-  auto fetch = [&](Fetched<D, WAVES>& f, const Pages& pages, int missing, int t0) {
+
+  // ---- this thread's chunks: 32 channels of a token, four tokens of a sixteenth of the channels
+  const int key_chunk = threadIdx.x, value_chunk = (int)threadIdx.x - S::kValueThread;
+  const bool has_keys = key_chunk < S::kKeyChunks, has_values = value_chunk >= 0;
+  const int key_token = key_chunk / (D / 32), key_group = key_chunk % (D / 32);
+  // of 32 neighbouring lanes two sixteenths and 16 fours of tokens: their LDS writes cover all banks
+  constexpr int kFours = S::kTokens / 4;
+  const int sixteenth = (value_chunk & 1) | (value_chunk / (2 * kFours) << 1), four = value_chunk >> 1 & (kFours - 1);
+  const int in_page = P - 1, key_at = key_token & in_page, value_at = four * 4 & in_page;
+  const int key_offset = L::key(key_at) + key_group * 16, key_scale_offset = L::key_scale(P, key_at, key_group);
+  const int value_offset = L::value(P, value_at, sixteenth);
+  const int value_scale_offset = L::value_scale(P, value_at, sixteenth * (D / 16) / 32);
+  const int key_place = key_token * S::kKeyRow + key_group * 64;
+  // fours 0, 1, 2, 3 of 16 tokens lie in the order 0, 2, 1, 3
+  const int value_place = sixteenth * (D / 16) * S::kValueRow + ((four & ~3) | (four & 1) << 1 | (four >> 1 & 1)) * 8;
+
+  Fetched<D> next;
+  auto fetch_keys = [&](const Pages& p, int at) {
+    if (!has_keys) return;
+    const uint8_t* block = block_at(p, key_token >> 4);
+    const int t = at * S::kTokens & in_page;  // (0 where pages are smaller than the tile)
+    load_words(next.keys(), block + (key_offset + t * L::kRow));
+    next.first_scale = block[key_scale_offset + t];
+  };
+  auto fetch_values = [&](const Pages& p, int at, int missing) {
+    if (!has_values) return;
+    const uint8_t* block = block_at(p, four >> 2);
+    const int t0 = at * S::kTokens, t = t0 & in_page;
+    load_words(next.values(), block + (value_offset + t * L::kRow));
+    next.value_scale() = *reinterpret_cast<const uint32_t*>(block + (value_scale_offset + t));
+    // what no row sees may hold anything, and nothing times zero has to be zero
+    if (t0 + S::kTokens > length || t0 < some_from || missing) {
 #pragma unroll
-    for (int i = 0; i < S::kKeyTurns; ++i) {
-      const int chunk = (int)threadIdx.x + i * S::kThreads;
-      if (S::kKeyChunks % S::kThreads == 0 || chunk < S::kKeyChunks) {
-        const int t = chunk / (D / 32), g = chunk % (D / 32), at = (t0 + t) & (P - 1);
-        bool there;
-        const uint8_t* b = block_of(pages, missing, t, &there);
-        load_words(f.k[i], b + (L::key(at) + g * 16));
-        f.ks[i] = b[L::key_scale(P, at, g)];
+      for (int j = 0; j < 4; ++j) {
+        const int token = t0 + four * 4 + j;
+        if (token >= length || token < some_from || missing >> (four >> 2) & 1)
+          next.value_scale() = (next.value_scale() & ~(255u << (8 * j))) | 127u << (8 * j);
       }
     }
-#pragma unroll
-    for (int i = 0; i < S::kValueTurns; ++i) {
-      const int chunk = (int)threadIdx.x - S::kValueThread + i * S::kThreads;
-      if (S::kValueChunks % S::kThreads == 0 || (chunk >= 0 && chunk < S::kValueChunks)) {
-        // of 32 neighbouring lanes two sixteenths and all 16 fours of tokens: their LDS writes cover all banks
-        const int sixteenth = (chunk & 1) | (chunk >> 5 << 1), t = (chunk >> 1 & 15) * 4, at = (t0 + t) & (P - 1);
-        bool there;
-        const uint8_t* b = block_of(pages, missing, t, &there);
-        load_words(f.v[i], b + L::value(P, at, sixteenth));
-        uint32_t vs = *reinterpret_cast<const uint32_t*>(b + L::value_scale(P, at, sixteenth * (D / 16) / 32));
-        // what no row sees may hold anything, and nothing times zero has to be zero
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (!there || t0 + t + j >= length || t0 + t + j < some_from) vs = (vs & ~(255u << (8 * j))) | 127u << (8 * j);
-        f.vs[i] = vs;
-      }
-    }
   };
-  auto spread = [&](const Fetched<D, WAVES>& f, TileBuffer<D, WAVES>& to) {
+  auto spread_keys = [&](uint8_t* to) {
+    if (!has_keys) return;
+    const float ks = __uint_as_float(next.first_scale << 23);
 #pragma unroll
-    for (int i = 0; i < S::kKeyTurns; ++i) {
-      const int chunk = (int)threadIdx.x + i * S::kThreads;
-      if (S::kKeyChunks % S::kThreads == 0 || chunk < S::kKeyChunks) {
-        uint8_t* at = to.k + chunk / (D / 32) * S::kKeyRow + chunk % (D / 32) * 64;
-        const float ks = __uint_as_float(f.ks[i] << 23);
+    for (int w = 0; w < 4; ++w) *reinterpret_cast<half8_t*>(to + key_place + w * 16) = eight_values(next.keys()[w], ks);
+  };
+  auto spread_values = [&](uint8_t* to) {
+    if (!has_values) return;
+    float vs[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) *reinterpret_cast<half8_t*>(at + w * 16) = eight_values(f.k[i][w], ks);
+    for (int j = 0; j < 4; ++j) vs[j] = __uint_as_float((next.value_scale() >> (8 * j) & 255) << 23);
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b) {  // byte b of each token: two channels
+      half2_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int byte = j * (D / 32) + b;
+        const uint32_t w = next.values()[byte / 4];
+        x[j] = byte % 4 == 0 ? two_values<0>(w, vs[j]) : byte % 4 == 1 ? two_values<1>(w, vs[j])
+             : byte % 4 == 2 ? two_values<2>(w, vs[j]) : two_values<3>(w, vs[j]);
       }
-    }
+      typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int i = 0; i < S::kValueTurns; ++i) {
-      const int chunk = (int)threadIdx.x - S::kValueThread + i * S::kThreads;
-      if (S::kValueChunks % S::kThreads == 0 || (chunk >= 0 && chunk < S::kValueChunks)) {
-        const int sixteenth = (chunk & 1) | (chunk >> 5 << 1), four = chunk >> 1 & 15;
-        // fours 0, 1, 2, 3 of 16 tokens lie in the order 0, 2, 1, 3
-        uint8_t* at = to.v + sixteenth * (D / 16) * S::kValueRow +
-                      ((four & ~3) | (four & 1) << 1 | (four >> 1 & 1)) * 8;
-        float vs[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vs[j] = __uint_as_float((f.vs[i] >> (8 * j) & 255) << 23);
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) {  // byte b of each token: two channels
-          half2_t x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int byte = j * (D / 32) + b;
-            const uint32_t w = f.v[i][byte / 4];
-            x[j] = byte % 4 == 0 ? two_values<0>(w, vs[j]) : byte % 4 == 1 ? two_values<1>(w, vs[j])
-                 : byte % 4 == 2 ? two_values<2>(w, vs[j]) : two_values<3>(w, vs[j]);
-          }
-          typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            *reinterpret_cast<half4_t*>(at + (2 * b + c) * S::kValueRow) = half4_t{x[0][c], x[1][c], x[2][c], x[3][c]};
-        }
-      }
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<half4_t*>(to + value_place + (2 * b + c) * S::kValueRow) = half4_t{x[0][c], x[1][c], x[2][c], x[3][c]};
     }
   };
 
-  Fetched<D, WAVES> next;
-  Pages pages = pages_of(tile_from);
-  int missing = missing_of(pages), missing_next = 0, missing_after = 0;  // of this tile, the next, the one after
-  if (tile_from < tile_to) {
-    fetch(next, pages, missing, tile_from * kTileTokens);
-    pages = pages_of(tile_from + 1);
-    spread(next, buffers[0]);
-    missing_next = missing_of(pages);
-    if (tile_from + 1 < tile_to) fetch(next, pages, missing_next, (tile_from + 1) * kTileTokens);
-    pages = pages_of(tile_from + 2);
-  }
-  __syncthreads();
-  for (int at = tile_from; at < tile_to; ++at) {
-    const TileBuffer<D, WAVES>& now = buffers[(at - tile_from) & 1];
-    const int t0 = at * kTileTokens;
-    if (at + 1 < tile_to) spread(next, buffers[(at - tile_from + 1) & 1]);
-    missing_after = missing_of(pages);
-    if (at + 2 < tile_to) fetch(next, pages, missing_after, t0 + 2 * kTileTokens);
-    pages = pages_of(at + 3);
-    if (t0 < wave_to && t0 + kTileTokens > wave_from) {
-      float16_t sc[2];
+  // ---- a unit of 32 tokens
+  auto key = [&](const uint8_t* keys, int c) {
+    return *reinterpret_cast<const half8_t*>(keys + n * S::kKeyRow + h * 16 + c * 32);
+  };
+  auto scores = [&](float16_t& sc, const uint8_t* keys) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 16; ++j) sc[j] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sc[i][j] = 0.0f;
+    for (int c = 0; c < D / 16; ++c) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(keys, c), q[c], sc, 0, 0, 0);
+  };
+  auto mask = [&](float16_t& sc, int t0, int missing) {  // missing: of the unit's two sixteens
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const half8_t k = *reinterpret_cast<const half8_t*>(now.k + (i * 32 + n) * S::kKeyRow + c * 32 + h * 16);
-          sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[c], sc[i], 0, 0, 0);
-        }
-      const bool whole = t0 >= all_from && t0 + kTileTokens <= all_to && missing == 0;
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int t = t0 + i * 32 + (j / 4) * 8 + h * 4 + j % 4;
-            if (t >= row_end || t < row_begin || missing >> (i * 2 + j / 8) & 1) sc[i][j] = -__builtin_inff();
-          }
-      }
-      float most = -__builtin_inff();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) most = fmaxf(most, sc[i][j]);
-      most = fmaxf(most, __shfl_xor(most, 32)) * scale;
-      if (__builtin_amdgcn_ballot_w64(most > m)) {
-        const float higher = fmaxf(m, most);
-        const float old = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
-        m = higher;
-        l *= old;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) o[c] *= old;
-      }
-      const float add = kLift - (m == -__builtin_inff() ? 0.0f : m);
-      half8_t p[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][j], scale, add));
-          l += x;
-          p[i * 2 + j / 8][j % 8] = (_Float16)x;
-        }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          const half8_t v = *reinterpret_cast<const half8_t*>(now.v + (c * 32 + n) * S::kValueRow + k * 32 + h * 16);
-          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[k], o[c], 0, 0, 0);
-        }
+    for (int j = 0; j < 16; ++j) {
+      const int t = t0 + (j / 4) * 8 + h * 4 + j % 4;
+      if (t >= row_end || t < row_begin || missing >> (j / 8) & 1) sc[j] = -__builtin_inff();
     }
-    missing = missing_next;
-    missing_next = missing_after;
-    __syncthreads();
+  };
+  auto largest = [&](const float16_t& sc) {
+    float most[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most[j] = fmaxf(fmaxf(sc[j], sc[j + 4]), fmaxf(sc[j + 8], sc[j + 12]));
+    return max32(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * scale;
+  };
+  // LDS is read kAhead products before the product, the first keys of a unit in the unit before it.
+  constexpr int kProducts = D / 16, kAhead = 4;
+  auto value = [&](const uint8_t* values, int z) {
+    return *reinterpret_cast<const half8_t*>(values + (z % (D / 32) * 32 + n) * S::kValueRow + h * 16 + z / (D / 32) * 32);
+  };
+  half8_t ahead[kAhead];
+  auto first_keys = [&](const uint8_t* keys) {
+#pragma unroll
+    for (int z = 0; z < kAhead; ++z) ahead[z] = key(keys, z);
+  };
+  // The next unit's scores and the present probabilities, product by product: each with its share of the 16
+  // exponentials, whose sums and roundings come one product later.
+  auto scores_beside_probabilities = [&](float16_t& sc_next, const uint8_t* keys, const uint8_t* values, half8_t (&p)[2],
+                                         const float16_t& sc, float add) {
+    constexpr int kEach = 16 / kProducts;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sc_next[j] = 0.0f;
+    float x[kEach];
+#pragma unroll
+    for (int z = 0; z <= kProducts; ++z) {
+      float last[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) last[e] = x[e];
+      if (z < kProducts) {
+        sc_next = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], q[z], sc_next, 0, 0, 0);
+        ahead[z % kAhead] = z + kAhead < kProducts ? key(keys, z + kAhead) : value(values, z + kAhead - kProducts);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[z * kEach + e], scale, add));
+      }
+      if (z > 0) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int i = (z - 1) * kEach + e;
+          l[i % 4] += last[e];
+          p[i / 8][i % 8] = (_Float16)last[e];
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // The present products with the values, the next unit's maximum among them once its scores are there.
+  auto gather_beside_largest = [&](const half8_t (&p)[2], const uint8_t* values, const uint8_t* keys_after,
+                                   const float16_t& sc_next) {
+    float most[4];
+#pragma unroll
+    for (int z = 0; z < kProducts; ++z) {
+      o[z % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], p[z / (D / 32)], o[z % (D / 32)], 0, 0, 0);
+      ahead[z % kAhead] = z + kAhead < kProducts ? value(values, z + kAhead) : key(keys_after, z + kAhead - kProducts);
+      if (z >= kProducts / 2) {
+        constexpr int kEach = kProducts >= 8 ? 1 : 2, kFrom = kProducts / 2;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int j = (z - kFrom) * kEach + e;
+          if (j < 4) most[j] = fmaxf(fmaxf(sc_next[j], sc_next[j + 4]), fmaxf(sc_next[j + 8], sc_next[j + 12]));
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return max32(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * scale;
+  };
+  auto sees = [&](int t0) { return t0 < min(wave_to, tile_to * S::kTokens) && t0 + 32 > wave_from; };
+  auto all_see = [&](int t0, int missing) { return t0 >= all_from && t0 + 32 <= all_to && (missing & 3) == 0; };
+
+  float most = -__builtin_inff();  // of the unit that comes next
+  // The unit of tokens t0 .. t0 + 31, whose scores are there; the scores of the next come.
+  auto work_on = [&](int t0, float16_t& sc, float16_t& sc_next, const uint8_t* keys_next, const uint8_t* keys_after,
+                     const uint8_t* values, int missing_next) {
+    const int t1 = t0 + 32;
+    const bool mine = sees(t0), mine_next = sees(t1);
+    if (!mine && !mine_next) {
+      first_keys(keys_after);
+      return;
+    }
+    if (__builtin_amdgcn_ballot_w64(most > m)) {
+      const float higher = fmaxf(m, most);
+      const float old = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
+      m = higher;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[j] *= old;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) o[c] *= old;
+    }
+    const float add = kLift - (m == -__builtin_inff() ? 0.0f : m);
+    half8_t p[2];
+    scores_beside_probabilities(sc_next, keys_next, values, p, sc, add);
+    // (the probabilities stay before the branch)
+    asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l[0]), "+v"(l[1]), "+v"(l[2]), "+v"(l[3]));
+    if (!mine_next || !all_see(t1, missing_next)) mask(sc_next, mine_next ? t1 : 1 << 30, missing_next);
+    most = gather_beside_largest(p, values, keys_after, sc_next);
+  };
+
+  // ---- While tile `at` is worked on, its keys and values and the next tile's keys are in LDS.  Keys are laid out
+  // two tiles ahead and values one, and fetched one tile before that.
+  uint8_t *keys_now = key_buffers[0], *keys_next = key_buffers[1], *keys_later = key_buffers[S::kKeyBuffers - 1];
+  float16_t even, odd;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) even[j] = odd[j] = -__builtin_inff();  // of a unit that the wave does not see
+  Pages pages_now = pages_of(tile_from), pages_next = pages_of(tile_from + 1), pages_later = pages_of(tile_from + 2);
+  int missing0 = missing_of(pages_now), missing1 = missing_of(pages_next), missing2 = missing_of(pages_later);
+  if (tile_from < tile_to) {
+    fetch_values(pages_now, tile_from, missing0);
+    if constexpr (S::kApart) {
+      fetch_keys(pages_now, tile_from);
+      spread_keys(keys_now);
+      spread_values(value_buffers[0]);
+    } else {
+      spread_values(value_buffers[0]);
+      fetch_keys(pages_now, tile_from);
+      spread_keys(keys_now);
+    }
+    if (tile_from + 1 < tile_to) {
+      fetch_keys(pages_next, tile_from + 1);
+      spread_keys(keys_next);
+      fetch_values(pages_next, tile_from + 1, missing1);
+    }
+    if (tile_from + 2 < tile_to) fetch_keys(pages_later, tile_from + 2);
+    pages_next = pages_later;
+    pages_later = pages_of(tile_from + 3);
   }
-  l += __shfl_xor(l, 32);
+  lds_barrier();
+  if (tile_from < tile_to && sees(tile_from * S::kTokens)) {
+    scores(even, keys_now);
+    if (!all_see(tile_from * S::kTokens, missing0)) mask(even, tile_from * S::kTokens, missing0);
+    most = largest(even);
+  }
+  // (with two key buffers the first keys are written over from here on)
+  if constexpr (S::kKeyBuffers == 2) lds_barrier();
+  // Keys of the unit after next, whatever is there where there is none: they are read and not used.
+  first_keys(S::kUnits == 2 ? keys_now + 32 * S::kKeyRow : keys_next);
+  auto advance = [&](int at, float16_t& first, float16_t& second) {
+    const int t0 = at * S::kTokens;
+    const uint8_t* values = value_buffers[(at - tile_from) & 1];
+    if constexpr (S::kUnits == 2) {
+      const uint8_t *second_now = keys_now + 32 * S::kKeyRow, *second_next = keys_next + 32 * S::kKeyRow;
+      work_on(t0, first, second, second_now, keys_next, values, missing0 >> 2);
+      work_on(t0 + 32, second, first, keys_next, second_next, values + 64, missing1);
+    } else {
+      // (the keys after next are being written where the present ones were: read behind the barrier)
+      work_on(t0, first, second, keys_next, keys_next, values, missing1);
+    }
+    uint8_t* const write = S::kUnits == 2 ? keys_later : keys_now;
+    if (at + 2 < tile_to) spread_keys(write);
+    if (at + 1 < tile_to) spread_values(value_buffers[(at - tile_from + 1) & 1]);
+    if (at + 3 < tile_to) fetch_keys(pages_later, at + 3);
+    if (at + 2 < tile_to) fetch_values(pages_next, at + 2, missing2);
+    pages_next = pages_later;
+    missing0 = missing1;
+    missing1 = missing2;
+    missing2 = missing_of(pages_later);
+    pages_later = pages_of(at + 4);
+    keys_later = keys_now;
+    keys_now = keys_next;
+    keys_next = write;
+    lds_barrier();
+    if constexpr (S::kUnits == 1) first_keys(keys_next);
+  };
+  for (int at = tile_from; at < tile_to; at += 3 - S::kUnits) {
+    advance(at, even, odd);
+    if (S::kUnits == 1 && at + 1 < tile_to) advance(at + 1, odd, even);
+  }
+  const Both sums = across32((l[0] + l[1]) + (l[2] + l[3]));
+  const float sum = sums.a + sums.b;
   if (row >= rows) return;
   if (pieces == 1) {
     T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
@@ -1080,61 +1230,79 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_tile_kernel(T
         *reinterpret_cast<float4_t*>(part + c * 32 + i * 2 + h * 4) = float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]};
     if (h == 0) {
       part[D] = m;
-      part[D + 1] = l;
+      part[D + 1] = sum;
     }
   }
 }
 
-// Joins the pieces of a tile's rows: a wave takes one row.
-template <typename T, int D, int WAVES>
+// Joins the pieces of a tile's rows: a block takes kJoinRows of them, D / 4 lanes a row, and has the first two
+// pieces of all its rows under way at once.
+constexpr int kJoinRows = 32;
+
+template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args) {
-  using S = TileShape<D, WAVES>;
+  using S = TileShape<D>;
   const AttentionArgs& a = args.a;
   __shared__ int found[2 * 4 + 2];
-  const int tile = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63;
-  int s, place;
-  int64_t total;
-  find_tile<256>(a, tile, S::kRows, &s, &place, &total, found);
-  if (s < 0) return;
-  const Sequence seq = sequence<true>(a, s);
-  const int rows = min(seq.count, a.max_queries) * a.group;
-  const int in_tile = blockIdx.z * 4 + (threadIdx.x >> 6), row = place * S::kRows + in_tile;
-  const Span span = span_of(a, seq, place * S::kRows, min((place + 1) * S::kRows, rows) - 1);
-  const int pieces = pieces_of_tile(args, span.to - span.from, total);
-  if (row >= rows || pieces == 1) return;
-  const float* part = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows + in_tile) * (D + 4);
+  const int tile = blockIdx.x, head = blockIdx.y;
+  const FoundTile own = find_tile<256>(a, tile, S::kRows, true, found);
+  if (own.seq < 0) return;
+  const Sequence seq = sequence<true>(a, own.seq);
+  const int rows = min(seq.count, a.max_queries) * a.group, row0 = own.place * S::kRows;
+  const Span span = span_of(a, seq, row0, min(row0 + S::kRows, rows) - 1);
+  const int pieces = pieces_of_tile(args, span.to - span.from, own.total);
+  if (pieces == 1) return;
+  constexpr int kLanes = D / 4, kAtOnce = 256 / kLanes, kTurns = kJoinRows / kAtOnce;
+  const int lane = threadIdx.x % kLanes, first = blockIdx.z * kJoinRows + threadIdx.x / kLanes;
   const int64_t stride = (int64_t)S::kRows * (D + 4);
-  float m = -__builtin_inff(), l = 0.0f, o[D / 64] = {};
-  for (int c = 0; c < pieces; ++c) m = fmaxf(m, part[c * stride + D]);
-#pragma unroll 4
-  for (int c = 0; c < pieces; ++c) {
-    const float* p = part + c * stride;
-    const float weight = p[D] == m ? 1.0f : __builtin_amdgcn_exp2f(p[D] - m);
-    l += p[D + 1] * weight;
+  const float* base = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows) * (D + 4);
+  float4_t x[kTurns][2];
+  float2 ml[kTurns][2];
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k) o[k] += p[k * 64 + lane] * weight;
+  for (int k = 0; k < kTurns; ++k)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      // (rows behind the last are not written, but they are there)
+      const float* p = base + c * stride + (int64_t)(first + k * kAtOnce) * (D + 4);
+      x[k][c] = *reinterpret_cast<const float4_t*>(p + lane * 4);
+      ml[k][c] = *reinterpret_cast<const float2*>(p + D);
+    }
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    const int in_tile = first + k * kAtOnce, row = row0 + in_tile;
+    if (row >= rows) continue;
+    float m = fmaxf(ml[k][0].x, ml[k][1].x);
+    float w0 = ml[k][0].x == m ? 1.0f : __builtin_amdgcn_exp2f(ml[k][0].x - m);
+    float w1 = ml[k][1].x == m ? 1.0f : __builtin_amdgcn_exp2f(ml[k][1].x - m);
+    float l = ml[k][0].y * w0 + ml[k][1].y * w1;
+    float4_t o = x[k][0] * w0 + x[k][1] * w1;
+    for (int c = 2; c < pieces; ++c) {
+      const float* p = base + c * stride + (int64_t)in_tile * (D + 4);
+      const float2 more = *reinterpret_cast<const float2*>(p + D);
+      const float higher = fmaxf(m, more.x);
+      w0 = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
+      w1 = more.x == higher ? 1.0f : __builtin_amdgcn_exp2f(more.x - higher);
+      m = higher;
+      l = l * w0 + more.y * w1;
+      o = o * w0 + *reinterpret_cast<const float4_t*>(p + lane * 4) * w1;
+    }
+    const int query = row / a.group;
+    T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token +
+             (int64_t)(head * a.group + row - query * a.group) * a.out_head + lane * 4;
+    store4(out, o * (l > 0.0f || l != l ? 1.0f / l : 0.0f), a.out_wide);
   }
-  const int query = row / a.group;
-  T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token +
-           (int64_t)(head * a.group + row - query * a.group) * a.out_head;
-#pragma unroll
-  for (int k = 0; k < D / 64; ++k) out[k * 64 + lane] = (T)(l > 0.0f || l != l ? o[k] / l : 0.0f);
 }
 
 // Tiles and pieces of a call.
 struct TilePlan {
-  int waves, tiles, splits, budget;
+  int tiles, splits, budget;
   int64_t bytes;
 };
-
-// Eight waves, two a SIMD unit, share a tile's keys and values; heads of 256 channels leave registers for one.
-int tile_waves(int head_size) { return head_size == 256 ? 4 : 8; }
 
 TilePlan plan_tiles(int64_t T, int group, int kv_heads, int head_size, int64_t num_seqs, int64_t max_queries,
                     int64_t table_width, int page_size) {
   TilePlan plan;
-  plan.waves = tile_waves(head_size);
-  const int64_t rows = 32 * plan.waves;
+  const int64_t rows = head_size == 256 ? TileShape<256>::kRows : TileShape<128>::kRows;
   // every sequence may leave one tile that is not full
   const int64_t tiles = min((T * group + rows - 1) / rows + num_seqs, num_seqs * ((max_queries * group + rows - 1) / rows));
   const int cus = device_compute_units();
@@ -1148,23 +1316,23 @@ TilePlan plan_tiles(int64_t T, int group, int kv_heads, int head_size, int64_t n
   return plan;
 }
 
-template <typename T, int D, int WAVES>
+template <typename T, int D>
 int launch_tiles(const TileArgs& args, void* stream) {
   const unsigned heads = (unsigned)args.a.pages.heads;
-  launch_kernel(attention_tile_kernel<T, D, WAVES>, dim3((unsigned)args.tiles, heads, (unsigned)args.splits),
-                dim3(64 * WAVES), 0, static_cast<hipStream_t>(stream), args);
+  launch_kernel(attention_tile_kernel<T, D>, dim3((unsigned)args.tiles, heads, (unsigned)args.splits),
+                dim3(TileShape<D>::kThreads), 0, static_cast<hipStream_t>(stream), args);
   int rc = finish_launch("kv4_attention");
   if (rc != TW_OK || args.splits == 1) return rc;
-  launch_kernel(attention_join_tile_kernel<T, D, WAVES>, dim3((unsigned)args.tiles, heads, 32 * WAVES / 4), dim3(256), 0,
+  launch_kernel(attention_join_tile_kernel<T, D>, dim3((unsigned)args.tiles, heads, TileShape<D>::kRows / kJoinRows), dim3(256), 0,
                 static_cast<hipStream_t>(stream), args);
   return finish_launch("kv4_attention");
 }
 
 template <typename T>
 int launch_tiles(const TileArgs& args, int D, void* stream) {
-  if (D == 64) return launch_tiles<T, 64, 8>(args, stream);
-  if (D == 128) return launch_tiles<T, 128, 8>(args, stream);
-  return launch_tiles<T, 256, 4>(args, stream);
+  if (D == 64) return launch_tiles<T, 64>(args, stream);
+  if (D == 128) return launch_tiles<T, 128>(args, stream);
+  return launch_tiles<T, 256>(args, stream);
 }
 
 bool wide_rows(const tw_heads* h) {
