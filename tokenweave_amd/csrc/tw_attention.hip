@@ -743,10 +743,19 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kSpan = 64;  // tokens in which tiles are measured and cut
 
+// Of a tile's key head that is worked on in even shares: whose rows they are, and the workgroups from `first` to
+// `last` that hold parts of it.
+struct TileHeader {
+  int32_t seq, row0, head, first, last;
+};
+
 struct TileArgs {
   AttentionArgs a;
-  float* parts;  // of up to `splits` pieces of every tile's tokens: [tile][head][split][rows][D + 4]
-  int tiles, splits, budget;
+  // Even shares: one header for each tile and key head, and two parts a workgroup, [rows][D + 4]: of the tile that
+  // it ends and of the one that it begins.  Null: a workgroup for each tile and key head.
+  TileHeader* headers;
+  float* parts;
+  int tiles;
 };
 
 // Tokens that the rows [row, last] of a sequence see, in spans: [from, to).
@@ -759,61 +768,51 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, const Sequence& 
   return {from, max((min(new_from + last / a.group + 1, q.length) + kSpan - 1) / kSpan, from)};
 }
 
-// Pieces of a tile of `count` spans: none longer than an even share of all tiles' spans over the budget, none
-// shorter than 256 tokens.
-__device__ __forceinline__ int pieces_of_tile(const TileArgs& args, int count, int64_t total) {
-  const int share = max((int)((total + args.budget - 1) / args.budget), 256 / kSpan);
-  return min(max((count + share - 1) / share, 1), args.splits);
+constexpr int kMostShared = 1024;  // tiles times key heads that are worked on in even shares
+
+// Sum over the workgroup's threads before this one, and over all.
+template <int THREADS>
+__device__ __forceinline__ int block_scan(int x, int* total, int* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sum = wave_scan(x);
+  __syncthreads();
+  if (lane == 63) lds[wave] = sum;
+  __syncthreads();
+  int before = sum - x, all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const int y = lds[w];
+    before += w < wave ? y : 0;
+    all += y;
+  }
+  *total = all;
+  return before;
 }
 
-// Whose tile it is and its place there (uniform); a tile behind the last: seq < 0.  `total`, where it is asked for:
-// the spans of all tiles of all key heads, a sequence's taken to grow evenly from its first tile to its last.
+__device__ __forceinline__ int tiles_in(const AttentionArgs& a, const Sequence& q, int rows_of_tile) {
+  return (min(q.count, a.max_queries) * a.group + rows_of_tile - 1) / rows_of_tile;
+}
+
+// Whose tile it is and its place there (uniform); a tile behind the last: seq < 0.
 struct FoundTile {
   int seq, place;
-  int64_t total;
 };
 template <int THREADS>
-__device__ __forceinline__ FoundTile find_tile(const AttentionArgs& a, int tile, int rows_of_tile, bool total, int* lds) {
-  constexpr int kW = THREADS / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x == 0) lds[kW] = -1;
+__device__ __forceinline__ FoundTile find_tile(const AttentionArgs& a, int tile, int rows_of_tile, int* lds) {
+  int* const found = lds + THREADS / 64;
+  if (threadIdx.x == 0) found[0] = -1;
   int base = 0;
-  int64_t spans = 0;
-  for (int s0 = 0; s0 < a.num_seqs; s0 += THREADS) {
-    const int s = s0 + threadIdx.x;
-    int count = 0, span = 0;
-    if (s < a.num_seqs) {
-      const Sequence q = sequence(a, s);
-      const int rows = min(q.count, a.max_queries) * a.group;
-      count = (rows + rows_of_tile - 1) / rows_of_tile;
-      if (total && count > 0) {
-        const Span first = span_of(a, q, 0, min(rows_of_tile, rows) - 1);
-        const Span last = span_of(a, q, (count - 1) * rows_of_tile, rows - 1);
-        span = (int)min((int64_t)count * (first.to - first.from + last.to - last.from) / 2, (int64_t)1 << 24);
-      }
-    }
-    const int sum = wave_scan(count);
-    if (total) span = wave_scan(span);
-    __syncthreads();
-    if (lane == 63) {
-      lds[wave] = sum;
-      lds[kW + 2 + wave] = span;
-    }
-    __syncthreads();
-    int before = base + sum - count;
-    for (int w = 0; w < kW; ++w) {
-      before += w < wave ? lds[w] : 0;
-      base += lds[w];
-      spans += total ? lds[kW + 2 + w] : 0;
-    }
+  for (int s0 = 0; s0 < a.num_seqs && base <= tile; s0 += THREADS) {
+    const int s = s0 + threadIdx.x, count = s < a.num_seqs ? tiles_in(a, sequence(a, s), rows_of_tile) : 0;
+    int all;
+    const int before = base + block_scan<THREADS>(count, &all, lds);
     if (tile >= before && tile < before + count) {
-      lds[kW] = s;
-      lds[kW + 1] = tile - before;
+      found[0] = s;
+      found[1] = tile - before;
     }
-    if (base > tile && !total) break;
+    base += all;
   }
   __syncthreads();
-  return {uniform(lds[kW]), uniform(lds[kW + 1]), spans * a.pages.heads};
+  return {uniform(found[0]), uniform(found[1])};
 }
 
 template <int D>
@@ -863,32 +862,110 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
   const AttentionArgs& a = args.a;
   __shared__ __align__(16) uint8_t key_buffers[S::kKeyBuffers][S::kKeyBytes];
   __shared__ __align__(16) uint8_t value_buffers[2][S::kValueBytes];
-  __shared__ int found[2 * S::kWaves + 2];
+  __shared__ int scan[S::kWaves + 2];
+  __shared__ int first_tile[kMostShared + 1], unit_end[kMostShared];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads;
-  const int tile = args.tiles - 1 - (int)blockIdx.x;  // a prompt's last tiles see the most: they go first
-  const int head = blockIdx.y, split = blockIdx.z;
+  const int window = a.window > 0 ? a.window : 1 << 30;
 
-  const FoundTile own = find_tile<S::kThreads>(a, tile, S::kRows, args.splits > 1, found);
-  if (own.seq < 0) return;
+  // ---- Which tiles: one, or an even share of all tiles' spans.  In the order of the shares a long tile of a prompt
+  // and a short one take turns: the last, the first, the last but one, ...
+  const bool shared = args.headers != nullptr;
+  int tiles = 0, units = 0, share = 1, unit = 0, at = 0, end = 1;
+  if (shared) {
+    for (int s0 = 0; s0 < a.num_seqs; s0 += S::kThreads) {
+      const int s = s0 + threadIdx.x, count = s < a.num_seqs ? tiles_in(a, sequence(a, s), S::kRows) : 0;
+      int all;
+      const int before = block_scan<S::kThreads>(count, &all, scan);
+      if (s < a.num_seqs) first_tile[s] = tiles + before;
+      tiles += all;
+    }
+    if (threadIdx.x == 0) first_tile[a.num_seqs] = tiles;
+    __syncthreads();
+    tiles = min(tiles, args.tiles);  // (more only where query_starts does not rise)
+    units = tiles * heads;
+  }
+  auto find = [&](int unit) {  // the tile of a unit of the shares
+    const int k = unit / heads, tile = k & 1 ? k >> 1 : tiles - 1 - (k >> 1);
+    int low = 0, high = a.num_seqs;  // the last sequence whose first tile is not behind it
+    while (high - low > 1) {
+      const int middle = (low + high) >> 1;
+      if (first_tile[middle] <= tile) low = middle;
+      else high = middle;
+    }
+    return FoundTile{low, tile - first_tile[low]};
+  };
+  auto span_in = [&](const Sequence& seq, int row0) {
+    return span_of(a, seq, row0, min(row0 + S::kRows, min(seq.count, a.max_queries) * a.group) - 1);
+  };
+  if (shared) {
+    int total = 0;
+    for (int u0 = 0; u0 < units; u0 += S::kThreads) {
+      const int u = u0 + threadIdx.x;
+      int count = 0, all;
+      if (u < units) {
+        const FoundTile own = find(u);
+        const Span span = span_in(sequence(a, own.seq), own.place * S::kRows);
+        count = max(span.to - span.from, 1);
+      }
+      const int before = total + block_scan<S::kThreads>(count, &all, scan);
+      if (u < units) unit_end[u] = before + count;
+      total += all;
+    }
+    __syncthreads();
+    // headers that no tile has
+    for (int u = units + blockIdx.x * S::kThreads + threadIdx.x; u < args.tiles * heads; u += gridDim.x * S::kThreads)
+      args.headers[u] = TileHeader{0, 0, 0, 0, 0};
+    share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+    at = blockIdx.x * share;
+    end = min(at + share, total);
+    if (at >= end) return;
+    int low = -1, high = units - 1;  // the first unit that ends behind `at`
+    while (high - low > 1) {
+      const int middle = (low + high) >> 1;
+      if (unit_end[middle] > at) high = middle;
+      else low = middle;
+    }
+    unit = uniform(high);
+  }
+
+  for (; at < end; ++unit) {
+  FoundTile own;
+  int head = blockIdx.y;
+  if (shared) {
+    own = find(unit);
+    own = {uniform(own.seq), uniform(own.place)};
+    head = unit - unit / heads * heads;
+  } else {
+    // a prompt's last tiles see the most: they go first
+    own = find_tile<S::kThreads>(a, args.tiles - 1 - (int)blockIdx.x, S::kRows, scan);
+    if (own.seq < 0) return;
+  }
   const Sequence seq = sequence<true>(a, own.seq);
   const int queries = min(seq.count, a.max_queries), rows = queries * a.group, length = seq.length;
   const int new_from = length - seq.count;
-  const int row0 = own.place * S::kRows, last_row = min(row0 + S::kRows, rows) - 1;
+  const int row0 = own.place * S::kRows;
 
-  // ---- tokens that the tile's rows see, and this piece of them
-  const int window = a.window > 0 ? a.window : 1 << 30;
+  // ---- tokens that the tile's rows see, and this share of them
   auto end_of = [&](int row) { return min(new_from + row / a.group + 1, length); };
   auto begin_of = [&](int row) { return max(new_from + row / a.group + 1 - window, 0); };
   const int some_from = begin_of(row0);
-  const Span span = span_of(a, seq, row0, last_row);
-  const int pieces = args.splits > 1 ? pieces_of_tile(args, span.to - span.from, own.total) : 1;
-  if (split >= pieces) return;
-  const int each = (span.to - span.from) / pieces, longer = (span.to - span.from) - each * pieces;
-  const int span_from = span.from + split * each + min(split, longer);
-  const int tile_from = span_from * (kSpan / S::kTokens);
-  const int tile_to = (span_from + each + (split < longer ? 1 : 0)) * (kSpan / S::kTokens);
+  Span span = span_in(seq, row0);
+  bool starts = true, ends = true;
+  if (shared) {
+    const int count = max(span.to - span.from, 1), unit_from = uniform(unit_end[unit]) - count;
+    starts = at == unit_from;
+    ends = unit_from + count <= end;
+    const int first = at - unit_from, last = min(end - unit_from, count);
+    if (starts && threadIdx.x == 0)
+      args.headers[unit] = TileHeader{own.seq, row0, head, (int)blockIdx.x, (unit_from + count - 1) / share};
+    at = unit_from + last;
+    span = {min(span.from + first, span.to), min(span.from + last, span.to)};
+  } else {
+    at = end;
+  }
+  const int tile_from = span.from * (kSpan / S::kTokens), tile_to = span.to * (kSpan / S::kTokens);
 
   // ---- this wave's rows
   const int row = row0 + wave * 32 + n, query = row / a.group, q_head = head * a.group + row - query * a.group;
@@ -1212,8 +1289,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
   }
   const Both sums = across32((l[0] + l[1]) + (l[2] + l[3]));
   const float sum = sums.a + sums.b;
-  if (row >= rows) return;
-  if (pieces == 1) {
+  if (row < rows && starts && ends) {
     T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
 #pragma unroll
@@ -1221,8 +1297,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
         store4(out + c * 32 + i * 2 + h * 4, float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv, a.out_wide);
-  } else {
-    float* part = args.parts + ((((int64_t)tile * heads + head) * args.splits + split) * S::kRows + row - row0) * (D + 4);
+  } else if (row < rows) {
+    float* part = args.parts + ((int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * S::kRows + row - row0) * (D + 4);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
@@ -1233,29 +1309,30 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
       part[D + 1] = sum;
     }
   }
+  lds_barrier();  // (the next tile's keys and values are written over these)
+  }
 }
 
-// Joins the pieces of a tile's rows: a block takes kJoinRows of them, D / 4 lanes a row, and has the first two
-// pieces of all its rows under way at once.
+// Joins the parts of a tile's rows: a block takes kJoinRows of them, D / 4 lanes a row, and has the first two parts
+// of all its rows under way at once.
 constexpr int kJoinRows = 32;
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args) {
   using S = TileShape<D>;
   const AttentionArgs& a = args.a;
-  __shared__ int found[2 * 4 + 2];
-  const int tile = blockIdx.x, head = blockIdx.y;
-  const FoundTile own = find_tile<256>(a, tile, S::kRows, true, found);
-  if (own.seq < 0) return;
-  const Sequence seq = sequence<true>(a, own.seq);
-  const int rows = min(seq.count, a.max_queries) * a.group, row0 = own.place * S::kRows;
-  const Span span = span_of(a, seq, row0, min(row0 + S::kRows, rows) - 1);
-  const int pieces = pieces_of_tile(args, span.to - span.from, own.total);
-  if (pieces == 1) return;
+  const TileHeader header = args.headers[blockIdx.x];
+  const int parts = header.last - header.first + 1, row0 = header.row0, head = header.head;
+  if (parts == 1) return;
+  const Sequence seq = sequence<true>(a, header.seq);
+  const int rows = min(seq.count, a.max_queries) * a.group;
   constexpr int kLanes = D / 4, kAtOnce = 256 / kLanes, kTurns = kJoinRows / kAtOnce;
-  const int lane = threadIdx.x % kLanes, first = blockIdx.z * kJoinRows + threadIdx.x / kLanes;
-  const int64_t stride = (int64_t)S::kRows * (D + 4);
-  const float* base = args.parts + (((int64_t)tile * a.pages.heads + head) * args.splits * S::kRows) * (D + 4);
+  const int lane = threadIdx.x % kLanes, first = blockIdx.y * kJoinRows + threadIdx.x / kLanes;
+  // the second part of the workgroup that begins the tile, the first of those behind it
+  auto part = [&](int c, int row) {
+    const int place = 2 * (header.first + c) + (c == 0 ? 1 : 0);
+    return args.parts + ((int64_t)place * S::kRows + row) * (D + 4);
+  };
   float4_t x[kTurns][2];
   float2 ml[kTurns][2];
 #pragma unroll
@@ -1263,7 +1340,7 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       // (rows behind the last are not written, but they are there)
-      const float* p = base + c * stride + (int64_t)(first + k * kAtOnce) * (D + 4);
+      const float* p = part(c, first + k * kAtOnce);
       x[k][c] = *reinterpret_cast<const float4_t*>(p + lane * 4);
       ml[k][c] = *reinterpret_cast<const float2*>(p + D);
     }
@@ -1276,8 +1353,8 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
     float w1 = ml[k][1].x == m ? 1.0f : __builtin_amdgcn_exp2f(ml[k][1].x - m);
     float l = ml[k][0].y * w0 + ml[k][1].y * w1;
     float4_t o = x[k][0] * w0 + x[k][1] * w1;
-    for (int c = 2; c < pieces; ++c) {
-      const float* p = base + c * stride + (int64_t)in_tile * (D + 4);
+    for (int c = 2; c < parts; ++c) {
+      const float* p = part(c, in_tile);
       const float2 more = *reinterpret_cast<const float2*>(p + D);
       const float higher = fmaxf(m, more.x);
       w0 = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
@@ -1293,46 +1370,48 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
   }
 }
 
-// Tiles and pieces of a call.
+// Tiles of a call, and whether they are worked on in even shares: while there are few they do not even out among
+// themselves (a prompt's tiles reach back differently far, and what is left over of a last round of workgroups
+// counts), and a part more or less is little beside a compute unit that waits.
 struct TilePlan {
-  int tiles, splits, budget;
-  int64_t bytes;
+  int tiles, grid;  // grid: of the even shares; 0: none
+  int64_t header_bytes, bytes;
 };
 
 TilePlan plan_tiles(int64_t T, int group, int kv_heads, int head_size, int64_t num_seqs, int64_t max_queries,
-                    int64_t table_width, int page_size) {
+                    int64_t capacity) {
   TilePlan plan;
   const int64_t rows = head_size == 256 ? TileShape<256>::kRows : TileShape<128>::kRows;
   // every sequence may leave one tile that is not full
   const int64_t tiles = min((T * group + rows - 1) / rows + num_seqs, num_seqs * ((max_queries * group + rows - 1) / rows));
   const int cus = device_compute_units();
-  // Two tiles and more a compute unit even out among themselves, the longest first.  Fewer are cut so that no
-  // piece is longer than an even share.
-  const int64_t units = tiles * kv_heads, most = max(table_width * page_size / 256, (int64_t)1);
-  plan.budget = cus > 0 ? cus : 256;
-  plan.splits = units >= 2 * plan.budget ? 1 : (int)min((2 * plan.budget + units - 1) / units, most);
   plan.tiles = (int)min(tiles, (int64_t)0x7fffffff);
-  plan.bytes = plan.splits == 1 ? 0 : tiles * kv_heads * plan.splits * rows * (head_size + 4) * (int64_t)sizeof(float);
+  // (spans are counted in 32 bits)
+  const bool few = tiles * kv_heads <= kMostShared && num_seqs <= kMostShared &&
+                   (double)(tiles * kv_heads) * (double)(capacity / kSpan + 1) < 2e9;
+  plan.grid = few ? (cus > 0 ? cus : 256) : 0;
+  plan.header_bytes = (tiles * kv_heads * (int64_t)sizeof(TileHeader) + 15) / 16 * 16;
+  plan.bytes = plan.grid == 0 ? 0 : plan.header_bytes + 2 * plan.grid * rows * (head_size + 4) * (int64_t)sizeof(float);
   return plan;
 }
 
 template <typename T, int D>
-int launch_tiles(const TileArgs& args, void* stream) {
-  const unsigned heads = (unsigned)args.a.pages.heads;
-  launch_kernel(attention_tile_kernel<T, D>, dim3((unsigned)args.tiles, heads, (unsigned)args.splits),
-                dim3(TileShape<D>::kThreads), 0, static_cast<hipStream_t>(stream), args);
+int launch_tiles(const TileArgs& args, int grid, void* stream) {
+  const unsigned tiles = (unsigned)args.tiles, heads = (unsigned)args.a.pages.heads;
+  launch_kernel(attention_tile_kernel<T, D>, grid ? dim3((unsigned)grid) : dim3(tiles, heads), dim3(TileShape<D>::kThreads),
+                0, static_cast<hipStream_t>(stream), args);
   int rc = finish_launch("kv4_attention");
-  if (rc != TW_OK || args.splits == 1) return rc;
-  launch_kernel(attention_join_tile_kernel<T, D>, dim3((unsigned)args.tiles, heads, TileShape<D>::kRows / kJoinRows), dim3(256), 0,
+  if (rc != TW_OK || grid == 0) return rc;
+  launch_kernel(attention_join_tile_kernel<T, D>, dim3(tiles * heads, TileShape<D>::kRows / kJoinRows), dim3(256), 0,
                 static_cast<hipStream_t>(stream), args);
   return finish_launch("kv4_attention");
 }
 
 template <typename T>
-int launch_tiles(const TileArgs& args, int D, void* stream) {
-  if (D == 64) return launch_tiles<T, 64>(args, stream);
-  if (D == 128) return launch_tiles<T, 128>(args, stream);
-  return launch_tiles<T, 256>(args, stream);
+int launch_tiles(const TileArgs& args, int D, int grid, void* stream) {
+  if (D == 64) return launch_tiles<T, 64>(args, grid, stream);
+  if (D == 128) return launch_tiles<T, 128>(args, grid, stream);
+  return launch_tiles<T, 256>(args, grid, stream);
 }
 
 bool wide_rows(const tw_heads* h) {
@@ -1348,7 +1427,7 @@ int64_t kv4_attention_workspace(int q_heads, int kv_heads, int head_size, int64_
   max_queries = min(max_queries, num_tokens);
   if (max_queries * group <= kMostRows)
     return plan_split(num_seqs, kv_heads, table_width, page_size, (int)max_queries * group, head_size).bytes;
-  return plan_tiles(num_tokens, group, kv_heads, head_size, num_seqs, max_queries, table_width, page_size).bytes;
+  return plan_tiles(num_tokens, group, kv_heads, head_size, num_seqs, max_queries, table_width * page_size).bytes;
 }
 
 int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages, int64_t num_pages, int page_size,
@@ -1416,12 +1495,16 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
     return dtype == TW_DTYPE_BF16 ? launch_split<__bf16>(args, head_size, plan.grid, stream)
                                   : launch_split<_Float16>(args, head_size, plan.grid, stream);
   }
-  const TilePlan plan = plan_tiles(T, a.group, kv_heads, head_size, num_seqs, max_queries, table_width, page_size);
+  const TilePlan plan = plan_tiles(T, a.group, kv_heads, head_size, num_seqs, max_queries, a.capacity);
   if ((double)T * a.group + (double)num_seqs * 256 > 2e9 || kv_heads > 65535)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too many rows", what);
-  const TileArgs args{a, static_cast<float*>(workspace), plan.tiles, plan.splits, plan.budget};
-  return dtype == TW_DTYPE_BF16 ? launch_tiles<__bf16>(args, head_size, stream)
-                                : launch_tiles<_Float16>(args, head_size, stream);
+  TileArgs args{a, nullptr, nullptr, plan.tiles};
+  if (plan.grid > 0) {
+    args.headers = static_cast<TileHeader*>(workspace);
+    args.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.header_bytes);
+  }
+  return dtype == TW_DTYPE_BF16 ? launch_tiles<__bf16>(args, head_size, plan.grid, stream)
+                                : launch_tiles<_Float16>(args, head_size, plan.grid, stream);
 }
 
 }  // namespace tw
