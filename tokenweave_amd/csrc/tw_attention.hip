@@ -815,6 +815,12 @@ __device__ __forceinline__ FoundTile find_tile(const AttentionArgs& a, int tile,
   return {uniform(found[0]), uniform(found[1])};
 }
 
+// Many rows: probabilities are held times 2^(kTileLift - m).  m need not be the maximum so far, only within kSlack of
+// it: so they stay below 2^15, fp16's normal range reaches down to 2^-13 of the largest or lower and its subnormals to
+// 2^-31, and a row's sums are multiplied anew a few times in all instead of in most units (one of 64 rows has a new
+// maximum in most of the first hundred units: 211 us with the maximum itself and 188 us so, for 8192 rows of 8 heads).
+constexpr float kTileLift = 7.0f, kSlack = 8.0f;
+
 template <int D>
 struct TileShape {
   // eight waves, two a SIMD unit, share a tile's keys and values; heads of 256 channels leave registers for one
@@ -1120,12 +1126,6 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
       if (t >= row_end || t < row_begin || missing >> (j / 8) & 1) sc[j] = -__builtin_inff();
     }
   };
-  auto largest = [&](const float16_t& sc) {
-    float most[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) most[j] = fmaxf(fmaxf(sc[j], sc[j + 4]), fmaxf(sc[j + 8], sc[j + 12]));
-    return max32(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * scale;
-  };
   // LDS is read kAhead products before the product, the first keys of a unit in the unit before it.
   constexpr int kProducts = D / 16, kAhead = 4;
   auto value = [&](const uint8_t* values, int z) {
@@ -1137,60 +1137,54 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     for (int z = 0; z < kAhead; ++z) ahead[z] = key(keys, z);
   };
   // The next unit's scores and the present probabilities, product by product: each with its share of the 16
-  // exponentials, whose sums and roundings come one product later.
-  auto scores_beside_probabilities = [&](float16_t& sc_next, const uint8_t* keys, const uint8_t* values, half8_t (&p)[2],
-                                         const float16_t& sc, float add) {
+  // exponentials, whose rounding comes one product later.  Returns the largest exponent.
+  auto scores_beside_probabilities = [&](float16_t& sc_next, const uint8_t* keys, const uint8_t* values, float16_t& x,
+                                         half8_t (&p)[2], const float16_t& sc, float add) {
     constexpr int kEach = 16 / kProducts;
 #pragma unroll
     for (int j = 0; j < 16; ++j) sc_next[j] = 0.0f;
-    float x[kEach];
+    float most = -__builtin_inff();
 #pragma unroll
     for (int z = 0; z <= kProducts; ++z) {
-      float last[kEach];
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) last[e] = x[e];
       if (z < kProducts) {
         sc_next = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], q[z], sc_next, 0, 0, 0);
         ahead[z % kAhead] = z + kAhead < kProducts ? key(keys, z + kAhead) : value(values, z + kAhead - kProducts);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e)
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[z * kEach + e], scale, add));
+        for (int e = 0; e < kEach; ++e) {
+          const float t = __builtin_fmaf(sc[z * kEach + e], scale, add);
+          most = fmaxf(most, t);
+          x[z * kEach + e] = __builtin_amdgcn_exp2f(t);
+        }
       }
       if (z > 0) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
           const int i = (z - 1) * kEach + e;
-          l[i % 4] += last[e];
-          p[i / 8][i % 8] = (_Float16)last[e];
+          p[i / 8][i % 8] = (_Float16)x[i];
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    return most;
   };
-  // The present products with the values, the next unit's maximum among them once its scores are there.
-  auto gather_beside_largest = [&](const half8_t (&p)[2], const uint8_t* values, const uint8_t* keys_after,
-                                   const float16_t& sc_next) {
-    float most[4];
+  // The present products with the values, the probabilities' sums among them.
+  auto gather_beside_sums = [&](const half8_t (&p)[2], const float16_t& x, const uint8_t* values, const uint8_t* keys_after) {
+    constexpr int kEach = 16 / kProducts;
 #pragma unroll
     for (int z = 0; z < kProducts; ++z) {
       o[z % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], p[z / (D / 32)], o[z % (D / 32)], 0, 0, 0);
       ahead[z % kAhead] = z + kAhead < kProducts ? value(values, z + kAhead) : key(keys_after, z + kAhead - kProducts);
-      if (z >= kProducts / 2) {
-        constexpr int kEach = kProducts >= 8 ? 1 : 2, kFrom = kProducts / 2;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const int j = (z - kFrom) * kEach + e;
-          if (j < 4) most[j] = fmaxf(fmaxf(sc_next[j], sc_next[j + 4]), fmaxf(sc_next[j + 8], sc_next[j + 12]));
-        }
-      }
+      for (int e = 0; e < kEach; ++e) l[(z * kEach + e) % 4] += x[z * kEach + e];
       __builtin_amdgcn_sched_barrier(0);
     }
-    return max32(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * scale;
   };
   auto sees = [&](int t0) { return t0 < min(wave_to, tile_to * S::kTokens) && t0 + 32 > wave_from; };
   auto all_see = [&](int t0, int missing) { return t0 >= all_from && t0 + 32 <= all_to && (missing & 3) == 0; };
 
-  float most = -__builtin_inff();  // of the unit that comes next
+  // Probabilities are held times 2^(kTileLift - m), where m need not be the maximum so far: it is raised to the
+  // maximum where a row sees its first token and where the maximum is kSlack above it.
+  float add = kTileLift, limit = row < rows ? -__builtin_inff() : __builtin_inff();
   // The unit of tokens t0 .. t0 + 31, whose scores are there; the scores of the next come.
   auto work_on = [&](int t0, float16_t& sc, float16_t& sc_next, const uint8_t* keys_next, const uint8_t* keys_after,
                      const uint8_t* values, int missing_next) {
@@ -1200,22 +1194,29 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
       first_keys(keys_after);
       return;
     }
-    if (__builtin_amdgcn_ballot_w64(most > m)) {
-      const float higher = fmaxf(m, most);
-      const float old = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
-      m = higher;
+    half8_t p[2];
+    float16_t x;
+    const float most = scores_beside_probabilities(sc_next, keys_next, values, x, p, sc, add);
+    // (the probabilities stay before the branch)
+    asm volatile("" : "+v"(p[0]), "+v"(p[1]));
+    if (__builtin_amdgcn_ballot_w64(most > limit)) {
+      const float higher = max32(most) - add, raised = max32(most) > limit ? higher : m;
+      const float old = m == raised ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
+      m = raised;
+      limit = m == -__builtin_inff() ? limit : kTileLift + kSlack;
+      add = m == -__builtin_inff() ? kTileLift : kTileLift - m;
 #pragma unroll
       for (int j = 0; j < 4; ++j) l[j] *= old;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) o[c] *= old;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j], scale, add));
+        p[j / 8][j % 8] = (_Float16)x[j];
+      }
     }
-    const float add = kLift - (m == -__builtin_inff() ? 0.0f : m);
-    half8_t p[2];
-    scores_beside_probabilities(sc_next, keys_next, values, p, sc, add);
-    // (the probabilities stay before the branch)
-    asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l[0]), "+v"(l[1]), "+v"(l[2]), "+v"(l[3]));
     if (!mine_next || !all_see(t1, missing_next)) mask(sc_next, mine_next ? t1 : 1 << 30, missing_next);
-    most = gather_beside_largest(p, values, keys_after, sc_next);
+    gather_beside_sums(p, x, values, keys_after);
   };
 
   // ---- While tile `at` is worked on, its keys and values and the next tile's keys are in LDS.  Keys are laid out
@@ -1250,7 +1251,6 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
   if (tile_from < tile_to && sees(tile_from * S::kTokens)) {
     scores(even, keys_now);
     if (!all_see(tile_from * S::kTokens, missing0)) mask(even, tile_from * S::kTokens, missing0);
-    most = largest(even);
   }
   // (with two key buffers the first keys are written over from here on)
   if constexpr (S::kKeyBuffers == 2) lds_barrier();
