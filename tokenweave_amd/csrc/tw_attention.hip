@@ -937,379 +937,384 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
   }
 
   for (; at < end; ++unit) {
-  FoundTile own;
-  int head = blockIdx.y;
-  if (shared) {
-    own = find(unit);
-    own = {uniform(own.seq), uniform(own.place)};
-    head = unit - unit / heads * heads;
-  } else {
-    // a prompt's last tiles see the most: they go first
-    own = find_tile<S::kThreads>(a, args.tiles - 1 - (int)blockIdx.x, S::kRows, scan);
-    if (own.seq < 0) return;
-  }
-  const Sequence seq = sequence<true>(a, own.seq);
-  const int queries = min(seq.count, a.max_queries), rows = queries * a.group, length = seq.length;
-  const int new_from = length - seq.count;
-  const int row0 = own.place * S::kRows;
-
-  // ---- tokens that the tile's rows see, and this share of them
-  auto end_of = [&](int row) { return min(new_from + row / a.group + 1, length); };
-  auto begin_of = [&](int row) { return max(new_from + row / a.group + 1 - window, 0); };
-  const int some_from = begin_of(row0);
-  Span span = span_in(seq, row0);
-  bool starts = true, ends = true;
-  if (shared) {
-    const int count = max(span.to - span.from, 1), unit_from = uniform(unit_end[unit]) - count;
-    starts = at == unit_from;
-    ends = unit_from + count <= end;
-    const int first = at - unit_from, last = min(end - unit_from, count);
-    if (starts && threadIdx.x == 0)
-      args.headers[unit] = TileHeader{own.seq, row0, head, (int)blockIdx.x, (unit_from + count - 1) / share};
-    at = unit_from + last;
-    span = {min(span.from + first, span.to), min(span.from + last, span.to)};
-  } else {
-    at = end;
-  }
-  const int tile_from = span.from * (kSpan / S::kTokens), tile_to = span.to * (kSpan / S::kTokens);
-
-  // ---- this wave's rows
-  const int row = row0 + wave * 32 + n, query = row / a.group, q_head = head * a.group + row - query * a.group;
-  const int row_end = row < rows ? end_of(row) : 0, row_begin = row < rows ? begin_of(row) : 0;
-  const int wave_row = row0 + wave * 32, wave_last = min(wave_row + 31, rows - 1);
-  const bool idle = wave_row >= rows;
-  const int wave_to = uniform(idle ? 0 : end_of(wave_last)), wave_from = uniform(idle ? 0 : begin_of(wave_row));
-  const int all_to = uniform(idle ? 0 : end_of(wave_row)), all_from = uniform(idle ? 0 : begin_of(wave_last));
-  half8_t q[D / 16];
-  float scale;
-  {
-    const T* from = static_cast<const T*>(a.q) + (int64_t)(seq.first + query) * a.q_token + (int64_t)q_head * a.q_head + h * 8;
-    float most = 0.0f;
-    float x[D / 16][8] = {};
-    if (row < rows) {
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) load_row(x[c], from + c * 16, a.q_wide);
+    FoundTile own;
+    int head = blockIdx.y;
+    if (shared) {
+      own = find(unit);
+      own = {uniform(own.seq), uniform(own.place)};
+      head = unit - unit / heads * heads;
+    } else {
+      // a prompt's last tiles see the most: they go first
+      own = find_tile<S::kThreads>(a, args.tiles - 1 - (int)blockIdx.x, S::kRows, scan);
+      if (own.seq < 0) return;
     }
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(x[c][j]));
-    const float up = lift_of(max32(most), a.scale, &scale);
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[c][j] = (_Float16)(x[c][j] * up);
-  }
-  float m = -__builtin_inff(), l[4] = {};  // l: in four strands, so that no addition waits for the last
-  float16_t o[D / 32];
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
+    const Sequence seq = sequence<true>(a, own.seq);
+    const int queries = min(seq.count, a.max_queries), rows = queries * a.group, length = seq.length;
+    const int new_from = length - seq.count;
+    const int row0 = own.place * S::kRows;
 
-  // ---- Pages.  A lane holds the number of one sixteen's page, 1024 tokens in a wave; they are asked for tile by
-  // tile.  A missing page is -1, its tokens are read from page 0 and masked.
-  const int32_t* table = a.block_table + own.seq * a.table_stride;
-  constexpr int kSixteens = S::kTokens / 16, kTilesHeld = 64 / kSixteens;
-  struct Pages {
-    int a, b, c, d;
-  };
-  int held = -1;
-  auto pages_of = [&](int at) {
-    if (at % kTilesHeld == 0 || at == tile_from) {
-      const int64_t t = ((int64_t)(at / kTilesHeld) * 64 + lane) * 16;
-      const int id = t < length && t < (int64_t)tile_to * S::kTokens ? table[t >> a.pages.page_log2] : -1;
-      held = id < a.pages.num_pages ? max(id, -1) : -1;  // (used here, so that the wait for it is here too)
+    // ---- tokens that the tile's rows see, and this share of them
+    auto end_of = [&](int row) { return min(new_from + row / a.group + 1, length); };
+    auto begin_of = [&](int row) { return max(new_from + row / a.group + 1 - window, 0); };
+    const int some_from = begin_of(row0);
+    Span span = span_in(seq, row0);
+    bool starts = true, ends = true;
+    if (shared) {
+      const int count = max(span.to - span.from, 1), unit_from = uniform(unit_end[unit]) - count;
+      starts = at == unit_from;
+      ends = unit_from + count <= end;
+      const int first = at - unit_from, last = min(end - unit_from, count);
+      if (starts && threadIdx.x == 0)
+        args.headers[unit] = TileHeader{own.seq, row0, head, (int)blockIdx.x, (unit_from + count - 1) / share};
+      at = unit_from + last;
+      span = {min(span.from + first, span.to), min(span.from + last, span.to)};
+    } else {
+      at = end;
     }
-    const int i = at % kTilesHeld * kSixteens;
-    auto one = [&](int j) { return j < kSixteens ? __builtin_amdgcn_readlane(held, i + j) : -1; };
-    return Pages{one(0), one(1), one(2), one(3)};
-  };
-  auto missing_of = [&](const Pages& p) {  // a bit for each sixteen
-    const int first = (p.a < 0 ? 1 : 0) | (p.b < 0 ? 2 : 0);
-    return S::kTokens == 32 ? first : first | (p.c < 0 ? 4 : 0) | (p.d < 0 ? 8 : 0);
-  };
-  auto block_of = [&](int id) { return a.pages.data + ((int64_t)max(id, 0) * heads + head) * a.pages.head_bytes; };
-  // Base of the block that holds a thread's sixteen `i` of the tile: the same for all where a page holds the tile.
-  auto block_at = [&](const Pages& p, int i) {
-    const uint8_t* block = block_of(p.a);
-    if (P < S::kTokens) {
-      const uint8_t *b = block_of(p.b), *c = block_of(p.c), *d = block_of(p.d);
-      block = i == 1 ? b : block;
-      block = i == 2 ? c : block;
-      block = i == 3 ? d : block;
-    }
-    return block;
-  };
+    const int tile_from = span.from * (kSpan / S::kTokens), tile_to = span.to * (kSpan / S::kTokens);
 
-  // ---- this thread's chunks: 32 channels of a token, four tokens of a sixteenth of the channels
-  const int key_chunk = threadIdx.x, value_chunk = (int)threadIdx.x - S::kValueThread;
-  const bool has_keys = key_chunk < S::kKeyChunks, has_values = value_chunk >= 0;
-  const int key_token = key_chunk / (D / 32), key_group = key_chunk % (D / 32);
-  // of 32 neighbouring lanes two sixteenths and 16 fours of tokens: their LDS writes cover all banks
-  constexpr int kFours = S::kTokens / 4;
-  const int sixteenth = (value_chunk & 1) | (value_chunk / (2 * kFours) << 1), four = value_chunk >> 1 & (kFours - 1);
-  const int in_page = P - 1, key_at = key_token & in_page, value_at = four * 4 & in_page;
-  const int key_offset = L::key(key_at) + key_group * 16, key_scale_offset = L::key_scale(P, key_at, key_group);
-  const int value_offset = L::value(P, value_at, sixteenth);
-  const int value_scale_offset = L::value_scale(P, value_at, sixteenth * (D / 16) / 32);
-  const int key_place = key_token * S::kKeyRow + key_group * 64;
-  // fours 0, 1, 2, 3 of 16 tokens lie in the order 0, 2, 1, 3
-  const int value_place = sixteenth * (D / 16) * S::kValueRow + ((four & ~3) | (four & 1) << 1 | (four >> 1 & 1)) * 8;
-
-  Fetched<D> next;
-  auto fetch_keys = [&](const Pages& p, int at) {
-    if (!has_keys) return;
-    const uint8_t* block = block_at(p, key_token >> 4);
-    const int t = at * S::kTokens & in_page;  // (0 where pages are smaller than the tile)
-    load_words(next.keys(), block + (key_offset + t * L::kRow));
-    next.first_scale = block[key_scale_offset + t];
-  };
-  auto fetch_values = [&](const Pages& p, int at, int missing) {
-    if (!has_values) return;
-    const uint8_t* block = block_at(p, four >> 2);
-    const int t0 = at * S::kTokens, t = t0 & in_page;
-    load_words(next.values(), block + (value_offset + t * L::kRow));
-    next.value_scale() = *reinterpret_cast<const uint32_t*>(block + (value_scale_offset + t));
-    // what no row sees may hold anything, and nothing times zero has to be zero
-    if (t0 + S::kTokens > length || t0 < some_from || missing) {
+    // ---- this wave's rows
+    const int row = row0 + wave * 32 + n, query = row / a.group, q_head = head * a.group + row - query * a.group;
+    const int row_end = row < rows ? end_of(row) : 0, row_begin = row < rows ? begin_of(row) : 0;
+    const int wave_row = row0 + wave * 32, wave_last = min(wave_row + 31, rows - 1);
+    const bool idle = wave_row >= rows;
+    const int wave_to = uniform(idle ? 0 : end_of(wave_last)), wave_from = uniform(idle ? 0 : begin_of(wave_row));
+    const int all_to = uniform(idle ? 0 : end_of(wave_row)), all_from = uniform(idle ? 0 : begin_of(wave_last));
+    half8_t q[D / 16];
+    float scale;
+    {
+      const T* from = static_cast<const T*>(a.q) + (int64_t)(seq.first + query) * a.q_token + (int64_t)q_head * a.q_head + h * 8;
+      float most = 0.0f;
+      float x[D / 16][8] = {};
+      if (row < rows) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int token = t0 + four * 4 + j;
-        if (token >= length || token < some_from || missing >> (four >> 2) & 1)
-          next.value_scale() = (next.value_scale() & ~(255u << (8 * j))) | 127u << (8 * j);
+        for (int c = 0; c < D / 16; ++c) load_row(x[c], from + c * 16, a.q_wide);
       }
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(x[c][j]));
+      const float up = lift_of(max32(most), a.scale, &scale);
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[c][j] = (_Float16)(x[c][j] * up);
     }
-  };
-  auto spread_keys = [&](uint8_t* to) {
-    if (!has_keys) return;
-    const float ks = __uint_as_float(next.first_scale << 23);
+    float m = -__builtin_inff(), l[4] = {};  // l: in four strands, so that no addition waits for the last
+    float16_t o[D / 32];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) *reinterpret_cast<half8_t*>(to + key_place + w * 16) = eight_values(next.keys()[w], ks);
-  };
-  auto spread_values = [&](uint8_t* to) {
-    if (!has_values) return;
-    float vs[4];
+    for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vs[j] = __uint_as_float((next.value_scale() >> (8 * j) & 255) << 23);
-#pragma unroll
-    for (int b = 0; b < D / 32; ++b) {  // byte b of each token: two channels
-      half2_t x[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int byte = j * (D / 32) + b;
-        const uint32_t w = next.values()[byte / 4];
-        x[j] = byte % 4 == 0 ? two_values<0>(w, vs[j]) : byte % 4 == 1 ? two_values<1>(w, vs[j])
-             : byte % 4 == 2 ? two_values<2>(w, vs[j]) : two_values<3>(w, vs[j]);
-      }
-      typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<half4_t*>(to + value_place + (2 * b + c) * S::kValueRow) = half4_t{x[0][c], x[1][c], x[2][c], x[3][c]};
-    }
-  };
+      for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
 
-  // ---- a unit of 32 tokens
-  auto key = [&](const uint8_t* keys, int c) {
-    return *reinterpret_cast<const half8_t*>(keys + n * S::kKeyRow + h * 16 + c * 32);
-  };
-  auto scores = [&](float16_t& sc, const uint8_t* keys) {
+    // ---- Pages.  A lane holds the number of one sixteen's page, 1024 tokens in a wave; they are asked for tile by
+    // tile.  A missing page is -1, its tokens are read from page 0 and masked.
+    const int32_t* table = a.block_table + own.seq * a.table_stride;
+    constexpr int kSixteens = S::kTokens / 16, kTilesHeld = 64 / kSixteens;
+    struct Pages {
+      int a, b, c, d;
+    };
+    int held = -1;
+    auto pages_of = [&](int at) {
+      if (at % kTilesHeld == 0 || at == tile_from) {
+        const int64_t t = ((int64_t)(at / kTilesHeld) * 64 + lane) * 16;
+        const int id = t < length && t < (int64_t)tile_to * S::kTokens ? table[t >> a.pages.page_log2] : -1;
+        held = id < a.pages.num_pages ? max(id, -1) : -1;  // (used here, so that the wait for it is here too)
+      }
+      const int i = at % kTilesHeld * kSixteens;
+      auto one = [&](int j) { return j < kSixteens ? __builtin_amdgcn_readlane(held, i + j) : -1; };
+      return Pages{one(0), one(1), one(2), one(3)};
+    };
+    auto missing_of = [&](const Pages& p) {  // a bit for each sixteen
+      const int first = (p.a < 0 ? 1 : 0) | (p.b < 0 ? 2 : 0);
+      return S::kTokens == 32 ? first : first | (p.c < 0 ? 4 : 0) | (p.d < 0 ? 8 : 0);
+    };
+    auto block_of = [&](int id) { return a.pages.data + ((int64_t)max(id, 0) * heads + head) * a.pages.head_bytes; };
+    // Base of the block that holds a thread's sixteen `i` of the tile: the same for all where a page holds the tile.
+    auto block_at = [&](const Pages& p, int i) {
+      const uint8_t* block = block_of(p.a);
+      if (P < S::kTokens) {
+        const uint8_t *b = block_of(p.b), *c = block_of(p.c), *d = block_of(p.d);
+        block = i == 1 ? b : block;
+        block = i == 2 ? c : block;
+        block = i == 3 ? d : block;
+      }
+      return block;
+    };
+
+    // ---- this thread's chunks: 32 channels of a token, four tokens of a sixteenth of the channels
+    const int key_chunk = threadIdx.x, value_chunk = (int)threadIdx.x - S::kValueThread;
+    const bool has_keys = key_chunk < S::kKeyChunks, has_values = value_chunk >= 0;
+    const int key_token = key_chunk / (D / 32), key_group = key_chunk % (D / 32);
+    // of 32 neighbouring lanes two sixteenths and 16 fours of tokens: their LDS writes cover all banks
+    constexpr int kFours = S::kTokens / 4;
+    const int sixteenth = (value_chunk & 1) | (value_chunk / (2 * kFours) << 1), four = value_chunk >> 1 & (kFours - 1);
+    const int in_page = P - 1, key_at = key_token & in_page, value_at = four * 4 & in_page;
+    const int key_offset = L::key(key_at) + key_group * 16, key_scale_offset = L::key_scale(P, key_at, key_group);
+    const int value_offset = L::value(P, value_at, sixteenth);
+    const int value_scale_offset = L::value_scale(P, value_at, sixteenth * (D / 16) / 32);
+    const int key_place = key_token * S::kKeyRow + key_group * 64;
+    // fours 0, 1, 2, 3 of 16 tokens lie in the order 0, 2, 1, 3
+    const int value_place = sixteenth * (D / 16) * S::kValueRow + ((four & ~3) | (four & 1) << 1 | (four >> 1 & 1)) * 8;
+
+    Fetched<D> next;
+    auto fetch_keys = [&](const Pages& p, int at) {
+      if (!has_keys) return;
+      const uint8_t* block = block_at(p, key_token >> 4);
+      const int t = at * S::kTokens & in_page;  // (0 where pages are smaller than the tile)
+      load_words(next.keys(), block + (key_offset + t * L::kRow));
+      next.first_scale = block[key_scale_offset + t];
+    };
+    auto fetch_values = [&](const Pages& p, int at, int missing) {
+      if (!has_values) return;
+      const uint8_t* block = block_at(p, four >> 2);
+      const int t0 = at * S::kTokens, t = t0 & in_page;
+      load_words(next.values(), block + (value_offset + t * L::kRow));
+      next.value_scale() = *reinterpret_cast<const uint32_t*>(block + (value_scale_offset + t));
+      // what no row sees may hold anything, and nothing times zero has to be zero
+      if (t0 + S::kTokens > length || t0 < some_from || missing) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sc[j] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(keys, c), q[c], sc, 0, 0, 0);
-  };
-  auto mask = [&](float16_t& sc, int t0, int missing) {  // missing: of the unit's two sixteens
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int t = t0 + (j / 4) * 8 + h * 4 + j % 4;
-      if (t >= row_end || t < row_begin || missing >> (j / 8) & 1) sc[j] = -__builtin_inff();
-    }
-  };
-  // LDS is read kAhead products before the product, the first keys of a unit in the unit before it.
-  constexpr int kProducts = D / 16, kAhead = 4;
-  auto value = [&](const uint8_t* values, int z) {
-    return *reinterpret_cast<const half8_t*>(values + (z % (D / 32) * 32 + n) * S::kValueRow + h * 16 + z / (D / 32) * 32);
-  };
-  half8_t ahead[kAhead];
-  auto first_keys = [&](const uint8_t* keys) {
-#pragma unroll
-    for (int z = 0; z < kAhead; ++z) ahead[z] = key(keys, z);
-  };
-  // The next unit's scores and the present probabilities, product by product: each with its share of the 16
-  // exponentials, whose rounding comes one product later.  Returns the largest exponent.
-  auto scores_beside_probabilities = [&](float16_t& sc_next, const uint8_t* keys, const uint8_t* values, float16_t& x,
-                                         half8_t (&p)[2], const float16_t& sc, float add) {
-    constexpr int kEach = 16 / kProducts;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) sc_next[j] = 0.0f;
-    float most = -__builtin_inff();
-#pragma unroll
-    for (int z = 0; z <= kProducts; ++z) {
-      if (z < kProducts) {
-        sc_next = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], q[z], sc_next, 0, 0, 0);
-        ahead[z % kAhead] = z + kAhead < kProducts ? key(keys, z + kAhead) : value(values, z + kAhead - kProducts);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const float t = __builtin_fmaf(sc[z * kEach + e], scale, add);
-          most = fmaxf(most, t);
-          x[z * kEach + e] = __builtin_amdgcn_exp2f(t);
+        for (int j = 0; j < 4; ++j) {
+          const int token = t0 + four * 4 + j;
+          if (token >= length || token < some_from || missing >> (four >> 2) & 1)
+            next.value_scale() = (next.value_scale() & ~(255u << (8 * j))) | 127u << (8 * j);
         }
       }
-      if (z > 0) {
+    };
+    auto spread_keys = [&](uint8_t* to) {
+      if (!has_keys) return;
+      const float ks = __uint_as_float(next.first_scale << 23);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const int i = (z - 1) * kEach + e;
-          p[i / 8][i % 8] = (_Float16)x[i];
+      for (int w = 0; w < 4; ++w) *reinterpret_cast<half8_t*>(to + key_place + w * 16) = eight_values(next.keys()[w], ks);
+    };
+    auto spread_values = [&](uint8_t* to) {
+      if (!has_values) return;
+      float vs[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vs[j] = __uint_as_float((next.value_scale() >> (8 * j) & 255) << 23);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {  // byte b of each token: two channels
+        half2_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int byte = j * (D / 32) + b;
+          const uint32_t w = next.values()[byte / 4];
+          x[j] = byte % 4 == 0 ? two_values<0>(w, vs[j]) : byte % 4 == 1 ? two_values<1>(w, vs[j])
+               : byte % 4 == 2 ? two_values<2>(w, vs[j]) : two_values<3>(w, vs[j]);
         }
+        typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<half4_t*>(to + value_place + (2 * b + c) * S::kValueRow) = half4_t{x[0][c], x[1][c], x[2][c], x[3][c]};
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    return most;
-  };
-  // The present products with the values, the probabilities' sums among them.
-  auto gather_beside_sums = [&](const half8_t (&p)[2], const float16_t& x, const uint8_t* values, const uint8_t* keys_after) {
-    constexpr int kEach = 16 / kProducts;
-#pragma unroll
-    for (int z = 0; z < kProducts; ++z) {
-      o[z % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], p[z / (D / 32)], o[z % (D / 32)], 0, 0, 0);
-      ahead[z % kAhead] = z + kAhead < kProducts ? value(values, z + kAhead) : key(keys_after, z + kAhead - kProducts);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) l[(z * kEach + e) % 4] += x[z * kEach + e];
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  auto sees = [&](int t0) { return t0 < min(wave_to, tile_to * S::kTokens) && t0 + 32 > wave_from; };
-  auto all_see = [&](int t0, int missing) { return t0 >= all_from && t0 + 32 <= all_to && (missing & 3) == 0; };
+    };
 
-  // Probabilities are held times 2^(kTileLift - m), where m need not be the maximum so far: it is raised to the
-  // maximum where a row sees its first token and where the maximum is kSlack above it.
-  float add = kTileLift, limit = row < rows ? -__builtin_inff() : __builtin_inff();
-  // The unit of tokens t0 .. t0 + 31, whose scores are there; the scores of the next come.
-  auto work_on = [&](int t0, float16_t& sc, float16_t& sc_next, const uint8_t* keys_next, const uint8_t* keys_after,
-                     const uint8_t* values, int missing_next) {
-    const int t1 = t0 + 32;
-    const bool mine = sees(t0), mine_next = sees(t1);
-    if (!mine && !mine_next) {
-      first_keys(keys_after);
-      return;
-    }
-    half8_t p[2];
-    float16_t x;
-    const float most = scores_beside_probabilities(sc_next, keys_next, values, x, p, sc, add);
-    // (the probabilities stay before the branch)
-    asm volatile("" : "+v"(p[0]), "+v"(p[1]));
-    if (__builtin_amdgcn_ballot_w64(most > limit)) {
-      const float higher = max32(most) - add, raised = max32(most) > limit ? higher : m;
-      const float old = m == raised ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
-      m = raised;
-      limit = m == -__builtin_inff() ? limit : kTileLift + kSlack;
-      add = m == -__builtin_inff() ? kTileLift : kTileLift - m;
+    // ---- a unit of 32 tokens
+    auto key = [&](const uint8_t* keys, int c) {
+      return *reinterpret_cast<const half8_t*>(keys + n * S::kKeyRow + h * 16 + c * 32);
+    };
+    auto scores = [&](float16_t& sc, const uint8_t* keys) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) l[j] *= old;
+      for (int j = 0; j < 16; ++j) sc[j] = 0.0f;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) o[c] *= old;
+      for (int c = 0; c < D / 16; ++c) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(keys, c), q[c], sc, 0, 0, 0);
+    };
+    auto mask = [&](float16_t& sc, int t0, int missing) {  // missing: of the unit's two sixteens
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j], scale, add));
-        p[j / 8][j % 8] = (_Float16)x[j];
+        const int t = t0 + (j / 4) * 8 + h * 4 + j % 4;
+        if (t >= row_end || t < row_begin || missing >> (j / 8) & 1) sc[j] = -__builtin_inff();
+      }
+    };
+    // LDS is read kAhead products before the product, the first keys of a unit in the unit before it.
+    constexpr int kProducts = D / 16, kAhead = 4;
+    auto value = [&](const uint8_t* values, int z) {
+      return *reinterpret_cast<const half8_t*>(values + (z % (D / 32) * 32 + n) * S::kValueRow + h * 16 + z / (D / 32) * 32);
+    };
+    half8_t ahead[kAhead];
+    auto first_keys = [&](const uint8_t* keys) {
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) ahead[z] = key(keys, z);
+    };
+    // The next unit's scores and the present probabilities, product by product: each with its share of the 16
+    // exponentials, whose rounding comes one product later.  Returns the largest exponent.
+    auto scores_beside_probabilities = [&](float16_t& sc_next, const uint8_t* keys, const uint8_t* values, float16_t& x,
+                                           half8_t (&p)[2], const float16_t& sc, float add) {
+      constexpr int kEach = 16 / kProducts;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc_next[j] = 0.0f;
+      float most = -__builtin_inff();
+#pragma unroll
+      for (int z = 0; z <= kProducts; ++z) {
+        if (z < kProducts) {
+          sc_next = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], q[z], sc_next, 0, 0, 0);
+          ahead[z % kAhead] = z + kAhead < kProducts ? key(keys, z + kAhead) : value(values, z + kAhead - kProducts);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            const float t = __builtin_fmaf(sc[z * kEach + e], scale, add);
+            most = fmaxf(most, t);
+            x[z * kEach + e] = __builtin_amdgcn_exp2f(t);
+          }
+        }
+        if (z > 0) {
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            const int i = (z - 1) * kEach + e;
+            p[i / 8][i % 8] = (_Float16)x[i];
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return most;
+    };
+    // The present products with the values, the probabilities' sums among them.
+    auto gather_beside_sums = [&](const half8_t (&p)[2], const float16_t& x, const uint8_t* values, const uint8_t* keys_after) {
+      constexpr int kEach = 16 / kProducts;
+#pragma unroll
+      for (int z = 0; z < kProducts; ++z) {
+        o[z % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], p[z / (D / 32)], o[z % (D / 32)], 0, 0, 0);
+        ahead[z % kAhead] = z + kAhead < kProducts ? value(values, z + kAhead) : key(keys_after, z + kAhead - kProducts);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) l[(z * kEach + e) % 4] += x[z * kEach + e];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto sees = [&](int t0) { return t0 < min(wave_to, tile_to * S::kTokens) && t0 + 32 > wave_from; };
+    auto all_see = [&](int t0, int missing) { return t0 >= all_from && t0 + 32 <= all_to && (missing & 3) == 0; };
+
+    // Probabilities are held times 2^(kTileLift - m), where m need not be the maximum so far: it is raised to the
+    // maximum where a row sees its first token and where the maximum is kSlack above it.
+    float add = kTileLift, limit = row < rows ? -__builtin_inff() : __builtin_inff();
+    // The unit of tokens t0 .. t0 + 31, whose scores are there; the scores of the next come.
+    auto work_on = [&](int t0, float16_t& sc, float16_t& sc_next, const uint8_t* keys_next, const uint8_t* keys_after,
+                       const uint8_t* values, int missing_next) {
+      const int t1 = t0 + 32;
+      const bool mine = sees(t0), mine_next = sees(t1);
+      if (!mine && !mine_next) {
+        first_keys(keys_after);
+        return;
+      }
+      half8_t p[2];
+      float16_t x;
+      const float most = scores_beside_probabilities(sc_next, keys_next, values, x, p, sc, add);
+      // (the probabilities stay before the branch)
+      asm volatile("" : "+v"(p[0]), "+v"(p[1]));
+      if (__builtin_amdgcn_ballot_w64(most > limit)) {
+        const float higher = max32(most) - add, raised = max32(most) > limit ? higher : m;
+        const float old = m == raised ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
+        m = raised;
+        limit = m == -__builtin_inff() ? limit : kTileLift + kSlack;
+        add = m == -__builtin_inff() ? kTileLift : kTileLift - m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[j] *= old;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) o[c] *= old;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j], scale, add));
+          p[j / 8][j % 8] = (_Float16)x[j];
+        }
+      }
+      if (!mine_next || !all_see(t1, missing_next)) mask(sc_next, mine_next ? t1 : 1 << 30, missing_next);
+      gather_beside_sums(p, x, values, keys_after);
+    };
+
+    // ---- While tile `at` is worked on, its keys and values and the next tile's keys are in LDS.  Keys are laid out
+    // two tiles ahead and values one, and fetched one tile before that.
+    uint8_t *keys_now = key_buffers[0], *keys_next = key_buffers[1], *keys_later = key_buffers[S::kKeyBuffers - 1];
+    float16_t even, odd;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) even[j] = odd[j] = -__builtin_inff();  // of a unit that the wave does not see
+    Pages pages_now = pages_of(tile_from), pages_next = pages_of(tile_from + 1), pages_later = pages_of(tile_from + 2);
+    int missing0 = missing_of(pages_now), missing1 = missing_of(pages_next), missing2 = missing_of(pages_later);
+    if (tile_from < tile_to) {
+      fetch_values(pages_now, tile_from, missing0);
+      if constexpr (S::kApart) {
+        fetch_keys(pages_now, tile_from);
+        spread_keys(keys_now);
+        spread_values(value_buffers[0]);
+      } else {
+        spread_values(value_buffers[0]);
+        fetch_keys(pages_now, tile_from);
+        spread_keys(keys_now);
+      }
+      if (tile_from + 1 < tile_to) {
+        fetch_keys(pages_next, tile_from + 1);
+        spread_keys(keys_next);
+        fetch_values(pages_next, tile_from + 1, missing1);
+      }
+      if (tile_from + 2 < tile_to) fetch_keys(pages_later, tile_from + 2);
+      pages_next = pages_later;
+      pages_later = pages_of(tile_from + 3);
+    }
+    lds_barrier();
+    if (tile_from < tile_to && sees(tile_from * S::kTokens)) {
+      scores(even, keys_now);
+      if (!all_see(tile_from * S::kTokens, missing0)) mask(even, tile_from * S::kTokens, missing0);
+    }
+    // (with two key buffers the first keys are written over from here on)
+    if constexpr (S::kKeyBuffers == 2) lds_barrier();
+    // Keys of the unit after next, whatever is there where there is none: they are read and not used.
+    first_keys(S::kUnits == 2 ? keys_now + 32 * S::kKeyRow : keys_next);
+    auto advance = [&](int at, float16_t& first, float16_t& second) {
+      const int t0 = at * S::kTokens;
+      const uint8_t* values = value_buffers[(at - tile_from) & 1];
+      auto move_values = [&]() {
+        if (at + 1 < tile_to) spread_values(value_buffers[(at - tile_from + 1) & 1]);
+        if (at + 2 < tile_to) fetch_values(pages_next, at + 2, missing2);
+      };
+      // of the two waves of a SIMD unit one lays out values before its products, the other keys after them
+      if constexpr (S::kApart) move_values();
+      if constexpr (S::kUnits == 2) {
+        const uint8_t *second_now = keys_now + 32 * S::kKeyRow, *second_next = keys_next + 32 * S::kKeyRow;
+        work_on(t0, first, second, second_now, keys_next, values, missing0 >> 2);
+        work_on(t0 + 32, second, first, keys_next, second_next, values + 64, missing1);
+      } else {
+        // (the keys after next are being written where the present ones were: read behind the barrier)
+        work_on(t0, first, second, keys_next, keys_next, values, missing1);
+      }
+      uint8_t* const write = S::kUnits == 2 ? keys_later : keys_now;
+      if (at + 2 < tile_to) spread_keys(write);
+      if (at + 3 < tile_to) fetch_keys(pages_later, at + 3);
+      if constexpr (!S::kApart) move_values();
+      pages_next = pages_later;
+      missing0 = missing1;
+      missing1 = missing2;
+      missing2 = missing_of(pages_later);
+      pages_later = pages_of(at + 4);
+      keys_later = keys_now;
+      keys_now = keys_next;
+      keys_next = write;
+      lds_barrier();
+      if constexpr (S::kUnits == 1) first_keys(keys_next);
+    };
+    for (int at = tile_from; at < tile_to; at += 3 - S::kUnits) {
+      advance(at, even, odd);
+      if (S::kUnits == 1 && at + 1 < tile_to) advance(at + 1, odd, even);
+    }
+    const Both sums = across32((l[0] + l[1]) + (l[2] + l[3]));
+    const float sum = sums.a + sums.b;
+    if (row < rows && starts && ends) {
+      T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
+      const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          store4(out + c * 32 + i * 2 + h * 4, float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv, a.out_wide);
+    } else if (row < rows) {
+      float* part = args.parts + ((int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * S::kRows + row - row0) * (D + 4);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4_t*>(part + c * 32 + i * 2 + h * 4) = float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]};
+      if (h == 0) {
+        part[D] = m;
+        part[D + 1] = sum;
       }
     }
-    if (!mine_next || !all_see(t1, missing_next)) mask(sc_next, mine_next ? t1 : 1 << 30, missing_next);
-    gather_beside_sums(p, x, values, keys_after);
-  };
-
-  // ---- While tile `at` is worked on, its keys and values and the next tile's keys are in LDS.  Keys are laid out
-  // two tiles ahead and values one, and fetched one tile before that.
-  uint8_t *keys_now = key_buffers[0], *keys_next = key_buffers[1], *keys_later = key_buffers[S::kKeyBuffers - 1];
-  float16_t even, odd;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) even[j] = odd[j] = -__builtin_inff();  // of a unit that the wave does not see
-  Pages pages_now = pages_of(tile_from), pages_next = pages_of(tile_from + 1), pages_later = pages_of(tile_from + 2);
-  int missing0 = missing_of(pages_now), missing1 = missing_of(pages_next), missing2 = missing_of(pages_later);
-  if (tile_from < tile_to) {
-    fetch_values(pages_now, tile_from, missing0);
-    if constexpr (S::kApart) {
-      fetch_keys(pages_now, tile_from);
-      spread_keys(keys_now);
-      spread_values(value_buffers[0]);
-    } else {
-      spread_values(value_buffers[0]);
-      fetch_keys(pages_now, tile_from);
-      spread_keys(keys_now);
-    }
-    if (tile_from + 1 < tile_to) {
-      fetch_keys(pages_next, tile_from + 1);
-      spread_keys(keys_next);
-      fetch_values(pages_next, tile_from + 1, missing1);
-    }
-    if (tile_from + 2 < tile_to) fetch_keys(pages_later, tile_from + 2);
-    pages_next = pages_later;
-    pages_later = pages_of(tile_from + 3);
-  }
-  lds_barrier();
-  if (tile_from < tile_to && sees(tile_from * S::kTokens)) {
-    scores(even, keys_now);
-    if (!all_see(tile_from * S::kTokens, missing0)) mask(even, tile_from * S::kTokens, missing0);
-  }
-  // (with two key buffers the first keys are written over from here on)
-  if constexpr (S::kKeyBuffers == 2) lds_barrier();
-  // Keys of the unit after next, whatever is there where there is none: they are read and not used.
-  first_keys(S::kUnits == 2 ? keys_now + 32 * S::kKeyRow : keys_next);
-  auto advance = [&](int at, float16_t& first, float16_t& second) {
-    const int t0 = at * S::kTokens;
-    const uint8_t* values = value_buffers[(at - tile_from) & 1];
-    if constexpr (S::kUnits == 2) {
-      const uint8_t *second_now = keys_now + 32 * S::kKeyRow, *second_next = keys_next + 32 * S::kKeyRow;
-      work_on(t0, first, second, second_now, keys_next, values, missing0 >> 2);
-      work_on(t0 + 32, second, first, keys_next, second_next, values + 64, missing1);
-    } else {
-      // (the keys after next are being written where the present ones were: read behind the barrier)
-      work_on(t0, first, second, keys_next, keys_next, values, missing1);
-    }
-    uint8_t* const write = S::kUnits == 2 ? keys_later : keys_now;
-    if (at + 2 < tile_to) spread_keys(write);
-    if (at + 1 < tile_to) spread_values(value_buffers[(at - tile_from + 1) & 1]);
-    if (at + 3 < tile_to) fetch_keys(pages_later, at + 3);
-    if (at + 2 < tile_to) fetch_values(pages_next, at + 2, missing2);
-    pages_next = pages_later;
-    missing0 = missing1;
-    missing1 = missing2;
-    missing2 = missing_of(pages_later);
-    pages_later = pages_of(at + 4);
-    keys_later = keys_now;
-    keys_now = keys_next;
-    keys_next = write;
-    lds_barrier();
-    if constexpr (S::kUnits == 1) first_keys(keys_next);
-  };
-  for (int at = tile_from; at < tile_to; at += 3 - S::kUnits) {
-    advance(at, even, odd);
-    if (S::kUnits == 1 && at + 1 < tile_to) advance(at + 1, odd, even);
-  }
-  const Both sums = across32((l[0] + l[1]) + (l[2] + l[3]));
-  const float sum = sums.a + sums.b;
-  if (row < rows && starts && ends) {
-    T* out = static_cast<T*>(a.out) + (int64_t)(seq.first + query) * a.out_token + (int64_t)q_head * a.out_head;
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        store4(out + c * 32 + i * 2 + h * 4, float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv, a.out_wide);
-  } else if (row < rows) {
-    float* part = args.parts + ((int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * S::kRows + row - row0) * (D + 4);
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4_t*>(part + c * 32 + i * 2 + h * 4) = float4_t{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]};
-    if (h == 0) {
-      part[D] = m;
-      part[D + 1] = sum;
-    }
-  }
-  lds_barrier();  // (the next tile's keys and values are written over these)
+    lds_barrier();  // (the next tile's keys and values are written over these)
   }
 }
 
