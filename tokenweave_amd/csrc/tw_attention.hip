@@ -522,6 +522,39 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
         }
         vs[i] = __uint_as_float(b << 23);
       }
+      // Where some rows see a token and others do not, a value that is not a number is kept out of the products (times
+      // zero it is not zero) and put into the sums of the rows that see it, which a product of ones and zeros finds.
+      if (!whole) {
+        bool any = false;
+        half8_t odd_ones;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool odd_one = vs[i] == __builtin_inff();
+          any = any || odd_one;
+          odd_ones[i] = odd_one ? (_Float16)1.0f : (_Float16)0.0f;
+        }
+        if (__builtin_amdgcn_ballot_w64(any)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (vs[i] == __builtin_inff()) vs[i] = 1.0f;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            half8_t seen;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int token = t0 + (i / 4) * 16 + h4 * 4 + i % 4;
+              seen[i] = token < row_end[t] && token >= row_begin[t] ? (_Float16)1.0f : (_Float16)0.0f;
+            }
+            const float4_t found = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd_ones, seen, float4_t{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (found[r] > 0.0f) {
+#pragma unroll
+                for (int c = 0; c < kTiles; ++c) o[t][c][r] = __builtin_nanf("");
+              }
+          }
+        }
+      }
       auto channels = [&](auto sel, int word) {  // two channels of the lane's: 2 * sel, 2 * sel + 1 of a word
         constexpr int S = decltype(sel)::value;
         half2_t x[8];
@@ -869,11 +902,14 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
   __shared__ __align__(16) uint8_t key_buffers[S::kKeyBuffers][S::kKeyBytes];
   __shared__ __align__(16) uint8_t value_buffers[2][S::kValueBytes];
   __shared__ int scan[S::kWaves + 2];
+  __shared__ int odd_unit;  // the last unit with values that are not numbers
   __shared__ int first_tile[kMostShared + 1], unit_end[kMostShared];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads;
   const int window = a.window > 0 ? a.window : 1 << 30;
+
+  if (threadIdx.x == 0) odd_unit = -1;  // (a barrier follows, with the search for the tiles)
 
   // ---- Which tiles: one, or an even share of all tiles' spans.  In the order of the shares a long tile of a prompt
   // and a short one take turns: the last, the first, the last but one, ...
@@ -1089,6 +1125,15 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     };
     auto spread_values = [&](uint8_t* to) {
       if (!has_values) return;
+      // A value that is not a number is kept out of the products, times zero it would not be zero: the sums of the rows
+      // that see it get it after the last tile.
+      uint32_t& scales = next.value_scale();
+      if (((scales & 0x7f7f7f7f) + 0x01010101) & scales & 0x80808080) {
+        odd_unit = unit;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if ((scales >> (8 * j) & 255) == 255) scales ^= 128u << (8 * j);
+      }
       float vs[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) vs[j] = __uint_as_float((next.value_scale() >> (8 * j) & 255) << 23);
@@ -1291,6 +1336,27 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     for (int at = tile_from; at < tile_to; at += 3 - S::kUnits) {
       advance(at, even, odd);
       if (S::kUnits == 1 && at + 1 < tile_to) advance(at + 1, odd, even);
+    }
+    if (odd_unit == unit) {
+      uint32_t mine = 0;  // a bit for each 32 channels
+#pragma unroll 1
+      for (int t0 = tile_from * S::kTokens; t0 < tile_to * S::kTokens; t0 += 32) {
+        const int t = t0 + n, id = t < length ? table[t >> a.pages.page_log2] : -1;
+        const bool there = id >= 0 && id < a.pages.num_pages;
+        const uint8_t* scales = block_of(there ? id : 0);
+        const int from = min(max(row_begin - t0, 0), 32), to = min(max(row_end - t0, 0), 32);
+        const uint32_t seen = from < to ? (uint32_t)(((uint64_t)1 << to) - ((uint64_t)1 << from)) : 0;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const bool odd_one = there && scales[L::value_scale(P, t & in_page, c)] == 255;
+          mine |= (uint32_t)__builtin_amdgcn_ballot_w64(odd_one) & seen ? 1u << c : 0;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (mine >> c & 1) o[c][j] = __builtin_nanf("");
     }
     const Both sums = across32((l[0] + l[1]) + (l[2] + l[3]));
     const float sum = sums.a + sums.b;
