@@ -37,19 +37,6 @@ struct Kv4 {
 
 constexpr int kMinExponent = -23, kMaxExponent = 13, kNanScale = 255;
 
-// 2^(b - 127); the format's byte for a block that is no number gives NaN.
-__device__ __forceinline__ float scale_of(uint32_t b) {
-  return b == kNanScale ? __builtin_nanf("") : __uint_as_float(b << 23);
-}
-
-// The value of a code without its scale.
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-  const uint32_t m = code & 7;
-  // 0, 0.5: m / 2; above: 2^(m/2 - 1) * (1 + (m & 1) / 2), the bits of a float shifted up
-  const float f = m < 2 ? 0.5f * (float)m : __uint_as_float((126u << 23) + (m << 22));
-  return code & 8 ? -f : f;
-}
-
 }  // namespace tw
 
 #endif

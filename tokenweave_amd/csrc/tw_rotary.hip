@@ -132,10 +132,19 @@ struct RotaryArgs {
 
 template <typename T, int W>
 __device__ __forceinline__ void rotary_item(const RotaryArgs& a, int64_t item) {
-  const int64_t row = item / a.columns;
-  const int column = (int)(item - row * a.columns);
-  const int64_t token = row / a.heads;
-  const int head = (int)(row - token * a.heads);
+  int64_t token;
+  int head, column;
+  if (a.items <= 0x7fffffff) {  // (a division of 64 bits takes longer than the rest)
+    const uint32_t row = (uint32_t)item / (uint32_t)a.columns;
+    column = (int)((uint32_t)item - row * (uint32_t)a.columns);
+    token = row / (uint32_t)a.heads;
+    head = (int)(row - (uint32_t)token * (uint32_t)a.heads);
+  } else {
+    const int64_t row = item / a.columns;
+    column = (int)(item - row * a.columns);
+    token = row / a.heads;
+    head = (int)(row - token * a.heads);
+  }
   const bool is_q = head < a.q_heads;
   const Heads& in = is_q ? a.q : a.k;
   const Heads& out = is_q ? a.q_out : a.k_out;
@@ -161,11 +170,11 @@ struct AppendArgs {
   Heads k, v;
   const int64_t* slots;
   int64_t tokens;
-  int64_t items;   // threads that code keys and values: 2 * heads * tokens * D/8
+  int blocks;      // of one head's keys or values: tokens * D/8 threads
+  int kv_blocks;   // of all heads' keys and values
   bool turned;
   Rotary r;
   RotaryArgs q;    // the queries (no keys); items = 0: none
-  int64_t kv_blocks;
 };
 
 // Codes of 8 values of a block of 32 whose other 24 are in the three neighbouring lanes.
@@ -178,15 +187,13 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t* scale
   // the exponent of most / 7, rounded up: 7 = 1.75 * 2^2
   const int e = min(max((int)((most + 0x1fffffu) >> 23) - 129, kMinExponent), kMaxExponent);
   *scale = most >= 0x7f800000u ? kNanScale : (uint32_t)(e + 127);
-  const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+  // two values an instruction: the nearest magnitude, ties to the even code, no further than the largest
+  const float size = __uint_as_float((uint32_t)(e + 127) << 23);
   uint32_t word = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = __builtin_fabsf(x[i]) * up;
-    // thresholds half way between the magnitudes; a tie goes to the even code
-    const uint32_t m = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-    word |= (m | (__float_as_uint(x[i]) >> 31 << 3)) << (4 * i);
-  }
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[0], x[1], size, 0);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[2], x[3], size, 1);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[4], x[5], size, 2);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[6], x[7], size, 3);
   return word;
 }
 
@@ -263,21 +270,20 @@ __device__ __forceinline__ bool inside(const Kv4Pages& p, int64_t slot) {
 // neighbouring tokens of one head, whose bytes are neighbours in a page.
 template <typename T, int D, bool VEC, int WQ>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
-  if ((int64_t)blockIdx.x >= a.kv_blocks) {
-    const int64_t item = ((int64_t)blockIdx.x - a.kv_blocks) * kThreads + threadIdx.x;
+  if ((int)blockIdx.x >= a.kv_blocks) {
+    const int64_t item = (int64_t)((int)blockIdx.x - a.kv_blocks) * kThreads + threadIdx.x;
     if (item < a.q.items) rotary_item<T, WQ>(a.q, item);
     return;
   }
   constexpr int kLanes = D / 8;
-  const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int part = (int)(item % kLanes), ch = part * 8;
-  const int64_t row = item / kLanes;
-  const int64_t token = row % a.tokens;
-  const int which = (int)(row / a.tokens);  // keys of all heads, then values of all heads
+  const int which = (int)blockIdx.x / a.blocks;  // keys of all heads, then values of all heads
+  const int64_t item = (int64_t)((int)blockIdx.x - which * a.blocks) * kThreads + threadIdx.x;
+  const int part = (int)item & (kLanes - 1), ch = part * 8;
+  const int64_t token = item / kLanes;
   const bool is_key = which < a.pages.heads;
   const int head = is_key ? which : which - a.pages.heads;
   // whole rows end together: the lanes of a block of 32 stay together
-  if (item >= a.items) return;
+  if (token >= a.tokens) return;
   const int64_t slot = a.slots[token];
   if (!inside(a.pages, slot)) return;
   const Heads& h = is_key ? a.k : a.v;
@@ -310,27 +316,35 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
     at[is_key ? L::key_scale(P, t, part >> 2) : L::value_scale(P, t, part >> 2)] = (uint8_t)scale;
 }
 
+template <int I>
+__device__ __forceinline__ void pair_of(float (&x)[8], uint32_t word, float scale) {
+  typedef float float2_t __attribute__((ext_vector_type(2)));
+  const float2_t v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, I);
+  x[2 * I] = v[0];
+  x[2 * I + 1] = v[1];
+}
+
 struct ReadArgs {
   Kv4Pages pages;
   Heads k, v;
   const int64_t* slots;
-  int64_t tokens, items;
+  int64_t tokens;
+  int blocks;  // of one head's keys or values
 };
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
   constexpr int kLanes = D / 8;
-  const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (item >= a.items) return;
-  const int part = (int)(item % kLanes);
-  const int64_t row = item / kLanes;
-  const int64_t token = row % a.tokens;
-  const int which = (int)(row / a.tokens);
+  const int which = (int)blockIdx.x / a.blocks;
+  const int64_t item = (int64_t)((int)blockIdx.x - which * a.blocks) * kThreads + threadIdx.x;
+  const int part = (int)item & (kLanes - 1);
+  const int64_t token = item / kLanes;
+  if (token >= a.tokens) return;
   const bool is_key = which < a.pages.heads;
   const int head = is_key ? which : which - a.pages.heads;
   const int64_t slot = a.slots[token];
   uint32_t word = 0;
-  float scale = 0.0f;
+  float scale = 1.0f;
   if (inside(a.pages, slot)) {
     using L = Kv4<D>;
     const int P = 1 << a.pages.page_log2;
@@ -345,11 +359,14 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
       constexpr int kWords = D / 128;
       word = *reinterpret_cast<const uint32_t*>(at + L::value(P, t, part / kWords) + part % kWords * 4);
     }
-    scale = scale_of(at[is_key ? L::key_scale(P, t, part >> 2) : L::value_scale(P, t, part >> 2)]);
+    // (255 is infinity's exponent, and what is scaled by it is no number)
+    scale = __uint_as_float((uint32_t)at[is_key ? L::key_scale(P, t, part >> 2) : L::value_scale(P, t, part >> 2)] << 23);
   }
   float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = e2m1_value(word >> (4 * i)) * scale;
+  pair_of<0>(x, word, scale);
+  pair_of<1>(x, word, scale);
+  pair_of<2>(x, word, scale);
+  pair_of<3>(x, word, scale);
   const Heads& h = is_key ? a.k : a.v;
   T* out = static_cast<T*>(h.data) + token * h.token_stride + head * h.head_stride + part * 8;
   if constexpr (VEC) {
@@ -538,7 +555,6 @@ int run_kv4_append(void* pages, int64_t num_pages, int page_size, const tw_heads
   a.v = heads_of(v);
   a.slots = slots;
   a.tokens = T;
-  a.items = 2 * k->heads * T * (head_size / 8);
   a.r = Rotary{positions, cos_sin, max_positions, rotary_dim, (flags & TW_ROTARY_INTERLEAVED) != 0,
                (flags & TW_ROTARY_INVERSE) != 0};
   const bool wide = a.turned && wide_columns(head_size, rotary_dim, cos_sin);
@@ -553,11 +569,14 @@ int run_kv4_append(void* pages, int64_t num_pages, int page_size, const tw_heads
                      columns_of(head_size, rotary_dim, q_vec ? 8 : 1), head_size, 0, a.r};
     a.q.items = T * a.q.heads * a.q.columns;
   }
-  int64_t q_blocks;
-  if (int rc = grid_of(what, a.items, &a.kv_blocks)) return rc;
+  int64_t kv_blocks, q_blocks;
+  if (int rc = grid_of(what, T * (head_size / 8), &kv_blocks)) return rc;
   if (int rc = grid_of(what, a.q.items, &q_blocks)) return rc;
-  if (a.kv_blocks + q_blocks > 0x7fffffff) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too many tokens", what);
-  return by_dtype<RunAppend>(dtype, a, head_size, vec, q_vec, a.kv_blocks + q_blocks, stream);
+  a.blocks = (int)kv_blocks;
+  kv_blocks *= 2 * k->heads;
+  if (kv_blocks + q_blocks > 0x7fffffff) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too many tokens", what);
+  a.kv_blocks = (int)kv_blocks;
+  return by_dtype<RunAppend>(dtype, a, head_size, vec, q_vec, kv_blocks + q_blocks, stream);
 }
 
 int run_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void* pages, int64_t num_pages, int page_size,
@@ -576,9 +595,11 @@ int run_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void* pages
   a.v = heads_of(v_out);
   a.slots = slots;
   a.tokens = T;
-  a.items = 2 * k_out->heads * T * (head_size / 8);
   int64_t blocks;
-  if (int rc = grid_of(what, a.items, &blocks)) return rc;
+  if (int rc = grid_of(what, T * (head_size / 8), &blocks)) return rc;
+  a.blocks = (int)blocks;
+  blocks *= 2 * k_out->heads;
+  if (blocks > 0x7fffffff) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too many tokens", what);
   const bool vec = vector_ok(k_out, bytes_of(dtype)) && vector_ok(v_out, bytes_of(dtype));
   return by_dtype<RunRead>(dtype, a, head_size, vec, blocks, stream);
 }
