@@ -76,6 +76,12 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int s) {
 // A sequence's 128-token steps are cut into even pieces, as many in all as the grid holds workgroups,
 // whatever the lengths: a workgroup finds its pieces from the lengths on the device.  The pieces of a
 // sequence that has several go to the workspace as (m, l, O), and attention_join_kernel joins them.
+//
+// What bounds it: the cache's bytes where there are many (256 sequences of 4096 tokens, 8 key heads, D = 128, 1.15 GB:
+// 238 us = 4.8 TB/s, where a large copy reaches 5.16), latencies below some 50 MB: lengths, pages' numbers and keys
+// wait for each other, and the join is a launch of its own (a sequence of 700 tokens 6.7 + 3.5 us, 64 ragged ones of
+// 29.7 MB 13.4 + 3.9).  Two tiles of keys and values are under way in registers, not LDS: no wave needs another's
+// keys, so none waits at a barrier (those 256 sequences took 282 us with barriers, 268 without, 239 with two tiles).
 // ---------------------------------------------------------------------------
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -717,11 +723,16 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
   store4(out, sum * (all > 0.0f || all != all ? 1.0f / all : 0.0f), a.out_wide);
 }
 
-constexpr int kMostRows = 32;  // of the split kernel
+// Of the split kernel, two operands' width.  One new token of each of 8 sequences of 4096, 8 rows: 11 us, in tiles 23;
+// of 300 of 700 with 8 key heads 74 and 211; four new tokens of each of 32 of 4096, 32 rows: 21 and 34.  Up to 16 rows
+// one operand is enough (8 sequences 11 us, with two operands 13; 300 sequences 74 and 91).
+constexpr int kMostRows = 32;
 
 // Cut of a call's steps.  While there is room, every piece has a workgroup of its own and all run at once, two a
 // compute unit (their registers allow no third); sequences and key heads beyond half of that are cut in four
-// pieces a compute unit on top, which the workgroups take in turn.
+// pieces a compute unit on top, which the workgroups take in turn.  8 heads over a key head, D = 128: 64 sequences of
+// 1 to 4096 tokens and 8 key heads 44.7 us so, 47.7 with two pieces a compute unit and 48.5 with eight (all of 2048
+// tokens: 40.9, 33.3 and 46.8), 40 of 16 to 8192 tokens 29.8, 32.4 and 31.7.
 struct SplitPlan {
   int grid, budget;
   int64_t header_bytes, bytes;
@@ -746,8 +757,9 @@ int launch_split(const SplitArgs& args, int grid, void* stream) {
   auto kernel = args.rows <= 16 ? attention_split_kernel<T, D, 1> : attention_split_kernel<T, D, 2>;
   launch_kernel(kernel, dim3((unsigned)grid), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), args);
   if (int rc = finish_launch("kv4_attention")) return rc;
-  // few sequences may be in very many pieces: more workgroups then share a row's channels
-  const bool few = (int64_t)args.a.num_seqs * args.a.pages.heads <= 16;
+  // Few rows may be in very many pieces: more workgroups then share a row's channels (one sequence of 65536 tokens,
+  // 8 rows: 12.3 us so and 13.7 with whole rows; two of 32768 and 8 key heads, 128 rows: 25.7 and 23.9).
+  const bool few = (int64_t)args.a.num_seqs * args.a.pages.heads * args.rows <= 32;
   launch_kernel(few ? attention_join_kernel<T, D, 32> : attention_join_kernel<T, D, D>,
                 dim3((unsigned)(args.a.num_seqs * args.a.pages.heads), (unsigned)args.rows, few ? D / 32 : 1), dim3(kJoinThreads), 0,
                 static_cast<hipStream_t>(stream), args);
@@ -770,7 +782,12 @@ int launch_split(const SplitArgs& args, int D, int grid, void* stream) {
 // tokens in the order in which the scores' registers hold them: of 16 tokens 0-3, 8-11, 4-7, 12-15.
 //
 // The matrix and the vector units work side by side: the scores of the next 32 tokens are computed between the
-// exponentials of the present ones, and their maximum is found between the present products with the values.
+// exponentials of the present ones, whose sums come between the present products with the values.  Two waves a SIMD
+// unit with 32 rows each: one wave with 64 rows reads LDS half as often, but nothing runs while it moves data (229
+// us against 188, for 8192 queries of 8 heads over one key head, D = 128).  What bounds it: the vector unit; of a
+// wave's 32 tokens the products take 512 cycles, the 16 exponentials a lane 256 and some 55 other vector
+// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 172 us with its
+// join of 15, 797 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
@@ -801,7 +818,7 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, const Sequence& 
   return {from, max((min(new_from + last / a.group + 1, q.length) + kSpan - 1) / kSpan, from)};
 }
 
-constexpr int kMostShared = 1024;  // tiles times key heads that are worked on in even shares
+constexpr int kMostShared = 4096;  // tiles times key heads that are worked on in even shares (their ends are in LDS)
 
 // Sum over the workgroup's threads before this one, and over all.
 template <int THREADS>
@@ -849,7 +866,7 @@ __device__ __forceinline__ FoundTile find_tile(const AttentionArgs& a, int tile,
 }
 
 // Many rows: probabilities are held times 2^(kTileLift - m).  m need not be the maximum so far, only within kSlack of
-// it: so they stay below 2^15, fp16's normal range reaches down to 2^-13 of the largest or lower and its subnormals to
+// it: so they stay below 2^15, fp16's normal range reaches down to 2^-21 of the largest or lower and its subnormals to
 // 2^-31, and a row's sums are multiplied anew a few times in all instead of in most units (one of 64 rows has a new
 // maximum in most of the first hundred units: 211 us with the maximum itself and 188 us so, for 8192 rows of 8 heads).
 constexpr float kTileLift = 7.0f, kSlack = 8.0f;
@@ -1441,9 +1458,12 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
   }
 }
 
-// Tiles of a call, and whether they are worked on in even shares: while there are few they do not even out among
-// themselves (a prompt's tiles reach back differently far, and what is left over of a last round of workgroups
-// counts), and a part more or less is little beside a compute unit that waits.
+// Tiles of a call, and whether they are worked on in even shares: they do not even out among themselves (a prompt's
+// tiles reach back differently far, and what is left over of a last round of workgroups counts), and a part more or
+// less is little beside a compute unit that waits.  Not where a sequence has room for 256 tokens or less, whose tiles
+// are about equal and soon done, and not for more tiles than there is LDS for.  In even shares and in a workgroup
+// each, 8 heads over one key head, D = 128: a prompt of 8192 tokens 196 and 259 us, eight of them 1121 and 1178, 32 of
+// 2048 359 and 484, 64 of 512 95 and 113; 400 of 200 tokens 216 and 198, 500 of 64 70 and 65.
 struct TilePlan {
   int tiles, grid;  // grid: of the even shares; 0: none
   int64_t header_bytes, bytes;
@@ -1458,7 +1478,7 @@ TilePlan plan_tiles(int64_t T, int group, int kv_heads, int head_size, int64_t n
   const int cus = device_compute_units();
   plan.tiles = (int)min(tiles, (int64_t)0x7fffffff);
   // (spans are counted in 32 bits)
-  const bool few = tiles * kv_heads <= kMostShared && num_seqs <= kMostShared &&
+  const bool few = tiles * kv_heads <= kMostShared && num_seqs <= kMostShared && capacity > 256 &&
                    (double)(tiles * kv_heads) * (double)(capacity / kSpan + 1) < 2e9;
   plan.grid = few ? (cus > 0 ? cus : 256) : 0;
   plan.header_bytes = (tiles * kv_heads * (int64_t)sizeof(TileHeader) + 15) / 16 * 16;
