@@ -786,8 +786,8 @@ int launch_split(const SplitArgs& args, int D, int grid, void* stream) {
 // unit with 32 rows each: one wave with 64 rows reads LDS half as often, but nothing runs while it moves data (229
 // us against 188, for 8192 queries of 8 heads over one key head, D = 128).  What bounds it: the vector unit; of a
 // wave's 32 tokens the products take 512 cycles, the 16 exponentials a lane 256 and some 55 other vector
-// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 172 us with its
-// join of 15, 797 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
+// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 174 us with its
+// join of 15, 789 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
