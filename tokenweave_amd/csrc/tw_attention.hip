@@ -786,8 +786,8 @@ int launch_split(const SplitArgs& args, int D, int grid, void* stream) {
 // unit with 32 rows each: one wave with 64 rows reads LDS half as often, but nothing runs while it moves data (229
 // us against 188, for 8192 queries of 8 heads over one key head, D = 128).  What bounds it: the vector unit; of a
 // wave's 32 tokens the products take 512 cycles, the 16 exponentials a lane 256 and some 55 other vector
-// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 174 us with its
-// join of 15, 789 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
+// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 168 us with its
+// join of 15, 819 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
@@ -1188,8 +1188,9 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
         if (t >= row_end || t < row_begin || missing >> (j / 8) & 1) sc[j] = -__builtin_inff();
       }
     };
-    // LDS is read kAhead products before the product, the first keys of a unit in the unit before it.
-    constexpr int kProducts = D / 16, kAhead = 4;
+    // LDS is read kAhead products before the product, the first keys of a unit in the unit before it (two, three or
+    // four ahead: the same time; two leave registers).
+    constexpr int kProducts = D / 16, kAhead = 2;
     auto value = [&](const uint8_t* values, int z) {
       return *reinterpret_cast<const half8_t*>(values + (z % (D / 32) * 32 + n) * S::kValueRow + h * 16 + z / (D / 32) * 32);
     };
@@ -1241,8 +1242,12 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    auto sees = [&](int t0) { return t0 < min(wave_to, tile_to * S::kTokens) && t0 + 32 > wave_from; };
-    auto all_see = [&](int t0, int missing) { return t0 >= all_from && t0 + 32 <= all_to && (missing & 3) == 0; };
+    // Of the unit that begins at a token: whether a row of the wave sees some of it, whether all see all of it.
+    const int piece_to = tile_to * S::kTokens, see_from = wave_from - 31;
+    const uint32_t see_span = max(min(wave_to, piece_to) - see_from, 0);
+    const uint32_t all_span = max(min(all_to, piece_to) - 31 - all_from, 0);
+    auto sees = [&](int t0) { return (uint32_t)(t0 - see_from) < see_span; };
+    auto all_see = [&](int t0, int missing) { return (uint32_t)(t0 - all_from) < all_span && (missing & 3) == 0; };
 
     // Probabilities are held times 2^(kTileLift - m), where m need not be the maximum so far: it is raised to the
     // maximum where a row sees its first token and where the maximum is kSlack above it.
@@ -1251,8 +1256,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     auto work_on = [&](int t0, float16_t& sc, float16_t& sc_next, const uint8_t* keys_next, const uint8_t* keys_after,
                        const uint8_t* values, int missing_next) {
       const int t1 = t0 + 32;
-      const bool mine = sees(t0), mine_next = sees(t1);
-      if (!mine && !mine_next) {
+      const bool mine_next = sees(t1);
+      if (!mine_next && !sees(t0)) {
         first_keys(keys_after);
         return;
       }
@@ -1277,7 +1282,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
           p[j / 8][j % 8] = (_Float16)x[j];
         }
       }
-      if (!mine_next || !all_see(t1, missing_next)) mask(sc_next, mine_next ? t1 : 1 << 30, missing_next);
+      if (!all_see(t1, missing_next)) mask(sc_next, mine_next ? t1 : 1 << 30, missing_next);
       gather_beside_sums(p, x, values, keys_after);
     };
 
@@ -1318,6 +1323,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     if constexpr (S::kKeyBuffers == 2) lds_barrier();
     // Keys of the unit after next, whatever is there where there is none: they are read and not used.
     first_keys(S::kUnits == 2 ? keys_now + 32 * S::kKeyRow : keys_next);
+    // (what comes last in a step goes first where both waves of a SIMD unit could: 174 us without, 169 with it)
+    if (S::kApart && wave * 64 >= S::kValueThread) __builtin_amdgcn_s_setprio(1);
     auto advance = [&](int at, float16_t& first, float16_t& second) {
       const int t0 = at * S::kTokens;
       const uint8_t* values = value_buffers[(at - tile_from) & 1];
@@ -1354,6 +1361,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
       advance(at, even, odd);
       if (S::kUnits == 1 && at + 1 < tile_to) advance(at + 1, odd, even);
     }
+    if (S::kApart) __builtin_amdgcn_s_setprio(0);
     if (odd_unit == unit) {
       uint32_t mine = 0;  // a bit for each 32 channels
 #pragma unroll 1
