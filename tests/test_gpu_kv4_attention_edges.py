@@ -83,6 +83,30 @@ def test_running_maxima_that_move(lengths, news, D, how, dtype):
     check(c, c.run())
 
 
+@pytest.mark.parametrize("news", [3, 200])
+@pytest.mark.parametrize("first, second", [(-2000.0, 300.0), (-30000.0, 5.0), (4000.0, 4002.0), (700.0, -900.0)])
+def test_scores_far_from_zero(first, second, news):
+    """Scores around one value in the first half and around another in the second.  Beside the reference's bound:
+    a score's own error, the sum of |q k| 2^-21, is as large as some of these scores' differences, so a probability is
+    off by no more than a factor of exp of twice it."""
+    c = Case([400], [news], 8, 1, 128, 32)
+    direction = torch.where(torch.arange(128, device=DEV) % 2 == 0, 1.0, -1.0)
+    t = torch.arange(400, device=DEV)
+    by = torch.where(t < 100, first, second)[:, None, None]
+    k = torch.randn(400, 1, 128, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)) * by.abs() * 2.0 ** -10
+    slots = c.slots(0, 400)
+    c.cache.append(k + by * direction / 128 ** 0.5, c.values[0].transpose(0, 1).float().to(DEV).contiguous(), slots)
+    c.keys[0] = c.cache.read(slots, torch.float32)[0].double().cpu().transpose(0, 1)
+    c.q = direction.expand(news, 8, 128).contiguous().to(torch.bfloat16)
+    got = c.run()
+    want, mean, size = attend(c.q, c.keys, c.values, c.lengths, c.news, 128 ** -0.5)
+    most = float(c.values[0].abs().max())
+    off = torch.expm1(2 * size * 2.0 ** -21)
+    bound = attend_bound(want, mean, 0 * size, got.dtype, 400) + (mean + want.abs()) * off + 400 * 2.0 ** -32 * most
+    far = (got.double().cpu() - want).abs()
+    assert (far <= bound).all(), (float((far - bound).max()), float((far / bound).max()))
+
+
 def test_more_sequences_than_a_wave_holds():
     g = torch.Generator().manual_seed(5)
     lengths = torch.randint(0, 200, (330,), generator=g).tolist()

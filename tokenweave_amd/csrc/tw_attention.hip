@@ -498,7 +498,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
           }
           most = fmaxf(most, x[i]);
         }
-        most = max32(max16(most)) * scale[t];
+        // (a whole number: neither kLift - m nor the factor from one m to the next is rounded)
+        most = __builtin_rintf(max32(max16(most)) * scale[t]);
         if (__builtin_amdgcn_ballot_w64(most > m[t])) {
           const float now = fmaxf(m[t], most);
           const float old = m[t] == now ? 1.0f : __builtin_amdgcn_exp2f(m[t] - now);
@@ -866,7 +867,7 @@ __device__ __forceinline__ FoundTile find_tile(const AttentionArgs& a, int tile,
 }
 
 // Many rows: probabilities are held times 2^(kTileLift - m).  m need not be the maximum so far, only within kSlack of
-// it: so they stay below 2^15, fp16's normal range reaches down to 2^-21 of the largest or lower and its subnormals to
+// it: so they stay within 2^15, fp16's normal range reaches down to 2^-21 of the largest or lower and its subnormals to
 // 2^-31, and a row's sums are multiplied anew a few times in all instead of in most units (one of 64 rows has a new
 // maximum in most of the first hundred units: 211 us with the maximum itself and 188 us so, for 8192 rows of 8 heads).
 constexpr float kTileLift = 7.0f, kSlack = 8.0f;
@@ -1250,7 +1251,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     auto all_see = [&](int t0, int missing) { return (uint32_t)(t0 - all_from) < all_span && (missing & 3) == 0; };
 
     // Probabilities are held times 2^(kTileLift - m), where m need not be the maximum so far: it is raised to the
-    // maximum where a row sees its first token and where the maximum is kSlack above it.
+    // maximum where a row sees its first token and where the maximum is kSlack above it.  It is a whole number, so
+    // that neither kTileLift - m nor the factor from one m to the next is rounded, however large the scores.
     float add = kTileLift, limit = row < rows ? -__builtin_inff() : __builtin_inff();
     // The unit of tokens t0 .. t0 + 31, whose scores are there; the scores of the next come.
     auto work_on = [&](int t0, float16_t& sc, float16_t& sc_next, const uint8_t* keys_next, const uint8_t* keys_after,
@@ -1267,7 +1269,10 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
       // (the probabilities stay before the branch)
       asm volatile("" : "+v"(p[0]), "+v"(p[1]));
       if (__builtin_amdgcn_ballot_w64(most > limit)) {
-        const float higher = max32(most) - add, raised = max32(most) > limit ? higher : m;
+        float top = sc[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[j]);
+        const float raised = max32(most) > limit ? __builtin_rintf(max32(top) * scale) : m;
         const float old = m == raised ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
         m = raised;
         limit = m == -__builtin_inff() ? limit : kTileLift + kSlack;
