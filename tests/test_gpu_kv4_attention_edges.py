@@ -107,6 +107,34 @@ def test_scores_far_from_zero(first, second, news):
     assert (far <= bound).all(), (float((far - bound).max()), float((far / bound).max()))
 
 
+@pytest.mark.parametrize("news", [1, 100])
+def test_many_small_probabilities_beside_a_large_one(news):
+    """One token, and 8000 that are 2^-22 of it each: together they are 0.2 % of the sum, and of the output."""
+    c = Case([8001], [news], 4, 1, 128, 64)
+    direction = torch.where(torch.arange(128, device=DEV) % 2 == 0, 1.0, -1.0)
+    by = torch.full((8001, 1, 1), -8.0, device=DEV)
+    by[5] = 8.0
+    v = torch.ones(8001, 1, 128, device=DEV)
+    v[5] = 0.5
+    slots = c.slots(0, 8001)
+    c.cache.append((by * direction).contiguous(), v, slots)
+    c.keys[0], c.values[0] = (x.double().cpu().transpose(0, 1) for x in c.cache.read(slots, torch.float32))
+    # a score is +-8 * 128 * size * 128^-0.5
+    size = 22 * math.log(2) / 16 / 128 ** 0.5
+    c.q = (direction * size).expand(news, 4, 128).contiguous().to(torch.float16)
+    check(c, c.run())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("news", [1, 40])
+def test_one_visible_token_is_copied(news, dtype):
+    """A softmax over one token is one: the output is the value, which both types hold exactly."""
+    c = Case([50], [news], 8, 2, 64, 16, dtype)
+    got = c.run(window=1)
+    want = c.values[0][:, 50 - news:].transpose(0, 1).repeat_interleave(4, 1)
+    assert torch.equal(got.double().cpu(), want)
+
+
 def test_more_sequences_than_a_wave_holds():
     g = torch.Generator().manual_seed(5)
     lengths = torch.randint(0, 200, (330,), generator=g).tolist()

@@ -305,6 +305,10 @@ __device__ __forceinline__ void store4(T* out, const float4_t& x, bool wide) {
   }
 }
 
+// The exponents' base for a maximum: the next 64th.  Neither kLift - m nor the factor from one m to the next is rounded
+// then, however large the scores, and the largest probabilities are just below a power of two, where fp16 is finest.
+__device__ __forceinline__ float base_of(float most) { return __builtin_ceilf(most * 64.0f) * 0.015625f; }
+
 constexpr float kLift = 14.0f;  // probabilities are held times 2^14: fp16's normal range reaches down to 2^-28 of the largest
 
 template <typename T, int D, int NT>
@@ -434,6 +438,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
       row_end[t] = row < rows ? new_from + i + 1 : 0;
       row_begin[t] = a.window > 0 ? max(new_from + i + 1 - a.window, 0) : 0;
     }
+    float one = 1.0f;
+    asm volatile("" : "+s"(one));  // (not known: a conversion and an addition are one instruction then)
     Tile<D> even, odd;
     Place even_place = place_of(step0, first_ids), odd_place = place_of(step0 + 1, ids);
     load_keys<D>(even, even_place, offsets, P);
@@ -498,8 +504,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
           }
           most = fmaxf(most, x[i]);
         }
-        // (a whole number: neither kLift - m nor the factor from one m to the next is rounded)
-        most = __builtin_rintf(max32(max16(most)) * scale[t]);
+        most = base_of(max32(max16(most)) * scale[t]);
         if (__builtin_amdgcn_ballot_w64(most > m[t])) {
           const float now = fmaxf(m[t], most);
           const float old = m[t] == now ? 1.0f : __builtin_amdgcn_exp2f(m[t] - now);
@@ -512,9 +517,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale[t], add));
-          sum += x[i];
-          p[t][i] = (_Float16)x[i];
+          p[t][i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale[t], add));
+          sum = __builtin_fmaf((float)p[t][i], one, sum);  // (as rounded: one token's output is its value, to the bit)
         }
         l[t] += sum;
       }
@@ -1202,12 +1206,12 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     };
     // The next unit's scores and the present probabilities, product by product: each with its share of the 16
     // exponentials, whose rounding comes one product later.  Returns the largest exponent.
-    auto scores_beside_probabilities = [&](float16_t& sc_next, const uint8_t* keys, const uint8_t* values, float16_t& x,
+    auto scores_beside_probabilities = [&](float16_t& sc_next, const uint8_t* keys, const uint8_t* values,
                                            half8_t (&p)[2], const float16_t& sc, float add) {
       constexpr int kEach = 16 / kProducts;
 #pragma unroll
       for (int j = 0; j < 16; ++j) sc_next[j] = 0.0f;
-      float most = -__builtin_inff();
+      float most = -__builtin_inff(), x[16];
 #pragma unroll
       for (int z = 0; z <= kProducts; ++z) {
         if (z < kProducts) {
@@ -1231,15 +1235,20 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
       }
       return most;
     };
-    // The present products with the values, the probabilities' sums among them.
-    auto gather_beside_sums = [&](const half8_t (&p)[2], const float16_t& x, const uint8_t* values, const uint8_t* keys_after) {
+    // The present products with the values, the sums of the probabilities as rounded among them (`one`: as above).
+    float one = 1.0f;
+    asm volatile("" : "+s"(one));
+    auto gather_beside_sums = [&](const half8_t (&p)[2], const uint8_t* values, const uint8_t* keys_after) {
       constexpr int kEach = 16 / kProducts;
 #pragma unroll
       for (int z = 0; z < kProducts; ++z) {
         o[z % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[z % kAhead], p[z / (D / 32)], o[z % (D / 32)], 0, 0, 0);
         ahead[z % kAhead] = z + kAhead < kProducts ? value(values, z + kAhead) : key(keys_after, z + kAhead - kProducts);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) l[(z * kEach + e) % 4] += x[z * kEach + e];
+        for (int e = 0; e < kEach; ++e) {
+          const int i = z * kEach + e;
+          l[i % 4] = __builtin_fmaf((float)p[i / 8][i % 8], one, l[i % 4]);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -1251,8 +1260,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     auto all_see = [&](int t0, int missing) { return (uint32_t)(t0 - all_from) < all_span && (missing & 3) == 0; };
 
     // Probabilities are held times 2^(kTileLift - m), where m need not be the maximum so far: it is raised to the
-    // maximum where a row sees its first token and where the maximum is kSlack above it.  It is a whole number, so
-    // that neither kTileLift - m nor the factor from one m to the next is rounded, however large the scores.
+    // maximum where a row sees its first token and where the maximum is kSlack above it.
     float add = kTileLift, limit = row < rows ? -__builtin_inff() : __builtin_inff();
     // The unit of tokens t0 .. t0 + 31, whose scores are there; the scores of the next come.
     auto work_on = [&](int t0, float16_t& sc, float16_t& sc_next, const uint8_t* keys_next, const uint8_t* keys_after,
@@ -1264,15 +1272,14 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
         return;
       }
       half8_t p[2];
-      float16_t x;
-      const float most = scores_beside_probabilities(sc_next, keys_next, values, x, p, sc, add);
+      const float most = scores_beside_probabilities(sc_next, keys_next, values, p, sc, add);
       // (the probabilities stay before the branch)
       asm volatile("" : "+v"(p[0]), "+v"(p[1]));
       if (__builtin_amdgcn_ballot_w64(most > limit)) {
         float top = sc[0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[j]);
-        const float raised = max32(most) > limit ? __builtin_rintf(max32(top) * scale) : m;
+        const float raised = max32(most) > limit ? base_of(max32(top) * scale) : m;
         const float old = m == raised ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
         m = raised;
         limit = m == -__builtin_inff() ? limit : kTileLift + kSlack;
@@ -1282,13 +1289,10 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) o[c] *= old;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j], scale, add));
-          p[j / 8][j % 8] = (_Float16)x[j];
-        }
+        for (int j = 0; j < 16; ++j) p[j / 8][j % 8] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sc[j], scale, add));
       }
       if (!all_see(t1, missing_next)) mask(sc_next, mine_next ? t1 : 1 << 30, missing_next);
-      gather_beside_sums(p, x, values, keys_after);
+      gather_beside_sums(p, values, keys_after);
     };
 
     // ---- While tile `at` is worked on, its keys and values and the next tile's keys are in LDS.  Keys are laid out
