@@ -1,9 +1,10 @@
 // Attention over the 4-bit paged cache (tw_kv4.h) for gfx950 (wave64).
 //
-//   o = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),  s_t = scale * log2(e) * q k_t,  m = max_t s_t
+//   o = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),  s_t = scale * log2(e) * q k_t,  any m near max_t s_t
 //
 // in one pass over the tokens: when a larger s appears, what has been summed is multiplied by
-// 2^(m - m').  Scores, m, sums and the output are fp32; the output is rounded once.
+// 2^(m - m').  Scores, m, sums and the output are fp32, the probabilities in both sums fp16; the output
+// is rounded once.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -78,7 +79,7 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int s) {
 // sequence that has several go to the workspace as (m, l, O), and attention_join_kernel joins them.
 //
 // What bounds it: the cache's bytes where there are many (256 sequences of 4096 tokens, 8 key heads, D = 128, 1.15 GB:
-// 238 us = 4.8 TB/s, where a large copy reaches 5.16), latencies below some 50 MB: lengths, pages' numbers and keys
+// 240 us = 4.8 TB/s, where a large copy reaches 5.16), latencies below some 50 MB: lengths, pages' numbers and keys
 // wait for each other, and the join is a launch of its own (a sequence of 700 tokens 6.7 + 3.5 us, 64 ragged ones of
 // 29.7 MB 13.4 + 3.9).  Two tiles of keys and values are under way in registers, not LDS: no wave needs another's
 // keys, so none waits at a barrier (those 256 sequences took 282 us with barriers, 268 without, 239 with two tiles).
@@ -791,8 +792,8 @@ int launch_split(const SplitArgs& args, int D, int grid, void* stream) {
 // unit with 32 rows each: one wave with 64 rows reads LDS half as often, but nothing runs while it moves data (229
 // us against 188, for 8192 queries of 8 heads over one key head, D = 128).  What bounds it: the vector unit; of a
 // wave's 32 tokens the products take 512 cycles, the 16 exponentials a lane 256 and some 55 other vector
-// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 168 us with its
-// join of 15, 819 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
+// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 169 us with its
+// join of 15, 813 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
