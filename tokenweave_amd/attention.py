@@ -169,19 +169,54 @@ class CachedBatch:
 
     def split(self, tokens: int) -> Tuple["CachedBatch", "CachedBatch"]:
         """The first `tokens` tokens and the rest, as the woven schedule runs them one after the other.
-        A sequence that both hold ends, in the first, with its last token there."""
-        if tokens not in self._splits:
-            starts = self.query_starts
-            if starts is None:
-                n = self.seq_lens.numel()
-                starts = torch.arange(n + 1, dtype=torch.int32, device=self.seq_lens.device) * (self.slots.numel() // max(n, 1))
-            first, second = starts.clamp(max=tokens), (starts - tokens).clamp(min=0)
-            hidden = (second[1:] - second[:-1]).to(self.seq_lens.dtype)
-            self._splits[tokens] = tuple(
-                CachedBatch(slots, self.block_table, lens, at.contiguous(), self.max_queries)
-                for slots, lens, at in ((self.slots[:tokens], self.seq_lens - hidden, first),
-                                        (self.slots[tokens:], self.seq_lens, second)))
-        return self._splits[tokens]
+        A sequence that both hold ends, in the first, with its last token there.  The halves hold no
+        lengths or starts of their own: they follow this batch's tensors where those change in place."""
+        whole = (self.slots, self.block_table, self.seq_lens, self.query_starts, self.max_queries)
+        halves = self._splits.get(tokens)
+        if halves is None or any(a is not b for a, b in zip(halves[0].whole, whole)):
+            halves = self._splits[tokens] = (_Half(whole, tokens, False), _Half(whole, tokens, True))
+        return halves
+
+
+class _Half(CachedBatch):
+    """A batch's first tokens or the others.  What it says of them is computed from the whole batch's
+    tensors every time it is asked for: lengths and starts may change in place, and where the question
+    is part of a captured step, so is the answer (five small operations for a first half, two for a second)."""
+
+    def __init__(self, whole: Tuple[Any, ...], tokens: int, second: bool) -> None:
+        self.whole, self.tokens, self.second = whole, tokens, second
+        self._splits = {}
+
+    def _starts(self) -> torch.Tensor:
+        """The whole batch's query_starts."""
+        slots, _, lens, starts, _ = self.whole
+        if starts is None:
+            n = lens.numel()
+            starts = torch.arange(n + 1, dtype=torch.int32, device=lens.device) * (slots.numel() // max(n, 1))
+        return starts
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self.whole[0][self.tokens:] if self.second else self.whole[0][:self.tokens]
+
+    @property
+    def block_table(self) -> torch.Tensor:
+        return self.whole[1]
+
+    @property
+    def seq_lens(self) -> torch.Tensor:
+        if self.second:
+            return self.whole[2]
+        behind = (self._starts() - self.tokens).clamp_(min=0)
+        return self.whole[2] - (behind[1:] - behind[:-1])
+
+    @property
+    def query_starts(self) -> torch.Tensor:
+        return (self._starts() - self.tokens).clamp_(min=0) if self.second else self._starts().clamp(max=self.tokens)
+
+    @property
+    def max_queries(self) -> Optional[int]:
+        return self.whole[4]
 
 
 class PagedSelfAttention(nn.Module):
