@@ -1,4 +1,5 @@
 """The halves of a step's tokens: they follow their batch's tensors."""
+import pytest
 import torch
 
 import tokenweave_amd as tw
@@ -39,3 +40,30 @@ def test_halves_follow_tensors_that_are_replaced():
     first, second = batch.split(2)
     assert first.seq_lens[:2].tolist() == [1, 2] and second.seq_lens[-2:].tolist() == [3, 4]
     assert first.slots.tolist() + second.slots.tolist() == [7, 8, 9, 10]
+
+
+def test_halves_keep_a_bound_on_a_sequences_new_tokens():
+    """The bound picks the kernel: without one, a half with starts counts all its tokens as one sequence's."""
+    table = torch.zeros(4, 2, dtype=torch.int32)
+    for each, cut in ((1, 2), (1, 4), (3, 6), (3, 5), (3, 0)):
+        lens = torch.full((4,), 40, dtype=torch.int32)
+        batch = tw.CachedBatch(torch.arange(4 * each), table, lens)
+        covered = []
+        for half, base in zip(batch.split(cut), (0, cut)):
+            n, starts = half.seq_lens.numel(), half.query_starts
+            assert half.block_table.shape == (n, 2)
+            if starts is None:     # the op's own bound: the same number each
+                assert half.max_queries in (None, each) and half.slots.numel() == n * each
+                starts = torch.arange(n + 1) * each
+            else:
+                assert half.max_queries == each
+            assert (starts[1:] - starts[:-1]).max() <= each if n else half.slots.numel() == 0
+            covered += half.slots[int(starts[0]):int(starts[-1])].tolist()
+        assert covered == list(range(4 * each))
+    starts = torch.tensor([0, 3, 4], dtype=torch.int32)
+    for bound in (None, 3):
+        batch = tw.CachedBatch(torch.arange(4), table[:2], torch.tensor([9, 9], dtype=torch.int32), starts, bound)
+        assert all(half.max_queries == bound for half in batch.split(2))
+    # what the op refuses of a whole batch is refused of its halves
+    with pytest.raises(RuntimeError, match="same number for each"):
+        tw.CachedBatch(torch.arange(5), table[:2], torch.tensor([9, 9], dtype=torch.int32)).split(2)

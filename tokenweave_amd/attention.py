@@ -181,18 +181,29 @@ class CachedBatch:
 class _Half(CachedBatch):
     """A batch's first tokens or the others.  What it says of them is computed from the whole batch's
     tensors every time it is asked for: lengths and starts may change in place, and where the question
-    is part of a captured step, so is the answer (five small operations for a first half, two for a second)."""
+    is part of a captured step, so is the answer (five small operations for a first half, two for a second).
+    Whole sequences with the same number of new tokens each are views, without any operation."""
 
     def __init__(self, whole: Tuple[Any, ...], tokens: int, second: bool) -> None:
         self.whole, self.tokens, self.second = whole, tokens, second
         self._splits = {}
+        slots, _, lens, starts, _ = whole
+        # new tokens of each sequence; 0: not the same for all
+        self._each = slots.numel() // max(lens.numel(), 1) if starts is None else 0
+        if starts is None and slots.numel() != self._each * lens.numel():
+            raise RuntimeError(f"{slots.numel()} tokens are not the same number for each of {lens.numel()} sequences: "
+                               "pass query_starts")
+        # the sequences of this half, where none is in both
+        self._rows = None
+        if self._each and tokens % self._each == 0:
+            at = tokens // self._each
+            self._rows = slice(at, None) if second else slice(0, at)
 
     def _starts(self) -> torch.Tensor:
         """The whole batch's query_starts."""
-        slots, _, lens, starts, _ = self.whole
+        lens, starts = self.whole[2:4]
         if starts is None:
-            n = lens.numel()
-            starts = torch.arange(n + 1, dtype=torch.int32, device=lens.device) * (slots.numel() // max(n, 1))
+            starts = torch.arange(lens.numel() + 1, dtype=torch.int32, device=lens.device) * self._each
         return starts
 
     @property
@@ -201,22 +212,28 @@ class _Half(CachedBatch):
 
     @property
     def block_table(self) -> torch.Tensor:
-        return self.whole[1]
+        return self.whole[1] if self._rows is None else self.whole[1][self._rows]
 
     @property
     def seq_lens(self) -> torch.Tensor:
+        if self._rows is not None:
+            return self.whole[2][self._rows]
         if self.second:
             return self.whole[2]
         behind = (self._starts() - self.tokens).clamp_(min=0)
         return self.whole[2] - (behind[1:] - behind[:-1])
 
     @property
-    def query_starts(self) -> torch.Tensor:
+    def query_starts(self) -> Optional[torch.Tensor]:
+        if self._rows is not None:
+            return None
         return (self._starts() - self.tokens).clamp_(min=0) if self.second else self._starts().clamp(max=self.tokens)
 
     @property
     def max_queries(self) -> Optional[int]:
-        return self.whole[4]
+        """The whole batch's bound; where it names none and its sequences have the same number, that number."""
+        bound = self.whole[4]
+        return self._each if bound is None and self.whole[3] is None else bound
 
 
 class PagedSelfAttention(nn.Module):
