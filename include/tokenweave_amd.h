@@ -384,8 +384,10 @@ TW_API int tw_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void*
  *                query_starts[s+1] - 1 of q and out, the last of its cached tokens; NULL:
  *                num_tokens / num_seqs tokens each
  * Query i of n sees the tokens up to its own, seq_len - n + i, and of these the last
- * `window` where window > 0.  A query that sees none gives zeros.  max_queries: at least the
- * largest number of new tokens of a sequence (more than that are not computed).
+ * `window` where window > 0.  A query that sees none gives zeros, and so do tokens of q before
+ * query_starts[0] and from query_starts[num_seqs] on, which no sequence has (padding).
+ * max_queries: at least the largest number of new tokens of a sequence (tokens of a sequence
+ * behind that many are not computed, and their rows of out are left as they were).
  * bf16 or fp16; scores and sums in fp32.  seq_lens may change between the replays of a
  * captured call.
  * workspace: tw_kv4_attention_workspace() bytes, 16-byte aligned, contents of no meaning

@@ -918,8 +918,9 @@ def kv4_attention(out: torch.Tensor, q: torch.Tensor, pages: torch.Tensor, block
     head g.  `block_table` [sequences, pages] int32 names a sequence's pages, `seq_lens` its cached
     tokens, `query_starts` [sequences + 1] int32 its first token in q (None: the same number of tokens
     for each sequence).  A token sees the cached tokens up to its own, of these the last `window` where
-    that is above 0; one that sees none gives zeros.  `max_queries`: the most new tokens of a sequence
-    (needed with query_starts, where it defaults to all of q's)."""
+    that is above 0; one that sees none gives zeros, and so does one before or behind all sequences'
+    (padding).  `max_queries`: the most new tokens of a sequence (needed with query_starts, where it
+    defaults to all of q's); rows of a sequence's tokens behind it are left as they were."""
     if _fast is not None and not _tracing() and _fast.kv4_attention(out, q, pages, block_table, seq_lens, scale,
                                                                     query_starts, max_queries, window):
         return

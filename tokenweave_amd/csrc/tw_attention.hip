@@ -321,6 +321,34 @@ __device__ __forceinline__ float below(float x, float scale, float m) {
   return s - m;
 }
 
+// Rows of tokens that no sequence has, before the first one's and behind the last one's: zeros, by all
+// threads of the launch.
+struct Rest {
+  int before, behind;  // [0, before) and [behind, num_tokens)
+};
+__device__ __forceinline__ Rest rest_of(const AttentionArgs& a) {
+  if (!a.query_starts) return {0, a.num_tokens};
+  const int first = constant(a.query_starts)[0], last = constant(a.query_starts)[a.num_seqs];
+  const int before = min(max(first, 0), a.num_tokens);
+  return {before, min(max(last, before), a.num_tokens)};
+}
+template <typename T, int D, int THREADS>
+__device__ __forceinline__ void clear_rest(const AttentionArgs& a) {
+  const Rest rest = rest_of(a);
+  const int tokens = rest.before + a.num_tokens - rest.behind;
+  if (tokens == 0) return;
+  const int64_t heads = a.pages.heads * a.group, columns = D / 4;
+  const int64_t block = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  const int64_t threads = (int64_t)gridDim.x * gridDim.y * gridDim.z * THREADS;
+  for (int64_t i = block * THREADS + threadIdx.x; i < tokens * heads * columns; i += threads) {
+    const int64_t row = i / columns;
+    const int at = (int)(row / heads), token = at < rest.before ? at : at - rest.before + rest.behind;
+    store4(static_cast<T*>(a.out) + (int64_t)token * a.out_token + (row - at * heads) * a.out_head +
+               (i - row * columns) * 4,
+           float4_t{0, 0, 0, 0}, a.out_wide);
+  }
+}
+
 constexpr float kLift = 14.0f;  // probabilities are held times 2^14: fp16's normal range reaches down to 2^-28 of the largest
 
 template <typename T, int D, int NT>
@@ -690,6 +718,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
   const int s = blockIdx.x / a.pages.heads, head = blockIdx.x - s * a.pages.heads, row = blockIdx.y, ch0 = blockIdx.z * CH;
   const PieceHeader header = args.headers[blockIdx.x];
   const Sequence seq = sequence<true>(a, s);
+  clear_rest<T, D, kJoinThreads>(a);
   // (a sequence without new tokens has no piece and leaves its header as it was)
   if (row >= min(seq.count, a.max_queries) * a.group || header.count < 2) return;
   constexpr int kLanes = CH / 4, kGroups = kJoinThreads / kLanes, kAtOnce = 8;
@@ -955,6 +984,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads;
   const int window = a.window > 0 ? a.window : 1 << 30;
 
+  clear_rest<T, D, S::kThreads>(a);
   if (threadIdx.x == 0) odd_unit = -1;  // (a barrier follows, with the search for the tiles)
 
   // ---- Which tiles: one, or an even share of all tiles' spans.  In the order of the shares a long tile of a prompt
@@ -1555,6 +1585,21 @@ int launch_tiles(const TileArgs& args, int D, int grid, void* stream) {
   return launch_tiles<T, 256>(args, grid, stream);
 }
 
+// A call without a new token of any sequence: all tokens are padding.
+template <typename T, int D>
+__global__ __launch_bounds__(kJoinThreads) void attention_clear_kernel(AttentionArgs a) {
+  clear_rest<T, D, kJoinThreads>(a);
+}
+
+template <typename T>
+int launch_clear(const AttentionArgs& a, int D, void* stream) {
+  const int64_t items = (int64_t)a.num_tokens * a.pages.heads * a.group * (D / 4);
+  const unsigned grid = (unsigned)min((items + kJoinThreads - 1) / kJoinThreads, (int64_t)2048);
+  launch_kernel(D == 64 ? attention_clear_kernel<T, 64> : D == 128 ? attention_clear_kernel<T, 128> : attention_clear_kernel<T, 256>,
+                dim3(grid), dim3(kJoinThreads), 0, static_cast<hipStream_t>(stream), a);
+  return finish_launch("kv4_attention");
+}
+
 bool wide_rows(const tw_heads* h) {
   return reinterpret_cast<uintptr_t>(h->data) % 16 == 0 && h->token_stride % 8 == 0 && h->head_stride % 8 == 0;
 }
@@ -1580,7 +1625,8 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   if (dtype != TW_DTYPE_BF16 && dtype != TW_DTYPE_F16) return set_error(TW_ERR_DTYPE, "%s: unsupported dtype %d", what, dtype);
   if (T < 0 || num_seqs < 0 || max_queries < 0 || window < 0 || table_width < 0 || table_stride < 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: a size is negative", what);
-  if (T == 0 || num_seqs == 0 || max_queries == 0) return TW_OK;
+  const bool nothing = num_seqs == 0 || max_queries == 0;
+  if (T == 0 || (nothing && !query_starts)) return TW_OK;
   AttentionArgs a{};
   if (int rc = check_kv4_pages(what, pages, num_pages, page_size, kv_heads, head_size, &a.pages)) return rc;
   if (!out || !q || !out->data || !q->data) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: out or q is null", what);
@@ -1589,7 +1635,7 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   if (out->heads != q->heads) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: out and q have different heads", what);
   if (out->token_stride < 0 || out->head_stride < 0 || q->token_stride < 0 || q->head_stride < 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: a stride is negative", what);
-  if (!seq_lens || (!block_table && table_width > 0))
+  if (!nothing && (!seq_lens || (!block_table && table_width > 0)))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table or seq_lens is null", what);
   if (table_width > ((int64_t)1 << 30) / page_size)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table has room for more than 2^30 tokens", what);
@@ -1598,7 +1644,7 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   if (!query_starts && T % num_seqs != 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld tokens are not the same number for each of %lld sequences", what,
                      (long long)T, (long long)num_seqs);
-  const int64_t need = kv4_attention_workspace((int)q->heads, kv_heads, head_size, num_seqs, T, max_queries,
+  const int64_t need = nothing ? 0 : kv4_attention_workspace((int)q->heads, kv_heads, head_size, num_seqs, T, max_queries,
                                                table_width, page_size);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, need %lld, 16-byte aligned", what,
@@ -1623,6 +1669,7 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   a.window = (int)min(window, (int64_t)1 << 30);
   a.q_wide = wide_rows(q);
   a.out_wide = wide_rows(out);
+  if (nothing) return dtype == TW_DTYPE_BF16 ? launch_clear<__bf16>(a, head_size, stream) : launch_clear<_Float16>(a, head_size, stream);
   max_queries = a.max_queries;
   if (max_queries * a.group <= kMostRows) {
     // steps are counted in 32 bits
