@@ -789,6 +789,13 @@ def _check_heads(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.d
     _require(t.stride(2) == 1 or t.size(2) == 1, f"the channels of {name} must be contiguous; got stride {t.stride()}")
 
 
+def _refuse_gradients(op: str, *tensors: Optional[torch.Tensor]) -> None:
+    """These ops are not part of autograd: where it records, a gradient through one would be lost without a word."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op} records no gradient and a tensor requires one: pass it detached, or call under "
+                           "torch.no_grad() (rotary_positions(inverse=True) is the gradient of a rotation)")
+
+
 def _check_index(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, numel: int) -> None:
     _require(isinstance(t, torch.Tensor) and t.is_cuda and t.device == device and t.dtype == dtype
              and t.is_contiguous() and t.dim() == 1, f"{name} must be a contiguous 1-D {dtype} tensor on {device}")
@@ -821,10 +828,12 @@ def rotary_positions(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     becomes (x1 cos - x2 sin, x2 cos + x1 sin), computed in fp32 and rounded once.  `cos_sin`
     [positions, rotary_dim] fp32 holds a position's cosines and then its sines
     (`RotaryPositions.cos_sin`).  `interleaved`: pairs are neighbours, else (j, j + rotary_dim / 2).
-    `inverse` turns back: the gradient of the rotation."""
+    `inverse` turns back: the gradient of the rotation.  (Autograd does not know these ops: a tensor that
+    requires a gradient is refused while one is recorded.)"""
     if _fast is not None and not _tracing() and _fast.rotary_positions(q, k, positions, cos_sin, interleaved, inverse,
                                                                        q_out, k_out):
         return
+    _refuse_gradients("rotary_positions", q, k, cos_sin, q_out, k_out)
     code = _dtype_code("rotary_positions_kernel", q)
     dev = q.device
     _check_heads("q", q, q.dtype, dev)
@@ -867,6 +876,7 @@ def kv4_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: tor
     if _fast is not None and not _tracing() and _fast.kv4_append(pages, k, v, slots, positions, cos_sin, interleaved,
                                                                  q, q_out):
         return
+    _refuse_gradients("kv4_append", k, v, cos_sin, q, q_out)
     code = _dtype_code("kv4_append_kernel", k)
     dev = k.device
     _check_heads("k", k, k.dtype, dev)
@@ -898,6 +908,7 @@ def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, pages: torch.Tensor, slot
     where a slot is outside the cache.  Values up to 6 * 2^13 are exact in every type."""
     if _fast is not None and not _tracing() and _fast.kv4_read(k_out, v_out, pages, slots):
         return
+    _refuse_gradients("kv4_read", k_out, v_out)
     code = _dtype_code("kv4_read_kernel", k_out)
     dev = k_out.device
     _check_heads("k_out", k_out, k_out.dtype, dev)
@@ -924,6 +935,7 @@ def kv4_attention(out: torch.Tensor, q: torch.Tensor, pages: torch.Tensor, block
     if _fast is not None and not _tracing() and _fast.kv4_attention(out, q, pages, block_table, seq_lens, scale,
                                                                     query_starts, max_queries, window):
         return
+    _refuse_gradients("kv4_attention", out, q)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f'"kv4_attention_kernel" not implemented for \'{q.dtype}\'')
     code = _DTYPE_CODE[q.dtype]
