@@ -320,7 +320,8 @@ TW_API int tw_gemm_bf16_nt_partials_bias(void* const* outs, const void* const* a
  * counterpart on the reference's path; head counts and lengths are the caller's.)
  *
  * tw_heads: a tensor [num_tokens, heads, head_size] whose channels are contiguous; the
- * strides are in elements (views of a wider projection output are fine).
+ * strides are in elements (views of a wider projection output are fine).  Rows of an output
+ * must not share memory: TW_ERR_INVALID_ARGUMENT.
  * ------------------------------------------------------------------------- */
 typedef struct tw_heads {
   void* data;

@@ -1635,6 +1635,7 @@ int run_kv4_attention(const tw_heads* out, const tw_heads* q, const void* pages,
   if (out->heads != q->heads) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: out and q have different heads", what);
   if (out->token_stride < 0 || out->head_stride < 0 || q->token_stride < 0 || q->head_stride < 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: a stride is negative", what);
+  if (int rc = check_rows_apart(what, "out", out, T, head_size)) return rc;
   if (!nothing && (!seq_lens || (!block_table && table_width > 0)))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: block_table or seq_lens is null", what);
   if (table_width > ((int64_t)1 << 30) / page_size)

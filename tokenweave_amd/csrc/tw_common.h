@@ -78,6 +78,9 @@ int run_gemm_bf16_nt_partials(void* const* outs, const void* const* as, const vo
 
 struct Kv4Pages;
 
+// Whether an output's rows of head_size values are apart, whatever the order of its strides.
+int check_rows_apart(const char* what, const char* name, const tw_heads* h, int64_t T, int head_size);
+
 int check_kv4_pages(const char* what, const void* pages, int64_t num_pages, int page_size, int64_t heads, int head_size,
                     Kv4Pages* out);
 

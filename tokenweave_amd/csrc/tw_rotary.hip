@@ -397,14 +397,18 @@ bool vector_ok(const tw_heads* h, int bytes) {
                 h->head_stride * bytes % 16 == 0);
 }
 
-int check_heads(const char* what, const char* name, const tw_heads* h, int head_size) {
+int check_heads(const char* what, const char* name, const tw_heads* h) {
   if (!h || !h->data) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %s is null", what, name);
   if (h->heads < 1 || h->heads > (1 << 20))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %s has %lld heads", what, name, (long long)h->heads);
   if (h->token_stride < 0 || h->head_stride < 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %s has a negative stride", what, name);
-  (void)head_size;
   return TW_OK;
+}
+
+int check_out_heads(const char* what, const char* name, const tw_heads* h, int64_t T, int head_size) {
+  const int rc = check_heads(what, name, h);
+  return rc ? rc : check_rows_apart(what, name, h, T, head_size);
 }
 
 int check_dtype(const char* what, int dtype) {
@@ -491,6 +495,23 @@ int bytes_of(int dtype) { return dtype == TW_DTYPE_F32 ? 4 : 2; }
 
 }  // namespace
 
+int check_rows_apart(const char* what, const char* name, const tw_heads* h, int64_t T, int head_size) {
+  typedef __int128 wide;  // (strides are the caller's)
+  const wide a = h->token_stride, b = h->head_stride, D = head_size, tokens = T - 1, heads = h->heads - 1;
+  bool apart = (tokens == 0 || a >= D) && (heads == 0 || b >= D);
+  // neither a token's heads within a token's stride nor a head's tokens within a head's: head by head, the nearest tokens
+  if (apart && tokens > 0 && heads > 0 && heads * b + D > a && tokens * a + D > b) {
+    for (wide x = b; x <= heads * b && apart; x += b) {
+      const wide k = x / a;
+      apart = (k > tokens || x - k * a >= D) && (k + 1 > tokens || (k + 1) * a - x >= D);
+    }
+  }
+  if (!apart)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: rows of %s share memory: %lld tokens, stride %lld, %lld heads, stride %lld",
+                     what, name, (long long)T, (long long)h->token_stride, (long long)h->heads, (long long)h->head_stride);
+  return TW_OK;
+}
+
 int check_kv4_pages(const char* what, const void* pages, int64_t num_pages, int page_size, int64_t heads, int head_size,
                     Kv4Pages* out) {
   if (head_size != 64 && head_size != 128 && head_size != 256)
@@ -515,12 +536,12 @@ int run_rotary_positions(const tw_heads* q_out, const tw_heads* q, const tw_head
   if (int rc = check_dtype(what, dtype)) return rc;
   if (T == 0) return TW_OK;
   if (int rc = check_rotary(what, positions, cos_sin, max_positions, head_size, rotary_dim, flags)) return rc;
-  if (int rc = check_heads(what, "q", q, head_size)) return rc;
-  if (int rc = check_heads(what, "q_out", q_out, head_size)) return rc;
+  if (int rc = check_heads(what, "q", q)) return rc;
+  if (int rc = check_out_heads(what, "q_out", q_out, T, head_size)) return rc;
   if (!k != !k_out) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: k and k_out must both be given or both be null", what);
   if (k) {
-    if (int rc = check_heads(what, "k", k, head_size)) return rc;
-    if (int rc = check_heads(what, "k_out", k_out, head_size)) return rc;
+    if (int rc = check_heads(what, "k", k)) return rc;
+    if (int rc = check_out_heads(what, "k_out", k_out, T, head_size)) return rc;
   }
   if (q_out->heads != q->heads || (k && k_out->heads != k->heads))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: input and output have different heads", what);
@@ -545,8 +566,8 @@ int run_kv4_append(void* pages, int64_t num_pages, int page_size, const tw_heads
   if (T < 0) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad num_tokens", what);
   if (int rc = check_dtype(what, dtype)) return rc;
   if (T == 0) return TW_OK;
-  if (int rc = check_heads(what, "k", k, head_size)) return rc;
-  if (int rc = check_heads(what, "v", v, head_size)) return rc;
+  if (int rc = check_heads(what, "k", k)) return rc;
+  if (int rc = check_heads(what, "v", v)) return rc;
   if (k->heads != v->heads) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: k and v have different heads", what);
   AppendArgs a{};
   if (int rc = check_kv4_pages(what, pages, num_pages, page_size, k->heads, head_size, &a.pages)) return rc;
@@ -568,8 +589,8 @@ int run_kv4_append(void* pages, int64_t num_pages, int page_size, const tw_heads
   const bool vec = (!a.turned || wide) && vector_ok(k, size) && vector_ok(v, size);
   bool q_vec = false;
   if (q) {
-    if (int rc = check_heads(what, "q", q, head_size)) return rc;
-    if (int rc = check_heads(what, "q_out", q_out, head_size)) return rc;
+    if (int rc = check_heads(what, "q", q)) return rc;
+    if (int rc = check_out_heads(what, "q_out", q_out, T, head_size)) return rc;
     if (q->heads != q_out->heads) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: q and q_out have different heads", what);
     q_vec = wide && vector_ok(q, size) && vector_ok(q_out, size);
     a.q = RotaryArgs{heads_of(q_out), heads_of(q), Heads{}, Heads{}, (int)q->heads, (int)q->heads,
@@ -592,8 +613,8 @@ int run_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void* pages
   if (T < 0) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad num_tokens", what);
   if (int rc = check_dtype(what, dtype)) return rc;
   if (T == 0) return TW_OK;
-  if (int rc = check_heads(what, "k_out", k_out, head_size)) return rc;
-  if (int rc = check_heads(what, "v_out", v_out, head_size)) return rc;
+  if (int rc = check_out_heads(what, "k_out", k_out, T, head_size)) return rc;
+  if (int rc = check_out_heads(what, "v_out", v_out, T, head_size)) return rc;
   if (k_out->heads != v_out->heads) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: k_out and v_out have different heads", what);
   ReadArgs a{};
   if (int rc = check_kv4_pages(what, pages, num_pages, page_size, k_out->heads, head_size, &a.pages)) return rc;
