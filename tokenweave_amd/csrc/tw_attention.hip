@@ -60,7 +60,8 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int s) {
   }
   const int length = UNIFORM ? constant(a.seq_lens)[s] : a.seq_lens[s];
   first = min(max(first, 0), a.num_tokens);
-  return {first, max(min(end, a.num_tokens) - first, 0), min(max(length, 0), a.capacity)};
+  end = min(max(end, 0), a.num_tokens);  // (before the subtraction: it would not fit 32 bits)
+  return {first, max(end - first, 0), min(max(length, 0), a.capacity)};
 }
 
 // ---------------------------------------------------------------------------
@@ -330,7 +331,7 @@ __device__ __forceinline__ Rest rest_of(const AttentionArgs& a) {
   if (!a.query_starts) return {0, a.num_tokens};
   const int first = constant(a.query_starts)[0], last = constant(a.query_starts)[a.num_seqs];
   const int before = min(max(first, 0), a.num_tokens);
-  return {before, min(max(last, before), a.num_tokens)};
+  return {before, last < first ? a.num_tokens : min(max(last, 0), a.num_tokens)};  // (in no order: nothing is behind)
 }
 template <typename T, int D, int THREADS>
 __device__ __forceinline__ void clear_rest(const AttentionArgs& a) {
