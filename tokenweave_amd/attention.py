@@ -87,6 +87,14 @@ class RotaryPositions(nn.Module):
         angle = torch.arange(max_position, dtype=torch.float64)[:, None] * inv
         self.register_buffer("cos_sin", (torch.cat((angle.cos(), angle.sin()), 1) * factor).float(), persistent=False)
 
+    def _apply(self, fn: Any, recurse: bool = True) -> "RotaryPositions":
+        """A model's type (`model.bfloat16()`) is not the table's: it stays fp32, on the device it is moved to."""
+        table = self.cos_sin
+        super()._apply(fn, recurse)
+        if self.cos_sin.dtype != torch.float32:
+            self.cos_sin = table.to(self.cos_sin.device)
+        return self
+
     def forward(self, positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor] = None,
                 q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
                 inverse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
