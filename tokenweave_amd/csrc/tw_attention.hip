@@ -308,22 +308,17 @@ __device__ __forceinline__ void store4(T* out, const float4_t& x, bool wide) {
 }
 
 // The exponents' base for a maximum: the next 64th.  Neither kLift - m nor the factor from one m to the next is rounded
-// then, and the largest probabilities are just below a power of two, where fp16 is finest.  A base of kFar and more is
-// the maximum itself: neighbouring fp32 values are half and more apart there, up to far more than the exponents' range,
-// so that s - m has to be taken of scores rounded as the maximum was (the largest has exactly zero) and lifted after.
-constexpr float kFar = 0x1p22f;
-__device__ __forceinline__ float base_of(float most) {
-  return __builtin_fabsf(most) < kFar ? __builtin_ceilf(most * 64.0f) * 0.015625f : most;
-}
-__device__ __forceinline__ bool is_far(float m) { return __builtin_fabsf(m) >= kFar && __builtin_fabsf(m) < __builtin_inff(); }
-__device__ __forceinline__ float below(float x, float scale, float m) {
-#pragma clang fp contract(off)
-  const float s = x * scale;
-  return s - m;
-}
+// then, and the largest probabilities are just below a power of two, where fp16 is finest.
+__device__ __forceinline__ float base_of(float most) { return __builtin_ceilf(most * 64.0f) * 0.015625f; }
 
-// Rows of tokens that no sequence has, before the first one's and behind the last one's: zeros, by all
-// threads of the launch.
+// From kFar on neighbouring fp32 values are half and more apart, up to far more than the exponents' range: a score's
+// product with the scale, which is not rounded where m is subtracted, may be that much above or below the maximum, which
+// was.  (From 2^25 on, where scores of 3e7 are, a row's largest probability was infinite or zero.)
+constexpr float kFar = 0x1p22f;
+__device__ __forceinline__ bool is_far(float m) { return __builtin_fabsf(m) >= kFar && __builtin_fabsf(m) < __builtin_inff(); }
+
+// Rows of tokens that no sequence has, before the first one's and behind the last one's: zeros, by the
+// workgroups of a launch that have no second place in the grid (those of a join's first rows).
 struct Rest {
   int before, behind;  // [0, before) and [behind, num_tokens)
 };
@@ -339,8 +334,7 @@ __device__ __forceinline__ void clear_rest(const AttentionArgs& a) {
   const int tokens = rest.before + a.num_tokens - rest.behind;
   if (tokens == 0) return;
   const int64_t heads = a.pages.heads * a.group, columns = D / 4;
-  const int64_t block = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-  const int64_t threads = (int64_t)gridDim.x * gridDim.y * gridDim.z * THREADS;
+  const int64_t block = (int64_t)blockIdx.z * gridDim.x + blockIdx.x, threads = (int64_t)gridDim.x * gridDim.z * THREADS;
   for (int64_t i = block * THREADS + threadIdx.x; i < tokens * heads * columns; i += threads) {
     const int64_t row = i / columns;
     const int at = (int)(row / heads), token = at < rest.before ? at : at - rest.before + rest.behind;
@@ -350,7 +344,29 @@ __device__ __forceinline__ void clear_rest(const AttentionArgs& a) {
   }
 }
 
-constexpr float kLift = 14.0f;  // probabilities are held times 2^14: fp16's normal range reaches down to 2^-28 of the largest
+// Few rows: probabilities are held times 2^14, so that fp16's normal range reaches down to 2^-28 of the largest.  A far
+// maximum's base is two to four neighbouring values below it: the largest exponent is kLift or more, and what is above
+// kMost counts as kMost, so that scores closer than their own rounding errors weigh the same.
+// (Four instructions of 32 tokens: 243.3 us instead of 240.5 for 256 sequences of 4096 tokens, 64 + 8 heads of 128; a base
+// that is the maximum itself, as of many rows, took three more registers and 245.3.)
+constexpr float kLift = 14.0f;
+constexpr _Float16 kMost = (_Float16)0x1p15f;
+__device__ __forceinline__ float low_base_of(float most) {
+  return is_far(most) ? __builtin_fmaf(__builtin_fabsf(most), -0x1p-22f, most) : base_of(most);
+}
+
+// Many rows: probabilities are held times 2^(kTileLift - m).  m need not be the maximum so far, only within kSlack of
+// it: so they stay within 2^15, fp16's normal range reaches down to 2^-21 of the largest or lower and its subnormals to
+// 2^-31, and a row's sums are multiplied anew a few times in all instead of in most units (one of 64 rows has a new
+// maximum in most of the first hundred units: 211 us with the maximum itself and 188 us so, for 8192 rows of 8 heads).
+// A far maximum is the base itself and scores are rounded as it was: the largest is exactly zero below it.
+constexpr float kTileLift = 7.0f, kSlack = 8.0f;
+__device__ __forceinline__ float tile_base_of(float most) { return is_far(most) ? most : base_of(most); }
+__device__ __forceinline__ float below(float x, float scale, float m) {
+#pragma clang fp contract(off)
+  const float s = x * scale;
+  return s - m;
+}
 
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split_kernel(SplitArgs args) {
@@ -492,17 +508,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
     ids_of(step0 + 2, ids);
 
     half8_t q[NT][D / 32];
-    // A probability is 2^(x * by + add).  limit: m, above which the base rises; of a far row less than any score, so that
-    // its scores are turned into differences from the base there, in every tile.  (What this costs the other rows: 66.3 us
-    // instead of 65.2 for 64 sequences of 4096 tokens, 32 heads over 8 key heads, D = 128.)
-    float scale[NT], m[NT], l[NT], limit[NT], by[NT], add[NT];
+    float scale[NT], m[NT], l[NT];
     float4_t o[NT][kTiles];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       scale[t] = raw[t].lift(q[t], a.scale);
-      m[t] = limit[t] = -__builtin_inff();
-      by[t] = scale[t];
-      add[t] = kLift;
+      m[t] = -__builtin_inff();
       l[t] = 0.0f;
 #pragma unroll
       for (int c = 0; c < kTiles; ++c) o[t][c] = float4_t{0, 0, 0, 0};
@@ -551,28 +562,22 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attention_split
           most = fmaxf(most, x[i]);
         }
         most = max32(max16(most)) * scale[t];
-        if (__builtin_amdgcn_ballot_w64(most > limit[t])) {
-          const float now = fmaxf(m[t], base_of(most));
+        if (__builtin_amdgcn_ballot_w64(most > m[t])) {
+          const float now = fmaxf(m[t], low_base_of(most));
           const float old = m[t] == now ? 1.0f : __builtin_amdgcn_exp2f(m[t] - now);
-          const bool far = is_far(now);
           m[t] = now;
-          limit[t] = far ? -__builtin_inff() : now;
-          by[t] = far ? 1.0f : scale[t];
-          add[t] = kLift - (far || now == -__builtin_inff() ? 0.0f : now);
           l[t] *= old;
 #pragma unroll
           for (int c = 0; c < kTiles; ++c) o[t][c] *= old;
-          if (__builtin_expect(__builtin_amdgcn_ballot_w64(far) != 0, 0)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = far ? below(x[i], scale[t], now) : x[i];
-          }
         }
+        const float add = kLift - (m[t] == -__builtin_inff() ? 0.0f : m[t]);
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[t][i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by[t], add[t]));
-          sum = __builtin_fmaf((float)p[t][i], one, sum);  // (as rounded: one token's output is its value, to the bit)
-        }
+        for (int i = 0; i < 8; ++i) p[t][i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale[t], add));
+        p[t] = __builtin_elementwise_minimum(p[t], half8_t(kMost));  // (what is not a number stays so)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // (as rounded: one token's output is its value, to the bit)
+          sum = __builtin_fmaf((float)p[t][i], one, sum);
         l[t] += sum;
       }
       // ---- values: what no row sees may hold anything, and nothing times zero has to be zero
@@ -719,7 +724,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
   const int s = blockIdx.x / a.pages.heads, head = blockIdx.x - s * a.pages.heads, row = blockIdx.y, ch0 = blockIdx.z * CH;
   const PieceHeader header = args.headers[blockIdx.x];
   const Sequence seq = sequence<true>(a, s);
-  clear_rest<T, D, kJoinThreads>(a);
+  if (blockIdx.y == 0) clear_rest<T, D, kJoinThreads>(a);
   // (a sequence without new tokens has no piece and leaves its header as it was)
   if (row >= min(seq.count, a.max_queries) * a.group || header.count < 2) return;
   constexpr int kLanes = CH / 4, kGroups = kJoinThreads / kLanes, kAtOnce = 8;
@@ -924,12 +929,6 @@ __device__ __forceinline__ FoundTile find_tile(const AttentionArgs& a, int tile,
   return {uniform(found[0]), uniform(found[1])};
 }
 
-// Many rows: probabilities are held times 2^(kTileLift - m).  m need not be the maximum so far, only within kSlack of
-// it: so they stay within 2^15, fp16's normal range reaches down to 2^-21 of the largest or lower and its subnormals to
-// 2^-31, and a row's sums are multiplied anew a few times in all instead of in most units (one of 64 rows has a new
-// maximum in most of the first hundred units: 211 us with the maximum itself and 188 us so, for 8192 rows of 8 heads).
-constexpr float kTileLift = 7.0f, kSlack = 8.0f;
-
 template <int D>
 struct TileShape {
   // eight waves, two a SIMD unit, share a tile's keys and values; heads of 256 channels leave registers for one
@@ -985,7 +984,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
   const int P = 1 << a.pages.page_log2, heads = a.pages.heads;
   const int window = a.window > 0 ? a.window : 1 << 30;
 
-  clear_rest<T, D, S::kThreads>(a);
+  if (blockIdx.y == 0) clear_rest<T, D, S::kThreads>(a);
   if (threadIdx.x == 0) odd_unit = -1;  // (a barrier follows, with the search for the tiles)
 
   // ---- Which tiles: one, or an even share of all tiles' spans.  In the order of the shares a long tile of a prompt
@@ -1335,7 +1334,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
         float top = sc[0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[j]);
-        const float raised = max32(most) > limit ? fmaxf(m, base_of(max32(top) * scale)) : m;
+        const float raised = max32(most) > limit ? fmaxf(m, tile_base_of(max32(top) * scale)) : m;
         const float old = m == raised ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
         m = raised;
         const bool far = is_far(m);
