@@ -383,7 +383,9 @@ TW_API int tw_kv4_read(const tw_heads* k_out, const tw_heads* v_out, const void*
  *   seq_lens     [num_seqs] int32: cached tokens, the new ones among them (appended before)
  *   query_starts [num_seqs + 1] int32: sequence s has the tokens query_starts[s] ..
  *                query_starts[s+1] - 1 of q and out, the last of its cached tokens; NULL:
- *                num_tokens / num_seqs tokens each
+ *                num_tokens / num_seqs tokens each.  A batch may be attended in parts: tokens
+ *                below 0 are an earlier call's, those from num_tokens on a later one's (and
+ *                not seen here, though seq_lens counts them)
  * Query i of n sees the tokens up to its own, seq_len - n + i, and of these the last
  * `window` where window > 0.  A query that sees none gives zeros, and so do tokens of q before
  * query_starts[0] and from query_starts[num_seqs] on, which no sequence has (padding).

@@ -928,7 +928,8 @@ def kv4_attention(out: torch.Tensor, q: torch.Tensor, pages: torch.Tensor, block
     ones there), q and out [tokens, heads, head_size] in bf16 or fp16; heads g*G .. g*G + G-1 share key
     head g.  `block_table` [sequences, pages] int32 names a sequence's pages, `seq_lens` its cached
     tokens, `query_starts` [sequences + 1] int32 its first token in q (None: the same number of tokens
-    for each sequence).  A token sees the cached tokens up to its own, of these the last `window` where
+    for each sequence; starts below 0 or past q's tokens are of other parts of a batch, attended in calls
+    of their own, and `seq_lens` is the whole batch's).  A token sees the cached tokens up to its own, of these the last `window` where
     that is above 0; one that sees none gives zeros, and so does one before or behind all sequences'
     (padding).  `max_queries`: the most new tokens of a sequence (needed with query_starts, where it
     defaults to all of q's); rows of a sequence's tokens behind it are left as they were."""

@@ -59,9 +59,11 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int s) {
     end = first + a.per_seq;
   }
   const int length = UNIFORM ? constant(a.seq_lens)[s] : a.seq_lens[s];
+  // New tokens behind q's last belong to a later call: here the sequence ends before them.
+  const int later = max(end, a.num_tokens) - a.num_tokens;
   first = min(max(first, 0), a.num_tokens);
   end = min(max(end, 0), a.num_tokens);  // (before the subtraction: it would not fit 32 bits)
-  return {first, max(end - first, 0), min(max(length, 0), a.capacity)};
+  return {first, max(end - first, 0), max(min(max(length, 0), a.capacity) - later, 0)};
 }
 
 // ---------------------------------------------------------------------------
