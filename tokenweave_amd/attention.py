@@ -292,7 +292,7 @@ class PagedSelfAttention(nn.Module):
         x, D, Hq, Hk = hidden_states[:n], self.head_size, self.num_heads, self.num_kv_heads
         qkv = torch.empty((n, self.qkv_weight.shape[0]), dtype=x.dtype, device=x.device)
         ops.gemm_bf16_nt(qkv, x, self.qkv_weight.data, None, None if self.qkv_bias is None else self.qkv_bias.data)
-        q, k, v = (t.view(n, -1, D) for t in qkv.split((Hq * D, Hk * D, Hk * D), 1))
+        q, k, v = (t.view(n, t.shape[1] // D, D) for t in qkv.split((Hq * D, Hk * D, Hk * D), 1))
         self.cache.append(k, v, batch.slots, positions[:n], self.rotary, q)
         table, lens, starts, bound = batch._operands()
         out = self.cache.attend(q, table, lens, None, starts, bound, self.window,
