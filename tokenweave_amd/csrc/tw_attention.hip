@@ -3,8 +3,11 @@
 //   o = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m),  s_t = scale * log2(e) * q k_t,  any m near max_t s_t
 //
 // in one pass over the tokens: when a larger s appears, what has been summed is multiplied by
-// 2^(m - m').  Scores, m, sums and the output are fp32, the probabilities in both sums fp16; the output
-// is rounded once.
+// 2^(m - m').  Scores, m, sums and the output are fp32; the output is rounded once.  Queries (lifted by a
+// power of two) and cached values are exact in fp16, the type of both products.  Probabilities are not:
+// they are rounded to it for the second product (2^-11 each) and summed as rounded, so that their
+// weights still sum to one.  An fp16 output is then 1.1 to 1.4 times as far from 64 bits as with fp32
+// probabilities (2.6e-4 and 2.1e-4 of its size for four drafted tokens), a bf16 one under 1 % farther.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -82,10 +85,12 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& a, int s) {
 // sequence that has several go to the workspace as (m, l, O), and attention_join_kernel joins them.
 //
 // What bounds it: the cache's bytes where there are many (256 sequences of 4096 tokens, 8 key heads, D = 128, 1.15 GB:
-// 240 us = 4.8 TB/s, where a large copy reaches 5.16), latencies below some 50 MB: lengths, pages' numbers and keys
-// wait for each other, and the join is a launch of its own (a sequence of 700 tokens 6.7 + 3.5 us, 64 ragged ones of
-// 29.7 MB 13.4 + 3.9).  Two tiles of keys and values are under way in registers, not LDS: no wave needs another's
-// keys, so none waits at a barrier (those 256 sequences took 282 us with barriers, 268 without, 239 with two tiles).
+// 243 us = 4.7 TB/s, where a large copy reaches 5.16), latencies below some 50 MB: lengths, pages' numbers and keys
+// wait for each other, and the join is a launch of its own (traced: a sequence of 700 tokens 6.7 + 4.2 us, 64 ragged
+// ones of 29.7 MB 14.2 + 3.9).  Of 17 to 32 rows the vector unit as well: 32 sequences of 4096 with four new tokens 22 us
+// (D = 256: 46; without the bound on probabilities, kMost, 21.7 and 43.4).  Two tiles of keys and values are under way
+// in registers, not LDS: no wave needs another's keys, so none waits at a barrier (those 256 sequences took, step by
+// step, 282 us with barriers, 268 without, 239 with two tiles).
 // ---------------------------------------------------------------------------
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -360,7 +365,8 @@ __device__ __forceinline__ float low_base_of(float most) {
 // Many rows: probabilities are held times 2^(kTileLift - m).  m need not be the maximum so far, only within kSlack of
 // it: so they stay within 2^15, fp16's normal range reaches down to 2^-21 of the largest or lower and its subnormals to
 // 2^-31, and a row's sums are multiplied anew a few times in all instead of in most units (one of 64 rows has a new
-// maximum in most of the first hundred units: 211 us with the maximum itself and 188 us so, for 8192 rows of 8 heads).
+// maximum in most of the first hundred units: 211 us with the maximum itself and 188 us so, before the later steps, for
+// 8192 queries of 8 heads).
 // A far maximum is the base itself and scores are rounded as it was: the largest is exactly zero below it.
 constexpr float kTileLift = 7.0f, kSlack = 8.0f;
 __device__ __forceinline__ float tile_base_of(float most) { return is_far(most) ? most : base_of(most); }
@@ -789,16 +795,17 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(SplitArgs 
   store4(out, sum * (all > 0.0f || all != all ? 1.0f / all : 0.0f), a.out_wide);
 }
 
-// Of the split kernel, two operands' width.  One new token of each of 8 sequences of 4096, 8 rows: 11 us, in tiles 23;
-// of 300 of 700 with 8 key heads 74 and 211; four new tokens of each of 32 of 4096, 32 rows: 21 and 34.  Up to 16 rows
-// one operand is enough (8 sequences 11 us, with two operands 13; 300 sequences 74 and 91).
+// Of the split kernel, two operands' width.  One new token of each of 8 sequences of 4096, 8 rows: 10 us, in tiles 23;
+// of 300 of 700 with 8 key heads 78 and 232; four new tokens of each of 32 of 4096, 32 rows: 22 and 34.  Up to 16 rows
+// one operand is enough (8 sequences 10 us, with two operands 11; 300 sequences 78 and 96).
 constexpr int kMostRows = 32;
 
-// Cut of a call's steps.  While there is room, every piece has a workgroup of its own and all run at once, two a
-// compute unit (their registers allow no third); sequences and key heads beyond half of that are cut in four
-// pieces a compute unit on top, which the workgroups take in turn.  8 heads over a key head, D = 128: 64 sequences of
-// 1 to 4096 tokens and 8 key heads 44.7 us so, 47.7 with two pieces a compute unit and 48.5 with eight (all of 2048
-// tokens: 40.9, 33.3 and 46.8), 40 of 16 to 8192 tokens 29.8, 32.4 and 31.7.
+// Cut of a call's steps.  While there is room, every piece has a workgroup of its own, two a compute unit, which is how
+// many of them run at once at D = 128 (their registers allow no third; of D = 256 one runs, the other after it, of D = 64
+// a third could); sequences and key heads beyond half of that are cut in four pieces a compute unit on top, which the
+// workgroups take in turn.  8 heads over a key head, D = 128: 64 sequences of 1 to 4096 tokens and 8 key heads 45.1 us
+// so, 48.5 with two pieces a compute unit and 49.7 with eight, 40 of 16 to 8192 tokens 30.3, 32.0 and 31.2; but 64 that
+// are all of 2048 tokens 41.8, 35.8 and 50.6: lengths that differ are taken to be the ordinary case.
 struct SplitPlan {
   int grid, budget;
   int64_t header_bytes, bytes;
@@ -824,7 +831,7 @@ int launch_split(const SplitArgs& args, int grid, void* stream) {
   launch_kernel(kernel, dim3((unsigned)grid), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), args);
   if (int rc = finish_launch("kv4_attention")) return rc;
   // Few rows may be in very many pieces: more workgroups then share a row's channels (one sequence of 65536 tokens,
-  // 8 rows: 12.3 us so and 13.7 with whole rows; two of 32768 and 8 key heads, 128 rows: 25.7 and 23.9).
+  // 8 rows: 12.3 us so and 13.6 with whole rows; two of 32768 and 8 key heads, 128 rows: 26.1 and 24.4).
   const bool few = (int64_t)args.a.num_seqs * args.a.pages.heads * args.rows <= 32;
   launch_kernel(few ? attention_join_kernel<T, D, 32> : attention_join_kernel<T, D, D>,
                 dim3((unsigned)(args.a.num_seqs * args.a.pages.heads), (unsigned)args.rows, few ? D / 32 : 1), dim3(kJoinThreads), 0,
@@ -850,10 +857,12 @@ int launch_split(const SplitArgs& args, int D, int grid, void* stream) {
 // The matrix and the vector units work side by side: the scores of the next 32 tokens are computed between the
 // exponentials of the present ones, whose sums come between the present products with the values.  Two waves a SIMD
 // unit with 32 rows each: one wave with 64 rows reads LDS half as often, but nothing runs while it moves data (229
-// us against 188, for 8192 queries of 8 heads over one key head, D = 128).  What bounds it: the vector unit; of a
-// wave's 32 tokens the products take 512 cycles, the 16 exponentials a lane 256 and some 55 other vector
-// instructions 220, and laying out the tile, addresses and the barrier come on top.  That call takes 169 us with its
-// join of 15, 813 TFLOP/s, where a product of 8192 x 8192 x 8192 by the library reaches 1332.
+// us against 188 before the later steps, for 8192 queries of 8 heads over one key head, D = 128).  What bounds it:
+// neither unit by itself.  Of a wave's 32 tokens the products take 512 cycles, the 16 exponentials a lane 256 and some
+// 55 other vector instructions 220; laying out the tile, addresses and the barrier come on top.  The matrix unit is
+// busy in 34 % of the kernel's cycles and the vector unit in 38 %: the two waves of a SIMD unit pass the barrier
+// together and are in the same phase for much of a tile.  That call takes 170 us with its join of 15, 808 TFLOP/s,
+// where a product of 8192 x 8192 x 8192 by the library reaches 1332.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
@@ -1397,7 +1406,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, TileShape<D>::kWaves / 4) v
     if constexpr (S::kKeyBuffers == 2) lds_barrier();
     // Keys of the unit after next, whatever is there where there is none: they are read and not used.
     first_keys(S::kUnits == 2 ? keys_now + 32 * S::kKeyRow : keys_next);
-    // (what comes last in a step goes first where both waves of a SIMD unit could: 174 us without, 169 with it)
+    // (what comes last in a step goes first where both waves of a SIMD unit could: 174.8 us without, 173.2 with it)
     if (S::kApart && wave * 64 >= S::kValueThread) __builtin_amdgcn_s_setprio(1);
     auto advance = [&](int at, float16_t& first, float16_t& second) {
       const int t0 = at * S::kTokens;
@@ -1543,9 +1552,9 @@ __global__ __launch_bounds__(256) void attention_join_tile_kernel(TileArgs args)
 // Tiles of a call, and whether they are worked on in even shares: they do not even out among themselves (a prompt's
 // tiles reach back differently far, and what is left over of a last round of workgroups counts), and a part more or
 // less is little beside a compute unit that waits.  Not where a sequence has room for 256 tokens or less, whose tiles
-// are about equal and soon done, and not for more tiles than there is LDS for.  In even shares and in a workgroup
-// each, 8 heads over one key head, D = 128: a prompt of 8192 tokens 196 and 259 us, eight of them 1121 and 1178, 32 of
-// 2048 359 and 484, 64 of 512 95 and 113; 400 of 200 tokens 216 and 198, 500 of 64 70 and 65.
+// about equal and soon done, and not for more tiles than there is LDS for.  In even shares and in a workgroup
+// each, 8 heads over one key head, D = 128: a prompt of 8192 tokens 170 and 236 us, eight of them 1094 and 1137, 32 of
+// 2048 348 and 461, 64 of 512 93 and 109; 400 of 200 tokens 224 and 198, 500 of 64 72 and 67.
 struct TilePlan {
   int tiles, grid;  // grid: of the even shares; 0: none
   int64_t header_bytes, bytes;
