@@ -406,6 +406,59 @@ TW_API int tw_kv4_attention(const tw_heads* out, const tw_heads* q, const void* 
                             int64_t window, int dtype, void* workspace, int64_t workspace_bytes,
                             void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The feed-forward half of a decoder layer: a gated product with its gradients, rows to
+ * 8-bit codes with a scale for 128 channels, the product of such codes.  (No counterpart on
+ * the reference's path; every size is the caller's.)
+ * ------------------------------------------------------------------------- */
+#define TW_ACT_SILU 0      /* x / (1 + e^-x)                                        */
+#define TW_ACT_GELU 1      /* x (1 + erf(x / sqrt 2)) / 2                           */
+#define TW_ACT_GELU_TANH 2 /* x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2       */
+
+/* out[M, I] = act(G) * U,  G = a[M, K] b[0:I, K]^T,  U = a b[I:2I, K]^T:  bf16, both sums in
+ * fp32, the result rounded once.  b is one contiguous [2 I, K] (gate rows, then up rows), out has
+ * rows of stride ldc.  gate_up, where not NULL, takes G and U, rounded, as [M, 2 I] (stride
+ * ld_gate_up): what the gradient needs.  K % 8 == 0, K <= 2^24, I % 4 == 0, strides % 4 == 0; a, b
+ * 16-byte, out, gate_up 8-byte aligned; max_cus as for tw_gemm_bf16_nt. */
+TW_API int tw_gated_gemm_bf16_nt(void* out, void* gate_up, const void* a, const void* b, int64_t M,
+                                 int64_t I, int64_t K, int64_t ldc, int64_t ld_gate_up,
+                                 int activation, int max_cus, void* stream);
+
+/* Its gradients, with D = [grad_out * U * act'(G), grad_out * act(G)] rounded to bf16:
+ *   grad_a[M, K] = D b,  grad_b[2 I, K] = D^T a     (either may be NULL; contiguous)
+ * workspace: tw_gated_gemm_bf16_nt_backward_workspace() bytes, 256-byte aligned, contents of no
+ * meaning before and after; calls that may run at the same time need one each. */
+TW_API int64_t tw_gated_gemm_bf16_nt_backward_workspace(int64_t M, int64_t I, int64_t K, int want_a,
+                                                        int want_b);
+TW_API int tw_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad_out,
+                                          int64_t ld_grad_out, const void* a, const void* b,
+                                          const void* gate_up, int64_t ld_gate_up, int64_t M,
+                                          int64_t I, int64_t K, int activation, int max_cus,
+                                          void* workspace, int64_t workspace_bytes, void* stream);
+
+#define TW_FP8_GROUP 128 /* channels of a scale; the last group of a row holds what is left */
+
+/* Rows to OCP float8 e4m3fn codes with one fp32 scale for TW_FP8_GROUP channels of a row:
+ *   scale = max(max |y|, 1e-10) / 448, rounded to fp32 ;  code = the e4m3 value next to y / scale
+ * (the exact quotient: ties to the even code).  y is the input's row (activation < 0), or, of an
+ * input of 2 K channels, act(first half) * second half in fp32, not rounded in between.  A group that
+ * holds an infinity or a NaN gives NaN codes.  out is [num_rows, K] contiguous; the scale of
+ * row t, group g is scales[t * scale_row_stride + g * scale_group_stride] (the product below reads
+ * scale_row_stride == 1 fastest).  dtype TW_DTYPE_*; any K, any alignment of whole elements. */
+TW_API int tw_quant_fp8_groups(void* out, float* scales, int64_t scale_row_stride,
+                               int64_t scale_group_stride, const void* input, int64_t ld_input,
+                               int64_t num_rows, int64_t K, int activation, int dtype, void* stream);
+
+/* out[M, N] = sum over blocks k of 128:  a_scale[m, k] * b_scale[n / 128, k] * (a b^T over the block)
+ * a [M, K] and b [N, K] e4m3fn codes, contiguous; a's scales at any strides (elements), b's
+ * [ceil(N / 128), ceil(K / 128)] contiguous; sums in fp32, rounded once to dtype (TW_DTYPE_BF16 or
+ * TW_DTYPE_F16), rows of out at stride ldc.  K % 16 == 0, K <= 2^22, N % 4 == 0, ldc % 4 == 0; a, b
+ * 16-byte, out 8-byte aligned; max_cus as for tw_gemm_bf16_nt. */
+TW_API int tw_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales,
+                                int64_t scale_row_stride, int64_t scale_block_stride, const void* b,
+                                const float* b_scales, int64_t M, int64_t N, int64_t K, int64_t ldc,
+                                int dtype, int max_cus, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,175 @@
+"""The gated product and its gradients against 64 bits: every row count at which another kernel or tile serves, odd
+sizes, views, the smallest and the ragged; captured calls; values that are not numbers."""
+import pytest
+import torch
+
+import feed_forward_reference as R
+from tokenweave_amd import ops
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def make(M, inner, K, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((M, K), generator=g, device="cuda").to(BF16)
+    w = (torch.randn((2 * inner, K), generator=g, device="cuda") * (scale * K ** -0.5)).to(BF16)
+    return x, w
+
+
+def wide(rows, width, extra=12):
+    """A row slice of a wider buffer, and the buffer, whose other places hold a mark."""
+    buf = torch.full((rows + 2, width + extra), 777.0, dtype=BF16, device="cuda")
+    return buf[1:1 + rows, 4:4 + width], buf
+
+
+def untouched(buf, rows, width):
+    keep = buf.clone()
+    keep[1:1 + rows, 4:4 + width] = 777.0
+    return bool((keep == 777.0).all())
+
+
+def check_forward(M, inner, K, kind, seed=0, max_cus=None):
+    x, w = make(M, inner, K, seed)
+    out, buf = wide(M, inner)
+    both, both_buf = wide(M, 2 * inner, 16)
+    ops.gated_gemm_bf16_nt(out, x, w, kind, max_cus, gate_up=both)
+    want, bound, products, off = R.gated(x, w, kind)
+    R.assert_within(out, want, bound, "out")
+    R.assert_within(both, products, off, "gate_up")
+    assert untouched(buf, M, inner) and untouched(both_buf, M, 2 * inner)
+    again = torch.empty((M, inner), dtype=BF16, device="cuda")
+    ops.gated_gemm_bf16_nt(again, x, w, kind, max_cus)
+    assert torch.equal(again, out), "the same call without gate_up gives other bits"
+    return x, w, both.contiguous(), out
+
+
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 16, 17, 31, 32, 33, 40, 41, 48, 64, 65, 72, 80, 96, 97, 128])
+@pytest.mark.parametrize("inner,K", [(4, 8), (100, 72), (704, 1024), (260, 136)])
+def test_few_rows(M, inner, K):
+    check_forward(M, inner, K, R.ACTIVATIONS[M % 3], seed=M)
+
+
+@pytest.mark.parametrize("M", [129, 160, 200, 256, 257, 300, 384, 511, 1001])
+@pytest.mark.parametrize("inner,K", [(32, 64), (100, 72), (704, 1024), (1376, 520), (36, 8)])
+def test_many_rows(M, inner, K):
+    check_forward(M, inner, K, R.ACTIVATIONS[M % 3], seed=M)
+
+
+@pytest.mark.parametrize("M,inner,K", [(1000, 2048, 256), (2458, 1376, 192), (700, 3696, 320), (4096, 512, 64)])
+def test_all_tile_shapes(M, inner, K):
+    check_forward(M, inner, K, "silu", seed=M)
+
+
+@pytest.mark.parametrize("M", [5, 64, 300])
+def test_grid_caps_give_the_same_bits(M):
+    x, w = make(M, 704, 520)
+    outs = []
+    for cap in (None, 1, 3, 64):
+        out = torch.empty((M, 704), dtype=BF16, device="cuda")
+        ops.gated_gemm_bf16_nt(out, x, w, "gelu", cap)
+        outs.append(out)
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+def test_products_that_are_large_or_no_numbers():
+    """An infinity or a NaN stays in its row (of x) or its column (of b); saturated gates are exact zeros and products."""
+    for M in (3, 200):
+        x, w = make(M, 64, 64)
+        x[1, 5] = float("inf")
+        w[7, 3] = float("nan")       # a gate row
+        w[64 + 9, 3] = float("inf")  # an up row
+        out = torch.empty((M, 64), dtype=BF16, device="cuda")
+        ops.gated_gemm_bf16_nt(out, x, w)
+        ok = torch.ones_like(out, dtype=torch.bool)
+        ok[1], ok[:, 7], ok[:, 9] = False, False, False
+        assert torch.isfinite(out[ok]).all() and torch.isnan(out[:, 7]).all() and not torch.isfinite(out[:, 9]).any()
+        x, w = make(M, 64, 64, scale=100.0)
+        for kind in R.ACTIVATIONS:
+            ops.gated_gemm_bf16_nt(out, x, w, kind)
+            want, bound, _, _ = R.gated(x, w, kind)
+            R.assert_within(out, want, bound + 1e-35, kind)
+
+
+@pytest.mark.parametrize("M,inner,K", [(1, 4, 8), (3, 36, 72), (64, 64, 64), (65, 100, 136), (129, 100, 72), (257, 704, 520),
+                                       (1001, 260, 1024)])
+@pytest.mark.parametrize("kind", R.ACTIVATIONS)
+def test_gradients(M, inner, K, kind):
+    x, w, both, out = check_forward(M, inner, K, kind)
+    grad_buf = torch.randn((M, inner + 8), device="cuda").to(BF16)
+    grad = grad_buf[:, 4:4 + inner]
+    gx, gw = torch.empty_like(x), torch.empty_like(w)
+    ops.gated_gemm_bf16_nt_backward(gx, gw, grad, x, w, both, kind)
+    want_x, bound_x, want_w, bound_w = R.gated_gradients(grad, x, w, both, kind)
+    R.assert_within(gx, want_x, bound_x, "grad_x")
+    R.assert_within(gw, want_w, bound_w, "grad_w")
+    only_x, only_w = torch.full_like(x, 5.0), torch.full_like(w, 5.0)
+    ops.gated_gemm_bf16_nt_backward(only_x, None, grad, x, w, both, kind)
+    ops.gated_gemm_bf16_nt_backward(None, only_w, grad, x, w, both, kind)
+    assert torch.equal(only_x, gx) and torch.equal(only_w, gw)
+
+
+def test_slopes_far_out_are_finite():
+    """Gates of +-3e38 and of 0: slopes of 1, 0 and 1/2, not a product of zero and infinity."""
+    gate = torch.tensor([[3e38, -3e38, 0.0, -90.0, 90.0, -5e19, 5e19, 1.0]], device="cuda").to(BF16)
+    up = torch.ones_like(gate)
+    x = torch.ones((1, 8), dtype=BF16, device="cuda")
+    w = torch.zeros((16, 8), dtype=BF16, device="cuda")
+    for kind in R.ACTIVATIONS:
+        gw = torch.empty_like(w)
+        ops.gated_gemm_bf16_nt_backward(None, gw, torch.ones_like(gate) * 1e-3, x, w, torch.cat((gate, up), 1), kind)
+        assert torch.isfinite(gw).all()
+        want = R.slope(gate.double(), kind)[0] * float(torch.tensor(1e-3).to(BF16))
+        R.assert_within(gw[:8, 0], want, want.abs() * 2 ** -7 + 1e-8, kind)
+
+
+def test_no_rows():
+    x, w = make(0, 36, 72)
+    ops.gated_gemm_bf16_nt(torch.empty((0, 36), dtype=BF16, device="cuda"), x, w,
+                           gate_up=torch.empty((0, 72), dtype=BF16, device="cuda"))
+    gx, gw = torch.empty_like(x), torch.full_like(w, 3.0)
+    ops.gated_gemm_bf16_nt_backward(gx, gw, torch.empty((0, 36), dtype=BF16, device="cuda"), x, w,
+                                    torch.empty((0, 72), dtype=BF16, device="cuda"))
+    assert (gw == 0).all()
+
+
+@pytest.mark.parametrize("M", [7, 300])
+def test_captured_and_on_another_stream(M):
+    x, w = make(M, 100, 136)
+    out, both = (torch.empty((M, n), dtype=BF16, device="cuda") for n in (100, 200))
+    grad = torch.randn((M, 100), device="cuda").to(BF16)
+    gx, gw = torch.empty_like(x), torch.empty_like(w)
+
+    def step():
+        ops.gated_gemm_bf16_nt(out, x, w, "gelu_tanh", gate_up=both)
+        ops.gated_gemm_bf16_nt_backward(gx, gw, grad, x, w, both, "gelu_tanh")
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in range(3):
+        x2, w2 = make(M, 100, 136, seed + 5)
+        x.copy_(x2), w.copy_(w2)
+        step()
+        torch.cuda.synchronize()
+        want = [t.clone() for t in (out, both, gx, gw)]
+        for t in (out, both, gx, gw):
+            t.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, o) for t, o in zip((out, both, gx, gw), want)), seed
+
+
+def test_both_routes_give_the_same_bits(monkeypatch):
+    x, w = make(70, 100, 136)
+    a, b = (torch.empty((70, 100), dtype=BF16, device="cuda") for _ in range(2))
+    ops.gated_gemm_bf16_nt(a, x, w)
+    monkeypatch.setattr(ops, "_fast", None)
+    ops.gated_gemm_bf16_nt(b, x, w)
+    assert torch.equal(a, b)

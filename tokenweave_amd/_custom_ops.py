@@ -971,6 +971,182 @@ def kv4_attention(out: torch.Tensor, q: torch.Tensor, pages: torch.Tensor, block
             None if ws is None else ws.data_ptr(), need, _stream_ptr(q)))
 
 
+# ---------------------------------------------------------------------------
+# the feed-forward half of a layer: a gated product with its gradients, rows to 8-bit codes,
+# the block-scaled product of such codes (no counterpart on the reference's path)
+# ---------------------------------------------------------------------------
+FP8_GROUP = _lib.TW_FP8_GROUP   # channels (and, of a weight, rows) that share a scale
+_ACTIVATIONS = {"silu": _lib.TW_ACT_SILU, "gelu": _lib.TW_ACT_GELU, "gelu_tanh": _lib.TW_ACT_GELU_TANH}
+
+
+def _activation_code(activation: str) -> int:
+    code = _ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"unknown activation {activation!r}, expected one of {sorted(_ACTIVATIONS)}")
+    return code
+
+
+def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, shape: Tuple[int, int]) -> int:
+    """A 2-D tensor whose rows are contiguous and apart; returns the distance of two rows in elements."""
+    _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}: tokenweave_amd ops run on the GPU only "
+                           "(there is no CPU implementation)")
+    _require(t.device == device, f"{name} is on {t.device}, expected {device}")
+    _require(t.dtype == dtype, f"{name} has dtype {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    rows, width = shape
+    _require((t.stride(1) == 1 or width <= 1) and (rows <= 1 or t.stride(0) >= width),
+             f"rows of {name} must be contiguous and apart; got stride {tuple(t.stride())}")
+    return t.stride(0) if rows > 1 else max(width, t.stride(0))
+
+
+def _refuse_recording(op: str, instead: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op} records no gradient and a tensor requires one: {instead}")
+
+
+def _check_gated(a: torch.Tensor, b: torch.Tensor) -> Tuple[int, int, int]:
+    """(M, I, K) of a [M, K] and b [2 I, K]."""
+    _require_bf16("gated_gemm_bf16_nt_kernel", a)
+    _check_tensor("a", a, torch.bfloat16, a.device)
+    _check_tensor("b", b, torch.bfloat16, a.device)
+    _require(a.dim() == 2 and b.dim() == 2, "gemm operands must be 2-D")
+    _require(a.size(1) == b.size(1), f"inner dimensions differ: a is {tuple(a.shape)}, b is {tuple(b.shape)}")
+    _require(b.size(0) % 2 == 0, f"b has {b.size(0)} rows: as many gate rows as up rows are expected")
+    return a.size(0), b.size(0) // 2, a.size(1)
+
+
+def gated_gemm_bf16_nt(out: torch.Tensor, a: torch.Tensor, b: torch.Tensor, activation: str = "silu",
+                       max_cus: Optional[int] = None, gate_up: Optional[torch.Tensor] = None) -> None:
+    """out[M, I] <- act(a @ b[:I]^T) * (a @ b[I:]^T) in one kernel: bf16, both products in fp32, the result
+    rounded once.  a [M, K], b [2 I, K] (a merged gate and up projection), `activation` "silu", "gelu" or
+    "gelu_tanh".  `gate_up` [M, 2 I] takes both products, rounded: what `gated_gemm_bf16_nt_backward` needs.
+    out and gate_up may be row slices of wider buffers.  `GatedLinear` is the layer with its gradient."""
+    if _fast is not None and not _tracing() and _fast.gated_gemm_bf16_nt(out, a, b, activation, max_cus, gate_up):
+        return
+    _refuse_recording("gated_gemm_bf16_nt", "use gated_linear or GatedLinear", out, a, b, gate_up)
+    act = _activation_code(activation)
+    M, inner, K = _check_gated(a, b)
+    ldc = _check_rows("out", out, torch.bfloat16, a.device, (M, inner))
+    ld_both = 0 if gate_up is None else _check_rows("gate_up", gate_up, torch.bfloat16, a.device, (M, 2 * inner))
+    with _on_device(a):
+        _lib.check(_lib.lib().tw_gated_gemm_bf16_nt(
+            out.data_ptr(), None if gate_up is None else gate_up.data_ptr(), a.data_ptr(), b.data_ptr(), M, inner, K,
+            ldc, ld_both, act, _cap(max_cus), _stream_ptr(a)))
+
+
+def gated_gemm_bf16_nt_backward(grad_a: Optional[torch.Tensor], grad_b: Optional[torch.Tensor], grad_out: torch.Tensor,
+                                a: torch.Tensor, b: torch.Tensor, gate_up: torch.Tensor, activation: str = "silu",
+                                max_cus: Optional[int] = None) -> None:
+    """The gradients of `gated_gemm_bf16_nt`: grad_a [M, K] and grad_b [2 I, K] are overwritten (either may be
+    None), from the gradient of out, the operands and the `gate_up` that the forward call filled.  The gradient
+    of both products is rounded to bf16 on the way, every sum is in fp32."""
+    if _fast is not None and not _tracing() and _fast.gated_gemm_bf16_nt_backward(grad_a, grad_b, grad_out, a, b,
+                                                                                  gate_up, activation, max_cus):
+        return
+    _refuse_recording("gated_gemm_bf16_nt_backward", "call under torch.no_grad()", grad_a, grad_b, grad_out, a, b, gate_up)
+    act = _activation_code(activation)
+    M, inner, K = _check_gated(a, b)
+    dev = a.device
+    ld_grad = _check_rows("grad_out", grad_out, torch.bfloat16, dev, (M, inner))
+    ld_both = _check_rows("gate_up", gate_up, torch.bfloat16, dev, (M, 2 * inner))
+    for name, t, like in (("grad_a", grad_a, a), ("grad_b", grad_b, b)):
+        if t is not None:
+            _check_tensor(name, t, torch.bfloat16, dev)
+            _require(t.shape == like.shape, f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
+    L = _lib.lib()
+    with _on_device(a):
+        need = L.tw_gated_gemm_bf16_nt_backward_workspace(M, inner, K, grad_a is not None, grad_b is not None)
+        if need < 0:
+            _lib.check(need)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(L.tw_gated_gemm_bf16_nt_backward(
+            None if grad_a is None else grad_a.data_ptr(), None if grad_b is None else grad_b.data_ptr(),
+            grad_out.data_ptr(), ld_grad, a.data_ptr(), b.data_ptr(), gate_up.data_ptr(), ld_both, M, inner, K, act,
+            _cap(max_cus), None if ws is None else ws.data_ptr(), need, _stream_ptr(a)))
+
+
+def fp8_group_scales(rows: int, channels: int, device=None) -> torch.Tensor:
+    """Memory for the scales of [rows, channels] codes, [rows, ceil(channels / FP8_GROUP)] fp32 in the layout that
+    `gemm_fp8_block_nt` reads fastest: the rows of a group side by side."""
+    groups = -(-channels // FP8_GROUP)
+    return torch.empty((groups, rows), dtype=torch.float32, device="cuda" if device is None else device).t()
+
+
+def _check_group_scales(name: str, t: torch.Tensor, device: torch.device, rows: int, groups: int) -> None:
+    _require(isinstance(t, torch.Tensor) and t.is_cuda and t.device == device and t.dtype == torch.float32,
+             f"{name} must be a torch.float32 tensor on {device}")
+    if tuple(t.shape) != (rows, groups):
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {(rows, groups)}")
+
+
+def quant_fp8_groups(out: torch.Tensor, scales: torch.Tensor, input: torch.Tensor,
+                     activation: Optional[str] = None) -> None:
+    """out [rows, K] (e4m3) and scales [rows, ceil(K / FP8_GROUP)] (fp32, any strides; `fp8_group_scales` makes the
+    usual layout) <- the rows of `input` [rows, K] in bf16, fp16 or fp32: of each group of 128 channels
+    scale = max(largest magnitude, 1e-10) / 448 and code = the e4m3 value next to x / scale, ties to the even one.
+    With `activation`, input is [rows, 2 K] and the rows are act(first half) * second half, taken in fp32 on the way
+    (a gated block between its projections).  A group with an infinity or a NaN gives NaN codes."""
+    if _fast is not None and not _tracing() and _fast.quant_fp8_groups(out, scales, input, activation):
+        return
+    _refuse_recording("quant_fp8_groups", "pass it detached, or call under torch.no_grad()", input)
+    act = -1 if activation is None else _activation_code(activation)
+    code = _dtype_code("quant_fp8_groups_kernel", input)
+    _require(input.dim() == 2 and (activation is None or input.size(1) % 2 == 0),
+             f"input has shape {tuple(input.shape)}, expected rows of " + ("channels" if activation is None else
+                                                                          "gate channels and as many up channels"))
+    M, K = input.size(0), input.size(1) // (1 if activation is None else 2)
+    _require(K > 0, "rows without channels")
+    dev = input.device
+    ld = _check_rows("input", input, input.dtype, dev, tuple(input.shape))
+    if not isinstance(out, torch.Tensor) or out.dtype != FP8_DTYPE:
+        raise NotImplementedError(f'"quant_fp8_groups_kernel" not implemented for \'{getattr(out, "dtype", out)}\'')
+    _check_tensor("out", out, FP8_DTYPE, dev)
+    _require(tuple(out.shape) == (M, K), f"out has shape {tuple(out.shape)}, expected {(M, K)}")
+    groups = -(-K // FP8_GROUP)
+    _check_group_scales("scales", scales, dev, M, groups)
+    s0, s1 = scales.stride()
+    _require((M <= 1 or s0 > 0) and (groups <= 1 or s1 > 0) and
+             (M <= 1 or groups <= 1 or s0 >= groups * s1 or s1 >= M * s0),
+             f"scales must not share memory; got stride {tuple(scales.stride())}")
+    with _on_device(input):
+        _lib.check(_lib.lib().tw_quant_fp8_groups(out.data_ptr(), scales.data_ptr(), s0, s1, input.data_ptr(), ld, M, K,
+                                                  act, code, _stream_ptr(input)))
+
+
+def gemm_fp8_block_nt(out: torch.Tensor, a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor,
+                      b_scales: torch.Tensor, max_cus: Optional[int] = None) -> None:
+    """out[M, N] (bf16 or fp16) <- the product of e4m3 codes a [M, K] and b [N, K] with their scales: a_scales
+    [M, ceil(K / 128)] (what `quant_fp8_groups` gives, any strides), b_scales [ceil(N / 128), ceil(K / 128)], one
+    for each block of 128 x 128, contiguous.  The sum over a block is taken in fp32 and multiplied by both scales.
+    out may be a row slice of a wider buffer (the rank's staging rows)."""
+    if _fast is not None and not _tracing() and _fast.gemm_fp8_block_nt(out, a, a_scales, b, b_scales, max_cus):
+        return
+    _refuse_recording("gemm_fp8_block_nt", "pass it detached, or call under torch.no_grad()", out, a_scales, b_scales)
+    if a.dtype != FP8_DTYPE:
+        raise NotImplementedError(f'"gemm_fp8_block_nt_kernel" not implemented for \'{a.dtype}\'')
+    dev = a.device
+    _check_tensor("a", a, FP8_DTYPE, dev)
+    _check_tensor("b", b, FP8_DTYPE, dev)
+    _require(a.dim() == 2 and b.dim() == 2, "gemm operands must be 2-D")
+    M, K = a.shape
+    N, K2 = b.shape
+    _require(K == K2, f"inner dimensions differ: a is {tuple(a.shape)}, b is {tuple(b.shape)}")
+    if not isinstance(out, torch.Tensor) or out.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f'"gemm_fp8_block_nt_kernel" not implemented for \'{getattr(out, "dtype", out)}\'')
+    ldc = _check_rows("out", out, out.dtype, dev, (M, N))
+    blocks = -(-K // FP8_GROUP)
+    _check_group_scales("a_scales", a_scales, dev, M, blocks)
+    _check_group_scales("b_scales", b_scales, dev, -(-N // FP8_GROUP), blocks)
+    _require(b_scales.is_contiguous(), "b_scales must be contiguous")
+    with _on_device(a):
+        _lib.check(_lib.lib().tw_gemm_fp8_block_nt(
+            out.data_ptr(), a.data_ptr(), a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), b.data_ptr(),
+            b_scales.data_ptr(), M, N, K, ldc, _DTYPE_CODE[out.dtype], _cap(max_cus), _stream_ptr(a)))
+
+
 def num_compute_units(device=None) -> int:
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(dev):

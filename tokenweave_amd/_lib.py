@@ -26,6 +26,10 @@ TW_SPLIT_MAX_TOKENS = 256
 TW_SPLIT_WORKSPACE_BYTES = TW_SPLIT_MAX_TOKENS * 384
 TW_ROTARY_INTERLEAVED = 1
 TW_ROTARY_INVERSE = 2
+TW_ACT_SILU = 0
+TW_ACT_GELU = 1
+TW_ACT_GELU_TANH = 2
+TW_FP8_GROUP = 128
 
 _vp, _i64, _u64, _f32, _ci = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint64,
                               ctypes.c_float, ctypes.c_int)
@@ -73,9 +77,16 @@ PROTOTYPES = {
     "tw_kv4_attention_workspace": [_ci, _ci, _ci, _i64, _i64, _i64, _i64, _ci],
     "tw_kv4_attention": [_hp, _hp, _vp, _i64, _ci, _ci, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _ci, _f32, _i64,
                          _ci, _vp, _i64, _vp],
+    "tw_gated_gemm_bf16_nt": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _ci, _ci, _vp],
+    "tw_gated_gemm_bf16_nt_backward_workspace": [_i64, _i64, _i64, _ci, _ci],
+    "tw_gated_gemm_bf16_nt_backward": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _ci, _ci, _vp, _i64,
+                                       _vp],
+    "tw_quant_fp8_groups": [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _ci, _ci, _vp],
+    "tw_gemm_fp8_block_nt": [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _ci, _ci, _vp],
 }
 # what an entry point returns where it is no status code
-RETURNS = {"tw_last_error": ctypes.c_char_p, "tw_kv4_attention_workspace": _i64}
+RETURNS = {"tw_last_error": ctypes.c_char_p, "tw_kv4_attention_workspace": _i64,
+           "tw_gated_gemm_bf16_nt_backward_workspace": _i64}
 
 _lib = None
 

@@ -76,6 +76,23 @@ int run_gemm_bf16_nt_partials(void* const* outs, const void* const* as, const vo
                               const void* const* biases, int count, int64_t M, int64_t N, int64_t K,
                               int64_t ldc, int max_cus, void* stream);
 
+// out[M, I] = act(a b[:I]^T) * (a b[I:]^T); both: null or [M, 2 I] for the two products.
+int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, int64_t M, int64_t I, int64_t K,
+                           int64_t ldc, int64_t ld_both, int act, int max_cus, void* stream);
+
+int64_t gated_backward_workspace(int64_t M, int64_t I, int64_t K, bool want_a, bool want_b);
+
+int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad_out, int64_t ld_grad, const void* a,
+                                    const void* b, const void* both, int64_t ld_both, int64_t M, int64_t I, int64_t K,
+                                    int act, int max_cus, void* workspace, int64_t workspace_bytes, void* stream);
+
+int run_quant_fp8_groups(void* out, float* scales, int64_t scale_row, int64_t scale_group, const void* input,
+                         int64_t ld_in, int64_t M, int64_t K, int act, int dtype, void* stream);
+
+int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64_t scale_row, int64_t scale_block,
+                          const void* b, const float* b_scales, int64_t M, int64_t N, int64_t K, int64_t ldc, int dtype,
+                          int max_cus, void* stream);
+
 struct Kv4Pages;
 
 // Whether an output's rows of head_size values are apart, whatever the order of its strides.

@@ -1,0 +1,592 @@
+// Rows to e4m3 codes with a scale for 128 channels, and the product of such rows with a weight of
+// e4m3 codes that has a scale for each block of 128 x 128.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "tw_activation.h"
+#include "tw_common.h"
+
+namespace tw {
+
+namespace {
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
+typedef __attribute__((address_space(3))) const u32x4_t lds_chunk_t;
+typedef __attribute__((address_space(3))) const float lds_f32_t;
+
+constexpr int GROUP = TW_FP8_GROUP;
+
+// ---------------------------------------------------------------------------
+// Codes
+//
+// A group of 128 channels is 16 lanes of 8: their largest magnitude by four exchanges, their codes as 8 bytes a lane.
+// A workgroup takes 16 rows of one group, its neighbours the next groups of the same rows: whole lines are read, and
+// the 16 scales leave together where the scales' rows are adjacent.
+// ---------------------------------------------------------------------------
+constexpr int QUANT_THREADS = 256;
+constexpr int QUANT_ROWS = QUANT_THREADS / 16;
+
+struct QuantArgs {
+  uint8_t* out;
+  float* scales;
+  const void* input;
+  int64_t scale_row, scale_group, ld_in;
+  int M, K, groups, act;
+};
+
+template <int DTYPE>
+__device__ __forceinline__ float load_one(const void* p, int64_t i) {
+  if (DTYPE == TW_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (DTYPE == TW_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
+  return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+}
+
+// Eight values from element `at` on, the first `n` of them; the others are zeros.  VEC: all or none, and 16-byte
+// aligned.
+template <int DTYPE, bool VEC>
+__device__ __forceinline__ void load_eight(float (&v)[8], const void* p, int64_t at, int n) {
+  if (!VEC) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? load_one<DTYPE>(p, at + e) : 0.0f;
+    return;
+  }
+  if (n < 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  } else if (DTYPE == TW_DTYPE_F32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const float4 x = q[0], y = q[1];
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (DTYPE == TW_DTYPE_F16) {
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, w[e]);
+        v[2 * e] = (float)h.x, v[2 * e + 1] = (float)h.y;
+      } else {
+        v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      }
+    }
+  }
+}
+
+// y / s as a float that rounds to the same e4m3 code as the exact quotient.  `inverse` is 1 / s; one correction makes
+// q the nearest float.  That may lie on the border of two codes (its low 19 bits are then zero; also below the least
+// normal code, whose borders have fewer bits) where the quotient does not: there q goes towards zero to the odd
+// neighbour or keeps its place with the lowest bit set, as the remainder says.
+__device__ __forceinline__ float quotient(float y, float s, float inverse) {
+  float q = y * inverse;
+  q = __fmaf_rn(__fmaf_rn(-q, s, y), inverse, q);
+  if ((__float_as_uint(q) & 0x7ffffu) == 0) {
+    const float rest = __fmaf_rn(-q, s, y);
+    if (rest != 0.0f) {
+      uint32_t bits = __float_as_uint(q);
+      if ((__float_as_uint(rest) ^ __float_as_uint(y)) >> 31) bits -= 1;  // |q| is the larger one; bits end in zeros
+      q = __uint_as_float(bits | 1u);
+    }
+  }
+  return q;
+}
+
+template <int DTYPE, bool GATED, bool VEC>
+__global__ __launch_bounds__(QUANT_THREADS) void quant_fp8_groups_kernel(QuantArgs w) {
+  const int unit = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int group = blockIdx.x % w.groups, row = blockIdx.x / w.groups * QUANT_ROWS + unit;
+  if (row >= w.M) return;
+  const int c = group * GROUP + lane * 8, n = min(max(w.K - c, 0), 8);
+  const int64_t at = row * w.ld_in + c;
+  float y[8];
+  load_eight<DTYPE, VEC>(y, w.input, at, n);
+  if (GATED) {
+    float u[8];
+    load_eight<DTYPE, VEC>(u, w.input, at + w.K, n);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = activation(y[e], w.act) * u[e];
+  }
+  // as whole numbers magnitudes are in order, infinities and NaN above all others
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(y[e]) & 0x7fffffffu);
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, x, 16));
+  const float largest = __uint_as_float(max(most, __float_as_uint(1e-10f)));
+  const float s = __fdiv_rn(largest, 448.0f);
+  if (lane == 0) w.scales[row * w.scale_row + group * w.scale_group] = s;
+  uint32_t code[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
+  if (most < 0x7f800000u) {
+    const float inverse = __frcp_rn(s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = quotient(y[e], s, inverse);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+      code[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], v, true);
+    }
+  }
+  uint8_t* to = w.out + (int64_t)row * w.K + c;
+  if (VEC) {
+    if (n == 8) *reinterpret_cast<uint2*>(to) = make_uint2(code[0], code[1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) to[e] = (uint8_t)(code[e >> 2] >> (8 * (e & 3)));
+  }
+}
+
+template <int DTYPE>
+void launch_quant(const QuantArgs& w, bool vec, int64_t grid, hipStream_t hs) {
+  auto go = [&](auto kernel) { launch_kernel(kernel, dim3((unsigned)grid), dim3(QUANT_THREADS), 0, hs, w); };
+  if (w.act >= 0) vec ? go(quant_fp8_groups_kernel<DTYPE, true, true>) : go(quant_fp8_groups_kernel<DTYPE, true, false>);
+  else vec ? go(quant_fp8_groups_kernel<DTYPE, false, true>) : go(quant_fp8_groups_kernel<DTYPE, false, false>);
+}
+
+// ---------------------------------------------------------------------------
+// The product.  A slab is one block of 128 of the inner dimension: 128 bytes a row, one matrix instruction of
+// 16 x 16 x 128 (two of 32 x 32 x 64) without a running sum, whose result is added to the fp32 sums with the product
+// of both scales.  Slabs lie in LDS as the bf16 kernels' do (128-byte rows, 16-byte chunk c of row r at c ^ key(r)).  The
+// order of the inner dimension inside an instruction is the same for both operands and otherwise free: a lane takes
+// chunks q and q + 4 of a row.
+// ---------------------------------------------------------------------------
+constexpr int ROWB = 128;
+[[maybe_unused]] constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
+constexpr int64_t BLOCK_MAX_K = 1 << 22;  // a tile's rows span at most 1 GiB
+
+struct BlockArgs {
+  uint16_t* out;
+  const uint8_t *a, *b;
+  const float *a_scales, *b_scales;
+  int64_t scale_row, scale_block, ldc;
+  int M, N, K, half_out, tiles_m, tiles_n, cols;
+};
+
+[[maybe_unused]] __device__ __forceinline__ uint32_t pack_out(float lo, float hi, int half_out) {
+  const f32x2_t v = {lo, hi};
+  return half_out ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t))
+                  : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
+}
+
+// Few rows: bound by reading b once.  As in the bf16 K-split kernel four waves share the inner dimension, wave w takes
+// the slabs w, w + 4, ..., each brings its own slabs of both operands and the rows' scales into LDS of its own, and the
+// four sums meet at the end as ((w0 + w1) + w2) + w3.
+constexpr int SPLIT_WAVES = 4;
+constexpr int SPLIT_THREADS = SPLIT_WAVES * 64;
+constexpr int split_stage(int mt, int nt) { return 32 * (mt + nt) * ROWB + 256; }
+constexpr int split_lds(int mt, int nt, int stages) {
+  const int slabs = SPLIT_WAVES * stages * split_stage(mt, nt), sums = SPLIT_WAVES * 32 * mt * (32 * nt * 4 + 16);
+  return slabs > sums ? slabs : sums;
+}
+
+template <int MT, int NT, int STAGES, int LA>
+__global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(BlockArgs w) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int RA = 32 * MT, RB = 32 * NT, LB = RB / 8, ROWS = 8 * LA, STAGE = split_stage(MT, NT);
+  constexpr int LOADS = LA + LB + 1;
+  static_assert(ROWS <= RA && RA <= 64, "one load of 64 lanes brings the rows' scales");
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, lhi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int K = w.K, nk = (K + GROUP - 1) / GROUP, tail_chunks = (K % GROUP) / 16;
+  const bool even = ((lane & 7) ^ (lane >> 4)) < tail_chunks, odd = ((lane & 7) ^ (lane >> 4) ^ 4) < tail_chunks;
+  uint32_t v[LA > LB ? LA : LB], roff[4];
+#pragma unroll
+  for (int j = 0; j < (LA > LB ? LA : LB); ++j)
+    v[j] = (uint32_t)(j * 8 + (lane >> 3)) * (uint32_t)K + (((lane & 7) ^ (((j & 1) << 2) | (lane >> 4))) << 4);
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) roff[kk] = l32 * ROWB + ((((kk << 1) | lhi) ^ ((l32 >> 1) & 7)) << 4);
+  uint8_t* const mine = lds + wave * (STAGES * STAGE);
+
+  const int num_tiles = w.tiles_m * w.tiles_n;
+  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+    // every XCD a contiguous range of tiles, the row tiles of one column range next to each other
+    int pid = t;
+    const int per_xcd = num_tiles / 8;
+    if (t < per_xcd * 8) pid = (t & 7) * per_xcd + (t >> 3);
+    const int m0 = pid % w.tiles_m * ROWS, n0 = pid / w.tiles_m * w.cols;
+    const int rows = min(w.M - m0, ROWS);
+    const __amdgpu_buffer_rsrc_t da = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(w.a) + (size_t)m0 * K, 0, (uint32_t)rows * (uint32_t)K, 0x00020000);
+    const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(w.b) + (size_t)n0 * K, 0, (uint32_t)min(w.N - n0, w.cols) * (uint32_t)K, 0x00020000);
+    // a row's scales, one for each lane that has a row
+    const float* const my_scales = w.a_scales + (int64_t)(m0 + min(lane, rows - 1)) * w.scale_row;
+    // columns before `border` belong to the first of the two weight blocks that a tile may touch
+    const float* const sb = w.b_scales + (int64_t)(n0 / GROUP) * nk;
+    const int border = GROUP - n0 % GROUP;
+    const int64_t second = n0 / GROUP + 1 < (w.N + GROUP - 1) / GROUP ? nk : 0;
+
+    f32x16_t acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    int next = wave;
+    uint32_t fill = 0, use = 0;
+    auto issue = [&]() {
+      const bool last = tail_chunks && next == nk - 1;
+      uint8_t* s = mine + fill;
+      const uint32_t koff = (uint32_t)next * ROWB;
+#pragma unroll
+      for (int j = 0; j < LB; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(s + RA * ROWB + j * 1024), 16,
+                                                 !last || ((j & 1) ? odd : even) ? v[j] : OUT_OF_RANGE, koff, 0, 0);
+#pragma unroll
+      for (int j = 0; j < LA; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_void_t*)(s + j * 1024), 16,
+                                                 !last || ((j & 1) ? odd : even) ? v[j] : OUT_OF_RANGE, koff, 0, 0);
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(my_scales + (int64_t)next * w.scale_block),
+          (lds_void_t*)(s + (RA + RB) * ROWB), 4, 0, 0);
+      next += SPLIT_WAVES;
+      fill = fill == (STAGES - 1) * STAGE ? 0 : fill + STAGE;
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+      if (next < nk) issue();
+    for (int slab = wave; slab < nk; slab += SPLIT_WAVES, use = use == (STAGES - 1) * STAGE ? 0 : use + STAGE) {
+      const float sb0 = sb[slab], sb1 = sb[slab + second];
+      if (next < nk) {
+        issue();
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
+      } else if (STAGES == 3 && slab + SPLIT_WAVES < nk) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      const uint8_t* pa = mine + use;
+      const uint8_t* pb = pa + RA * ROWB;
+      f32x16_t part[MT][NT];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        i32x8_t fa[MT], fb[NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(pa + i * 32 * ROWB + roff[2 * h]);
+          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(pa + i * 32 * ROWB + roff[2 * h + 1]);
+          fa[i] = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(pb + j * 32 * ROWB + roff[2 * h]);
+          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(pb + j * 32 * ROWB + roff[2 * h + 1]);
+          fb[j] = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            part[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                fb[j], fa[i], h ? part[i][j] : f32x16_t{}, 0, 0, 0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const float sa = *reinterpret_cast<const float*>(mine + use + (RA + RB) * ROWB + (i * 32 + l32) * 4);
+        const float s0 = sa * sb0, s1 = sa * sb1;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float s = j * 32 + 8 * q + 4 * lhi < border ? s0 : s1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = __fmaf_rn(part[i][j][4 * q + e], s, acc[i][j][4 * q + e]);
+          }
+      }
+      // the fragments and scales are in registers: the loads issued next may overwrite this stage
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+
+    // acc[i][j][4 q + e]: sum of out[m0 + i*32 + l32][n0 + j*32 + 8 q + 4 lhi + e]
+    constexpr int PITCH = RB * 4 + 16;
+    __syncthreads();
+    uint8_t* const sums = lds + wave * (RA * PITCH);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4_t*>(sums + (i * 32 + l32) * PITCH + (j * 32 + 8 * q + 4 * lhi) * 4) =
+              f32x4_t{acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __syncthreads();
+    for (int g = tid; g < ROWS * RB / 4; g += SPLIT_THREADS) {
+      const int m = g / (RB / 4), c = (g % (RB / 4)) * 4;
+      if (m < rows && c < w.cols && n0 + c < w.N) {
+        const uint8_t* p = lds + m * PITCH + c * 4;
+        f32x4_t s = *reinterpret_cast<const f32x4_t*>(p);
+#pragma unroll
+        for (int x = 1; x < SPLIT_WAVES; ++x) s += *reinterpret_cast<const f32x4_t*>(p + x * (RA * PITCH));
+        *reinterpret_cast<uint2*>(w.out + (size_t)(m0 + m) * w.ldc + n0 + c) =
+            make_uint2(pack_out(s.x, s.y, w.half_out), pack_out(s.z, s.w, w.half_out));
+      }
+    }
+    __syncthreads();  // the next tile's slabs overwrite the sums
+  }
+#endif
+}
+
+// More rows: tiles of (32 TM) x (64 TN), eight waves (2 x 4) of (16 TM) x (16 TN), two slabs in LDS.  The sums cannot stay
+// in accumulation registers, which vector instructions do not reach; two waves a SIMD let one multiply while the
+// other's results are added.
+constexpr int WIDE_THREADS = 512;
+constexpr int wide_stage(int tm, int tn) { return (32 * tm + 64 * tn) * ROWB + 32 * tm * 4; }
+
+template <int TM, int TN>
+__global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(BlockArgs w) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int BM = 32 * TM, BN = 64 * TN, STAGE = wide_stage(TM, TN), PA = BM * ROWB, PB = BN * ROWB;
+  constexpr int BLOCKS = (BM + BN) / 8;  // 8-row blocks of both panels, dealt out to the waves
+  constexpr int LOADS = (BLOCKS + 7) / 8;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  lds_u8_t* const base = (lds_u8_t*)lds;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3, r16 = lane & 15, quad = lane >> 4;
+  const int K = w.K, nk = (K + GROUP - 1) / GROUP, tail_chunks = K % GROUP ? (K % GROUP) / 16 : 8;
+
+  const uint32_t row_a = (wm * 16 * TM + r16) * ROWB;
+  // MFMA row r of the pair of tiles (2 p, 2 p + 1) is column 32 p + 8 (r / 4) + 4 (tile & 1) + r % 4; a wave of one
+  // tile of columns keeps their order
+  const uint32_t row_b = PA + (wn * 16 * TN + (TN > 1 ? (r16 >> 2) * 8 + (r16 & 3) : r16)) * ROWB;
+  const uint32_t key_b = TN > 1 ? r16 >> 1 : ((r16 >> 1) & 1) | ((r16 >> 3) & 1) << 1 | (wn & 1) << 2;
+  const uint32_t a0 = row_a + ((quad ^ (r16 >> 1)) << 4), a1 = row_a + (((4 + quad) ^ (r16 >> 1)) << 4);
+  const uint32_t b0 = row_b + ((quad ^ key_b) << 4), b1 = row_b + (((4 + quad) ^ key_b) << 4);
+
+  const int num_tiles = w.tiles_m * w.tiles_n;
+  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+  int pid = t;
+  const int per_xcd = num_tiles / 8;
+  if (t < per_xcd * 8) pid = (t & 7) * per_xcd + (t >> 3);
+  const int sweep = 4 * w.tiles_n, group = pid / sweep, first = group * 4, in_group = min(w.tiles_m - first, 4);
+  const int m0 = (first + pid % sweep % in_group) * BM, n0 = pid % sweep / in_group * BN;
+  const int rows = min(w.M - m0, BM), cols = min(w.N - n0, BN);
+
+  const __amdgpu_buffer_rsrc_t da = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(w.a) + (size_t)m0 * K, 0, (uint32_t)rows * (uint32_t)K, 0x00020000);
+  const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(w.b) + (size_t)n0 * K, 0, (uint32_t)cols * (uint32_t)K, 0x00020000);
+  uint32_t v[LOADS];
+  int chunk[LOADS];
+#pragma unroll
+  for (int l = 0; l < LOADS; ++l) {
+    const int blk = wave + l * 8;
+    const bool of_a = blk < BM / 8;
+    const int in = of_a ? blk : blk - BM / 8;
+    const int key = of_a ? ((in & 1) << 2) | (lane >> 4) : ((lane >> 4) & 1) | ((in & 3) << 1);
+    chunk[l] = (lane & 7) ^ key;
+    v[l] = (uint32_t)(in * 8 + (lane >> 3)) * (uint32_t)K + (chunk[l] << 4);
+  }
+  auto load = [&](int slab, uint32_t stage) {
+    const int chunks = slab == nk - 1 ? tail_chunks : 8;
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      const int blk = wave + l * 8;
+      if (blk < BLOCKS)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(blk < BM / 8 ? da : db, (lds_void_t*)(base + stage + blk * 1024), 16,
+                                                 chunk[l] < chunks ? v[l] : OUT_OF_RANGE, (uint32_t)slab * ROWB, 0, 0);
+    }
+    if (wave * 64 < BM) {
+      const int row = m0 + min(wave * 64 + lane, rows - 1);
+      if (wave * 64 + lane < BM)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(w.a_scales + row * w.scale_row + slab * w.scale_block),
+            (lds_void_t*)(base + stage + PA + PB + wave * 256), 4, 0, 0);
+    }
+  };
+  const int block_n = min((n0 + wn * 16 * TN) / GROUP, (w.N - 1) / GROUP);
+  const float* const sb = w.b_scales + (int64_t)block_n * nk;
+
+  f32x4_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
+
+  float next_s = sb[0];
+  load(0, 0);
+  for (int slab = 0; slab < nk; ++slab) {
+    const uint32_t use = (slab & 1) * STAGE;
+    const float s = next_s;
+    // this slab has arrived (every wave waited for its own loads), the other stage's readers are done
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (slab + 1 < nk) {
+      load(slab + 1, STAGE - use);
+      next_s = sb[slab + 1];
+    }
+    i32x8_t fb[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const uint32_t at = use + (TN > 1 ? (j >> 1) * 4096 + (j & 1) * 512 : 0);
+      const u32x4_t x = *(lds_chunk_t*)(base + at + b0), y = *(lds_chunk_t*)(base + at + b1);
+      fb[j] = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const u32x4_t x = *(lds_chunk_t*)(base + use + i * 2048 + a0), y = *(lds_chunk_t*)(base + use + i * 2048 + a1);
+      const i32x8_t fa = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+      const float scale = s * *(lds_f32_t*)(base + use + PA + PB + (wm * 16 * TM + i * 16 + r16) * 4);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const f32x4_t part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, f32x4_t{}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(part[e], scale, acc[i][j][e]);
+      }
+    }
+  }
+
+  // a lane holds row r16 of each row tile: columns 8 quad + 0 .. 7 of a pair of tiles, 4 quad + 0 .. 3 of a single one
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = wm * 16 * TM + i * 16 + r16;
+    if (m >= rows) continue;
+    uint16_t* to = w.out + (size_t)(m0 + m) * w.ldc + n0;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int c = wn * 16 * TN + (TN > 1 ? (j >> 1) * 32 + quad * 8 + (j & 1) * 4 : quad * 4);
+      if (c < cols)
+        *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_out(acc[i][j][0], acc[i][j][1], w.half_out),
+                                                       pack_out(acc[i][j][2], acc[i][j][3], w.half_out));
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next tile's first slab goes where this one's last may be
+  }
+#endif
+}
+
+constexpr int kMaxDevices = 64;
+
+// More than 64 KiB of dynamic LDS must be allowed once per function and device.
+template <typename Kernel>
+int allow_lds(Kernel kernel, std::atomic<bool>* ok, int bytes) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices)
+    return set_error(TW_ERR_LAUNCH, "gemm_fp8_block_nt: no current device");
+  if (!ok[dev].load(std::memory_order_acquire)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+        hipSuccess)
+      return set_error(TW_ERR_LAUNCH, "gemm_fp8_block_nt: the device refused %d bytes of LDS", bytes);
+    ok[dev].store(true, std::memory_order_release);
+  }
+  return TW_OK;
+}
+
+template <int MT, int NT, int STAGES, int LA>
+int launch_split(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
+  constexpr int LDS = split_lds(MT, NT, STAGES);
+  static std::atomic<bool> ok[kMaxDevices];
+  const auto kernel = gemm_fp8_block_split_kernel<MT, NT, STAGES, LA>;
+  if (int rc = allow_lds(kernel, ok, LDS)) return rc;
+  // tiles just wide enough for a whole number of workgroups per compute unit
+  w.tiles_m = (w.M + 8 * LA - 1) / (8 * LA);
+  const int64_t full = (w.N + 32 * NT - 1) / (32 * NT), rounds = (w.tiles_m * full + cus - 1) / cus;
+  const int64_t columns = std::max<int64_t>(full, cus * rounds / w.tiles_m);
+  w.cols = (int)std::min<int64_t>(32 * NT, ((w.N + columns - 1) / columns + 3) / 4 * 4);
+  w.tiles_n = (w.N + w.cols - 1) / w.cols;
+  int64_t grid = (int64_t)w.tiles_m * w.tiles_n;
+  if (max_cus > 0 && grid > max_cus) grid = max_cus;
+  launch_kernel(kernel, dim3((unsigned)grid), dim3(SPLIT_THREADS), LDS, hs, w);
+  return TW_OK;
+}
+
+template <int TM, int TN>
+int launch_wide(BlockArgs w, int max_cus, hipStream_t hs) {
+  constexpr int LDS = 2 * wide_stage(TM, TN);
+  static std::atomic<bool> ok[kMaxDevices];
+  const auto kernel = gemm_fp8_block_tile_kernel<TM, TN>;
+  if (int rc = allow_lds(kernel, ok, LDS)) return rc;
+  w.tiles_m = (w.M + 32 * TM - 1) / (32 * TM);
+  w.tiles_n = (w.N + 64 * TN - 1) / (64 * TN);
+  int64_t grid = (int64_t)w.tiles_m * w.tiles_n;
+  if (max_cus > 0 && grid > max_cus) grid = max_cus;
+  launch_kernel(kernel, dim3((unsigned)grid), dim3(WIDE_THREADS), LDS, hs, w);
+  return TW_OK;
+}
+
+}  // namespace
+
+int run_quant_fp8_groups(void* out, float* scales, int64_t scale_row, int64_t scale_group, const void* input,
+                         int64_t ld_in, int64_t M, int64_t K, int act, int dtype, void* stream) {
+  const char* what = "quant_fp8_groups";
+  if (M < 0 || K <= 0 || M > INT32_MAX || K > INT32_MAX / 4)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad shape, %lld rows of %lld", what, (long long)M, (long long)K);
+  if (act > TW_ACT_GELU_TANH) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, act);
+  if (dtype != TW_DTYPE_BF16 && dtype != TW_DTYPE_F16 && dtype != TW_DTYPE_F32)
+    return set_error(TW_ERR_DTYPE, "%s: unknown dtype %d", what, dtype);
+  const int64_t width = act >= 0 ? 2 * K : K, size = dtype == TW_DTYPE_F32 ? 4 : 2;
+  if (M > 1 && ld_in < width)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: rows of %lld at a stride of %lld", what, (long long)width,
+                     (long long)ld_in);
+  if (M == 0) return TW_OK;
+  if (!out || !scales || !input) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
+  if (reinterpret_cast<uintptr_t>(input) % size || reinterpret_cast<uintptr_t>(scales) % 4)
+    return set_error(TW_ERR_ALIGNMENT, "%s: input and scales must be aligned to their elements", what);
+  QuantArgs w = {};
+  w.out = static_cast<uint8_t*>(out);
+  w.scales = scales;
+  w.input = input;
+  w.scale_row = scale_row, w.scale_group = scale_group, w.ld_in = ld_in;
+  w.M = (int)M, w.K = (int)K, w.groups = (int)((K + GROUP - 1) / GROUP), w.act = act < 0 ? -1 : act;
+  const int64_t grid = (M + QUANT_ROWS - 1) / QUANT_ROWS * w.groups;
+  if (grid > INT32_MAX) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too large", what);
+  const bool vec = K % 8 == 0 && ld_in * size % 16 == 0 && reinterpret_cast<uintptr_t>(input) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % 8 == 0;
+  const hipStream_t hs = static_cast<hipStream_t>(stream);
+  if (dtype == TW_DTYPE_BF16) launch_quant<TW_DTYPE_BF16>(w, vec, grid, hs);
+  else if (dtype == TW_DTYPE_F16) launch_quant<TW_DTYPE_F16>(w, vec, grid, hs);
+  else launch_quant<TW_DTYPE_F32>(w, vec, grid, hs);
+  return finish_launch(what);
+}
+
+int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64_t scale_row, int64_t scale_block,
+                          const void* b, const float* b_scales, int64_t M, int64_t N, int64_t K, int64_t ldc, int dtype,
+                          int max_cus, void* stream) {
+  const char* what = "gemm_fp8_block_nt";
+  if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > BLOCK_MAX_K || ldc < N)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad shape M=%lld N=%lld K=%lld ldc=%lld", what, (long long)M,
+                     (long long)N, (long long)K, (long long)ldc);
+  if (K % 16 != 0 || N % 4 != 0 || ldc % 4 != 0)
+    return set_error(TW_ERR_ALIGNMENT, "%s: needs K %% 16 == 0, N %% 4 == 0, ldc %% 4 == 0", what);
+  if (dtype != TW_DTYPE_BF16 && dtype != TW_DTYPE_F16)
+    return set_error(TW_ERR_DTYPE, "%s: out must be bf16 or fp16, got dtype %d", what, dtype);
+  if (M == 0) return TW_OK;
+  if (!out || !a || !a_scales || !b || !b_scales)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
+  auto misaligned = [](const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
+  if (misaligned(a, 16) || misaligned(b, 16) || misaligned(out, 8) || misaligned(a_scales, 4) || misaligned(b_scales, 4))
+    return set_error(TW_ERR_ALIGNMENT, "%s: needs 16-byte aligned a and b, 8-byte aligned out, 4-byte aligned scales",
+                     what);
+  BlockArgs w = {};
+  w.out = static_cast<uint16_t*>(out);
+  w.a = static_cast<const uint8_t*>(a);
+  w.b = static_cast<const uint8_t*>(b);
+  w.a_scales = a_scales, w.b_scales = b_scales;
+  w.scale_row = scale_row, w.scale_block = scale_block, w.ldc = ldc;
+  w.M = (int)M, w.N = (int)N, w.K = (int)K, w.half_out = dtype == TW_DTYPE_F16;
+  const hipStream_t hs = static_cast<hipStream_t>(stream);
+  int cus = device_compute_units(), rc;
+  if (cus <= 0) cus = 256;
+  if (M <= 8) rc = launch_split<1, 1, 3, 1>(w, max_cus, cus, hs);
+  else if (M <= 16) rc = launch_split<1, 1, 3, 2>(w, max_cus, cus, hs);
+  else if (M <= 32) rc = launch_split<1, 1, 3, 4>(w, max_cus, cus, hs);
+  else if (M <= 64) rc = launch_split<2, 1, 3, 8>(w, max_cus, cus, hs);
+  else if (M <= 128) rc = launch_split<2, 2, 2, 8>(w, max_cus, cus, hs);
+  else rc = launch_wide<8, 4>(w, max_cus, hs);
+  return rc ? rc : finish_launch(what);
+}
+
+}  // namespace tw

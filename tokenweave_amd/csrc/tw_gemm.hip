@@ -28,7 +28,9 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
+#include "tw_activation.h"
 #include "tw_common.h"
 
 namespace tw {
@@ -196,6 +198,19 @@ struct GemmBatch {
   const uint16_t* bias[TW_MAX_PARTIALS];  // [N] bf16 or null: added to that product only
 };
 
+// The gated form (GATED) of both kernels below: b is [2 I, K], a gate row and an up row for each of the I columns of
+// out, out = act(a gate^T) * (a up^T).  A tile's rows of b are half gate and half up rows of the same columns, so both
+// sums of an element meet in one lane (tile kernel) or one thread (K-split kernel) as fp32 and the product is rounded
+// once.  `both`, where given, also takes the two sums, rounded: [M][2 I], what the gradient needs.
+struct GatedOut {
+  uint16_t* both;
+  int64_t ld_both;
+  int act;  // TW_ACT_*
+};
+struct NotGated {};
+template <bool GATED>
+using GatedArg = std::conditional_t<GATED, GatedOut, NotGated>;
+
 // ---------------------------------------------------------------------------
 // K-split kernel: few rows (a decode step, a short prefill chunk).  The product is bound by
 // reading b once, so what counts is how many compute units stream it and how evenly.
@@ -256,9 +271,11 @@ __device__ __forceinline__ void ks_issue(__amdgpu_buffer_rsrc_t d, const uint32_
 // LA: the tile's 8-row blocks of a: 4 MT, or only as many as its share of the rows needs (the rest of its MFMA
 // blocks is then whatever LDS holds: it reaches no output row but its own, which is not stored).
 // BAUX: cache policy of b's loads.
-template <int MT, int NT, int STAGES, int LA, int BAUX, bool TAIL>
+// GATED: N and cols count columns of out; the upper half of a slab's b rows are up rows.
+template <int MT, int NT, int STAGES, int LA, int BAUX, bool TAIL, bool GATED = false>
 __global__ __launch_bounds__(KS_THREADS) void gemm_bf16_nt_ksplit_kernel(
-    GemmBatch batch, int count, int M, int N, int K, int64_t ldc, int tiles_m, int tiles_n, int cols) {
+    GemmBatch batch, int count, int M, int N, int K, int64_t ldc, int tiles_m, int tiles_n, int cols,
+    GatedArg<GATED> gated) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass only needs the stub, and cannot instantiate the device builtins
   constexpr int RA = 32 * MT, RB = 32 * NT, LB = RB / 8, ROWS = 8 * LA;
   static_assert(ROWS <= RA, "a tile's rows fit its MFMA blocks");
@@ -317,6 +334,9 @@ __global__ __launch_bounds__(KS_THREADS) void gemm_bf16_nt_ksplit_kernel(
         const_cast<uint16_t*>(a) + (size_t)m0 * K, 0, (uint32_t)min(M - m0, ROWS) * (uint32_t)K * 2u, 0x00020000);
     const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t*>(b) + (size_t)n0 * K, 0, (uint32_t)min(N - n0, cols) * (uint32_t)K * 2u, 0x00020000);
+    [[maybe_unused]] const __amdgpu_buffer_rsrc_t du = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(b) + (size_t)(N + n0) * K, 0,
+        GATED ? (uint32_t)min(N - n0, cols) * (uint32_t)K * 2u : 0u, 0x00020000);
 
     f32x16_t acc[MT][NT];
 #pragma unroll
@@ -332,7 +352,12 @@ __global__ __launch_bounds__(KS_THREADS) void gemm_bf16_nt_ksplit_kernel(
     auto issue = [&]() {
       const bool last = next == nk - 1;
       uint8_t* s = mine + fill;
-      ks_issue<LB, BAUX, TAIL>(db, vb, s + RA * KS_ROWB, (uint32_t)next * KS_ROWB, last, even, odd);
+      if constexpr (GATED) {  // an even number of 8-row blocks each: the offsets and the swizzle of a half are alike
+        ks_issue<LB / 2, BAUX, TAIL>(db, vb, s + RA * KS_ROWB, (uint32_t)next * KS_ROWB, last, even, odd);
+        ks_issue<LB / 2, BAUX, TAIL>(du, vb, s + (RA + RB / 2) * KS_ROWB, (uint32_t)next * KS_ROWB, last, even, odd);
+      } else {
+        ks_issue<LB, BAUX, TAIL>(db, vb, s + RA * KS_ROWB, (uint32_t)next * KS_ROWB, last, even, odd);
+      }
       ks_issue<LA, 0, TAIL>(da, va, s, (uint32_t)next * KS_ROWB, last, even, odd);
       next += KS_WAVES;
       fill = fill == (STAGES - 1) * STAGE ? 0 : fill + STAGE;
@@ -384,6 +409,30 @@ __global__ __launch_bounds__(KS_THREADS) void gemm_bf16_nt_ksplit_kernel(
           *reinterpret_cast<f32x4_t*>(sums + (i * 32 + l32) * PITCH + (j * 32 + 8 * q + 4 * lhi) * 4) =
               f32x4_t{acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     __syncthreads();
+    if constexpr (GATED) {
+      for (int g = tid; g < ROWS * RB / 8; g += KS_THREADS) {
+        const int m = g / (RB / 8), c = (g % (RB / 8)) * 4;
+        if (m0 + m < M && c < cols && n0 + c < N) {
+          const uint8_t* p = lds_ks + m * PITCH + c * 4;
+          f32x4_t s = *reinterpret_cast<const f32x4_t*>(p), u = *reinterpret_cast<const f32x4_t*>(p + RB * 2);
+#pragma unroll
+          for (int w = 1; w < KS_WAVES; ++w) {
+            s += *reinterpret_cast<const f32x4_t*>(p + w * (RA * PITCH));
+            u += *reinterpret_cast<const f32x4_t*>(p + w * (RA * PITCH) + RB * 2);
+          }
+          if (gated.both) {
+            uint16_t* to = gated.both + (size_t)(m0 + m) * gated.ld_both + n0 + c;
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
+            *reinterpret_cast<uint2*>(to + N) = make_uint2(pack2(u.x, u.y), pack2(u.z, u.w));
+          }
+          *reinterpret_cast<uint2*>(out + (size_t)(m0 + m) * ldc + n0 + c) =
+              make_uint2(pack2(activation(s.x, gated.act) * u.x, activation(s.y, gated.act) * u.y),
+                         pack2(activation(s.z, gated.act) * u.z, activation(s.w, gated.act) * u.w));
+        }
+      }
+      __syncthreads();  // the next tile's slabs overwrite the sums
+      continue;
+    }
     for (int g = tid; g < ROWS * RB / 4; g += KS_THREADS) {
       const int m = g / (RB / 4), c = (g % (RB / 4)) * 4;
       if (m0 + m < M && c < cols && n0 + c < N) {  // N and cols are multiples of 4
@@ -596,6 +645,51 @@ __device__ __forceinline__ void tile_store(const f32x4_t (&acc)[TM][TN], __amdgp
   }
 }
 
+__device__ __forceinline__ float acc_read(float x) {
+  float y;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(y) : "a"(x));
+  return y;
+}
+
+// The gated form: tiles 4 p .. 4 p + 3 of a row of tiles are gate, up, gate, up of eight columns, 32 p + 8 quad and up.
+// Rows of 8 bytes' alignment or I % 8 != 0 (narrow) take two stores.
+template <int TM, int TN, bool WIDE>
+__device__ __forceinline__ void tile_store_gated(const f32x4_t (&acc)[TM][TN], __amdgpu_buffer_rsrc_t dc,
+                                                 uint32_t row_off, uint32_t row_step, int n, int N, int m, int M,
+                                                 const GatedOut& gated) {
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int p = 0; p < TN / 4; ++p) {
+      const int c = n + p * 32;
+      u32x2_t v[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float g[4], u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = acc_read(acc[i][4 * p + 2 * s][e]), u[e] = acc_read(acc[i][4 * p + 2 * s + 1][e]);
+        if (gated.both && m + 16 * i < M && c + 4 * s < N) {
+          uint16_t* to = gated.both + (size_t)(m + 16 * i) * gated.ld_both + c + 4 * s;
+          *reinterpret_cast<uint2*>(to) = make_uint2(pack2(g[0], g[1]), pack2(g[2], g[3]));
+          *reinterpret_cast<uint2*>(to + N) = make_uint2(pack2(u[0], u[1]), pack2(u[2], u[3]));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = activation(g[e], gated.act) * u[e];
+        v[s] = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+      }
+      const uint32_t off = row_off + (uint32_t)i * row_step + (uint32_t)p * 64u;
+      if (WIDE) {
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{v[0].x, v[0].y, v[1].x, v[1].y}, dc,
+                                               c < N ? off : TILE_OUT_OF_RANGE, 0, kStoreThrough);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b64(v[0], dc, c < N ? off : TILE_OUT_OF_RANGE, 0, kStoreThrough);
+        __builtin_amdgcn_raw_buffer_store_b64(v[1], dc, c + 4 < N ? off + 8u : TILE_OUT_OF_RANGE, 0, kStoreThrough);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
 // Where the loader stands: product, tile and slab of the next slab to request.
 struct TilePlace {
   int product, m0, n0;
@@ -641,11 +735,19 @@ __device__ __forceinline__ TilePlace tile_place(int t, int num_tiles, int tiles_
 // -> 40.4 / 37.0 -> 33.5, 640: 69.4 -> 49.7 / 48.9 -> 41.4, 800: 71.5 -> 70.7 / 49.7 -> 50.6, 1000: 77.0 -> 71.1 /
 // 55.0 -> 51.8; K = 7392 (both from memory), 200 rows 61 -> 50, 256: 72 -> 57, 512: 85 -> 77, 640: 122 -> 96.  On one
 // set again and again the units are busy 4 % fewer cycles at 1000 rows and 3 to 7 % more at 200.
-template <int TM, int TN, TileRows ROWS>
+//
+// GATED: N counts columns of out, BN / 2 a tile.  Row x of b's panel is a gate row where bit 2 of x is clear and an up
+// row where it is set, of column 32 (x / 64) + 8 (x / 8 % 4) + 4 (x / 32 % 2) + x % 4 of the tile: a lane's accumulators
+// are then eight adjacent columns of both.
+template <int TM, int TN, TileRows ROWS, bool GATED = false>
 __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nt_tile_kernel(
-    GemmBatch batch, int count, int M, int N, int K, int64_t ldc, int tiles_m, int tiles_n, int wide_store) {
+    GemmBatch batch, int count, int M, int N, int K, int64_t ldc, int tiles_m, int tiles_n, int wide_store,
+    GatedArg<GATED> gated) {
 #ifdef __HIP_DEVICE_COMPILE__
+  static_assert(!GATED || (TN % 4 == 0 && ROWS != kLines), "gate and up rows alternate in groups of 64");
   using S = TileShape<TM, TN, ROWS>;
+  // after a tile: how many stores its first barrier does not wait for
+  constexpr int STORES = GATED ? S::STORES / 2 : S::STORES;
   constexpr int LA = S::LA, LB = S::LB, PA = S::PA, PB = S::PB, D = S::D;
   constexpr uint32_t AHEAD = S::LINES ? 128 : 0;  // the loads' offsets begin a line ahead of the tile
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_tile[];
@@ -678,7 +780,10 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     }                                                                                                        \
     _Pragma("unroll") for (int l = 0; l < LB; ++l) {                                                         \
       const int blk = wave * LB + l, c = (lane & 7) ^ (((lane >> 4) & 1) | ((blk & 3) << 1));                \
-      vb[l] = c < (chunks) ? (uint32_t)((blk * 8 + (lane >> 3)) * K + c * 8) * 2u : TILE_OUT_OF_RANGE;       \
+      const uint32_t row = !GATED ? blk * 8 + (lane >> 3)                                                    \
+                                  : (uint32_t)((lane >> 5) * N + 32 * (blk >> 3) + 8 * (blk & 3) +           \
+                                               4 * ((blk >> 2) & 1) + ((lane >> 3) & 3));                    \
+      vb[l] = c < (chunks) ? (row * (uint32_t)K + c * 8) * 2u : TILE_OUT_OF_RANGE;                           \
     }                                                                                                        \
   } while (0)
   // kLines: the same for line `line` of every row: lane position x holds the line's chunk x ^ key ^ flip, so
@@ -708,13 +813,15 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   do {                                                                                                       \
     const bool in = lt < num_tiles;                                                                          \
     const TilePlace p = tile_place<TM, TN>(in ? lt : 0, num_tiles, tiles_m, tiles_n);                        \
-    const uint16_t *pa = batch.a[p.product] + (size_t)p.m0 * K, *pb = batch.b[p.product] + (size_t)p.n0 * K; \
+    const uint16_t* pa = batch.a[p.product] + (size_t)p.m0 * K;                                              \
+    const uint16_t* pb = batch.b[p.product] + (size_t)(GATED ? p.n0 / 2 : p.n0) * K;                         \
     if (S::LINES) load_phase_a = line_phase(pa), load_phase_b = line_phase(pb);                              \
     da = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pa) - (int)AHEAD / 2, 0,                    \
                                            in ? (uint32_t)min(M - p.m0, S::BM) * (uint32_t)K * 2u + AHEAD : 0u, \
                                            0x00020000);                                                      \
     db = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pb) - (int)AHEAD / 2, 0,                    \
-                                           in ? (uint32_t)min(N - p.n0, S::BN) * (uint32_t)K * 2u + AHEAD : 0u, \
+                                           in ? (uint32_t)(GATED ? 2 * N - p.n0 / 2 : min(N - p.n0, S::BN)) * \
+                                                        (uint32_t)K * 2u + AHEAD : 0u,                       \
                                            0x00020000);                                                      \
   } while (0)
 #define TW_TILE_ADVANCE()                                                                                    \
@@ -782,7 +889,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
                                        TW_AT(use_b, b1, next_b1, PB, S::SB), \
                                        da, db, va, vb, wa + fill_a, wb + fill_b, lk * 128u);                 \
     if (AFTER_STORE)                                                                                         \
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT + S::STORES) : "memory"); \
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT + STORES) : "memory");   \
     else                                                                                                     \
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT) : "memory");            \
     TW_RING(use_a, PA, S::SA);                                                                               \
@@ -800,6 +907,16 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     for (int kt = 1; kt < nk; ++kt) TW_TILE_SLAB(false, false);
 
     const TilePlace p = tile_place<TM, TN>(t, num_tiles, tiles_m, tiles_n);
+    if constexpr (GATED) {
+      const int n0 = p.n0 / 2, col = wn * 8 * TN + quad * 8, row = wm * 16 * TM + r16;
+      const __amdgpu_buffer_rsrc_t dc = __builtin_amdgcn_make_buffer_rsrc(
+          batch.out[0] + (size_t)p.m0 * ldc + n0, 0, (uint32_t)min(M - p.m0, S::BM) * (uint32_t)ldc * 2u, 0x00020000);
+      const uint32_t row_off = (uint32_t)(row * (int)ldc + col) * 2u, row_step = (uint32_t)ldc * 32u;
+      asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMA's result is written
+      if (wide_store) tile_store_gated<TM, TN, true>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
+      else tile_store_gated<TM, TN, false>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
+      continue;
+    }
     const uint16_t* __restrict__ bias = batch.bias[p.product];
     const __amdgpu_buffer_rsrc_t dc = __builtin_amdgcn_make_buffer_rsrc(
         batch.out[p.product] + (size_t)p.m0 * ldc + p.n0, 0, (uint32_t)min(M - p.m0, S::BM) * (uint32_t)ldc * 2u,
@@ -817,7 +934,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     // The tile's rows have one line more than slabs: a slab without products between this tile and the next.
     if (S::LINES && t + (int)gridDim.x < num_tiles) {
       tile_loads<TM, TN, ROWS, 0>(da, db, va, vb, wa + fill_a, wb + fill_b, lk * 128u);
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT + S::STORES) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT + STORES) : "memory");
       TW_RING(use_a, PA, S::SA);
       TW_RING(use_b, PB, S::SB);
       place_reader(t + gridDim.x);
@@ -869,18 +986,18 @@ static KsTiles ksplit_tiles(int64_t M, int64_t N, int count, int rows, int most_
   return {tiles_m, (N + cols - 1) / cols, cols};
 }
 
-template <int MT, int NT, int STAGES, int LA, int BAUX, bool TAIL>
+template <int MT, int NT, int STAGES, int LA, int BAUX, bool TAIL, bool GATED>
 static int launch_ksplit(const GemmBatch& batch, int count, int64_t M, int64_t N, int64_t K, int64_t ldc, int max_cus,
-                         int cus, hipStream_t hs) {
+                         int cus, GatedArg<GATED> gated, hipStream_t hs) {
   constexpr int LDS = ks_lds_bytes(MT, NT, STAGES);
   static std::atomic<bool> lds_ok[kMaxDevices];
-  const auto kernel = gemm_bf16_nt_ksplit_kernel<MT, NT, STAGES, LA, BAUX, TAIL>;
+  const auto kernel = gemm_bf16_nt_ksplit_kernel<MT, NT, STAGES, LA, BAUX, TAIL, GATED>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, LDS)) return rc;
-  const KsTiles tiles = ksplit_tiles(M, N, count, 8 * LA, 32 * NT, cus);
+  const KsTiles tiles = ksplit_tiles(M, N, count, 8 * LA, GATED ? 16 * NT : 32 * NT, cus);
   int64_t grid = count * tiles.m * tiles.n;
   if (max_cus > 0 && grid > max_cus) grid = max_cus;
   launch_kernel(kernel, dim3((unsigned)grid), dim3(KS_THREADS), LDS, hs, batch, count, (int)M, (int)N, (int)K, ldc,
-                (int)tiles.m, (int)tiles.n, tiles.cols);
+                (int)tiles.m, (int)tiles.n, tiles.cols, gated);
   return TW_OK;
 }
 
@@ -959,29 +1076,31 @@ static KsForm ksplit_form(int64_t M, int64_t N, int64_t K, int count, int max_cu
   return {2, 2, 2, 8, false, !whole};
 }
 
+template <bool GATED = false>
 static int launch_ksplit_for(const GemmBatch& batch, int count, int64_t M, int64_t N, int64_t K, int64_t ldc,
-                             int max_cus, hipStream_t hs) {
+                             int max_cus, hipStream_t hs, GatedArg<GATED> gated = {}) {
   int cus = device_compute_units();
   if (cus <= 0) cus = 256;
-  const KsForm f = ksplit_form(M, N, K, count, max_cus, cus);
+  const KsForm f = ksplit_form(M, GATED ? 2 * N : N, K, count, max_cus, cus);  // a gated column is two rows of b
 #define TW_KSPLIT_LAUNCH(MT, NT, STAGES, LA, STREAM, TAIL)                                                     \
   if (f.mt == MT && f.nt == NT && f.stages == STAGES && f.la == LA && f.stream == STREAM && f.tail == TAIL)      \
-    return launch_ksplit<MT, NT, STAGES, LA, STREAM ? KS_STREAM : 0, TAIL>(batch, count, M, N, K, ldc, max_cus, cus, \
-                                                                           hs);
+    return launch_ksplit<MT, NT, STAGES, LA, STREAM ? KS_STREAM : 0, TAIL, GATED>(batch, count, M, N, K, ldc, \
+                                                                                  max_cus, cus, gated, hs);
   TW_KSPLIT_FORMS(TW_KSPLIT_LAUNCH)
 #undef TW_KSPLIT_LAUNCH
   return set_error(TW_ERR_INVALID_ARGUMENT, "gemm_bf16_nt: no kernel for %d rows", (int)M);
 }
 
-template <int TM, int TN, TileRows ROWS>
+template <int TM, int TN, TileRows ROWS, bool GATED = false>
 static int launch_tile_kernel(const GemmBatch& batch, int count, int64_t M, int64_t N, int64_t K, int64_t ldc,
-                       int max_cus, hipStream_t hs) {
+                       int max_cus, hipStream_t hs, GatedArg<GATED> gated = {}) {
   using S = TileShape<TM, TN, ROWS>;
   static std::atomic<bool> lds_ok[kMaxDevices];
-  if (int rc = allow_lds(reinterpret_cast<const void*>(gemm_bf16_nt_tile_kernel<TM, TN, ROWS>), lds_ok, kMaxDevices,
+  if (int rc = allow_lds(reinterpret_cast<const void*>(gemm_bf16_nt_tile_kernel<TM, TN, ROWS, GATED>), lds_ok, kMaxDevices,
                          S::LDS))
     return rc;
-  const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + S::BN - 1) / S::BN);
+  constexpr int COLS = GATED ? S::BN / 2 : S::BN;
+  const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + COLS - 1) / COLS);
   // a workgroup per compute unit at most: it fills the unit and walks its share of the tiles
   int cus = max_cus > 0 ? max_cus : device_compute_units();
   if (cus <= 0) cus = 256;
@@ -990,8 +1109,8 @@ static int launch_tile_kernel(const GemmBatch& batch, int count, int64_t M, int6
   int wide_store = (N % 8 == 0 && ldc % 8 == 0) ? 1 : 0;
   for (int p = 0; p < count; ++p)
     if (reinterpret_cast<uintptr_t>(batch.out[p]) & 15u) wide_store = 0;
-  launch_kernel(gemm_bf16_nt_tile_kernel<TM, TN, ROWS>, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, batch,
-                count, (int)M, (int)N, (int)K, ldc, tiles_m, tiles_n, wide_store);
+  launch_kernel(gemm_bf16_nt_tile_kernel<TM, TN, ROWS, GATED>, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs,
+                batch, count, (int)M, (int)N, (int)K, ldc, tiles_m, tiles_n, wide_store, gated);
   return TW_OK;
 }
 
@@ -1060,10 +1179,11 @@ static int launch_tile_shape(int tm, int tn, const GemmBatch& batch, int count, 
 // The shape whose rounds over the available units take the least time; ties go to the earlier
 // (larger) one.  The shape never changes a result bit: every output element is the same sequence
 // of MFMA k-steps whatever tile it lies in.
-static const TileChoice& pick_tile(int64_t M, int64_t N, int count, int cus) {
+static const TileChoice& pick_tile(int64_t M, int64_t N, int count, int cus, bool gated = false) {
   const TileChoice* best = &kTiles[0];
   double best_cost = 1e300;
   for (const TileChoice& t : kTiles) {
+    if (gated && t.tn % 4 != 0) continue;
     const int64_t tiles = count * ((M + 32 * t.tm - 1) / (32 * t.tm)) * ((N + 32 * t.tn - 1) / (32 * t.tn));
     const double cost = (double)((tiles + cus - 1) / cus) * t.cost;
     if (cost < best_cost) {
@@ -1086,6 +1206,24 @@ static int launch_tile_for(const GemmBatch& batch, int count, int64_t M, int64_t
   if (cus <= 0) cus = 256;
   const TileChoice& t = pick_tile(M, N, count, cus);
   return launch_tile_shape(t.tm, t.tn, batch, count, M, N, K, ldc, max_cus, hs);
+}
+
+// act(a b[:I]^T) * (a b[I:]^T).  The tile kernel reaches both halves of b through one descriptor: weights of less than
+// 2 GiB.  Larger ones take the K-split kernel whatever the rows, which has a descriptor for each half's rows of a tile.
+static int launch_gated_tile(const GemmBatch& batch, int64_t M, int64_t I, int64_t K, int64_t ldc, int max_cus,
+                             const GatedOut& gated, hipStream_t hs) {
+  int cus = max_cus > 0 ? max_cus : device_compute_units();
+  if (cus <= 0) cus = 256;
+  const TileChoice& t = pick_tile(M, 2 * I, 1, cus, true);
+#define TW_GATED_TILE(TM, TN, COST)                                                                                  \
+  if constexpr (TN % 4 == 0)                                                                                         \
+    if (t.tm == TM && t.tn == TN)                                                                                    \
+      return K % BK == 0                                                                                             \
+                 ? launch_tile_kernel<TM, TN, kWholeSlabs, true>(batch, 1, M, I, K, ldc, max_cus, hs, gated)         \
+                 : launch_tile_kernel<TM, TN, kPartialSlab, true>(batch, 1, M, I, K, ldc, max_cus, hs, gated);
+  TW_TILES(TW_GATED_TILE)
+#undef TW_GATED_TILE
+  return set_error(TW_ERR_INVALID_ARGUMENT, "gated_gemm_bf16_nt: no %d x %d tile", 32 * t.tm, 32 * t.tn);
 }
 
 static int check_gemm_shape(const char* what, int64_t M, int64_t N, int64_t K, int64_t ldc) {
@@ -1139,6 +1277,34 @@ int run_gemm_bf16_nt(void* out, const void* a, const void* b, const void* bias, 
   batch.b[0] = static_cast<const uint16_t*>(b);
   batch.bias[0] = static_cast<const uint16_t*>(bias);
   return run_products("gemm_bf16_nt", batch, 1, M, N, K, ldc, max_cus, static_cast<hipStream_t>(stream));
+}
+
+int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, int64_t M, int64_t I, int64_t K,
+                           int64_t ldc, int64_t ld_both, int act, int max_cus, void* stream) {
+  const char* what = "gated_gemm_bf16_nt";
+  if (I > INT32_MAX / 2) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld columns", what, (long long)I);
+  if (int rc = check_gemm_shape(what, M, I, K, ldc)) return rc;
+  if (act < TW_ACT_SILU || act > TW_ACT_GELU_TANH)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, act);
+  if (K > KS_MAX_K) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: K %lld exceeds %lld", what, (long long)K,
+                                     (long long)KS_MAX_K);
+  if (both && (ld_both < 2 * I || ld_both % 4 != 0))
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: gate_up rows of %lld at a stride of %lld", what, (long long)(2 * I),
+                     (long long)ld_both);
+  if (M == 0) return TW_OK;
+  if (int rc = check_gemm_pointers(what, out, a, b, both)) return rc;
+  GemmBatch batch = {};
+  batch.out[0] = static_cast<uint16_t*>(out);
+  batch.a[0] = static_cast<const uint16_t*>(a);
+  batch.b[0] = static_cast<const uint16_t*>(b);
+  const GatedOut gated = {static_cast<uint16_t*>(both), ld_both, act};
+  const hipStream_t hs = static_cast<hipStream_t>(stream);
+  int rc;
+  if (tile_kernel_fits(M, 2 * I, K, ldc) && 2 * I * K < (int64_t)1 << 30)
+    rc = launch_gated_tile(batch, M, I, K, ldc, max_cus, gated, hs);
+  else
+    rc = launch_ksplit_for<true>(batch, 1, M, I, K, ldc, max_cus, hs, gated);
+  return rc ? rc : finish_launch(what);
 }
 
 // outs[p][M, N] (row stride ldc) = as[p][M, K] * bs[p][N, K]^T (+ biases[p] when `biases` and

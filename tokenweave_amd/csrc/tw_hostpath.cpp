@@ -318,6 +318,58 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       enqueue([&] { tw_torch::kv4_attention(*out, *q, *pages, *table, *lens, scale, starts, most, window); }));
 }
 
+// The name of an activation (None where `optional`: below 0).
+bool as_activation(PyObject* o, bool optional, int* v) {
+  static const char* const names[] = {"silu", "gelu", "gelu_tanh"};  // TW_ACT_*
+  *v = -1;
+  if (optional && o == Py_None) return true;
+  if (!PyUnicode_CheckExact(o)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (PyUnicode_CompareWithASCIIString(o, names[i]) == 0) *v = i;
+  return *v >= 0;
+}
+
+// (out, a, b, activation, max_cus | None, gate_up | None)
+PyObject* gated_gemm_bf16_nt(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t cus;
+  int act;
+  const Tensor* both;
+  if (n != 6 || !direct_allowed()) Py_RETURN_FALSE;
+  const Tensor *o = plain(a[0]), *x = plain(a[1]), *w = plain(a[2]);
+  if (!o || !x || !w || !as_activation(a[3], false, &act) || !as_cap(a[4], &cus) || !optional_plain(a[5], &both))
+    Py_RETURN_FALSE;
+  return yes_no(enqueue([&] { tw_torch::gated_gemm_bf16_nt(*o, *x, *w, act, cus, both); }));
+}
+
+// (grad_a | None, grad_b | None, grad_out, a, b, gate_up, activation, max_cus | None)
+PyObject* gated_gemm_bf16_nt_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t cus;
+  int act;
+  const Tensor *ga, *gb;
+  if (n != 8 || !direct_allowed() || !optional_plain(a[0], &ga) || !optional_plain(a[1], &gb)) Py_RETURN_FALSE;
+  const Tensor *g = plain(a[2]), *x = plain(a[3]), *w = plain(a[4]), *both = plain(a[5]);
+  if (!g || !x || !w || !both || !as_activation(a[6], false, &act) || !as_cap(a[7], &cus)) Py_RETURN_FALSE;
+  return yes_no(enqueue([&] { tw_torch::gated_gemm_bf16_nt_backward(ga, gb, *g, *x, *w, *both, act, cus); }));
+}
+
+// (out, scales, input, activation | None)
+PyObject* quant_fp8_groups(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int act;
+  if (n != 4 || !direct_allowed()) Py_RETURN_FALSE;
+  const Tensor *o = plain(a[0]), *s = plain(a[1]), *x = plain(a[2]);
+  if (!o || !s || !x || !as_activation(a[3], true, &act)) Py_RETURN_FALSE;
+  return yes_no(enqueue([&] { tw_torch::quant_fp8_groups(*o, *s, *x, act); }));
+}
+
+// (out, a, a_scales, b, b_scales, max_cus | None)
+PyObject* gemm_fp8_block_nt(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t cus;
+  if (n != 6 || !direct_allowed()) Py_RETURN_FALSE;
+  const Tensor *o = plain(a[0]), *x = plain(a[1]), *xs = plain(a[2]), *w = plain(a[3]), *ws = plain(a[4]);
+  if (!o || !x || !xs || !w || !ws || !as_cap(a[5], &cus)) Py_RETURN_FALSE;
+  return yes_no(enqueue([&] { tw_torch::gemm_fp8_block_nt(*o, *x, *xs, *w, *ws, cus); }));
+}
+
 // ---------------------------------------------------------------------------
 // layers.  An nn.Module whose __call__ would do more than call the class's forward (hooks, a
 // compiled or replaced forward) is not handled here.
@@ -526,6 +578,10 @@ PyMethodDef g_methods[] = {
     TW_FAST("kv4_append", kv4_append),
     TW_FAST("kv4_read", kv4_read),
     TW_FAST("kv4_attention", kv4_attention),
+    TW_FAST("gated_gemm_bf16_nt", gated_gemm_bf16_nt),
+    TW_FAST("gated_gemm_bf16_nt_backward", gated_gemm_bf16_nt_backward),
+    TW_FAST("quant_fp8_groups", quant_fp8_groups),
+    TW_FAST("gemm_fp8_block_nt", gemm_fp8_block_nt),
     TW_FAST_RESULT("rms_norm_forward", rms_norm_forward),
     TW_FAST_RESULT("rms_norm_call", rms_norm_call),
     TW_FAST("fused_allreduce_layernorm", fused_allreduce_layernorm),

@@ -592,6 +592,115 @@ void kv4_attention(const Tensor& out, const Tensor& q, const Tensor& pages, cons
                             need, l.stream));
 }
 
+// ---------------------------------------------------------------------------
+// the feed-forward half: a gated product with its gradients, rows to 8-bit codes, the
+// block-scaled product
+// ---------------------------------------------------------------------------
+// The distance of two rows of a 2-D tensor whose rows are contiguous and apart.
+static int64_t check_rows(const char* name, const Tensor& t, at::ScalarType dtype, const c10::Device& device,
+                          int64_t rows, int64_t width) {
+  TORCH_CHECK(t.is_cuda() && t.device() == device, name, " is on ", t.device(), ", expected ", device);
+  TORCH_CHECK(t.scalar_type() == dtype, name, " has dtype ", dtype_name(t.scalar_type()), ", expected ",
+              dtype_name(dtype));
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == width, name, " has shape ", t.sizes(), ", expected (",
+              rows, ", ", width, ")");
+  TORCH_CHECK((t.stride(1) == 1 || width <= 1) && (rows <= 1 || t.stride(0) >= width), "rows of ", name,
+              " must be contiguous and apart; got stride ", t.strides());
+  return rows > 1 ? t.stride(0) : std::max(width, t.stride(0));
+}
+
+namespace {
+struct GatedShape { int64_t M, I, K; };
+}  // namespace
+
+static GatedShape check_gated(const Tensor& a, const Tensor& b) {
+  require_bf16("gated_gemm_bf16_nt_kernel", a);
+  check_tensor("a", a, at::kBFloat16, a.device());
+  check_tensor("b", b, at::kBFloat16, a.device());
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2, "gemm operands must be 2-D");
+  TORCH_CHECK(a.size(1) == b.size(1), "inner dimensions differ: a is ", a.sizes(), ", b is ", b.sizes());
+  TORCH_CHECK(b.size(0) % 2 == 0, "b has ", b.size(0), " rows: as many gate rows as up rows are expected");
+  return {a.size(0), b.size(0) / 2, a.size(1)};
+}
+
+void gated_gemm_bf16_nt(const Tensor& out, const Tensor& a, const Tensor& b, int activation, int64_t max_cus,
+                        const Tensor* gate_up) {
+  const GatedShape s = check_gated(a, b);
+  const int64_t ldc = check_rows("out", out, at::kBFloat16, a.device(), s.M, s.I);
+  const int64_t ld = gate_up ? check_rows("gate_up", *gate_up, at::kBFloat16, a.device(), s.M, 2 * s.I) : 0;
+  Launch l(a);
+  check_rc(tw_gated_gemm_bf16_nt(out.data_ptr(), gate_up ? gate_up->data_ptr() : nullptr, a.data_ptr(), b.data_ptr(),
+                                 s.M, s.I, s.K, ldc, ld, activation, (int)max_cus, l.stream));
+}
+
+void gated_gemm_bf16_nt_backward(const Tensor* grad_a, const Tensor* grad_b, const Tensor& grad_out, const Tensor& a,
+                                 const Tensor& b, const Tensor& gate_up, int activation, int64_t max_cus) {
+  const GatedShape s = check_gated(a, b);
+  const auto dev = a.device();
+  const int64_t ld_grad = check_rows("grad_out", grad_out, at::kBFloat16, dev, s.M, s.I);
+  const int64_t ld_both = check_rows("gate_up", gate_up, at::kBFloat16, dev, s.M, 2 * s.I);
+  if (grad_a) check_tensor("grad_a", *grad_a, at::kBFloat16, dev);
+  if (grad_b) check_tensor("grad_b", *grad_b, at::kBFloat16, dev);
+  TORCH_CHECK(!grad_a || grad_a->sizes() == a.sizes(), "grad_a must have the shape of a");
+  TORCH_CHECK(!grad_b || grad_b->sizes() == b.sizes(), "grad_b must have the shape of b");
+  Launch l(a);
+  const int64_t need = tw_gated_gemm_bf16_nt_backward_workspace(s.M, s.I, s.K, grad_a != nullptr, grad_b != nullptr);
+  if (need < 0) check_rc((int)need);
+  Tensor ws;
+  if (need > 0) ws = at::detail::empty_cuda({need}, at::kByte, dev, std::nullopt);
+  check_rc(tw_gated_gemm_bf16_nt_backward(grad_a ? grad_a->data_ptr() : nullptr, grad_b ? grad_b->data_ptr() : nullptr,
+                                          grad_out.data_ptr(), ld_grad, a.data_ptr(), b.data_ptr(), gate_up.data_ptr(),
+                                          ld_both, s.M, s.I, s.K, activation, (int)max_cus,
+                                          need > 0 ? ws.data_ptr() : nullptr, need, l.stream));
+}
+
+static void check_group_scales(const char* name, const Tensor& t, const c10::Device& device, int64_t rows,
+                               int64_t groups) {
+  TORCH_CHECK(t.is_cuda() && t.device() == device && t.scalar_type() == at::kFloat, name,
+              " must be a torch.float32 tensor on ", device);
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == groups, name, " has shape ", t.sizes(), ", expected (",
+              rows, ", ", groups, ")");
+}
+
+void quant_fp8_groups(const Tensor& out, const Tensor& scales, const Tensor& input, int activation) {
+  const int code = dtype_code("quant_fp8_groups_kernel", input);
+  const int parts = activation < 0 ? 1 : 2;
+  TORCH_CHECK(input.dim() == 2 && input.size(1) > 0 && input.size(1) % parts == 0, "input has shape ", input.sizes());
+  const auto dev = input.device();
+  const int64_t M = input.size(0), K = input.size(1) / parts, groups = (K + TW_FP8_GROUP - 1) / TW_FP8_GROUP;
+  const int64_t ld = check_rows("input", input, input.scalar_type(), dev, M, input.size(1));
+  check_tensor("out", out, at::kFloat8_e4m3fn, dev);
+  TORCH_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == K, "out has shape ", out.sizes());
+  check_group_scales("scales", scales, dev, M, groups);
+  const int64_t s0 = scales.stride(0), s1 = scales.stride(1);
+  TORCH_CHECK((M <= 1 || s0 > 0) && (groups <= 1 || s1 > 0) &&
+                  (M <= 1 || groups <= 1 || s0 >= groups * s1 || s1 >= M * s0),
+              "scales must not share memory; got stride ", scales.strides());
+  Launch l(input);
+  check_rc(tw_quant_fp8_groups(out.data_ptr(), static_cast<float*>(scales.data_ptr()), s0, s1, input.data_ptr(), ld, M,
+                               K, activation, code, l.stream));
+}
+
+void gemm_fp8_block_nt(const Tensor& out, const Tensor& a, const Tensor& a_scales, const Tensor& b,
+                       const Tensor& b_scales, int64_t max_cus) {
+  const auto dev = a.device();
+  check_tensor("a", a, at::kFloat8_e4m3fn, dev);
+  check_tensor("b", b, at::kFloat8_e4m3fn, dev);
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2, "gemm operands must be 2-D");
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0), blocks = (K + TW_FP8_GROUP - 1) / TW_FP8_GROUP;
+  TORCH_CHECK(b.size(1) == K, "inner dimensions differ: a is ", a.sizes(), ", b is ", b.sizes());
+  const int code = dtype_code("gemm_fp8_block_nt_kernel", out);
+  const int64_t ldc = check_rows("out", out, out.scalar_type(), dev, M, N);
+  check_group_scales("a_scales", a_scales, dev, M, blocks);
+  check_group_scales("b_scales", b_scales, dev, (N + TW_FP8_GROUP - 1) / TW_FP8_GROUP, blocks);
+  TORCH_CHECK(b_scales.is_contiguous(), "b_scales must be contiguous");
+  Launch l(a);
+  check_rc(tw_gemm_fp8_block_nt(out.data_ptr(), a.data_ptr(), static_cast<const float*>(a_scales.data_ptr()),
+                                a_scales.stride(0), a_scales.stride(1), b.data_ptr(),
+                                static_cast<const float*>(b_scales.data_ptr()), M, N, K, ldc, code, (int)max_cus,
+                                l.stream));
+}
+
 }  // namespace tw_torch
 
 namespace {

@@ -55,6 +55,17 @@ TW_TORCH_API void kv4_attention(const Tensor& out, const Tensor& q, const Tensor
                                 const Tensor& seq_lens, double scale, const Tensor* query_starts, int64_t max_queries,
                                 int64_t window);
 
+// The feed-forward half; activation: TW_ACT_*, below 0: none.  Optional tensors may be null.  Not
+// registered: no reference schema.
+TW_TORCH_API void gated_gemm_bf16_nt(const Tensor& out, const Tensor& a, const Tensor& b, int activation,
+                                     int64_t max_cus, const Tensor* gate_up);
+TW_TORCH_API void gated_gemm_bf16_nt_backward(const Tensor* grad_a, const Tensor* grad_b, const Tensor& grad_out,
+                                              const Tensor& a, const Tensor& b, const Tensor& gate_up, int activation,
+                                              int64_t max_cus);
+TW_TORCH_API void quant_fp8_groups(const Tensor& out, const Tensor& scales, const Tensor& input, int activation);
+TW_TORCH_API void gemm_fp8_block_nt(const Tensor& out, const Tensor& a, const Tensor& a_scales, const Tensor& b,
+                                    const Tensor& b_scales, int64_t max_cus);
+
 }  // namespace tw_torch
 
 #endif
