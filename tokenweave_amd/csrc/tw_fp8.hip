@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 #include "tw_activation.h"
 #include "tw_common.h"
@@ -165,6 +166,8 @@ constexpr int ROWB = 128;
 [[maybe_unused]] constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
 constexpr int64_t BLOCK_MAX_K = 1 << 22;  // a tile's rows span at most 1 GiB
 
+constexpr int64_t BLOCK_MAX_SCALE_ROW = 1 << 20;  // 32-bit offsets of a tile's scales
+
 struct BlockArgs {
   uint16_t* out;
   const uint8_t *a, *b;
@@ -175,9 +178,19 @@ struct BlockArgs {
 
 [[maybe_unused]] __device__ __forceinline__ uint32_t pack_out(float lo, float hi, int half_out) {
   const f32x2_t v = {lo, hi};
-  return half_out ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t))
-                  : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
+  const uint32_t half = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+  const uint32_t brain = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
+  return half_out ? half : brain;
 }
+
+#ifdef __HIP_DEVICE_COMPILE__
+// One fp32 a lane, `offset` bytes behind `from`, to LDS.  (A buffer load: behind a global load to LDS the compiler makes
+// every wait for an LDS read a wait for all of them, and for all loads.)
+__device__ __forceinline__ void load_scales(const float* from, uint32_t offset, lds_u8_t* to) {
+  const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, 0x7fffffffu, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void_t*)to, 4, offset, 0, 0, 0);
+}
+#endif
 
 // Few rows: bound by reading b once.  As in the bf16 K-split kernel four waves share the inner dimension, wave w takes
 // the slabs w, w + 4, ..., each brings its own slabs of both operands and the rows' scales into LDS of its own, and the
@@ -222,7 +235,8 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
     const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(w.b) + (size_t)n0 * K, 0, (uint32_t)min(w.N - n0, w.cols) * (uint32_t)K, 0x00020000);
     // a row's scales, one for each lane that has a row
-    const float* const my_scales = w.a_scales + (int64_t)(m0 + min(lane, rows - 1)) * w.scale_row;
+    const float* const scales = w.a_scales + (int64_t)m0 * w.scale_row;
+    const uint32_t my_scale = (uint32_t)min(lane, rows - 1) * (uint32_t)w.scale_row * 4u;
     // columns before `border` belong to the first of the two weight blocks that a tile may touch
     const float* const sb = w.b_scales + (int64_t)(n0 / GROUP) * nk;
     const int border = GROUP - n0 % GROUP;
@@ -250,9 +264,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
       for (int j = 0; j < LA; ++j)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_void_t*)(s + j * 1024), 16,
                                                  !last || ((j & 1) ? odd : even) ? v[j] : OUT_OF_RANGE, koff, 0, 0);
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void*)(my_scales + (int64_t)next * w.scale_block),
-          (lds_void_t*)(s + (RA + RB) * ROWB), 4, 0, 0);
+      load_scales(scales + next * w.scale_block, my_scale, (lds_u8_t*)(s + (RA + RB) * ROWB));
       next += SPLIT_WAVES;
       fill = fill == (STAGES - 1) * STAGE ? 0 : fill + STAGE;
     };
@@ -340,130 +352,182 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
 #endif
 }
 
-// More rows: tiles of (32 TM) x (64 TN), eight waves (2 x 4) of (16 TM) x (16 TN), two slabs in LDS.  The sums cannot stay
-// in accumulation registers, which vector instructions do not reach; two waves a SIMD let one multiply while the
-// other's results are added.
+// More rows: eight waves, WM x (8 / WM) of them, each (16 TM) x (16 TN) of the output, two slabs in LDS.  The sums cannot
+// stay in accumulation registers, which vector instructions do not reach: two waves a SIMD of 256 registers each.
+//
+// A slab is TM rows of TN matrix instructions; what goes on beside them is placed by hand:
+//  * behind each instruction the four multiply-adds of the one a row earlier, whose results have arrived;
+//  * a row's fragment of a is read from LDS one row ahead, the slab's fragments of b in the last row of the slab before,
+//    each as its register has served;
+//  * the slab's one barrier lies before its last row.  It says that the next slab has arrived and, as all fragments of
+//    this one are in registers, that its place in LDS is free: the slab after the next goes there, one load per SPACE
+//    instructions.  In a burst they hold up all waves: the unit's path to memory takes 64 bytes a cycle.
 constexpr int WIDE_THREADS = 512;
-constexpr int wide_stage(int tm, int tn) { return (32 * tm + 64 * tn) * ROWB + 32 * tm * 4; }
+template <int WM, int TM, int TN>
+struct WideShape {
+  static constexpr int WN = 8 / WM, BM = 16 * TM * WM, BN = 16 * TN * WN, PA = BM * ROWB, PB = BN * ROWB;
+  static constexpr int STAGE = PA + PB + 2048, LDS = 2 * STAGE, BLOCKS = (BM + BN) / 8, LOADS = BLOCKS / 8;
+  static constexpr int SPACE = TM * TN / (LOADS + 1) / 2 < 1 ? 1 : TM * TN / (LOADS + 1) / 2;
+  static_assert(TM % 2 == 0 && TN % 2 == 0 && BLOCKS % 8 == 0 && LDS <= 160 * 1024, "tiles come in pairs");
+  static_assert(LOADS * SPACE < TM * TN, "every load has a place");
+};
 
-template <int TM, int TN>
+#ifdef __HIP_DEVICE_COMPILE__
+__device__ __forceinline__ i32x8_t fragment(const lds_u8_t* p, const lds_u8_t* q) {
+  const u32x4_t x = *(lds_chunk_t*)p, y = *(lds_chunk_t*)q;
+  return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+}
+#endif
+
+// TAIL: the last slab is a partial one, whose chunks past K must arrive as zeros.
+template <int WM, int TM, int TN, bool TAIL>
 __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(BlockArgs w) {
 #ifdef __HIP_DEVICE_COMPILE__
-  constexpr int BM = 32 * TM, BN = 64 * TN, STAGE = wide_stage(TM, TN), PA = BM * ROWB, PB = BN * ROWB;
-  constexpr int BLOCKS = (BM + BN) / 8;  // 8-row blocks of both panels, dealt out to the waves
-  constexpr int LOADS = (BLOCKS + 7) / 8;
+  using S = WideShape<WM, TM, TN>;
+  constexpr int WN = S::WN, BM = S::BM, BN = S::BN, PA = S::PA, PB = S::PB, STAGE = S::STAGE, LOADS = S::LOADS;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   lds_u8_t* const base = (lds_u8_t*)lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 2, wn = wave & 3, r16 = lane & 15, quad = lane >> 4;
-  const int K = w.K, nk = (K + GROUP - 1) / GROUP, tail_chunks = K % GROUP ? (K % GROUP) / 16 : 8;
+  const int wm = wave / WN, wn = wave % WN, r16 = lane & 15, quad = lane >> 4;
+  const int K = w.K, nk = (K + GROUP - 1) / GROUP, tail_chunks = (K % GROUP) / 16;
 
-  const uint32_t row_a = (wm * 16 * TM + r16) * ROWB;
-  // MFMA row r of the pair of tiles (2 p, 2 p + 1) is column 32 p + 8 (r / 4) + 4 (tile & 1) + r % 4; a wave of one
-  // tile of columns keeps their order
-  const uint32_t row_b = PA + (wn * 16 * TN + (TN > 1 ? (r16 >> 2) * 8 + (r16 & 3) : r16)) * ROWB;
-  const uint32_t key_b = TN > 1 ? r16 >> 1 : ((r16 >> 1) & 1) | ((r16 >> 3) & 1) << 1 | (wn & 1) << 2;
-  const uint32_t a0 = row_a + ((quad ^ (r16 >> 1)) << 4), a1 = row_a + (((4 + quad) ^ (r16 >> 1)) << 4);
-  const uint32_t b0 = row_b + ((quad ^ key_b) << 4), b1 = row_b + (((4 + quad) ^ key_b) << 4);
+  // MFMA row r of the pair of tiles (2 p, 2 p + 1) is column 32 p + 8 (r / 4) + 4 (tile & 1) + r % 4.
+  const uint32_t row_a = (wm * 16 * TM + r16) * ROWB, row_b = PA + (wn * 16 * TN + (r16 >> 2) * 8 + (r16 & 3)) * ROWB;
+  const uint32_t chunk0 = (quad ^ (r16 >> 1)) << 4, chunk1 = ((4 + quad) ^ (r16 >> 1)) << 4;
+  const lds_u8_t *a0 = base + row_a + chunk0, *a1 = base + row_a + chunk1;
+  const lds_u8_t *b0 = base + row_b + chunk0, *b1 = base + row_b + chunk1;
+  const lds_u8_t* const at_scale = base + PA + PB + (wm * 16 * TM + r16) * 4;
 
-  const int num_tiles = w.tiles_m * w.tiles_n;
-  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-  int pid = t;
-  const int per_xcd = num_tiles / 8;
-  if (t < per_xcd * 8) pid = (t & 7) * per_xcd + (t >> 3);
-  const int sweep = 4 * w.tiles_n, group = pid / sweep, first = group * 4, in_group = min(w.tiles_m - first, 4);
-  const int m0 = (first + pid % sweep % in_group) * BM, n0 = pid % sweep / in_group * BN;
-  const int rows = min(w.M - m0, BM), cols = min(w.N - n0, BN);
-
-  const __amdgpu_buffer_rsrc_t da = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(w.a) + (size_t)m0 * K, 0, (uint32_t)rows * (uint32_t)K, 0x00020000);
-  const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(w.b) + (size_t)n0 * K, 0, (uint32_t)cols * (uint32_t)K, 0x00020000);
   uint32_t v[LOADS];
-  int chunk[LOADS];
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
     const int blk = wave + l * 8;
     const bool of_a = blk < BM / 8;
     const int in = of_a ? blk : blk - BM / 8;
     const int key = of_a ? ((in & 1) << 2) | (lane >> 4) : ((lane >> 4) & 1) | ((in & 3) << 1);
-    chunk[l] = (lane & 7) ^ key;
-    v[l] = (uint32_t)(in * 8 + (lane >> 3)) * (uint32_t)K + (chunk[l] << 4);
+    v[l] = (uint32_t)(in * 8 + (lane >> 3)) * (uint32_t)K + (((lane & 7) ^ key) << 4);
   }
-  auto load = [&](int slab, uint32_t stage) {
-    const int chunks = slab == nk - 1 ? tail_chunks : 8;
-#pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
+
+  const int num_tiles = w.tiles_m * w.tiles_n;
+  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+    int pid = t;
+    const int per_xcd = num_tiles / 8;
+    if (t < per_xcd * 8) pid = (t & 7) * per_xcd + (t >> 3);
+    const int sweep = 4 * w.tiles_n, group = pid / sweep, first = group * 4, in_group = min(w.tiles_m - first, 4);
+    const int m0 = (first + pid % sweep % in_group) * BM, n0 = pid % sweep / in_group * BN;
+    const int rows = min(w.M - m0, BM), cols = min(w.N - n0, BN);
+    const __amdgpu_buffer_rsrc_t da = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(w.a) + (size_t)m0 * K, 0, (uint32_t)rows * (uint32_t)K, 0x00020000);
+    const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(w.b) + (size_t)n0 * K, 0, (uint32_t)cols * (uint32_t)K, 0x00020000);
+    const float* const scales = w.a_scales + (int64_t)m0 * w.scale_row;
+    const uint32_t my_scale = (uint32_t)min(wave * 64 + lane, rows - 1) * (uint32_t)w.scale_row * 4u;
+    // load l of a slab into its place in LDS; the last one brings 64 rows' scales (waves behind the rows: copies)
+    auto load = [&](int l, int slab, uint32_t stage) {
+      if (l == LOADS) {
+        load_scales(scales + min(slab, nk - 1) * w.scale_block, my_scale, base + stage + PA + PB + wave * 256);
+        return;
+      }
       const int blk = wave + l * 8;
-      if (blk < BLOCKS)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(blk < BM / 8 ? da : db, (lds_void_t*)(base + stage + blk * 1024), 16,
-                                                 chunk[l] < chunks ? v[l] : OUT_OF_RANGE, (uint32_t)slab * ROWB, 0, 0);
-    }
-    if (wave * 64 < BM) {
-      const int row = m0 + min(wave * 64 + lane, rows - 1);
-      if (wave * 64 + lane < BM)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(w.a_scales + row * w.scale_row + slab * w.scale_block),
-            (lds_void_t*)(base + stage + PA + PB + wave * 256), 4, 0, 0);
-    }
-  };
-  const int block_n = min((n0 + wn * 16 * TN) / GROUP, (w.N - 1) / GROUP);
-  const float* const sb = w.b_scales + (int64_t)block_n * nk;
+      const bool of_a = blk < BM / 8;
+      uint32_t off = v[l];
+      if (TAIL) {
+        const int in = of_a ? blk : blk - BM / 8;
+        const int key = of_a ? ((in & 1) << 2) | (lane >> 4) : ((lane >> 4) & 1) | ((in & 3) << 1);
+        if (slab >= nk - 1 && ((lane & 7) ^ key) >= tail_chunks) off = OUT_OF_RANGE;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(of_a ? da : db, (lds_void_t*)(base + stage + blk * 1024), 16, off,
+                                               (uint32_t)min(slab, nk - 1) * ROWB, 0, 0);
+    };
+    // the wave's columns touch two weight blocks at most, and a pair of column tiles one
+    const int col = n0 + wn * 16 * TN, most_block = (w.N - 1) / GROUP;
+    // (fetched by vector loads: a scalar load under way makes every wait for LDS a wait for all of it)
+    int64_t none = 0;
+    asm volatile("" : "+v"(none));
+    const float* const sb = w.b_scales + (int64_t)min(col / GROUP, most_block) * nk + none;
+    const int64_t second = col / GROUP + 1 <= most_block ? nk : 0;
+    const int border = (GROUP - col % GROUP) / 16;  // column tiles of the first block
 
-  f32x4_t acc[TM][TN];
+    f32x4_t acc[TM][TN], part[2][TN];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
-
-  float next_s = sb[0];
-  load(0, 0);
-  for (int slab = 0; slab < nk; ++slab) {
-    const uint32_t use = (slab & 1) * STAGE;
-    const float s = next_s;
-    // this slab has arrived (every wave waited for its own loads), the other stage's readers are done
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (slab + 1 < nk) {
-      load(slab + 1, STAGE - use);
-      next_s = sb[slab + 1];
+      for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < TN; ++j) part[1][j] = f32x4_t{0, 0, 0, 0};
+    float first_scale = 0.0f, second_scale = 0.0f;  // of the row of tiles before
+    float s0 = sb[0], s1 = sb[second];
+#pragma unroll
+    for (int l = 0; l <= LOADS; ++l) load(l, 0, 0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    i32x8_t fa[2], fb[TN];
+    fa[0] = fragment(a0, a1);
+    float sa = *(lds_f32_t*)at_scale;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      fb[j] = fragment(b0 + (j >> 1) * 4096 + (j & 1) * 512, b1 + (j >> 1) * 4096 + (j & 1) * 512);
+#pragma unroll
+    for (int l = 0; l <= LOADS; ++l)
+      if (l * S::SPACE < TN) load(l, 1, STAGE);  // those that go out in a last row
+    for (int slab = 0; slab < nk; ++slab) {
+      const uint32_t use = (slab & 1) * STAGE, other = STAGE - use;
+      const int next = min(slab + 1, nk - 1);
+      const float next0 = sb[next], next1 = sb[next + second];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const float mine0 = sa * s0, mine1 = sa * s1;
+        if (i == TM - 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // Past the last slab loads bring that one again and fragments are read that nobody uses: branches cost more
+        // (a second set of registers for b's fragments, and spills).
+        const uint32_t at = i + 1 < TM ? use + (i + 1) * 2048 : other;
+        fa[(i + 1) & 1] = fragment(a0 + at, a1 + at);
+        sa = *(lds_f32_t*)(at_scale + (i + 1 < TM ? use + (i + 1) * 64 : other));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          part[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i & 1], f32x4_t{}, 0, 0, 0, 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (i == TM - 1)
+            fb[j] = fragment(b0 + other + (j >> 1) * 4096 + (j & 1) * 512, b1 + other + (j >> 1) * 4096 + (j & 1) * 512);
+          const int n = (i + 1) % TM * TN + j;  // instructions since the barrier
+          if (n % S::SPACE == 0 && n / S::SPACE <= LOADS) {
+            const int ahead = i == TM - 1 ? 2 : 1;
+            load(n / S::SPACE, slab + ahead, ahead == 2 ? use : other);
+          }
+          // the row of tiles before, of the slab before for the first one
+          const float scale = j < border ? first_scale : second_scale;
+          f32x4_t& sum = acc[(i + TM - 1) % TM][j];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] = __fmaf_rn(part[(i + 1) & 1][j][e], scale, sum[e]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        first_scale = mine0, second_scale = mine1;
+      }
+      s0 = next0, s1 = next1;
     }
-    i32x8_t fb[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const uint32_t at = use + (TN > 1 ? (j >> 1) * 4096 + (j & 1) * 512 : 0);
-      const u32x4_t x = *(lds_chunk_t*)(base + at + b0), y = *(lds_chunk_t*)(base + at + b1);
-      fb[j] = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+      const float scale = j < border ? first_scale : second_scale;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[TM - 1][j][e] = __fmaf_rn(part[1][j][e], scale, acc[TM - 1][j][e]);
     }
+
+    // a lane holds row r16 of each row of tiles, columns 8 quad + 0 .. 7 of a pair of column tiles
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      const u32x4_t x = *(lds_chunk_t*)(base + use + i * 2048 + a0), y = *(lds_chunk_t*)(base + use + i * 2048 + a1);
-      const i32x8_t fa = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-      const float scale = s * *(lds_f32_t*)(base + use + PA + PB + (wm * 16 * TM + i * 16 + r16) * 4);
+      const int m = wm * 16 * TM + i * 16 + r16;
+      if (m >= rows) continue;
+      uint16_t* to = w.out + (size_t)(m0 + m) * w.ldc + n0;
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const f32x4_t part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, f32x4_t{}, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(part[e], scale, acc[i][j][e]);
+        const int c = wn * 16 * TN + (j >> 1) * 32 + quad * 8 + (j & 1) * 4;
+        if (c < cols)
+          *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_out(acc[i][j][0], acc[i][j][1], w.half_out),
+                                                         pack_out(acc[i][j][2], acc[i][j][3], w.half_out));
       }
     }
-  }
-
-  // a lane holds row r16 of each row tile: columns 8 quad + 0 .. 7 of a pair of tiles, 4 quad + 0 .. 3 of a single one
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = wm * 16 * TM + i * 16 + r16;
-    if (m >= rows) continue;
-    uint16_t* to = w.out + (size_t)(m0 + m) * w.ldc + n0;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int c = wn * 16 * TN + (TN > 1 ? (j >> 1) * 32 + quad * 8 + (j & 1) * 4 : quad * 4);
-      if (c < cols)
-        *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_out(acc[i][j][0], acc[i][j][1], w.half_out),
-                                                       pack_out(acc[i][j][2], acc[i][j][3], w.half_out));
-    }
-  }
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next tile's first slab goes where this one's last may be
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next tile's slabs go where this one's were
   }
 #endif
 }
@@ -503,17 +567,18 @@ int launch_split(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
   return TW_OK;
 }
 
-template <int TM, int TN>
+template <int WM, int TM, int TN>
 int launch_wide(BlockArgs w, int max_cus, hipStream_t hs) {
-  constexpr int LDS = 2 * wide_stage(TM, TN);
-  static std::atomic<bool> ok[kMaxDevices];
-  const auto kernel = gemm_fp8_block_tile_kernel<TM, TN>;
-  if (int rc = allow_lds(kernel, ok, LDS)) return rc;
-  w.tiles_m = (w.M + 32 * TM - 1) / (32 * TM);
-  w.tiles_n = (w.N + 64 * TN - 1) / (64 * TN);
+  using S = WideShape<WM, TM, TN>;
+  static std::atomic<bool> ok[2][kMaxDevices];
+  const bool tail = w.K % GROUP != 0;
+  const auto kernel = tail ? gemm_fp8_block_tile_kernel<WM, TM, TN, true> : gemm_fp8_block_tile_kernel<WM, TM, TN, false>;
+  if (int rc = allow_lds(kernel, ok[tail], S::LDS)) return rc;
+  w.tiles_m = (w.M + S::BM - 1) / S::BM;
+  w.tiles_n = (w.N + S::BN - 1) / S::BN;
   int64_t grid = (int64_t)w.tiles_m * w.tiles_n;
   if (max_cus > 0 && grid > max_cus) grid = max_cus;
-  launch_kernel(kernel, dim3((unsigned)grid), dim3(WIDE_THREADS), LDS, hs, w);
+  launch_kernel(kernel, dim3((unsigned)grid), dim3(WIDE_THREADS), S::LDS, hs, w);
   return TW_OK;
 }
 
@@ -559,6 +624,9 @@ int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64
   if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > BLOCK_MAX_K || ldc < N)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad shape M=%lld N=%lld K=%lld ldc=%lld", what, (long long)M,
                      (long long)N, (long long)K, (long long)ldc);
+  if (scale_row < 0 || scale_block < 0 || scale_row > BLOCK_MAX_SCALE_ROW)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: the scales of two rows may be 0 to %lld elements apart, got %lld", what,
+                     (long long)BLOCK_MAX_SCALE_ROW, (long long)scale_row);
   if (K % 16 != 0 || N % 4 != 0 || ldc % 4 != 0)
     return set_error(TW_ERR_ALIGNMENT, "%s: needs K %% 16 == 0, N %% 4 == 0, ldc %% 4 == 0", what);
   if (dtype != TW_DTYPE_BF16 && dtype != TW_DTYPE_F16)
@@ -585,7 +653,17 @@ int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64
   else if (M <= 32) rc = launch_split<1, 1, 3, 4>(w, max_cus, cus, hs);
   else if (M <= 64) rc = launch_split<2, 1, 3, 8>(w, max_cus, cus, hs);
   else if (M <= 128) rc = launch_split<2, 2, 2, 8>(w, max_cus, cus, hs);
-  else rc = launch_wide<8, 4>(w, max_cus, hs);
+  else {
+    const char* e = getenv("TW_T");
+    int t = e ? atoi(e) : 284;
+    if (t == 244) rc = launch_wide<2, 4, 4>(w, max_cus, hs);
+    else if (t == 264) rc = launch_wide<2, 6, 4>(w, max_cus, hs);
+    else if (t == 444) rc = launch_wide<4, 4, 4>(w, max_cus, hs);
+    else if (t == 242) rc = launch_wide<2, 4, 2>(w, max_cus, hs);
+    else if (t == 446) rc = launch_wide<4, 4, 6>(w, max_cus, hs);
+    else if (t == 222) rc = launch_wide<2, 2, 2>(w, max_cus, hs);
+    else rc = launch_wide<2, 8, 4>(w, max_cus, hs);
+  }
   return rc ? rc : finish_launch(what);
 }
 
