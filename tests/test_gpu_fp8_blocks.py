@@ -153,7 +153,10 @@ def test_product_of_many_rows(M, N, K):
     check_product(M, N, K, (torch.bfloat16, torch.float16)[M % 2], seed=M)
 
 
-@pytest.mark.parametrize("M,N,K", [(2458, 1376, 512), (4096, 2048, 128), (700, 7392, 400), (384, 6144, 2048)])
+@pytest.mark.parametrize("M,N,K", [(2458, 1376, 512), (4096, 2048, 128), (700, 7392, 400), (384, 6144, 2048),
+                                   # one round of each shape: 256 x 224, 256 x 192, 192 x 256, 256 x 128, 128 x 256, ...
+                                   (4096, 3584, 400), (4090, 3068, 528), (3070, 4092, 1040), (4096, 2044, 9200),
+                                   (2047, 4096, 640), (2040, 2048, 144), (1020, 2048, 8336)])
 def test_product_of_all_tile_shapes(M, N, K):
     check_product(M, N, K)
 

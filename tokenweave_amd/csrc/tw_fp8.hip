@@ -5,7 +5,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 #include "tw_activation.h"
 #include "tw_common.h"
@@ -352,24 +351,38 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
 #endif
 }
 
-// More rows: eight waves, WM x (8 / WM) of them, each (16 TM) x (16 TN) of the output, two slabs in LDS.  The sums cannot
-// stay in accumulation registers, which vector instructions do not reach: two waves a SIMD of 256 registers each.
+// More rows: eight waves, WM x (8 / WM) of them, each (16 TM) x (16 TN) of the output.  The sums cannot stay in
+// accumulation registers, which vector instructions do not reach: two waves a SIMD of 256 registers each.
 //
 // A slab is TM rows of TN matrix instructions; what goes on beside them is placed by hand:
-//  * behind each instruction the four multiply-adds of the one a row earlier, whose results have arrived;
+//  * behind each instruction the four multiply-adds of the one LAG earlier, whose results have arrived;
 //  * a row's fragment of a is read from LDS one row ahead, the slab's fragments of b in the last row of the slab before,
 //    each as its register has served;
-//  * the slab's one barrier lies before its last row.  It says that the next slab has arrived and, as all fragments of
-//    this one are in registers, that its place in LDS is free: the slab after the next goes there, one load per SPACE
-//    instructions.  In a burst they hold up all waves: the unit's path to memory takes 64 bytes a cycle.
+//  * a barrier lies before a slab's last row.  It says that the next slab has arrived and, as all fragments of this one
+//    are in registers, that its place in LDS is free: a's rows of the slab NA ahead go there;
+//  * b's rows are all in registers a row into the slab.  Where LDS holds two slabs of them only, a second barrier says
+//    so there, and those of the slab after the next set out most of a slab earlier than they otherwise could.
+// Loads go out one per SPACE instructions: in a burst they hold up all waves, the unit's path to memory takes 64 bytes a
+// cycle.
 constexpr int WIDE_THREADS = 512;
-template <int WM, int TM, int TN>
+template <int WM, int TM, int TN, int NA, int NB>
 struct WideShape {
-  static constexpr int WN = 8 / WM, BM = 16 * TM * WM, BN = 16 * TN * WN, PA = BM * ROWB, PB = BN * ROWB;
-  static constexpr int STAGE = PA + PB + 2048, LDS = 2 * STAGE, BLOCKS = (BM + BN) / 8, LOADS = BLOCKS / 8;
-  static constexpr int SPACE = TM * TN / (LOADS + 1) / 2 < 1 ? 1 : TM * TN / (LOADS + 1) / 2;
-  static_assert(TM % 2 == 0 && TN % 2 == 0 && BLOCKS % 8 == 0 && LDS <= 160 * 1024, "tiles come in pairs");
-  static_assert(LOADS * SPACE < TM * TN, "every load has a place");
+  static constexpr int WN = 8 / WM, BM = 16 * TM * WM, BN = 16 * TN * WN, PA = BM * ROWB;
+  static constexpr int LA = BM / 64, LB = (BN + 63) / 64;  // loads of 8 rows a wave and slab
+  static constexpr int PB = BN * ROWB;                     // (BN % 64 != 0: some waves' last load goes nowhere)
+  static constexpr bool EARLY = NB < NA || NB == 2;        // b's rows by a barrier of their own
+  static constexpr int AT_B = NA * PA, AT_S = AT_B + NB * PB, AT_NONE = AT_S + NA * BM * 4;
+  static constexpr int LDS = AT_NONE + (BN % 64 ? 1024 : 0);
+  // loads under way that a slab's barrier does not wait for: what was issued behind the next slab's
+  static constexpr int PENDING = !EARLY ? (NA - 2) * (LA + LB + 1) : (NA - 2) * (LA + 1) + LB;
+  static constexpr int LATE = EARLY ? LA + 1 : LA + LB + 1;  // loads that follow the barrier before the last row
+  static constexpr int SPACE_LATE = EARLY ? 1 : TM * TN / LATE / 2 < 1 ? 1 : TM * TN / LATE / 2;
+  static constexpr int SPACE_EARLY = (TM - 2) * TN / LB / 2 < 1 ? 1 : (TM - 2) * TN / LB / 2;
+  static constexpr int TOTAL = TM * TN, LAG = TN < 3 ? TN : 3, RING = 4;  // results in registers
+  static_assert(TOTAL % RING == 0 && LAG < RING, "an instruction's results have one place in every slab");
+  static_assert(TM % 2 == 0 && BM % 64 == 0 && LDS <= 160 * 1024 && NA >= NB && (NA == NB || NA == 3), "shape");
+  static_assert(EARLY ? TM > 2 && NB == 2 && (LATE - 1) * SPACE_LATE < 2 * TN && (LB - 1) * SPACE_EARLY < (TM - 2) * TN
+                      : (LATE - 1) * SPACE_LATE < TM * TN, "every load has a place");
 };
 
 #ifdef __HIP_DEVICE_COMPILE__
@@ -377,14 +390,20 @@ __device__ __forceinline__ i32x8_t fragment(const lds_u8_t* p, const lds_u8_t* q
   const u32x4_t x = *(lds_chunk_t*)p, y = *(lds_chunk_t*)q;
   return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
 }
+__device__ __forceinline__ uint32_t after(uint32_t at, uint32_t panel, int n) {
+  return at == (n - 1) * panel ? 0u : at + panel;
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
 #endif
 
 // TAIL: the last slab is a partial one, whose chunks past K must arrive as zeros.
-template <int WM, int TM, int TN, bool TAIL>
+template <int WM, int TM, int TN, int NA, int NB, bool TAIL>
 __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(BlockArgs w) {
 #ifdef __HIP_DEVICE_COMPILE__
-  using S = WideShape<WM, TM, TN>;
-  constexpr int WN = S::WN, BM = S::BM, BN = S::BN, PA = S::PA, PB = S::PB, STAGE = S::STAGE, LOADS = S::LOADS;
+  using S = WideShape<WM, TM, TN, NA, NB>;
+  constexpr int WN = S::WN, BM = S::BM, BN = S::BN, PA = S::PA, PB = S::PB, LA = S::LA, LB = S::LB;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   lds_u8_t* const base = (lds_u8_t*)lds;
   const int lane = threadIdx.x & 63;
@@ -392,22 +411,33 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
   const int wm = wave / WN, wn = wave % WN, r16 = lane & 15, quad = lane >> 4;
   const int K = w.K, nk = (K + GROUP - 1) / GROUP, tail_chunks = (K % GROUP) / 16;
 
-  // MFMA row r of the pair of tiles (2 p, 2 p + 1) is column 32 p + 8 (r / 4) + 4 (tile & 1) + r % 4.
-  const uint32_t row_a = (wm * 16 * TM + r16) * ROWB, row_b = PA + (wn * 16 * TN + (r16 >> 2) * 8 + (r16 & 3)) * ROWB;
-  const uint32_t chunk0 = (quad ^ (r16 >> 1)) << 4, chunk1 = ((4 + quad) ^ (r16 >> 1)) << 4;
-  const lds_u8_t *a0 = base + row_a + chunk0, *a1 = base + row_a + chunk1;
-  const lds_u8_t *b0 = base + row_b + chunk0, *b1 = base + row_b + chunk1;
-  const lds_u8_t* const at_scale = base + PA + PB + (wm * 16 * TM + r16) * 4;
+  // Chunk c of row r lies at c ^ key: a's bits 1, 2, 3 of r, b's bits 1, 3, 4.  MFMA row r of the pair of column tiles
+  // (2 p, 2 p + 1) is column 32 p + 8 (r / 4) + 4 (tile & 1) + r % 4 of the wave's; a last single tile keeps the order.
+  auto key_b = [](int row) { return (uint32_t)(((row >> 1) & 1) | ((row >> 3) & 3) << 1); };
+  const int pair_row = wn * 16 * TN + (r16 >> 2) * 8 + (r16 & 3), single_row = wn * 16 * TN + 16 * (TN - 1) + r16;
+  const lds_u8_t* const a0 = base + (wm * 16 * TM + r16) * ROWB + ((quad ^ (r16 >> 1)) << 4);
+  const lds_u8_t* const a1 = base + (wm * 16 * TM + r16) * ROWB + (((4 + quad) ^ (r16 >> 1)) << 4);
+  const lds_u8_t* const b0 = base + S::AT_B + pair_row * ROWB + ((quad ^ key_b(pair_row)) << 4);
+  const lds_u8_t* const b1 = base + S::AT_B + pair_row * ROWB + (((4 + quad) ^ key_b(pair_row)) << 4);
+  [[maybe_unused]] const lds_u8_t* const c0 = base + S::AT_B + single_row * ROWB + ((quad ^ key_b(single_row)) << 4);
+  [[maybe_unused]] const lds_u8_t* const c1 = base + S::AT_B + single_row * ROWB + (((4 + quad) ^ key_b(single_row)) << 4);
+  const lds_u8_t* const at_scale = base + S::AT_S + (wm * 16 * TM + r16) * 4;
+  auto fragment_b = [&](int j, uint32_t use) {
+    if (TN % 2 && j == TN - 1) return fragment(c0 + use, c1 + use);
+    return fragment(b0 + use + (j >> 1) * 4096 + (j & 1) * 512, b1 + use + (j >> 1) * 4096 + (j & 1) * 512);
+  };
 
-  uint32_t v[LOADS];
+  // Loads: wave w fills the 8-row blocks w, w + 8, ... of a panel.
+  uint32_t va[LA], vb[LB];
+  const int chunk_a = (lane & 7) ^ ((wave & 1) << 2 | lane >> 4), chunk_b = (lane & 7) ^ (((lane >> 4) & 1) | (wave & 3) << 1);
 #pragma unroll
-  for (int l = 0; l < LOADS; ++l) {
-    const int blk = wave + l * 8;
-    const bool of_a = blk < BM / 8;
-    const int in = of_a ? blk : blk - BM / 8;
-    const int key = of_a ? ((in & 1) << 2) | (lane >> 4) : ((lane >> 4) & 1) | ((in & 3) << 1);
-    v[l] = (uint32_t)(in * 8 + (lane >> 3)) * (uint32_t)K + (((lane & 7) ^ key) << 4);
-  }
+  for (int l = 0; l < LA; ++l) va[l] = (uint32_t)((wave + 8 * l) * 8 + (lane >> 3)) * (uint32_t)K + (chunk_a << 4);
+#pragma unroll
+  for (int l = 0; l < LB; ++l)
+    vb[l] = (wave + 8 * l) * 8 < BN ? (uint32_t)((wave + 8 * l) * 8 + (lane >> 3)) * (uint32_t)K + (chunk_b << 4) : OUT_OF_RANGE;
+
+  const uint32_t past_a = TAIL && chunk_a >= tail_chunks ? OUT_OF_RANGE : 0u;  // of the last slab
+  const uint32_t past_b = TAIL && chunk_b >= tail_chunks ? OUT_OF_RANGE : 0u;
 
   const int num_tiles = w.tiles_m * w.tiles_n;
   for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
@@ -422,110 +452,140 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
     const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(w.b) + (size_t)n0 * K, 0, (uint32_t)cols * (uint32_t)K, 0x00020000);
     const float* const scales = w.a_scales + (int64_t)m0 * w.scale_row;
-    const uint32_t my_scale = (uint32_t)min(wave * 64 + lane, rows - 1) * (uint32_t)w.scale_row * 4u;
-    // load l of a slab into its place in LDS; the last one brings 64 rows' scales (waves behind the rows: copies)
-    auto load = [&](int l, int slab, uint32_t stage) {
-      if (l == LOADS) {
-        load_scales(scales + min(slab, nk - 1) * w.scale_block, my_scale, base + stage + PA + PB + wave * 256);
+    const int scale_part = wave % (BM / 64) * 64;  // 64 rows' scales a wave, some of them twice: all waves count alike
+    const uint32_t my_scale = (uint32_t)min(scale_part + lane, rows - 1) * (uint32_t)w.scale_row * 4u;
+    // Past the last slab loads bring that one again and fragments are read that nobody uses: branches cost more (a
+    // second set of registers for b's fragments, and spills).
+    auto load_a = [&](int l, int slab, uint32_t at, uint32_t at_s) {
+      const int k = min(slab, nk - 1);
+      if (l == LA) {
+        load_scales(scales + k * w.scale_block, my_scale, base + S::AT_S + at_s + scale_part * 4);
         return;
       }
-      const int blk = wave + l * 8;
-      const bool of_a = blk < BM / 8;
-      uint32_t off = v[l];
-      if (TAIL) {
-        const int in = of_a ? blk : blk - BM / 8;
-        const int key = of_a ? ((in & 1) << 2) | (lane >> 4) : ((lane >> 4) & 1) | ((in & 3) << 1);
-        if (slab >= nk - 1 && ((lane & 7) ^ key) >= tail_chunks) off = OUT_OF_RANGE;
-      }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(of_a ? da : db, (lds_void_t*)(base + stage + blk * 1024), 16, off,
+      const uint32_t off = TAIL ? va[l] | (slab >= nk - 1 ? past_a : 0u) : va[l];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_void_t*)(base + at + (wave + 8 * l) * 1024), 16, off,
+                                               (uint32_t)k * ROWB, 0, 0);
+    };
+    auto load_b = [&](int l, int slab, uint32_t at) {
+      const uint32_t off = TAIL ? vb[l] | (slab >= nk - 1 ? past_b : 0u) : vb[l];
+      const uint32_t to = BN % 64 == 0 || (wave + 8 * l) * 8 < BN ? S::AT_B + at + (wave + 8 * l) * 1024 : S::AT_NONE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(base + to), 16, off,
                                                (uint32_t)min(slab, nk - 1) * ROWB, 0, 0);
     };
-    // the wave's columns touch two weight blocks at most, and a pair of column tiles one
+    auto all_a = [&](int slab) {
+#pragma unroll
+      for (int l = 0; l <= LA; ++l) load_a(l, slab, slab * PA, slab * BM * 4);
+    };
+    auto all_b = [&](int slab) {
+#pragma unroll
+      for (int l = 0; l < LB; ++l) load_b(l, slab, slab * PB);
+    };
+    // The weight's scales: the wave's columns touch two blocks at most (one if it has 32, 64 or 128 columns).  Lane l
+    // keeps those of slab l of 64.
+    constexpr bool TWO = GROUP % (16 * TN) != 0;
     const int col = n0 + wn * 16 * TN, most_block = (w.N - 1) / GROUP;
-    // (fetched by vector loads: a scalar load under way makes every wait for LDS a wait for all of it)
-    int64_t none = 0;
-    asm volatile("" : "+v"(none));
-    const float* const sb = w.b_scales + (int64_t)min(col / GROUP, most_block) * nk + none;
-    const int64_t second = col / GROUP + 1 <= most_block ? nk : 0;
-    const int border = (GROUP - col % GROUP) / 16;  // column tiles of the first block
+    const float* const sb = w.b_scales + (int64_t)min(col / GROUP, most_block) * nk;
+    const int64_t second = TWO && col / GROUP + 1 <= most_block ? nk : 0;
+    const int border = GROUP - col % GROUP;  // columns of the first block
+    float sb0 = sb[min(lane, nk - 1)], sb1 = sb[min(lane, nk - 1) + second];
 
-    f32x4_t acc[TM][TN], part[2][TN];
+    f32x4_t acc[TM][TN], part[S::RING];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < TN; ++j) part[1][j] = f32x4_t{0, 0, 0, 0};
+    for (int x = 0; x < S::RING; ++x) part[x] = f32x4_t{0, 0, 0, 0};
     float first_scale = 0.0f, second_scale = 0.0f;  // of the row of tiles before
-    float s0 = sb[0], s1 = sb[second];
+    auto add = [&](int x, float in_first, float in_second) {  // the results of a slab's instruction x
+      const int i = x / TN, j = x % TN;
+      // (an even count of column tiles: the border lies between two pairs)
+      const int column = TN % 2 == 0 || j == TN - 1 ? 16 * j : (j >> 1) * 32 + quad * 8;
+      const float scale = !TWO || column < border ? in_first : in_second;
 #pragma unroll
-    for (int l = 0; l <= LOADS; ++l) load(l, 0, 0);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(part[x % S::RING][e], scale, acc[i][j][e]);
+    };
+
+    // as the loop would have left it
+    if (NA == 3) {
+      all_a(0), all_b(0), all_a(1), all_b(1);
+    } else {
+      all_b(0), all_a(0), all_b(1);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::PENDING) : "memory");
+    uint32_t use_a = 0, use_b = 0, use_s = 0;           // of the slab at work
+    uint32_t fill_a = (NA - 1) * PA, fill_s = (NA - 1) * BM * 4, fill_b = (NB - 1) * PB;
+    // what a last row sends out
+    constexpr int IN_LAST_ROW = (TN + S::SPACE_LATE - 1) / S::SPACE_LATE;
+#pragma unroll
+    for (int l = 0; l < S::LATE && l < IN_LAST_ROW; ++l) {
+      if (l <= LA) load_a(l, NA - 1, fill_a, fill_s);
+      else load_b(l - LA - 1, NB - 1, fill_b);
+    }
     i32x8_t fa[2], fb[TN];
     fa[0] = fragment(a0, a1);
     float sa = *(lds_f32_t*)at_scale;
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-      fb[j] = fragment(b0 + (j >> 1) * 4096 + (j & 1) * 512, b1 + (j >> 1) * 4096 + (j & 1) * 512);
-#pragma unroll
-    for (int l = 0; l <= LOADS; ++l)
-      if (l * S::SPACE < TN) load(l, 1, STAGE);  // those that go out in a last row
+    for (int j = 0; j < TN; ++j) fb[j] = fragment_b(j, 0);
+    if (S::EARLY) fill_b = 0;
     for (int slab = 0; slab < nk; ++slab) {
-      const uint32_t use = (slab & 1) * STAGE, other = STAGE - use;
-      const int next = min(slab + 1, nk - 1);
-      const float next0 = sb[next], next1 = sb[next + second];
+      if (slab && slab % 64 == 0) {
+        sb0 = sb[min(slab + lane, nk - 1)];
+        sb1 = sb[min(slab + lane, nk - 1) + second];
+        asm volatile("" : "+v"(sb0), "+v"(sb1));  // waited for here: not in every slab, for all loads under way
+      }
+      const float s0 = lane_value(sb0, slab & 63), s1 = lane_value(sb1, slab & 63);
+      const uint32_t next_a = after(use_a, PA, NA), next_b = after(use_b, PB, NB), next_s = after(use_s, BM * 4, NA);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const float mine0 = sa * s0, mine1 = sa * s1;
-        if (i == TM - 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        // Past the last slab loads bring that one again and fragments are read that nobody uses: branches cost more
-        // (a second set of registers for b's fragments, and spills).
-        const uint32_t at = i + 1 < TM ? use + (i + 1) * 2048 : other;
+        if (i == TM - 1) {
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::PENDING) : "memory");
+          fill_a = use_a, fill_s = use_s;
+          if (!S::EARLY) fill_b = use_b;
+        }
+        if (S::EARLY && i == 1) {  // every wave has multiplied with all of its fragments of b
+          asm volatile("s_barrier" ::: "memory");
+          fill_b = use_b;
+        }
+        const uint32_t at = i + 1 < TM ? use_a + (i + 1) * 2048 : next_a;
         fa[(i + 1) & 1] = fragment(a0 + at, a1 + at);
-        sa = *(lds_f32_t*)(at_scale + (i + 1 < TM ? use + (i + 1) * 64 : other));
+        sa = *(lds_f32_t*)(at_scale + (i + 1 < TM ? use_s + (i + 1) * 64 : next_s));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          part[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i & 1], f32x4_t{}, 0, 0, 0, 0, 0, 0);
+          part[(i * TN + j) % S::RING] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i & 1], f32x4_t{}, 0, 0, 0, 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
-          if (i == TM - 1)
-            fb[j] = fragment(b0 + other + (j >> 1) * 4096 + (j & 1) * 512, b1 + other + (j >> 1) * 4096 + (j & 1) * 512);
-          const int n = (i + 1) % TM * TN + j;  // instructions since the barrier
-          if (n % S::SPACE == 0 && n / S::SPACE <= LOADS) {
-            const int ahead = i == TM - 1 ? 2 : 1;
-            load(n / S::SPACE, slab + ahead, ahead == 2 ? use : other);
+          if (i == TM - 1) fb[j] = fragment_b(j, next_b);
+          const int late = (i + 1) % TM * TN + j, early = (i - 1) * TN + j;  // instructions since the barriers
+          if (late % S::SPACE_LATE == 0 && late / S::SPACE_LATE < S::LATE) {
+            const int l = late / S::SPACE_LATE, from = i == TM - 1 ? slab : slab - 1;
+            if (l <= LA) load_a(l, from + NA, fill_a, fill_s);
+            else load_b(l - LA - 1, from + NB, fill_b);
           }
-          // the row of tiles before, of the slab before for the first one
-          const float scale = j < border ? first_scale : second_scale;
-          f32x4_t& sum = acc[(i + TM - 1) % TM][j];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[e] = __fmaf_rn(part[(i + 1) & 1][j][e], scale, sum[e]);
+          if (S::EARLY && early >= 0 && early % S::SPACE_EARLY == 0 && early / S::SPACE_EARLY < LB)
+            load_b(early / S::SPACE_EARLY, slab + 2, fill_b);
+          // of this row, or of the one before (for the first row: the slab before)
+          if (j >= S::LAG) add(i * TN + j - S::LAG, mine0, mine1);
+          else add((i * TN + j - S::LAG + S::TOTAL) % S::TOTAL, first_scale, second_scale);
           __builtin_amdgcn_sched_barrier(0);
         }
         first_scale = mine0, second_scale = mine1;
       }
-      s0 = next0, s1 = next1;
+      use_a = next_a, use_b = next_b, use_s = next_s;
     }
+    const int m = wm * 16 * TM + r16;
+    uint16_t* const to = w.out + (size_t)(m0 + m) * w.ldc + n0;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const float scale = j < border ? first_scale : second_scale;
+      if (j >= TN - S::LAG) add((TM - 1) * TN + j, first_scale, second_scale);
+      // a lane holds row r16 of each row of tiles, columns 8 quad + 0 .. 7 of a pair of column tiles
+      const int c = wn * 16 * TN + (TN % 2 && j == TN - 1 ? 16 * j + quad * 4 : (j >> 1) * 32 + quad * 8 + (j & 1) * 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[TM - 1][j][e] = __fmaf_rn(part[1][j][e], scale, acc[TM - 1][j][e]);
-    }
-
-    // a lane holds row r16 of each row of tiles, columns 8 quad + 0 .. 7 of a pair of column tiles
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int m = wm * 16 * TM + i * 16 + r16;
-      if (m >= rows) continue;
-      uint16_t* to = w.out + (size_t)(m0 + m) * w.ldc + n0;
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int c = wn * 16 * TN + (j >> 1) * 32 + quad * 8 + (j & 1) * 4;
-        if (c < cols)
-          *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_out(acc[i][j][0], acc[i][j][1], w.half_out),
-                                                         pack_out(acc[i][j][2], acc[i][j][3], w.half_out));
-      }
+      for (int i = 0; i < TM; ++i)
+        if (c < cols && m + 16 * i < rows)
+          *reinterpret_cast<uint2*>(to + (size_t)(16 * i) * w.ldc + c) = make_uint2(
+              pack_out(acc[i][j][0], acc[i][j][1], w.half_out), pack_out(acc[i][j][2], acc[i][j][3], w.half_out));
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next tile's slabs go where this one's were
   }
@@ -567,12 +627,13 @@ int launch_split(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
   return TW_OK;
 }
 
-template <int WM, int TM, int TN>
+template <int WM, int TM, int TN, int NA, int NB>
 int launch_wide(BlockArgs w, int max_cus, hipStream_t hs) {
-  using S = WideShape<WM, TM, TN>;
+  using S = WideShape<WM, TM, TN, NA, NB>;
   static std::atomic<bool> ok[2][kMaxDevices];
   const bool tail = w.K % GROUP != 0;
-  const auto kernel = tail ? gemm_fp8_block_tile_kernel<WM, TM, TN, true> : gemm_fp8_block_tile_kernel<WM, TM, TN, false>;
+  const auto kernel = tail ? gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, true>
+                           : gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, false>;
   if (int rc = allow_lds(kernel, ok[tail], S::LDS)) return rc;
   w.tiles_m = (w.M + S::BM - 1) / S::BM;
   w.tiles_n = (w.N + S::BN - 1) / S::BN;
@@ -580,6 +641,38 @@ int launch_wide(BlockArgs w, int max_cus, hipStream_t hs) {
   if (max_cus > 0 && grid > max_cus) grid = max_cus;
   launch_kernel(kernel, dim3((unsigned)grid), dim3(WIDE_THREADS), S::LDS, hs, w);
   return TW_OK;
+}
+
+// The tile shapes (WM, TM, TN, slabs of a and of b in LDS) with the time that a round of one tile a compute unit takes,
+// relative to 256 x 224, measured at K = 8192 (106 us).  By area the large ones are alike (two rounds: 505 to 542 values
+// a ns, 128 x 128 441), so what counts is how the tile count fits the units: [4096, 8192] x [7168, 8192] has 512 tiles of
+// 256 x 224 and takes 205 us, with 192 x 256 256 us, 256 x 128 247, 128 x 128 292; [1000, 3696] x [8192, 3696] has 256
+// tiles of 128 x 256: 38.6 us, with 256 x 224 54.5, 192 x 256 47.0, 128 x 128 47.8.  64 x 128: two of them fit a unit.
+#define TW_WIDE_TILES(X)                                                                                    \
+  X(4, 4, 7, 3, 2, 1.0) X(4, 4, 6, 3, 2, 0.87) X(2, 6, 4, 3, 2, 0.83) X(4, 4, 4, 3, 3, 0.61) X(2, 4, 4, 3, 3, 0.59) \
+  X(2, 4, 2, 3, 3, 0.37) X(2, 2, 2, 3, 3, 0.22)
+
+struct WideTile { int wm, tm, tn; double cost; };
+#define TW_WIDE_TILE(WM, TM, TN, NA, NB, COST) {WM, TM, TN, COST},
+constexpr WideTile kWideTiles[] = {TW_WIDE_TILES(TW_WIDE_TILE)};
+#undef TW_WIDE_TILE
+
+// The shape whose rounds take the least time; no shape changes a result bit (an element's slabs are added in order).
+int launch_wide_for(const BlockArgs& w, int max_cus, int cus, hipStream_t hs) {
+  const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
+  const WideTile* best = &kWideTiles[0];
+  double best_cost = 1e300;
+  for (const WideTile& t : kWideTiles) {
+    const int64_t bm = 16 * t.tm * t.wm, bn = 16 * t.tn * (8 / t.wm);
+    const int64_t tiles = (w.M + bm - 1) / bm * ((w.N + bn - 1) / bn);
+    const double cost = (double)((tiles + units - 1) / units) * t.cost;
+    if (cost < best_cost) best = &t, best_cost = cost;
+  }
+#define TW_WIDE_LAUNCH(WM, TM, TN, NA, NB, COST) \
+  if (best->wm == WM && best->tm == TM && best->tn == TN) return launch_wide<WM, TM, TN, NA, NB>(w, max_cus, hs);
+  TW_WIDE_TILES(TW_WIDE_LAUNCH)
+#undef TW_WIDE_LAUNCH
+  return set_error(TW_ERR_INVALID_ARGUMENT, "gemm_fp8_block_nt: no tile for %d rows", w.M);
 }
 
 }  // namespace
@@ -653,17 +746,7 @@ int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64
   else if (M <= 32) rc = launch_split<1, 1, 3, 4>(w, max_cus, cus, hs);
   else if (M <= 64) rc = launch_split<2, 1, 3, 8>(w, max_cus, cus, hs);
   else if (M <= 128) rc = launch_split<2, 2, 2, 8>(w, max_cus, cus, hs);
-  else {
-    const char* e = getenv("TW_T");
-    int t = e ? atoi(e) : 284;
-    if (t == 244) rc = launch_wide<2, 4, 4>(w, max_cus, hs);
-    else if (t == 264) rc = launch_wide<2, 6, 4>(w, max_cus, hs);
-    else if (t == 444) rc = launch_wide<4, 4, 4>(w, max_cus, hs);
-    else if (t == 242) rc = launch_wide<2, 4, 2>(w, max_cus, hs);
-    else if (t == 446) rc = launch_wide<4, 4, 6>(w, max_cus, hs);
-    else if (t == 222) rc = launch_wide<2, 2, 2>(w, max_cus, hs);
-    else rc = launch_wide<2, 8, 4>(w, max_cus, hs);
-  }
+  else rc = launch_wide_for(w, max_cus, cus, hs);
   return rc ? rc : finish_launch(what);
 }
 
