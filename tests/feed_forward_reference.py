@@ -105,7 +105,7 @@ def weight_codes(w):
     N, K = w.shape
     padded = torch.nn.functional.pad(w.float(), (0, -K % GROUP, 0, -N % GROUP))
     blocks = padded.view(padded.shape[0] // GROUP, GROUP, -1, GROUP)
-    scales = (blocks.abs().amax((1, 3)).clamp(min=1e-10) / 448).contiguous()
+    scales = (blocks.abs().amax((1, 3)).clamp(min=1e-10).double() / 448).float().contiguous()   # (one rounding)
     return (w.float() / spread(spread(scales, N, 0), K, 1)).clamp(-448, 448).to(torch.float8_e4m3fn), scales
 
 

@@ -113,3 +113,64 @@ def test_a_tensor_that_wants_its_gradient_is_refused():
         ops.gated_gemm_bf16_nt(bf16(4, 8), x, bf16(16, 16))
     with pytest.raises(RuntimeError, match="records no gradient"):
         ops.quant_fp8_groups(torch.zeros((4, 16), dtype=torch.float8_e4m3fn), torch.zeros((4, 1)), x)
+
+
+def test_the_formulas_gradients_follow_differences():
+    """The 64-bit gradients that the kernel's are compared with, against central differences."""
+    import feed_forward_reference as R
+    g = torch.Generator().manual_seed(3)
+    x, w, c = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((3, 8), (12, 8), (3, 6)))
+    for kind in R.ACTIVATIONS:
+        both = x @ w.t()
+        gx, _, gw, _ = R.gated_gradients(c, x, w, both, kind)
+
+        def loss(x, w):
+            gate, up = (x @ w.t()).chunk(2, 1)
+            return float((R.act(gate, kind) * up * c).sum())
+
+        for t, grad in ((x, gx), (w, gw)):
+            for i in range(0, t.numel(), 5):
+                keep, h = t.view(-1)[i].item(), 1e-5
+                t.view(-1)[i] = keep + h
+                above = loss(x, w)
+                t.view(-1)[i] = keep - h
+                below = loss(x, w)
+                t.view(-1)[i] = keep
+                # a third derivative of order 100 times h^2, and 2^-50 of the loss over h
+                assert abs((above - below) / (2 * h) - grad.view(-1)[i].item()) < 1e-7
+
+
+def test_layers_check_their_sizes():
+    import tokenweave_amd as tw
+    with pytest.raises(ValueError, match="not divisible"):
+        tw.GatedLinear(16, 30, tp_size=4)
+    with pytest.raises(ValueError, match="Invalid rank"):
+        tw.GatedLinear(16, 32, tp_rank=4, tp_size=4)
+    with pytest.raises(ValueError, match="unknown activation"):
+        tw.FeedForward(16, 32, "swish")
+
+
+def test_sizes_without_8_bit_rows_are_refused_when_a_model_is_loaded():
+    import tokenweave_amd as tw
+    with pytest.raises(ValueError, match="multiple of 16"):
+        tw.FeedForward(64, 400, tp_size=2).to_fp8_blocks()
+    with pytest.raises(ValueError, match="multiple of 16"):
+        tw.Fp8BlockLinearMethod().process_weights(tw.RowParallelLinear(24, 64, bias=False))
+
+
+def test_weight_codes_on_the_cpu():
+    import feed_forward_reference as R
+    import tokenweave_amd as tw
+    w = torch.randn(300, 200)
+    codes, scales = tw.quantize_fp8_blocks(w)
+    want, want_scales = R.weight_codes(w)
+    assert codes.dtype == torch.float8_e4m3fn and scales.shape == (3, 2)
+    assert torch.allclose(scales, want_scales, rtol=2 ** -23, atol=0) and (codes.float() - want.float()).abs().max() <= 32
+
+
+def test_a_capture_is_refused_where_a_gradient_is_recorded(monkeypatch):
+    from tokenweave_amd import feed_forward
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="gated_gemm_bf16_nt_backward"):
+        feed_forward.gated_linear(bf16(4, 16).requires_grad_(), bf16(16, 16))
