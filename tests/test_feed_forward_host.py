@@ -174,3 +174,18 @@ def test_a_capture_is_refused_where_a_gradient_is_recorded(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="gated_gemm_bf16_nt_backward"):
         feed_forward.gated_linear(bf16(4, 16).requires_grad_(), bf16(16, 16))
+
+
+def test_a_models_type_leaves_codes_and_scales_as_they_are():
+    import tokenweave_amd as tw
+    block = tw.FeedForward(64, 96)
+    for p in block.parameters():
+        p.data.normal_()
+    block.to_fp8_blocks()
+    before = {k: v.clone() for k, v in block.state_dict().items()}
+    for model in (block.half(), block.bfloat16(), block.to(torch.float32)):
+        for name, value in model.state_dict().items():
+            assert value.dtype == before[name].dtype == (torch.float32 if "scale" in name else torch.float8_e4m3fn)
+            assert torch.equal(value.view(torch.uint8), before[name].view(torch.uint8))
+    plain = tw.RowParallelLinear(64, 64, bias=True).half()
+    assert plain.weight.dtype == plain.bias.dtype == torch.float16

@@ -7,7 +7,7 @@ activation and product are one kernel.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Any, Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 from torch.nn.parameter import Parameter
 
 from . import _custom_ops as ops
-from .linear import RowParallelLinear
+from .linear import RowParallelLinear, _apply_beside_codes
 
 
 def _refuse_capture() -> None:
@@ -78,6 +78,9 @@ class GatedLinear(nn.Module):
         self.input_size, self.intermediate_size = input_size, intermediate_size // tp_size
         self.weight = Parameter(torch.empty(2 * self.intermediate_size, input_size, dtype=torch.bfloat16),
                                 requires_grad=False)
+
+    def _apply(self, fn: Any, recurse: bool = True) -> "GatedLinear":
+        return _apply_beside_codes(self, super()._apply, fn, recurse)
 
     def weight_loader(self, param: Parameter, loaded_weight: torch.Tensor, shard_id: int) -> None:
         """This rank's rows of a full gate (``shard_id`` 0) or up (1) weight."""

@@ -54,6 +54,17 @@ def _is_unquantized(method: Any) -> bool:
             and "apply_inplace" not in method.__dict__)
 
 
+def _apply_beside_codes(layer: nn.Module, apply: Any, fn: Any, recurse: bool) -> nn.Module:
+    """A model's type (`model.bfloat16()`) is not that of 8-bit codes and of their fp32 scales: they stay what they
+    are, on the device they are moved to."""
+    held = {name: p.data for name, p in layer._parameters.items() if p is not None} if hasattr(layer, "weight_scale") else {}
+    apply(fn, recurse)
+    for name in ("weight", "weight_scale"):
+        if name in held and getattr(layer, name).dtype != held[name].dtype:
+            getattr(layer, name).data = held[name].to(getattr(layer, name).device)
+    return layer
+
+
 class RowParallelLinear(nn.Module):
     """Y = X A + b with A split along its first dimension (X along its last) over
     ``tp_size`` ranks; this module is rank ``tp_rank``'s share.  Constructor and
@@ -87,6 +98,9 @@ class RowParallelLinear(nn.Module):
             self.bias = Parameter(torch.empty(output_size, dtype=self.params_dtype), requires_grad=False)
         else:
             self.register_parameter("bias", None)
+
+    def _apply(self, fn: Any, recurse: bool = True) -> "RowParallelLinear":
+        return _apply_beside_codes(self, super()._apply, fn, recurse)
 
     def weight_loader(self, param: Parameter, loaded_weight: torch.Tensor) -> None:
         """This rank's slice of a full weight along the input dimension; biases whole
