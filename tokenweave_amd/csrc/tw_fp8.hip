@@ -189,6 +189,13 @@ __device__ __forceinline__ void load_scales(const float* from, uint32_t offset, 
   const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, 0x7fffffffu, 0x00020000);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void_t*)to, 4, offset, 0, 0, 0);
 }
+__device__ __forceinline__ i32x8_t fragment(const lds_u8_t* p, const lds_u8_t* q) {
+  const u32x4_t x = *(lds_chunk_t*)p, y = *(lds_chunk_t*)q;
+  return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
 #endif
 
 // Few rows: bound by reading b once.  As in the bf16 K-split kernel four waves share the inner dimension, wave w takes
@@ -197,8 +204,9 @@ __device__ __forceinline__ void load_scales(const float* from, uint32_t offset, 
 constexpr int SPLIT_WAVES = 4;
 constexpr int SPLIT_THREADS = SPLIT_WAVES * 64;
 constexpr int split_stage(int mt, int nt) { return 32 * (mt + nt) * ROWB + 256; }
+constexpr int split_wave(int mt, int nt, int stages) { return stages * split_stage(mt, nt) + 512; }
 constexpr int split_lds(int mt, int nt, int stages) {
-  const int slabs = SPLIT_WAVES * stages * split_stage(mt, nt), sums = SPLIT_WAVES * 32 * mt * (32 * nt * 4 + 16);
+  const int slabs = SPLIT_WAVES * split_wave(mt, nt, stages), sums = SPLIT_WAVES * 32 * mt * (32 * nt * 4 + 16);
   return slabs > sums ? slabs : sums;
 }
 
@@ -219,7 +227,9 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
     v[j] = (uint32_t)(j * 8 + (lane >> 3)) * (uint32_t)K + (((lane & 7) ^ (((j & 1) << 2) | (lane >> 4))) << 4);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) roff[kk] = l32 * ROWB + ((((kk << 1) | lhi) ^ ((l32 >> 1) & 7)) << 4);
-  uint8_t* const mine = lds + wave * (STAGES * STAGE);
+  // the wave's slabs, and the weight's scales of 64 of them, for both blocks that a tile may touch
+  uint8_t* const mine = lds + wave * split_wave(MT, NT, STAGES);
+  lds_u8_t* const block_scales = (lds_u8_t*)mine + STAGES * STAGE;
 
   const int num_tiles = w.tiles_m * w.tiles_n;
   for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
@@ -240,6 +250,13 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
     const float* const sb = w.b_scales + (int64_t)(n0 / GROUP) * nk;
     const int border = GROUP - n0 % GROUP;
     const int64_t second = n0 / GROUP + 1 < (w.N + GROUP - 1) / GROUP ? nk : 0;
+    auto fetch_blocks = [&](int from) {
+      const uint32_t at = (uint32_t)min(from + SPLIT_WAVES * lane, nk - 1) * 4u;
+      load_scales(sb, at, block_scales);
+      load_scales(sb + second, at, block_scales + 256);
+    };
+    fetch_blocks(wave);
+    uint32_t turn = 0;
 
     f32x16_t acc[MT][NT];
 #pragma unroll
@@ -271,7 +288,11 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
     for (int i = 0; i < STAGES - 1; ++i)
       if (next < nk) issue();
     for (int slab = wave; slab < nk; slab += SPLIT_WAVES, use = use == (STAGES - 1) * STAGE ? 0 : use + STAGE) {
-      const float sb0 = sb[slab], sb1 = sb[slab + second];
+      if (turn == 256) {
+        fetch_blocks(slab);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        turn = 0;
+      }
       if (next < nk) {
         issue();
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
@@ -283,32 +304,31 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
       const uint8_t* pa = mine + use;
       const uint8_t* pb = pa + RA * ROWB;
       f32x16_t part[MT][NT];
+      i32x8_t fa[2][MT], fb[2][NT];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        i32x8_t fa[MT], fb[NT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(pa + i * 32 * ROWB + roff[2 * h]);
-          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(pa + i * 32 * ROWB + roff[2 * h + 1]);
-          fa[i] = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-        }
+        for (int j = 0; j < NT; ++j)
+          fb[h][j] = fragment((lds_u8_t*)pb + j * 32 * ROWB + roff[2 * h], (lds_u8_t*)pb + j * 32 * ROWB + roff[2 * h + 1]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(pb + j * 32 * ROWB + roff[2 * h]);
-          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(pb + j * 32 * ROWB + roff[2 * h + 1]);
-          fb[j] = i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-        }
+        for (int i = 0; i < MT; ++i)
+          fa[h][i] = fragment((lds_u8_t*)pa + i * 32 * ROWB + roff[2 * h], (lds_u8_t*)pa + i * 32 * ROWB + roff[2 * h + 1]);
+      }
+      const float block0 = *(lds_f32_t*)(block_scales + turn), block1 = *(lds_f32_t*)(block_scales + 256 + turn);
+      turn += 4;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int j = 0; j < NT; ++j)
-            part[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                fb[j], fa[i], h ? part[i][j] : f32x16_t{}, 0, 0, 0, 0, 0, 0);
-      }
+            part[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][j], fa[h][i], h ? part[i][j] : f32x16_t{}, 0,
+                                                                         0, 0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const float sa = *reinterpret_cast<const float*>(mine + use + (RA + RB) * ROWB + (i * 32 + l32) * 4);
-        const float s0 = sa * sb0, s1 = sa * sb1;
+        const float s0 = sa * block0, s1 = sa * block1;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -386,15 +406,8 @@ struct WideShape {
 };
 
 #ifdef __HIP_DEVICE_COMPILE__
-__device__ __forceinline__ i32x8_t fragment(const lds_u8_t* p, const lds_u8_t* q) {
-  const u32x4_t x = *(lds_chunk_t*)p, y = *(lds_chunk_t*)q;
-  return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-}
 __device__ __forceinline__ uint32_t after(uint32_t at, uint32_t panel, int n) {
   return at == (n - 1) * panel ? 0u : at + panel;
-}
-__device__ __forceinline__ float lane_value(float v, int lane) {
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
 #endif
 
@@ -744,7 +757,9 @@ int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64
   if (M <= 8) rc = launch_split<1, 1, 3, 1>(w, max_cus, cus, hs);
   else if (M <= 16) rc = launch_split<1, 1, 3, 2>(w, max_cus, cus, hs);
   else if (M <= 32) rc = launch_split<1, 1, 3, 4>(w, max_cus, cus, hs);
-  else if (M <= 64) rc = launch_split<2, 1, 3, 8>(w, max_cus, cus, hs);
+  else if (M <= 64) rc = launch_split<2, 1, 2, 8>(w, max_cus, cus, hs);
+  else if (M <= 80) rc = launch_split<2, 2, 2, 5>(w, max_cus, cus, hs);
+  else if (M <= 96) rc = launch_split<2, 2, 2, 6>(w, max_cus, cus, hs);
   else if (M <= 128) rc = launch_split<2, 2, 2, 8>(w, max_cus, cus, hs);
   else rc = launch_wide_for(w, max_cus, cus, hs);
   return rc ? rc : finish_launch(what);
