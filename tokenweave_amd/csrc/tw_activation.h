@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/tokenweave_amd.h"
 
 namespace tw {
@@ -13,20 +15,22 @@ constexpr float kTanhA = 0.7978845608028654f, kTanhB = 0.044715f;  // sqrt(2 / p
 // 1 / (1 + e^-x).  e^-x overflows to an infinity below -88.7, whose reciprocal is the zero it should be.
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
-__device__ __forceinline__ float activation(float x, int act) {
-  if (act == TW_ACT_SILU) return x * sigmoid(x);
+template <int ACT>
+__device__ __forceinline__ float activation(float x) {
+  if (ACT == TW_ACT_SILU) return x * sigmoid(x);
   // 0.5 (1 + tanh z) = sigmoid(2 z): no cancellation for large negative z
-  if (act == TW_ACT_GELU_TANH) return x * sigmoid(2.0f * kTanhA * (x + kTanhB * x * x * x));
+  if (ACT == TW_ACT_GELU_TANH) return x * sigmoid(2.0f * kTanhA * (x + kTanhB * x * x * x));
   return 0.5f * x * erfcf(-0.70710678118654752f * x);
 }
 
 // act(x) and its derivative
-__device__ __forceinline__ void activation_and_slope(float x, int act, float& f, float& df) {
-  if (act == TW_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ void activation_and_slope(float x, float& f, float& df) {
+  if (ACT == TW_ACT_SILU) {
     const float s = sigmoid(x);
     f = x * s;
     df = s * (1.0f + x * (1.0f - s));
-  } else if (act == TW_ACT_GELU_TANH) {
+  } else if (ACT == TW_ACT_GELU_TANH) {
     const float z = 2.0f * kTanhA * (x + kTanhB * x * x * x), s = sigmoid(z);
     const float c = fminf(fmaxf(x, -16.0f), 16.0f);  // s (1 - s) is zero out there, and must not meet an infinity
     f = x * s;
@@ -36,6 +40,14 @@ __device__ __forceinline__ void activation_and_slope(float x, int act, float& f,
     f = x * cdf;
     df = cdf + x * 0.3989422804014327f * __expf(-0.5f * x * x);
   }
+}
+
+// f(integral_constant<act>): one branch on the activation, outside the loops that apply it.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  if (act == TW_ACT_SILU) f(std::integral_constant<int, TW_ACT_SILU>{});
+  else if (act == TW_ACT_GELU) f(std::integral_constant<int, TW_ACT_GELU>{});
+  else f(std::integral_constant<int, TW_ACT_GELU_TANH>{});
 }
 
 }  // namespace tw

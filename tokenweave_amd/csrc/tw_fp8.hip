@@ -114,8 +114,10 @@ __global__ __launch_bounds__(QUANT_THREADS) void quant_fp8_groups_kernel(QuantAr
   if (GATED) {
     float u[8];
     load_eight<DTYPE, VEC>(u, w.input, at + w.K, n);
+    with_activation(w.act, [&](auto act) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = activation(y[e], w.act) * u[e];
+      for (int e = 0; e < 8; ++e) y[e] = activation<act()>(y[e]) * u[e];
+    });
   }
   // as whole numbers magnitudes are in order, infinities and NaN above all others
   uint32_t most = 0;

@@ -92,13 +92,15 @@ __global__ __launch_bounds__(TURN_THREADS) void gated_grad_kernel(GradArgs w) {
       const float gate[4] = {low(g2.x), high(g2.x), low(g2.y), high(g2.y)};
       const float up[4] = {low(u2.x), high(u2.x), low(u2.y), high(u2.y)};
       float x[4], y[4];
+      with_activation(w.act, [&](auto act) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float f, df;
-        activation_and_slope(gate[e], w.act, f, df);
-        x[e] = h[e] * up[e] * df;
-        y[e] = h[e] * f;
-      }
+        for (int e = 0; e < 4; ++e) {
+          float f, df;
+          activation_and_slope<act()>(gate[e], f, df);
+          x[e] = h[e] * up[e] * df;
+          y[e] = h[e] * f;
+        }
+      });
       dg = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
       du = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
       if (w.d) {

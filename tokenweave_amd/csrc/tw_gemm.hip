@@ -410,26 +410,28 @@ __global__ __launch_bounds__(KS_THREADS) void gemm_bf16_nt_ksplit_kernel(
               f32x4_t{acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     __syncthreads();
     if constexpr (GATED) {
-      for (int g = tid; g < ROWS * RB / 8; g += KS_THREADS) {
-        const int m = g / (RB / 8), c = (g % (RB / 8)) * 4;
-        if (m0 + m < M && c < cols && n0 + c < N) {
-          const uint8_t* p = lds_ks + m * PITCH + c * 4;
-          f32x4_t s = *reinterpret_cast<const f32x4_t*>(p), u = *reinterpret_cast<const f32x4_t*>(p + RB * 2);
-#pragma unroll
-          for (int w = 1; w < KS_WAVES; ++w) {
-            s += *reinterpret_cast<const f32x4_t*>(p + w * (RA * PITCH));
-            u += *reinterpret_cast<const f32x4_t*>(p + w * (RA * PITCH) + RB * 2);
+      with_activation(gated.act, [&](auto act) {
+        for (int g = tid; g < ROWS * RB / 8; g += KS_THREADS) {
+          const int m = g / (RB / 8), c = (g % (RB / 8)) * 4;
+          if (m0 + m < M && c < cols && n0 + c < N) {
+            const uint8_t* p = lds_ks + m * PITCH + c * 4;
+            f32x4_t s = *reinterpret_cast<const f32x4_t*>(p), u = *reinterpret_cast<const f32x4_t*>(p + RB * 2);
+  #pragma unroll
+            for (int w = 1; w < KS_WAVES; ++w) {
+              s += *reinterpret_cast<const f32x4_t*>(p + w * (RA * PITCH));
+              u += *reinterpret_cast<const f32x4_t*>(p + w * (RA * PITCH) + RB * 2);
+            }
+            if (gated.both) {
+              uint16_t* to = gated.both + (size_t)(m0 + m) * gated.ld_both + n0 + c;
+              *reinterpret_cast<uint2*>(to) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
+              *reinterpret_cast<uint2*>(to + N) = make_uint2(pack2(u.x, u.y), pack2(u.z, u.w));
+            }
+            *reinterpret_cast<uint2*>(out + (size_t)(m0 + m) * ldc + n0 + c) =
+                make_uint2(pack2(activation<act()>(s.x) * u.x, activation<act()>(s.y) * u.y),
+                           pack2(activation<act()>(s.z) * u.z, activation<act()>(s.w) * u.w));
           }
-          if (gated.both) {
-            uint16_t* to = gated.both + (size_t)(m0 + m) * gated.ld_both + n0 + c;
-            *reinterpret_cast<uint2*>(to) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
-            *reinterpret_cast<uint2*>(to + N) = make_uint2(pack2(u.x, u.y), pack2(u.z, u.w));
-          }
-          *reinterpret_cast<uint2*>(out + (size_t)(m0 + m) * ldc + n0 + c) =
-              make_uint2(pack2(activation(s.x, gated.act) * u.x, activation(s.y, gated.act) * u.y),
-                         pack2(activation(s.z, gated.act) * u.z, activation(s.w, gated.act) * u.w));
         }
-      }
+      });
       __syncthreads();  // the next tile's slabs overwrite the sums
       continue;
     }
@@ -653,7 +655,7 @@ __device__ __forceinline__ float acc_read(float x) {
 
 // The gated form: tiles 4 p .. 4 p + 3 of a row of tiles are gate, up, gate, up of eight columns, 32 p + 8 quad and up.
 // Rows of 8 bytes' alignment or I % 8 != 0 (narrow) take two stores.
-template <int TM, int TN, bool WIDE>
+template <int TM, int TN, bool WIDE, int ACT>
 __device__ __forceinline__ void tile_store_gated(const f32x4_t (&acc)[TM][TN], __amdgpu_buffer_rsrc_t dc,
                                                  uint32_t row_off, uint32_t row_step, int n, int N, int m, int M,
                                                  const GatedOut& gated) {
@@ -674,7 +676,7 @@ __device__ __forceinline__ void tile_store_gated(const f32x4_t (&acc)[TM][TN], _
           *reinterpret_cast<uint2*>(to + N) = make_uint2(pack2(u[0], u[1]), pack2(u[2], u[3]));
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) g[e] = activation(g[e], gated.act) * u[e];
+        for (int e = 0; e < 4; ++e) g[e] = activation<ACT>(g[e]) * u[e];
         v[s] = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
       }
       const uint32_t off = row_off + (uint32_t)i * row_step + (uint32_t)p * 64u;
@@ -913,8 +915,11 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
           batch.out[0] + (size_t)p.m0 * ldc + n0, 0, (uint32_t)min(M - p.m0, S::BM) * (uint32_t)ldc * 2u, 0x00020000);
       const uint32_t row_off = (uint32_t)(row * (int)ldc + col) * 2u, row_step = (uint32_t)ldc * 32u;
       asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMA's result is written
-      if (wide_store) tile_store_gated<TM, TN, true>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
-      else tile_store_gated<TM, TN, false>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
+      with_activation(gated.act, [&](auto act) {
+        if (wide_store)
+          tile_store_gated<TM, TN, true, act()>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
+        else tile_store_gated<TM, TN, false, act()>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
+      });
       continue;
     }
     const uint16_t* __restrict__ bias = batch.bias[p.product];
