@@ -179,6 +179,42 @@ def test_what_the_instruction_keeps(M):
                 assert (out.abs() <= 2.0 ** least).all(), (place, e)
 
 
+@pytest.mark.parametrize("M", [3, 64, 100, 300])
+def test_long_inner_dimension(M):
+    check_product(M, 68, 33168)
+
+
+@pytest.mark.parametrize("M", [3, 130])
+def test_weight_of_more_than_two_gib(M):
+    N, K = 70000, 32768
+    a, a_scales, _, _ = operands(M, 4, K)
+    b = torch.empty((N, K), dtype=torch.uint8, device="cuda")
+    for part in b.split(10000):
+        part.copy_(torch.randint(0, 256, part.shape, dtype=torch.uint8, device="cuda"))
+        part[(part & 0x7f) == 0x7f] = 1
+    b_scales = torch.rand((-(-N // 128), K // 128), device="cuda")
+    out = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    ops.gemm_fp8_block_nt(out, a, a_scales, b.view(FP8), b_scales)
+    for first in (0, 35072, 69888):
+        part = b[first:first + 128].view(FP8)
+        want, off = R.block_product(a, a_scales, part, b_scales[first // 128:first // 128 + 1])
+        R.assert_within(out[:, first:first + 128], want, off + R.half(torch.bfloat16) * want.abs(), first)
+
+
+def test_scales_of_one_row_at_any_stride():
+    a, a_scales, b, b_scales = operands(1, 260, 272)
+    wide = torch.empty((1, 1 << 22), device="cuda").as_strided((1, 3), (1 << 22, 5))
+    wide.copy_(a_scales)
+    out, want = (torch.empty((1, 260), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ops.gemm_fp8_block_nt(want, a, a_scales, b, b_scales)
+    ops.gemm_fp8_block_nt(out, a, wide, b, b_scales)
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="elements apart"):
+        rows2 = torch.empty(1 << 22, device="cuda").as_strided((2, 3), (1 << 21, 1))
+        ops.gemm_fp8_block_nt(torch.empty((2, 260), dtype=torch.bfloat16, device="cuda"), a.expand(2, -1).contiguous(), rows2,
+                              b, b_scales)
+
+
 @pytest.mark.parametrize("M", [5, 64, 300])
 def test_grid_caps_give_the_same_bits(M):
     a, a_scales, b, b_scales = operands(M, 700, 528)

@@ -123,6 +123,20 @@ def test_slopes_far_out_are_finite():
         R.assert_within(gw[:8, 0], want, want.abs() * 2 ** -7 + 1e-8, kind)
 
 
+@pytest.mark.parametrize("M", [2, 130])
+def test_weight_halves_more_than_two_gib_apart(M):
+    inner, K = 69632, 16384
+    x = make(M, 4, K)[0]
+    w = torch.empty((2 * inner, K), dtype=BF16, device="cuda")
+    for part in w.split(8192):
+        part.normal_(0, K ** -0.5)
+    out = torch.empty((M, inner), dtype=BF16, device="cuda")
+    ops.gated_gemm_bf16_nt(out, x, w)
+    at = torch.tensor([0, 1, 127, 128, 35000, inner - 129, inner - 1], device="cuda")
+    want, bound, _, _ = R.gated(x, torch.cat((w[at], w[inner + at])), "silu")
+    R.assert_within(out[:, at], want, bound, "out")
+
+
 def test_no_rows():
     x, w = make(0, 36, 72)
     ops.gated_gemm_bf16_nt(torch.empty((0, 36), dtype=BF16, device="cuda"), x, w,

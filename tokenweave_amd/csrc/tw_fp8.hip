@@ -542,7 +542,6 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
     float sa = *(lds_f32_t*)at_scale;
 #pragma unroll
     for (int j = 0; j < TN; ++j) fb[j] = fragment_b(j, 0);
-    if (S::EARLY) fill_b = 0;
     for (int slab = 0; slab < nk; ++slab) {
       if (slab && slab % 64 == 0) {
         sb0 = sb[min(slab + lane, nk - 1)];
@@ -729,6 +728,7 @@ int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64
                           const void* b, const float* b_scales, int64_t M, int64_t N, int64_t K, int64_t ldc, int dtype,
                           int max_cus, void* stream) {
   const char* what = "gemm_fp8_block_nt";
+  if (M == 1) scale_row = 0;  // a single row's has no meaning
   if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > BLOCK_MAX_K || ldc < N)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad shape M=%lld N=%lld K=%lld ldc=%lld", what, (long long)M,
                      (long long)N, (long long)K, (long long)ldc);

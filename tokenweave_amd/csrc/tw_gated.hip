@@ -26,6 +26,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 constexpr int TURN = 64;          // rows and columns of a tile
 constexpr int TURN_PITCH = 66;    // elements of a tile's row in LDS: columns are read without conflicts
 constexpr int TURN_THREADS = 256;
+constexpr int TURN_ROWS = TURN_THREADS / (TURN / 4), TURN_STEPS = TURN / TURN_ROWS;  // four channels a thread and step
 
 struct GradArgs {
   const uint16_t *grad, *both, *a, *b;
@@ -59,13 +60,19 @@ __device__ __forceinline__ void write_turned(const uint16_t* tile, uint16_t* to,
 __device__ __forceinline__ void turn(uint16_t* tile, const uint16_t* from, uint16_t* to, int64_t rows, int64_t columns,
                                      int64_t pitch, int64_t t) {
   const int64_t across = (columns + TURN - 1) / TURN, m0 = t / across * TURN, c0 = t % across * TURN;
-  for (int g = threadIdx.x; g < TURN * TURN / 4; g += TURN_THREADS) {
-    const int m = g / (TURN / 4), c = (g % (TURN / 4)) * 4;
-    uint2 v = make_uint2(0, 0);
-    if (m0 + m < rows && c0 + c < columns) v = *reinterpret_cast<const uint2*>(from + (m0 + m) * columns + c0 + c);
-    uint32_t* p = reinterpret_cast<uint32_t*>(tile + m * TURN_PITCH + c);
-    p[0] = v.x;
-    p[1] = v.y;
+  const int m = threadIdx.x / (TURN / 4), c = threadIdx.x % (TURN / 4) * 4;
+  uint2 v[TURN_STEPS];  // all under way before the first is used
+#pragma unroll
+  for (int i = 0; i < TURN_STEPS; ++i) {
+    const int64_t row = m0 + m + i * TURN_ROWS;
+    v[i] = make_uint2(0, 0);
+    if (row < rows && c0 + c < columns) v[i] = *reinterpret_cast<const uint2*>(from + row * columns + c0 + c);
+  }
+#pragma unroll
+  for (int i = 0; i < TURN_STEPS; ++i) {
+    uint32_t* p = reinterpret_cast<uint32_t*>(tile + (m + i * TURN_ROWS) * TURN_PITCH + c);
+    p[0] = v[i].x;
+    p[1] = v[i].y;
   }
   __syncthreads();
   write_turned(tile, to, c0, columns, m0, pitch, pitch);
@@ -81,41 +88,49 @@ __global__ __launch_bounds__(TURN_THREADS) void gated_grad_kernel(GradArgs w) {
     return;
   }
   const int64_t across = (w.I + TURN - 1) / TURN, m0 = t / across * TURN, c0 = t % across * TURN;
-  for (int g = threadIdx.x; g < TURN * TURN / 4; g += TURN_THREADS) {
-    const int m = g / (TURN / 4), c = (g % (TURN / 4)) * 4;
-    uint2 dg = make_uint2(0, 0), du = make_uint2(0, 0);
-    if (m0 + m < w.M && c0 + c < w.I) {
-      const uint2 dh = *reinterpret_cast<const uint2*>(w.grad + (m0 + m) * w.ld_grad + c0 + c);
-      const uint16_t* both = w.both + (m0 + m) * w.ld_both + c0 + c;
-      const uint2 g2 = *reinterpret_cast<const uint2*>(both), u2 = *reinterpret_cast<const uint2*>(both + w.I);
-      const float h[4] = {low(dh.x), high(dh.x), low(dh.y), high(dh.y)};
-      const float gate[4] = {low(g2.x), high(g2.x), low(g2.y), high(g2.y)};
-      const float up[4] = {low(u2.x), high(u2.x), low(u2.y), high(u2.y)};
-      float x[4], y[4];
-      with_activation(w.act, [&](auto act) {
+  const int m = threadIdx.x / (TURN / 4), c = threadIdx.x % (TURN / 4) * 4;
+  uint2 dh[TURN_STEPS], g2[TURN_STEPS], u2[TURN_STEPS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float f, df;
-          activation_and_slope<act()>(gate[e], f, df);
-          x[e] = h[e] * up[e] * df;
-          y[e] = h[e] * f;
-        }
-      });
-      dg = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
-      du = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
-      if (w.d) {
-        uint16_t* d = w.d + (m0 + m) * 2 * w.I + c0 + c;
+  for (int i = 0; i < TURN_STEPS; ++i) {
+    const int64_t row = m0 + m + i * TURN_ROWS;
+    dh[i] = g2[i] = u2[i] = make_uint2(0, 0);  // past the rows: zeros, which give zeros
+    if (row < w.M && c0 + c < w.I) {
+      const uint16_t* both = w.both + row * w.ld_both + c0 + c;
+      dh[i] = *reinterpret_cast<const uint2*>(w.grad + row * w.ld_grad + c0 + c);
+      g2[i] = *reinterpret_cast<const uint2*>(both);
+      u2[i] = *reinterpret_cast<const uint2*>(both + w.I);
+    }
+  }
+  with_activation(w.act, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < TURN_STEPS; ++i) {
+      const int64_t row = m0 + m + i * TURN_ROWS;
+      const float h[4] = {low(dh[i].x), high(dh[i].x), low(dh[i].y), high(dh[i].y)};
+      const float gate[4] = {low(g2[i].x), high(g2[i].x), low(g2[i].y), high(g2[i].y)};
+      const float up[4] = {low(u2[i].x), high(u2[i].x), low(u2[i].y), high(u2[i].y)};
+      float x[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f, df;
+        activation_and_slope<act()>(gate[e], f, df);
+        x[e] = h[e] * up[e] * df;
+        y[e] = h[e] * f;
+      }
+      const uint2 dg = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+      const uint2 du = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+      if (w.d && row < w.M && c0 + c < w.I) {
+        uint16_t* d = w.d + row * 2 * w.I + c0 + c;
         *reinterpret_cast<uint2*>(d) = dg;
         *reinterpret_cast<uint2*>(d + w.I) = du;
       }
+      if (w.d_turned) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(tiles[0] + (m + i * TURN_ROWS) * TURN_PITCH + c);
+        p[0] = dg.x, p[1] = dg.y;
+        p = reinterpret_cast<uint32_t*>(tiles[1] + (m + i * TURN_ROWS) * TURN_PITCH + c);
+        p[0] = du.x, p[1] = du.y;
+      }
     }
-    if (w.d_turned) {
-      uint32_t* p = reinterpret_cast<uint32_t*>(tiles[0] + m * TURN_PITCH + c);
-      p[0] = dg.x, p[1] = dg.y;
-      p = reinterpret_cast<uint32_t*>(tiles[1] + m * TURN_PITCH + c);
-      p[0] = du.x, p[1] = du.y;
-    }
-  }
+  });
   if (!w.d_turned) return;
   __syncthreads();
   write_turned(tiles[0], w.d_turned, c0, w.I, m0, w.pitch, w.pitch);

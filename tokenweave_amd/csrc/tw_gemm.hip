@@ -563,12 +563,13 @@ __device__ __forceinline__ uint32_t tile_pack2(float lo, float hi) {
 
 // One phase: acc += fb x fa, and between the MFMAs the next phase's fragments (na, nb from pa, pb)
 // and this half's share of the loads of the slab D ahead.
-template <int TM, int TN, TileRows ROWS, bool FIRST, int HALF>
+template <int TM, int TN, TileRows ROWS, bool FIRST, int HALF, bool GATED>
 __device__ __forceinline__ void tile_phase(f32x4_t (&acc)[TM][TN], const bf16x8_t (&fa)[TM], const bf16x8_t (&fb)[TN],
                                            bf16x8_t (&na)[TM], bf16x8_t (&nb)[TN], const lds_u8_t* pa,
                                            const lds_u8_t* pb, __amdgpu_buffer_rsrc_t da,
-                                           __amdgpu_buffer_rsrc_t db, const uint32_t (&va)[TM],
-                                           const uint32_t (&vb)[TN], lds_u8_t* sa, lds_u8_t* sb, uint32_t koff) {
+                                           __amdgpu_buffer_rsrc_t db, __amdgpu_buffer_rsrc_t du,
+                                           const uint32_t (&va)[TM], const uint32_t (&vb)[TN], lds_u8_t* sa,
+                                           lds_u8_t* sb, uint32_t koff) {
   using S = TileShape<TM, TN, ROWS>;
 #pragma unroll
   for (int n = 0; n < S::SLOTS; ++n) {
@@ -578,7 +579,7 @@ __device__ __forceinline__ void tile_phase(f32x4_t (&acc)[TM][TN], const bf16x8_
     __builtin_amdgcn_sched_barrier(0);
     if (n % S::READ_STEP == 0 && n / S::READ_STEP < S::L) {
       const int r = n / S::READ_STEP;
-      if (r < TN) nb[r] = *(lds_frag_t*)(pb + (r >> 1) * 4096 + (r & 1) * 512);
+      if (r < TN) nb[r] = *(lds_frag_t*)(pb + (GATED ? r * 2048 : (r >> 1) * 4096 + (r & 1) * 512));
       else na[r - TN] = *(lds_frag_t*)(pa + (r - TN) * 2048);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -589,7 +590,8 @@ __device__ __forceinline__ void tile_phase(f32x4_t (&acc)[TM][TN], const bf16x8_
     }
     if (slot >= S::B0 && (slot - S::B0) % S::B_STEP == 0 && (slot - S::B0) / S::B_STEP < S::LB) {
       const int l = (slot - S::B0) / S::B_STEP;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(sb + l * 1024), 16, vb[l], koff, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(GATED && (l & 2) ? du : db, (lds_void_t*)(sb + l * 1024), 16, vb[l],
+                                               koff, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -738,9 +740,10 @@ __device__ __forceinline__ TilePlace tile_place(int t, int num_tiles, int tiles_
 // 55.0 -> 51.8; K = 7392 (both from memory), 200 rows 61 -> 50, 256: 72 -> 57, 512: 85 -> 77, 640: 122 -> 96.  On one
 // set again and again the units are busy 4 % fewer cycles at 1000 rows and 3 to 7 % more at 200.
 //
-// GATED: N counts columns of out, BN / 2 a tile.  Row x of b's panel is a gate row where bit 2 of x is clear and an up
-// row where it is set, of column 32 (x / 64) + 8 (x / 8 % 4) + 4 (x / 32 % 2) + x % 4 of the tile: a lane's accumulators
-// are then eight adjacent columns of both.
+// GATED: N counts columns of out, BN / 2 a tile.  Sixteen rows of b's panel are gate rows, the next sixteen up rows: a
+// tile of columns and a wave's load have one kind, which has its own descriptor.  Row x of the panel is of column
+// 32 (x / 64) + 8 (x / 4 % 4) + 4 (x / 32 % 2) + x % 4 of the tile, so that a lane's accumulators are eight adjacent
+// columns of both.  The panel is swizzled as a's.
 template <int TM, int TN, TileRows ROWS, bool GATED = false>
 __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nt_tile_kernel(
     GemmBatch batch, int count, int M, int N, int K, int64_t ldc, int tiles_m, int tiles_n, int wide_store,
@@ -763,7 +766,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   const int num_tiles = count * tiles_m * tiles_n;
 
   // Reader: the two 32-wide halves of a slab.
-  const uint32_t row_a = (wm * 16 * TM + r16) * 128, row_b = (wn * 16 * TN + (r16 >> 2) * 8 + (r16 & 3)) * 128;
+  const uint32_t row_a = (wm * 16 * TM + r16) * 128, row_b = (wn * 16 * TN + (GATED ? r16 : (r16 >> 2) * 8 + (r16 & 3))) * 128;
   const uint32_t chunk0 = (quad ^ (r16 >> 1)) << 4, chunk1 = ((4 + quad) ^ (r16 >> 1)) << 4;
   const lds_u8_t *a0 = lds_a + row_a + chunk0, *a1 = lds_a + row_a + chunk1;
   const lds_u8_t *b0 = lds_b + row_b + chunk0, *b1 = lds_b + row_b + chunk1;
@@ -781,11 +784,12 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
       va[l] = c < (chunks) ? (uint32_t)((blk * 8 + (lane >> 3)) * K + c * 8) * 2u : TILE_OUT_OF_RANGE;       \
     }                                                                                                        \
     _Pragma("unroll") for (int l = 0; l < LB; ++l) {                                                         \
-      const int blk = wave * LB + l, c = (lane & 7) ^ (((lane >> 4) & 1) | ((blk & 3) << 1));                \
-      const uint32_t row = !GATED ? blk * 8 + (lane >> 3)                                                    \
-                                  : (uint32_t)((lane >> 5) * N + 32 * (blk >> 3) + 8 * (blk & 3) +           \
-                                               4 * ((blk >> 2) & 1) + ((lane >> 3) & 3));                    \
-      vb[l] = c < (chunks) ? (row * (uint32_t)K + c * 8) * 2u : TILE_OUT_OF_RANGE;                           \
+      const int blk = wave * LB + l;                                                                         \
+      const int c = (lane & 7) ^ (GATED ? ((blk & 1) << 2) | (lane >> 4) : ((lane >> 4) & 1) | ((blk & 3) << 1)); \
+      const int row = !GATED ? blk * 8 + (lane >> 3)                                                         \
+                             : 32 * (blk >> 3) + 16 * (blk & 1) + 8 * (lane >> 5) + 4 * ((blk >> 2) & 1) +   \
+                                   ((lane >> 3) & 3);                                                        \
+      vb[l] = c < (chunks) ? (uint32_t)(row * K + c * 8) * 2u : TILE_OUT_OF_RANGE;                           \
     }                                                                                                        \
   } while (0)
   // kLines: the same for line `line` of every row: lane position x holds the line's chunk x ^ key ^ flip, so
@@ -810,7 +814,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   // its loads ask memory for nothing.  (The hardware compares with the extent less the slab's offset,
   // which for an extent of 0 must not go below 0.)
   int lt = blockIdx.x, lk = 0;
-  __amdgpu_buffer_rsrc_t da, db;
+  __amdgpu_buffer_rsrc_t da, db, du;  // du: b's up rows
 #define TW_TILE_DESCRIPTORS()                                                                                \
   do {                                                                                                       \
     const bool in = lt < num_tiles;                                                                          \
@@ -822,9 +826,12 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
                                            in ? (uint32_t)min(M - p.m0, S::BM) * (uint32_t)K * 2u + AHEAD : 0u, \
                                            0x00020000);                                                      \
     db = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pb) - (int)AHEAD / 2, 0,                    \
-                                           in ? (uint32_t)(GATED ? 2 * N - p.n0 / 2 : min(N - p.n0, S::BN)) * \
-                                                        (uint32_t)K * 2u + AHEAD : 0u,                       \
+                                           in ? (uint32_t)(GATED ? min(N - p.n0 / 2, S::BN / 2)              \
+                                                                 : min(N - p.n0, S::BN)) * (uint32_t)K * 2u + AHEAD : 0u, \
                                            0x00020000);                                                      \
+    du = !GATED ? db : __builtin_amdgcn_make_buffer_rsrc(                                                    \
+        const_cast<uint16_t*>(pb) + (size_t)N * K, 0,                                                        \
+        in ? (uint32_t)min(N - p.n0 / 2, S::BN / 2) * (uint32_t)K * 2u : 0u, 0x00020000);                     \
   } while (0)
 #define TW_TILE_ADVANCE()                                                                                    \
   do {                                                                                                       \
@@ -851,7 +858,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
       __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_void_t*)(wa + s * PA + l * 1024), 16, va[l], lk * 128u, 0, 0);
 #pragma unroll
     for (int l = 0; l < LB; ++l)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(wb + s * PB + l * 1024), 16, vb[l], lk * 128u, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(GATED && (l & 2) ? du : db, (lds_void_t*)(wb + s * PB + l * 1024), 16,
+                                               vb[l], lk * 128u, 0, 0);
     TW_TILE_ADVANCE();
   }
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((D - S::NEED) * S::L) : "memory");
@@ -880,25 +888,25 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   do {                                                                                                       \
     const lds_u8_t *const pb = TW_AT(use_b, b0, next_b0, PB, S::SB), *const pa = TW_AT(use_a, a0, next_a0, PA, S::SA); \
     _Pragma("unroll") for (int r = 0; r < TN; ++r)                                                           \
-        fb0[r] = *(lds_frag_t*)(pb + (r >> 1) * 4096 + (r & 1) * 512);                                       \
+        fb0[r] = *(lds_frag_t*)(pb + (GATED ? r * 2048 : (r >> 1) * 4096 + (r & 1) * 512));                  \
     _Pragma("unroll") for (int r = 0; r < TM; ++r) fa0[r] = *(lds_frag_t*)(pa + r * 2048);                   \
   } while (0)
   if (S::LINES) place_reader(blockIdx.x);
   TW_TILE_READ_FIRST();
 #define TW_TILE_SLAB(FIRST, AFTER_STORE)                                                                         \
   do {                                                                                                       \
-    tile_phase<TM, TN, ROWS, FIRST, 0>(acc, fa0, fb0, fa1, fb1, TW_AT(use_a, a1, next_a1, PA, S::SA),          \
+    tile_phase<TM, TN, ROWS, FIRST, 0, GATED>(acc, fa0, fb0, fa1, fb1, TW_AT(use_a, a1, next_a1, PA, S::SA),   \
                                        TW_AT(use_b, b1, next_b1, PB, S::SB), \
-                                       da, db, va, vb, wa + fill_a, wb + fill_b, lk * 128u);                 \
+                                       da, db, du, va, vb, wa + fill_a, wb + fill_b, lk * 128u);                 \
     if (AFTER_STORE)                                                                                         \
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT + STORES) : "memory");   \
     else                                                                                                     \
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT) : "memory");            \
     TW_RING(use_a, PA, S::SA);                                                                               \
     TW_RING(use_b, PB, S::SB);                                                                               \
-    tile_phase<TM, TN, ROWS, false, 1>(acc, fa1, fb1, fa0, fb0, TW_AT(use_a, a0, next_a0, PA, S::SA),          \
+    tile_phase<TM, TN, ROWS, false, 1, GATED>(acc, fa1, fb1, fa0, fb0, TW_AT(use_a, a0, next_a0, PA, S::SA),   \
                                        TW_AT(use_b, b0, next_b0, PB, S::SB), \
-                                       da, db, va, vb, wa + fill_a, wb + fill_b, lk * 128u);                 \
+                                       da, db, du, va, vb, wa + fill_a, wb + fill_b, lk * 128u);                 \
     TW_TILE_ADVANCE();                                                                                       \
     TW_RING(fill_a, PA, S::SA);                                                                              \
     TW_RING(fill_b, PB, S::SB);                                                                              \
@@ -1213,8 +1221,7 @@ static int launch_tile_for(const GemmBatch& batch, int count, int64_t M, int64_t
   return launch_tile_shape(t.tm, t.tn, batch, count, M, N, K, ldc, max_cus, hs);
 }
 
-// act(a b[:I]^T) * (a b[I:]^T).  The tile kernel reaches both halves of b through one descriptor: weights of less than
-// 2 GiB.  Larger ones take the K-split kernel whatever the rows, which has a descriptor for each half's rows of a tile.
+// act(a b[:I]^T) * (a b[I:]^T).
 static int launch_gated_tile(const GemmBatch& batch, int64_t M, int64_t I, int64_t K, int64_t ldc, int max_cus,
                              const GatedOut& gated, hipStream_t hs) {
   int cus = max_cus > 0 ? max_cus : device_compute_units();
@@ -1305,7 +1312,7 @@ int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, 
   const GatedOut gated = {static_cast<uint16_t*>(both), ld_both, act};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
   int rc;
-  if (tile_kernel_fits(M, 2 * I, K, ldc) && 2 * I * K < (int64_t)1 << 30)
+  if (tile_kernel_fits(M, 2 * I, K, ldc))
     rc = launch_gated_tile(batch, M, I, K, ldc, max_cus, gated, hs);
   else
     rc = launch_ksplit_for<true>(batch, 1, M, I, K, ldc, max_cus, hs, gated);
