@@ -80,6 +80,10 @@ int run_gemm_bf16_nt_partials(void* const* outs, const void* const* as, const vo
 int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, int64_t M, int64_t I, int64_t K,
                            int64_t ldc, int64_t ld_both, int act, int max_cus, void* stream);
 
+// out[M, N] = a[M, K] b[rows, N]; rows <= K end in the last slab of 64, a's columns from `rows` on are zeros.
+int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t rows, int max_cus,
+                     void* stream);
+
 int64_t gated_backward_workspace(int64_t M, int64_t I, int64_t K, bool want_a, bool want_b);
 
 int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad_out, int64_t ld_grad, const void* a,

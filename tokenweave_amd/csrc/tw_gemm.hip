@@ -971,6 +971,223 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
 #endif
 }
 
+// ---------------------------------------------------------------------------
+// "NN" product: out[M, N] = a[M, K] b[K, N], b read as it lies in memory.  The tile kernel above with another panel for b:
+// a slab is 64 rows of 64 TN bytes, brought into LDS as it is; its fragments come out turned, by LDS reads that hand lane
+// i of 16 the i-th column of four rows (lane i asks for eight bytes of row i / 4, and is given four values of one
+// column).  16-byte chunk c of row k lies at c ^ 2 f, f = k % 4 + 4 (k / 8 % 2), or k % 4 where a row is no 2^n bytes: the
+// rows that a read touches are spread over the banks.  A tile of columns is sixteen adjacent ones, so that a read takes
+// 32 bytes of a row; lanes then hold four adjacent columns of every tile, and exchange halves of a pair of tiles before
+// they store eight.
+//
+// 4096 x 8192 x 7168: 336 us, the "NT" kernel 326 on a b turned beforehand, which takes 50.  (With a turned on the way as
+// well the LDS reads are the bound: 388 us; so a^T b has a laid out turned where it is made.)
+// ---------------------------------------------------------------------------
+[[maybe_unused]] __host__ __device__ constexpr int nn_key(int T, int row) {
+  return T == 4 || T == 8 ? (row & 3) | ((row >> 3) & 1) << 2 : row & 3;
+}
+
+#ifdef __HIP_DEVICE_COMPILE__
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t lds_turn_t;
+__device__ __forceinline__ bf16x8_t nn_read(const lds_u8_t* p, int row_bytes) {
+  const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_turn_t*)p);
+  const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_turn_t*)(p + 4 * row_bytes));
+  return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The wave's accumulators: lanes 16 q .. 16 q + 15 hold columns 4 q .. 4 q + 3 of every tile of columns.  Of a pair of
+// tiles, odd groups of lanes give their columns of the first to the even group before them and get that group's of
+// the second: eight adjacent columns each.  N % 8 == 0.
+template <int TM, int TN, bool WIDE>
+__device__ __forceinline__ void nn_store(const f32x4_t (&acc)[TM][TN], __amdgpu_buffer_rsrc_t dc, uint32_t row_off,
+                                             uint32_t row_step, int n, int N) {
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const auto x = __builtin_amdgcn_permlane16_swap(tile_pack2(acc[i][j][0], acc[i][j][1]),
+                                                      tile_pack2(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
+      const auto y = __builtin_amdgcn_permlane16_swap(tile_pack2(acc[i][j][2], acc[i][j][3]),
+                                                      tile_pack2(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
+      const uint32_t off = n + j * 16 < N ? row_off + (uint32_t)i * row_step + (uint32_t)j * 32u : TILE_OUT_OF_RANGE;
+      if (WIDE) {
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{x[0], y[0], x[1], y[1]}, dc, off, 0, kStoreThrough);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{x[0], y[0]}, dc, off, 0, kStoreThrough);
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{x[1], y[1]}, dc, off + 8u, 0, kStoreThrough);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// (__restrict__: the panels read and those being filled are others.  Without it every turned read waits for all loads.)
+template <int TM, int TN, bool FIRST, int HALF>
+__device__ __forceinline__ void nn_phase(f32x4_t (&acc)[TM][TN], const bf16x8_t (&fa)[TM], const bf16x8_t (&fb)[TN],
+                                             bf16x8_t (&na)[TM], bf16x8_t (&nb)[TN], const lds_u8_t* __restrict__ pa,
+                                             const lds_u8_t* __restrict__ pb, uint32_t off_a,
+                                             const uint32_t (&off_b)[TN], __amdgpu_buffer_rsrc_t da,
+                                             __amdgpu_buffer_rsrc_t db, const uint32_t (&va)[TM],
+                                             const uint32_t (&vb)[TN], lds_u8_t* __restrict__ sa,
+                                             lds_u8_t* __restrict__ sb, uint32_t koff) {
+  using S = TileShape<TM, TN>;
+#pragma unroll
+  for (int n = 0; n < S::SLOTS; ++n) {
+    const int i = n / TN, j = n % TN, slot = n + HALF * S::SLOTS;
+    if (FIRST) tile_mfma_first(acc[i][j], fb[j], fa[i]);
+    else tile_mfma(acc[i][j], fb[j], fa[i]);
+    __builtin_amdgcn_sched_barrier(0);
+    if (n % S::READ_STEP == 0 && n / S::READ_STEP < S::L) {
+      const int r = n / S::READ_STEP;
+      if (r < TN) nb[r] = nn_read(pb + off_b[r] + (1 - HALF) * 32 * 64 * TN, 64 * TN);
+      else na[r - TN] = *(lds_frag_t*)(pa + off_a + (r - TN) * 2048);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (slot >= S::A0 && (slot - S::A0) % S::A_STEP == 0 && (slot - S::A0) / S::A_STEP < S::LA) {
+      const int l = (slot - S::A0) / S::A_STEP;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_void_t*)(sa + l * 1024), 16, va[l], koff, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (slot >= S::B0 && (slot - S::B0) % S::B_STEP == 0 && (slot - S::B0) / S::B_STEP < S::LB) {
+      const int l = (slot - S::B0) / S::B_STEP;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(sb + l * 1024), 16, vb[l], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+#endif
+
+constexpr int64_t NN_MAX_N = 1 << 23;  // 64 rows of b span less than 2 GiB
+
+// rows: b's, at most K; a's columns behind as many are zeros.  TAIL: K % 64 != 0, a's chunks past K must arrive as zeros.
+template <int TM, int TN, bool TAIL>
+__global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nn_kernel(
+    uint16_t* out, const uint16_t* a, const uint16_t* b, int M, int N, int K, int rows, int tiles_m, int tiles_n,
+    int wide_store) {
+#ifdef __HIP_DEVICE_COMPILE__
+  using S = TileShape<TM, TN>;
+  static_assert(TN % 2 == 0, "whole groups of eight chunks a row");
+  constexpr int LA = S::LA, LB = S::LB, PA = S::PA, PB = S::PB, D = S::D;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds_tile[];
+  lds_u8_t* const lds_a = (lds_u8_t*)lds_tile;
+  lds_u8_t* const lds_b = lds_a + S::SA * PA;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1, r16 = lane & 15, quad = lane >> 4;
+  const int nk = (K + BK - 1) / BK, tail_chunks = TAIL ? (K % BK) / 8 : 8;
+  const int num_tiles = tiles_m * tiles_n;
+
+  // Reader: a as the tile kernel; of b row 8 quad + r16 / 4 (and the one four below) of each half of a slab
+  const uint32_t row_a = (wm * 16 * TM + r16) * 128;
+  const uint32_t off0 = row_a + ((quad ^ (r16 >> 1)) << 4), off1 = row_a + (((4 + quad) ^ (r16 >> 1)) << 4);
+  const int row_b = 8 * quad + (r16 >> 2);
+  uint32_t off_b[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+    off_b[j] = row_b * 64 * TN + (((wn * 2 * TN + 2 * j) ^ (2 * nn_key(TN, row_b))) << 4) + (r16 & 3) * 8;
+
+  // Loader
+  lds_u8_t* const wa = lds_a + wave * LA * 1024;
+  lds_u8_t* const wb = lds_b + wave * LB * 1024;
+  uint32_t va[LA], vb[LB];
+  auto offsets = [&](int chunks) {
+#pragma unroll
+    for (int l = 0; l < LA; ++l) {
+      const int blk = wave * LA + l, c = (lane & 7) ^ (((blk & 1) << 2) | (lane >> 4));
+      va[l] = c < chunks ? (uint32_t)((blk * 8 + (lane >> 3)) * K + c * 8) * 2u : TILE_OUT_OF_RANGE;
+    }
+  };
+#pragma unroll
+  for (int l = 0; l < LB; ++l) {
+    const int place = (wave * LB + l) * 64 + lane, row = place / (4 * TN);
+    vb[l] = (uint32_t)row * (uint32_t)N * 2u + (uint32_t)(((place % (4 * TN)) ^ (2 * nn_key(TN, row))) << 4);
+  }
+  // Load cursor: slab lk of tile lt; past the last tile descriptors are empty.
+  int lt = blockIdx.x, lk = 0;
+  __amdgpu_buffer_rsrc_t da, db;
+  TilePlace lp;
+  auto place = [&]() {
+    lp = tile_place<TM, TN>(lt < num_tiles ? lt : 0, num_tiles, tiles_m, tiles_n);
+    da = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a) + (size_t)lp.m0 * K, 0,
+                                           lt < num_tiles ? (uint32_t)min(M - lp.m0, S::BM) * (uint32_t)K * 2u : 0u,
+                                           0x00020000);
+  };
+  // columns n0 and up of b's rows 64 lk and up: the descriptor ends with the last row's part of the tile
+  auto slab_of_b = [&]() {
+    const int last = min(rows - lk * BK, BK) - 1;
+    db = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(b) + (size_t)lk * BK * N + lp.n0, 0,
+        lt < num_tiles ? ((uint32_t)last * (uint32_t)N + (uint32_t)min(N - lp.n0, S::BN)) * 2u : 0u, 0x00020000);
+  };
+  auto advance = [&]() {
+    if (lt < num_tiles) ++lk;
+    if (lk == nk) {
+      lk = 0;
+      lt += gridDim.x;
+      place();
+      if (TAIL) offsets(nk == 1 ? tail_chunks : 8);
+    } else if (TAIL && lk == nk - 1) {
+      offsets(tail_chunks);
+    }
+    slab_of_b();
+  };
+  place();
+  slab_of_b();
+  offsets(TAIL && nk == 1 ? tail_chunks : 8);
+#pragma unroll
+  for (int s = 0; s < D; ++s) {
+#pragma unroll
+    for (int l = 0; l < LA; ++l)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_void_t*)(wa + s * PA + l * 1024), 16, va[l], lk * 128u, 0, 0);
+#pragma unroll
+    for (int l = 0; l < LB; ++l)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(wb + s * PB + l * 1024), 16, vb[l], 0, 0, 0);
+    advance();
+  }
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((D - S::NEED) * S::L) : "memory");
+  f32x4_t acc[TM][TN];
+  bf16x8_t fa0[TM], fb0[TN], fa1[TM], fb1[TN];
+  uint32_t use_a = 0, use_b = 0, fill_a = (D % S::SA) * PA, fill_b = (D % S::SB) * PB;
+#pragma unroll
+  for (int r = 0; r < TN; ++r) fb0[r] = nn_read(lds_b + off_b[r], 64 * TN);
+#pragma unroll
+  for (int r = 0; r < TM; ++r) fa0[r] = *(lds_frag_t*)(lds_a + off0 + r * 2048);
+#define TW_RING(x, panel, n) x = (x) + (panel) == (n) * (panel) ? 0u : (x) + (panel)
+#define TW_NN_SLAB(FIRST, AFTER_STORE)                                                                         \
+  do {                                                                                                         \
+    nn_phase<TM, TN, FIRST, 0>(acc, fa0, fb0, fa1, fb1, lds_a + use_a, lds_b + use_b, off1, off_b, da, db, va, vb, \
+                               wa + fill_a, wb + fill_b, lk * 128u);                                           \
+    if (AFTER_STORE)                                                                                           \
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT + S::STORES) : "memory");   \
+    else                                                                                                       \
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::IN_FLIGHT) : "memory");               \
+    TW_RING(use_a, PA, S::SA);                                                                                 \
+    TW_RING(use_b, PB, S::SB);                                                                                 \
+    nn_phase<TM, TN, false, 1>(acc, fa1, fb1, fa0, fb0, lds_a + use_a, lds_b + use_b, off0, off_b, da, db, va, vb, \
+                               wa + fill_a, wb + fill_b, lk * 128u);                                           \
+    advance();                                                                                                 \
+    TW_RING(fill_a, PA, S::SA);                                                                                \
+    TW_RING(fill_b, PB, S::SB);                                                                                \
+  } while (0)
+  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+    TW_NN_SLAB(true, t != (int)blockIdx.x);
+    for (int kt = 1; kt < nk; ++kt) TW_NN_SLAB(false, false);
+    const TilePlace p = tile_place<TM, TN>(t, num_tiles, tiles_m, tiles_n);
+    const __amdgpu_buffer_rsrc_t dc = __builtin_amdgcn_make_buffer_rsrc(
+        out + (size_t)p.m0 * N + p.n0, 0, (uint32_t)min(M - p.m0, S::BM) * (uint32_t)N * 2u, 0x00020000);
+    const int col = wn * 16 * TN + (quad & 1) * 16 + (quad >> 1) * 8;
+    const uint32_t row_off = (uint32_t)((wm * 16 * TM + r16) * N + col) * 2u, row_step = (uint32_t)N * 32u;
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMA's result is written
+    if (wide_store) nn_store<TM, TN, true>(acc, dc, row_off, row_step, p.n0 + col, N);
+    else nn_store<TM, TN, false>(acc, dc, row_off, row_step, p.n0 + col, N);
+  }
+#undef TW_NN_SLAB
+#undef TW_RING
+#endif
+}
+
 // More than 64 KiB of dynamic LDS must be allowed once per function and device.
 static int allow_lds(const void* kernel, std::atomic<bool>* ok, int max_devices, int bytes) {
   int dev = 0;
@@ -1219,6 +1436,45 @@ static int launch_tile_for(const GemmBatch& batch, int count, int64_t M, int64_t
   if (cus <= 0) cus = 256;
   const TileChoice& t = pick_tile(M, N, count, cus);
   return launch_tile_shape(t.tm, t.tn, batch, count, M, N, K, ldc, max_cus, hs);
+}
+
+template <int TM, int TN, bool TAIL>
+static int launch_nn(uint16_t* out, const uint16_t* a, const uint16_t* b, int64_t M, int64_t N, int64_t K, int64_t rows,
+                     int units, hipStream_t hs) {
+  using S = TileShape<TM, TN>;
+  static std::atomic<bool> lds_ok[kMaxDevices];
+  const auto kernel = gemm_bf16_nn_kernel<TM, TN, TAIL>;
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, S::LDS)) return rc;
+  const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + S::BN - 1) / S::BN);
+  const int64_t grid = std::min<int64_t>((int64_t)tiles_m * tiles_n, units);
+  const int wide_store = reinterpret_cast<uintptr_t>(out) % 16 == 0;  // N is a multiple of 8
+  launch_kernel(kernel, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, out, a, b, (int)M, (int)N, (int)K, (int)rows,
+                tiles_m, tiles_n, wide_store);
+  return TW_OK;
+}
+
+// out[M, N] = a[M, K] b[rows, N], everything contiguous, K and N multiples of 8, rows <= K, the last of them in the last
+// slab of 64, and a's columns from `rows` on zeros; a 16-byte aligned, out and b 8.
+int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t rows, int max_cus,
+                     void* stream) {
+  const char* what = "gemm_bf16_nn";
+  if (N > NN_MAX_N || K > TILE_MAX_K || N > TILE_MAX_LDC)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: an inner dimension of %lld or rows of %lld values are too long", what,
+                     (long long)K, (long long)N);
+  const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
+  const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
+  const TileChoice& t = pick_tile(M, N, 1, units);
+  uint16_t* const o = static_cast<uint16_t*>(out);
+  const uint16_t *const x = static_cast<const uint16_t*>(a), *const y = static_cast<const uint16_t*>(b);
+  const hipStream_t hs = static_cast<hipStream_t>(stream);
+  int rc = TW_OK;
+#define TW_NN_TILE(TM, TN, COST)                                                               \
+  if (t.tm == TM && t.tn == TN)                                                                \
+    rc = K % BK == 0 ? launch_nn<TM, TN, false>(o, x, y, M, N, K, rows, units, hs)             \
+                     : launch_nn<TM, TN, true>(o, x, y, M, N, K, rows, units, hs);
+  TW_TILES(TW_NN_TILE)
+#undef TW_NN_TILE
+  return rc ? rc : finish_launch(what);
 }
 
 // act(a b[:I]^T) * (a b[I:]^T).
