@@ -92,7 +92,8 @@ def test_products_that_are_large_or_no_numbers():
 
 
 @pytest.mark.parametrize("M,inner,K", [(1, 4, 8), (3, 36, 72), (64, 64, 64), (65, 100, 136), (129, 100, 72), (257, 704, 520),
-                                       (1001, 260, 1024)])
+                                       (1001, 260, 1024), (7, 704, 1024), (64, 1376, 520), (300, 100, 2048),
+                                       (64, 2100, 264), (2, 2048, 128), (4000, 36, 72), (130, 4100, 136)])
 @pytest.mark.parametrize("kind", R.ACTIVATIONS)
 def test_gradients(M, inner, K, kind):
     x, w, both, out = check_forward(M, inner, K, kind)

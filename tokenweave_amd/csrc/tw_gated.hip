@@ -128,7 +128,11 @@ int check_shape(const char* what, int64_t M, int64_t I, int64_t K) {
 
 int64_t gated_backward_workspace(int64_t M, int64_t I, int64_t K, bool want_a, bool want_b) {
   if (int rc = check_shape("gated_gemm_bf16_nt_backward_workspace", M, I, K)) return rc;
-  return 4 * I * ((want_a ? turned_pitch(M) : 0) + (want_b ? turned_pitch(M) : 0));
+  // D, D turned, and the partial sums of one product after the other
+  const int64_t pitch = turned_pitch(M);
+  const int64_t of_a = want_a && M ? gemm_bf16_nn_workspace(M, K, 2 * I) : 0;
+  const int64_t of_b = want_b && M ? gemm_bf16_nn_workspace(2 * I, K, pitch) : 0;
+  return 4 * I * ((want_a ? pitch : 0) + (want_b ? pitch : 0)) + std::max(of_a, of_b);
 }
 
 int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad_out, int64_t ld_grad, const void* a,
@@ -166,7 +170,8 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   w.both = static_cast<const uint16_t*>(both);
   w.pitch = turned_pitch(M);
   if (grad_a) w.d = ws, ws += 2 * I * w.pitch;
-  if (grad_b) w.d_turned = ws;
+  if (grad_b) w.d_turned = ws, ws += 2 * I * w.pitch;
+  float* const sums = reinterpret_cast<float*>(ws);
   w.ld_grad = ld_grad, w.ld_both = ld_both;
   w.M = (int)M, w.I = (int)I, w.act = act;
   w.across = (int)((I + TURN - 1) / TURN);
@@ -175,8 +180,8 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   launch_kernel(gated_grad_kernel, dim3((unsigned)grid), dim3(GRAD_THREADS), 0, hs, w);
   if (int rc = finish_launch(what)) return rc;
   if (grad_a)
-    if (int rc = run_gemm_bf16_nn(grad_a, w.d, b, M, K, 2 * I, 2 * I, max_cus, stream)) return rc;
-  if (grad_b) return run_gemm_bf16_nn(grad_b, w.d_turned, a, 2 * I, K, w.pitch, M, max_cus, stream);
+    if (int rc = run_gemm_bf16_nn(grad_a, w.d, b, M, K, 2 * I, 2 * I, max_cus, sums, stream)) return rc;
+  if (grad_b) return run_gemm_bf16_nn(grad_b, w.d_turned, a, 2 * I, K, w.pitch, M, max_cus, sums, stream);
   return TW_OK;
 }
 

@@ -1062,10 +1062,13 @@ __device__ __forceinline__ void nn_phase(f32x4_t (&acc)[TM][TN], const bf16x8_t 
 constexpr int64_t NN_MAX_N = 1 << 23;  // 64 rows of b span less than 2 GiB
 
 // rows: b's, at most K; a's columns behind as many are zeros.  TAIL: K % 64 != 0, a's chunks past K must arrive as zeros.
-template <int TM, int TN, bool TAIL>
+//
+// SPLIT: few tiles.  A tile's slabs are dealt out to `parts` workgroups, `per` each, whose fp32 sums go to sums[part][M][N];
+// nn_sum_kernel adds them in order.
+template <int TM, int TN, bool TAIL, bool SPLIT>
 __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nn_kernel(
     uint16_t* out, const uint16_t* a, const uint16_t* b, int M, int N, int K, int rows, int tiles_m, int tiles_n,
-    int wide_store) {
+    int wide_store, float* sums, int parts, int per) {
 #ifdef __HIP_DEVICE_COMPILE__
   using S = TileShape<TM, TN>;
   static_assert(TN % 2 == 0, "whole groups of eight chunks a row");
@@ -1077,7 +1080,10 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1, r16 = lane & 15, quad = lane >> 4;
   const int nk = (K + BK - 1) / BK, tail_chunks = TAIL ? (K % BK) / 8 : 8;
-  const int num_tiles = tiles_m * tiles_n;
+  const int whole = tiles_m * tiles_n, num_tiles = SPLIT ? whole * parts : whole;
+  auto tile_of = [&](int t) { return tile_place<TM, TN>(SPLIT ? t / parts : t, whole, tiles_m, tiles_n); };
+  auto first_slab = [&](int t) { return SPLIT ? t % parts * per : 0; };
+  auto slabs_of = [&](int first) { return SPLIT ? min(per, nk - first) : nk; };
 
   // Reader: a as the tile kernel; of b row 8 quad + r16 / 4 (and the one four below) of each half of a slab
   const uint32_t row_a = (wm * 16 * TM + r16) * 128;
@@ -1104,12 +1110,14 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     const int place = (wave * LB + l) * 64 + lane, row = place / (4 * TN);
     vb[l] = (uint32_t)row * (uint32_t)N * 2u + (uint32_t)(((place % (4 * TN)) ^ (2 * nn_key(TN, row))) << 4);
   }
-  // Load cursor: slab lk of tile lt; past the last tile descriptors are empty.
-  int lt = blockIdx.x, lk = 0;
+  // Load cursor: slab lk, before l_end, of tile lt; past the last tile it stays at slab 0 of empty descriptors.
+  int lt = blockIdx.x, lk = 0, l_end = nk;
   __amdgpu_buffer_rsrc_t da, db;
   TilePlace lp;
   auto place = [&]() {
-    lp = tile_place<TM, TN>(lt < num_tiles ? lt : 0, num_tiles, tiles_m, tiles_n);
+    lp = tile_of(lt < num_tiles ? lt : 0);
+    lk = lt < num_tiles ? first_slab(lt) : 0;
+    l_end = lk + slabs_of(lk);
     da = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a) + (size_t)lp.m0 * K, 0,
                                            lt < num_tiles ? (uint32_t)min(M - lp.m0, S::BM) * (uint32_t)K * 2u : 0u,
                                            0x00020000);
@@ -1123,11 +1131,10 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   };
   auto advance = [&]() {
     if (lt < num_tiles) ++lk;
-    if (lk == nk) {
-      lk = 0;
+    if (lk == l_end) {
       lt += gridDim.x;
       place();
-      if (TAIL) offsets(nk == 1 ? tail_chunks : 8);
+      if (TAIL) offsets(lk == nk - 1 ? tail_chunks : 8);
     } else if (TAIL && lk == nk - 1) {
       offsets(tail_chunks);
     }
@@ -1135,7 +1142,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   };
   place();
   slab_of_b();
-  offsets(TAIL && nk == 1 ? tail_chunks : 8);
+  offsets(TAIL && lk == nk - 1 ? tail_chunks : 8);
 #pragma unroll
   for (int s = 0; s < D; ++s) {
 #pragma unroll
@@ -1173,8 +1180,26 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   } while (0)
   for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
     TW_NN_SLAB(true, t != (int)blockIdx.x);
-    for (int kt = 1; kt < nk; ++kt) TW_NN_SLAB(false, false);
-    const TilePlace p = tile_place<TM, TN>(t, num_tiles, tiles_m, tiles_n);
+    const int slabs = slabs_of(first_slab(t));
+    for (int kt = 1; kt < slabs; ++kt) TW_NN_SLAB(false, false);
+    const TilePlace p = tile_of(t);
+    if constexpr (SPLIT) {
+      const __amdgpu_buffer_rsrc_t ds = __builtin_amdgcn_make_buffer_rsrc(
+          sums + ((size_t)(t % parts) * M + p.m0) * N + p.n0, 0, (uint32_t)min(M - p.m0, S::BM) * (uint32_t)N * 4u,
+          0x00020000);
+      asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMA's result is written
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int c = wn * 16 * TN + j * 16 + quad * 4;
+          const uint32_t off = (uint32_t)((wm * 16 * TM + i * 16 + r16) * N + c) * 4u;
+          const f32x4_t v = {acc_read(acc[i][j][0]), acc_read(acc[i][j][1]), acc_read(acc[i][j][2]), acc_read(acc[i][j][3])};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), ds,
+                                                 p.n0 + c < N ? off : TILE_OUT_OF_RANGE, 0, 0);
+        }
+      continue;
+    }
     const __amdgpu_buffer_rsrc_t dc = __builtin_amdgcn_make_buffer_rsrc(
         out + (size_t)p.m0 * N + p.n0, 0, (uint32_t)min(M - p.m0, S::BM) * (uint32_t)N * 2u, 0x00020000);
     const int col = wn * 16 * TN + (quad & 1) * 16 + (quad >> 1) * 8;
@@ -1186,6 +1211,16 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
 #undef TW_NN_SLAB
 #undef TW_RING
 #endif
+}
+
+constexpr int NN_SUM_THREADS = 256;
+// n: values of a part, a multiple of 8
+__global__ __launch_bounds__(NN_SUM_THREADS) void nn_sum_kernel(uint16_t* out, const float* sums, int64_t n, int parts) {
+  const int64_t i = ((int64_t)blockIdx.x * NN_SUM_THREADS + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4_t s = *reinterpret_cast<const f32x4_t*>(sums + i);
+  for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4_t*>(sums + p * n + i);
+  *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
 }
 
 // More than 64 KiB of dynamic LDS must be allowed once per function and device.
@@ -1438,40 +1473,71 @@ static int launch_tile_for(const GemmBatch& batch, int count, int64_t M, int64_t
   return launch_tile_shape(t.tm, t.tn, batch, count, M, N, K, ldc, max_cus, hs);
 }
 
-template <int TM, int TN, bool TAIL>
+// How many workgroups share a tile's slabs, and how many slabs each has.  Where 64 x 128 tiles leave half of the units
+// without one, as many as there are units for, with four slabs or more each.  With the launch that adds the sums:
+// [64, 7168] x [7168, 8192] 57 us in whole tiles, 28 in four parts (117 MB of b: 23 us at a copy's rate).  Not where it
+// saves a tile fewer than 32 slabs: [7, 1408] x [1408, 1024] 14.3 us in whole tiles, 16.7 in five parts, [1001, 1408]
+// 13.4, 17.0 in two.
+struct NnSplit { int parts, per; };
+static NnSplit nn_split(int64_t M, int64_t N, int64_t K) {
+  int cus = device_compute_units();
+  if (cus <= 0) cus = 256;
+  const int64_t tiles = ((M + 63) / 64) * ((N + 127) / 128), nk = (K + BK - 1) / BK;
+  if (2 * tiles > cus || nk < 8) return {1, (int)nk};
+  const int64_t parts = std::min<int64_t>(std::min<int64_t>(cus / tiles, nk / 4), 16), per = (nk + parts - 1) / parts;
+  if (nk - per < 32) return {1, (int)nk};
+  return {(int)((nk + per - 1) / per), (int)per};
+}
+
+int64_t gemm_bf16_nn_workspace(int64_t M, int64_t N, int64_t K) {
+  const NnSplit s = nn_split(M, N, K);
+  return s.parts > 1 ? 4 * s.parts * M * N : 0;
+}
+
+template <int TM, int TN, bool TAIL, bool SPLIT = false>
 static int launch_nn(uint16_t* out, const uint16_t* a, const uint16_t* b, int64_t M, int64_t N, int64_t K, int64_t rows,
-                     int units, hipStream_t hs) {
+                     int units, float* sums, const NnSplit& split, hipStream_t hs) {
   using S = TileShape<TM, TN>;
   static std::atomic<bool> lds_ok[kMaxDevices];
-  const auto kernel = gemm_bf16_nn_kernel<TM, TN, TAIL>;
+  const auto kernel = gemm_bf16_nn_kernel<TM, TN, TAIL, SPLIT>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, S::LDS)) return rc;
   const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + S::BN - 1) / S::BN);
-  const int64_t grid = std::min<int64_t>((int64_t)tiles_m * tiles_n, units);
+  const int64_t grid = std::min<int64_t>((int64_t)tiles_m * tiles_n * split.parts, units);
   const int wide_store = reinterpret_cast<uintptr_t>(out) % 16 == 0;  // N is a multiple of 8
   launch_kernel(kernel, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, out, a, b, (int)M, (int)N, (int)K, (int)rows,
-                tiles_m, tiles_n, wide_store);
+                tiles_m, tiles_n, wide_store, sums, split.parts, split.per);
   return TW_OK;
 }
 
 // out[M, N] = a[M, K] b[rows, N], everything contiguous, K and N multiples of 8, rows <= K, the last of them in the last
-// slab of 64, and a's columns from `rows` on zeros; a 16-byte aligned, out and b 8.
+// slab of 64, and a's columns from `rows` on zeros; a 16-byte aligned, out and b 8; sums: gemm_bf16_nn_workspace bytes.
 int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t rows, int max_cus,
-                     void* stream) {
+                     float* sums, void* stream) {
   const char* what = "gemm_bf16_nn";
   if (N > NN_MAX_N || K > TILE_MAX_K || N > TILE_MAX_LDC)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: an inner dimension of %lld or rows of %lld values are too long", what,
                      (long long)K, (long long)N);
   const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
   const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
-  const TileChoice& t = pick_tile(M, N, 1, units);
   uint16_t* const o = static_cast<uint16_t*>(out);
   const uint16_t *const x = static_cast<const uint16_t*>(a), *const y = static_cast<const uint16_t*>(b);
   const hipStream_t hs = static_cast<hipStream_t>(stream);
+  NnSplit split = nn_split(M, N, K);
   int rc = TW_OK;
-#define TW_NN_TILE(TM, TN, COST)                                                               \
-  if (t.tm == TM && t.tn == TN)                                                                \
-    rc = K % BK == 0 ? launch_nn<TM, TN, false>(o, x, y, M, N, K, rows, units, hs)             \
-                     : launch_nn<TM, TN, true>(o, x, y, M, N, K, rows, units, hs);
+  if (split.parts > 1) {
+    rc = K % BK == 0 ? launch_nn<2, 4, false, true>(o, x, y, M, N, K, rows, units, sums, split, hs)
+                     : launch_nn<2, 4, true, true>(o, x, y, M, N, K, rows, units, sums, split, hs);
+    if (rc) return rc;
+    if ((rc = finish_launch(what))) return rc;
+    launch_kernel(nn_sum_kernel, dim3((unsigned)((M * N / 4 + NN_SUM_THREADS - 1) / NN_SUM_THREADS)), dim3(NN_SUM_THREADS), 0,
+                  hs, o, sums, M * N, split.parts);
+    return finish_launch(what);
+  }
+  const TileChoice& t = pick_tile(M, N, 1, units);
+#define TW_NN_TILE(TM, TN, COST)                                                                       \
+  if (t.tm == TM && t.tn == TN)                                                                        \
+    rc = K % BK == 0 ? launch_nn<TM, TN, false>(o, x, y, M, N, K, rows, units, nullptr, split, hs)     \
+                     : launch_nn<TM, TN, true>(o, x, y, M, N, K, rows, units, nullptr, split, hs);
   TW_TILES(TW_NN_TILE)
 #undef TW_NN_TILE
   return rc ? rc : finish_launch(what);
