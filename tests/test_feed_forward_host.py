@@ -43,6 +43,8 @@ def test_gated_gradients():
     assert backward(ga=None, gb=None) == _lib.TW_OK
     assert backward(M=0, gb=None) == _lib.TW_OK
     for call in (dict(grad=None), dict(a=None), dict(b=None), dict(both=None), dict(ws=None), dict(size=4095),
+                 dict(K=(1 << 21) + 8), dict(inner=1 << 21, ld_grad=1 << 21, ld_both=1 << 22, gb=None, size=1 << 60),
+                 dict(M=(1 << 21) + 1, ga=None, size=1 << 60),
                  dict(ld_grad=4), dict(ld_grad=10), dict(ld_both=8), dict(ld_both=18), dict(act=3), dict(K=0), dict(M=-1)):
         assert backward(**call) == BAD, call
     for call in (dict(inner=6), dict(K=12), dict(a=AT + 8), dict(b=AT + 8), dict(ws=AT + 64), dict(ga=AT + 4),

@@ -9,7 +9,9 @@
 // matrix cores take it, and G and U were when they were kept: against 64 bits da and db of bf16 operands are off by
 // 0.29 % in the mean square, with neither rounding by 0.17 % (their own).
 //
-// [4096, 8192] x [7168, 8192]: D and D^T 45 us (206 MB read and written, 4.6 TB/s)
+// 4096 rows, K = 8192, I = 3584: D and D^T 42 us (88 MB read, 117 written: 4.9 TB/s), da 341, db 388; with b and a turned
+// beforehand as well, for the "NT" kernel, 104, 326 and 357, in a workspace of 302 MB instead of 118.  300 rows: 112
+// us, that way 134.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -29,6 +31,8 @@ constexpr int TURN = 64;          // rows and columns of a tile
 constexpr int TURN_PITCH = 66;    // elements of a tile's row in LDS: columns are read without conflicts
 constexpr int GRAD_THREADS = 256;
 constexpr int TURN_ROWS = GRAD_THREADS / (TURN / 4), TURN_STEPS = TURN / TURN_ROWS;  // four channels a thread and step
+
+constexpr int64_t GRAD_MAX_K = 1 << 21;  // what the products take
 
 struct GradArgs {
   const uint16_t *grad, *both;
@@ -142,6 +146,9 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   if (int rc = check_shape(what, M, I, K)) return rc;
   if (act < TW_ACT_SILU || act > TW_ACT_GELU_TANH)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, act);
+  if (K > GRAD_MAX_K || (grad_a && 2 * I > GRAD_MAX_K) || (grad_b && turned_pitch(M) > GRAD_MAX_K))
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: K, 2 I and, for grad_b, the rows may be %lld at most", what,
+                     (long long)GRAD_MAX_K);
   if (ld_grad < I || ld_grad % 4 != 0 || ld_both < 2 * I || ld_both % 4 != 0)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: rows of grad_out and gate_up need strides of at least %lld and %lld, "
                      "multiples of 4", what, (long long)I, (long long)(2 * I));

@@ -202,6 +202,11 @@ struct GemmBatch {
 // out, out = act(a gate^T) * (a up^T).  A tile's rows of b are half gate and half up rows of the same columns, so both
 // sums of an element meet in one lane (tile kernel) or one thread (K-split kernel) as fp32 and the product is rounded
 // once.  `both`, where given, also takes the two sums, rounded: [M][2 I], what the gradient needs.
+//
+// The product takes the time of the plain one over the same rows of b: [4096, 8192] x [7168, 8192]^T 337 us, plain 340
+// (1 430 TFLOP/s; the tile loop is the bound, see there), with `both` 348; one row 20.4 us (117 MB of weights at 5.7 TB/s),
+// 61 rows x [7392, 8192]^T 29.7 (4.1 TB/s: what a unit has under way is shared with a).  The activation is known outside the
+// loops that apply it: chosen per value the same call took 361, and [1001, 1024] x [1408, 1024]^T 9.3 instead of 8.6.
 struct GatedOut {
   uint16_t* both;
   int64_t ld_both;
@@ -1059,8 +1064,6 @@ __device__ __forceinline__ void nn_phase(f32x4_t (&acc)[TM][TN], const bf16x8_t 
 
 #endif
 
-constexpr int64_t NN_MAX_N = 1 << 23;  // 64 rows of b span less than 2 GiB
-
 // rows: b's, at most K; a's columns behind as many are zeros.  TAIL: K % 64 != 0, a's chunks past K must arrive as zeros.
 //
 // SPLIT: few tiles.  A tile's slabs are dealt out to `parts` workgroups, `per` each, whose fp32 sums go to sums[part][M][N];
@@ -1514,7 +1517,7 @@ static int launch_nn(uint16_t* out, const uint16_t* a, const uint16_t* b, int64_
 int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t rows, int max_cus,
                      float* sums, void* stream) {
   const char* what = "gemm_bf16_nn";
-  if (N > NN_MAX_N || K > TILE_MAX_K || N > TILE_MAX_LDC)
+  if (K > TILE_MAX_K || N > TILE_MAX_LDC)  // 32-bit offsets of a tile's rows of a and out, of 64 rows of b
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: an inner dimension of %lld or rows of %lld values are too long", what,
                      (long long)K, (long long)N);
   const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
