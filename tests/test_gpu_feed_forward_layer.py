@@ -195,3 +195,35 @@ def test_as_the_schedules_mlp(fp8, cus):
     y0, r0 = run_layers(T, False, fp8)
     y1, r1 = run_layers(T, True, fp8, cus)
     assert torch.equal(r0, r1) and torch.equal(y0, y1)
+
+
+def test_two_streams_at_once():
+    """The whole of it on two streams with operands of their own, many times: nothing is shared."""
+    def work(seed, T):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        x = torch.randn(T, H, generator=g, device=DEV).to(BF16)
+        w = (torch.randn(2 * INNER, H, generator=g, device=DEV) * H ** -0.5).to(BF16)
+        dh = torch.randn(T, INNER, generator=g, device=DEV).to(BF16)
+        block = filled(tw.FeedForward(H, INNER), seed).to_fp8_blocks()
+        out, both = (torch.empty(T, n, dtype=BF16, device=DEV) for n in (INNER, 2 * INNER))
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+
+        def run():
+            ops.gated_gemm_bf16_nt(out, x, w, gate_up=both)
+            ops.gated_gemm_bf16_nt_backward(dx, dw, dh, x, w, both)
+            return [t.clone() for t in (out, both, dx, dw)] + [block(x.clone())]
+        return run
+
+    pair = [work(1, 300), work(2, 40)]
+    want = [run() for run in pair]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in pair]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(pair[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for results in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(results, want[i]))

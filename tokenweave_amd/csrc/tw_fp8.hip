@@ -356,6 +356,8 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 
+    // A wave without a slab has its block scales under way still: they must not land among the sums.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // acc[i][j][4 q + e]: sum of out[m0 + i*32 + l32][n0 + j*32 + 8 q + 4 lhi + e]
     constexpr int PITCH = RB * 4 + 16;
     __syncthreads();
