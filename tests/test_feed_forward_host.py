@@ -36,13 +36,14 @@ def backward(ga=AT, gb=AT, grad=AT, ld_grad=8, a=AT, b=AT, both=AT, ld_both=16, 
 def test_gated_gradients():
     L = _lib.lib()
     size = L.tw_gated_gemm_bf16_nt_backward_workspace
-    # the gradient of both products, 2 bytes a value, and the same turned; whole slabs of 64 rows
-    assert size(4, 8, 16, 1, 0) == size(4, 8, 16, 0, 1) == 64 * 16 * 2 and size(65, 8, 16, 1, 1) == 2 * 128 * 16 * 2
+    # the gradient of both products, 2 bytes a value, and the same turned; rows of whole slabs of 64
+    assert size(4, 8, 16, 1, 0) == 4 * 64 * 2 and size(4, 8, 16, 0, 1) == 16 * 64 * 2
+    assert size(65, 40, 16, 1, 1) == (65 * 128 + 80 * 128) * 2
     assert size(0, 8, 16, 1, 1) == 0 and size(4, 8, 16, 0, 0) == 0
     assert size(4, 6, 16, 1, 1) == ALIGN and size(-1, 8, 16, 1, 1) == BAD
     assert backward(ga=None, gb=None) == _lib.TW_OK
     assert backward(M=0, gb=None) == _lib.TW_OK
-    for call in (dict(grad=None), dict(a=None), dict(b=None), dict(both=None), dict(ws=None), dict(size=4095),
+    for call in (dict(grad=None), dict(a=None), dict(b=None), dict(both=None), dict(ws=None), dict(size=2559),
                  dict(K=(1 << 21) + 8), dict(inner=1 << 21, ld_grad=1 << 21, ld_both=1 << 22, gb=None, size=1 << 60),
                  dict(M=(1 << 21) + 1, ga=None, size=1 << 60),
                  dict(ld_grad=4), dict(ld_grad=10), dict(ld_both=8), dict(ld_both=18), dict(act=3), dict(K=0), dict(M=-1)):

@@ -188,3 +188,32 @@ def test_both_routes_give_the_same_bits(monkeypatch):
     monkeypatch.setattr(ops, "_fast", None)
     ops.gated_gemm_bf16_nt(b, x, w)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("M,inner,K", [(1, 4, 8), (70, 100, 136), (300, 36, 200), (64, 2100, 264), (129, 64, 72)])
+def test_what_a_workspace_held_does_not_matter(M, inner, K):
+    """Not-a-numbers left in the workspace; gradients that begin 8, 16 and 64 bytes into a buffer."""
+    from tokenweave_amd import _lib
+    x, w = make(M, inner, K)
+    both = torch.empty((M, 2 * inner), dtype=BF16, device="cuda")
+    ops.gated_gemm_bf16_nt(torch.empty((M, inner), dtype=BF16, device="cuda"), x, w, gate_up=both)
+    grad = torch.randn((M, inner), device="cuda").to(BF16)
+    L = _lib.lib()
+    size = L.tw_gated_gemm_bf16_nt_backward_workspace(M, inner, K, 1, 1)
+    space = torch.full((size // 2,), float("nan"), dtype=BF16, device="cuda")
+    before = None
+    for skip in (4, 8, 32):
+        bufs = [torch.full((rows * K + 64,), 777.0, dtype=BF16, device="cuda") for rows in (M, 2 * inner)]
+        gx, gw = (b[skip:skip + rows * K].view(rows, K) for b, rows in zip(bufs, (M, 2 * inner)))
+        space.fill_(float("nan"))
+        _lib.check(L.tw_gated_gemm_bf16_nt_backward(
+            gx.data_ptr(), gw.data_ptr(), grad.data_ptr(), inner, x.data_ptr(), w.data_ptr(), both.data_ptr(), 2 * inner,
+            M, inner, K, 0, 0, space.data_ptr(), size, torch.cuda.current_stream().cuda_stream))
+        want_x, bound_x, want_w, bound_w = R.gated_gradients(grad, x, w, both, "silu")
+        R.assert_within(gx, want_x, bound_x, "grad_x")
+        R.assert_within(gw, want_w, bound_w, "grad_w")
+        for b, rows in zip(bufs, (M, 2 * inner)):
+            assert (b[:skip] == 777.0).all() and (b[skip + rows * K:] == 777.0).all()
+        if before:
+            assert torch.equal(gx, before[0]) and torch.equal(gw, before[1])
+        before = gx.clone(), gw.clone()

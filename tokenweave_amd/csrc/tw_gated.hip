@@ -37,7 +37,7 @@ constexpr int64_t GRAD_MAX_K = 1 << 21;  // what the products take
 struct GradArgs {
   const uint16_t *grad, *both;
   uint16_t *d, *d_turned;  // null: not wanted
-  int64_t ld_grad, ld_both, pitch;
+  int64_t ld_grad, ld_both, pitch, pitch_turned;
   int M, I, across, act;
 };
 
@@ -94,10 +94,12 @@ __global__ __launch_bounds__(GRAD_THREADS) void gated_grad_kernel(GradArgs w) {
       const uint2 dg = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
       const uint2 du = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
       if (w.d && row < w.M && c0 + c < w.I) {
-        uint16_t* d = w.d + (int64_t)row * 2 * w.I + c0 + c;
+        uint16_t* d = w.d + row * w.pitch + c0 + c;
         *reinterpret_cast<uint2*>(d) = dg;
         *reinterpret_cast<uint2*>(d + w.I) = du;
       }
+      if (w.d && row < w.M && c0 + TURN >= w.I && 2 * w.I + c < w.pitch)  // behind D's columns: zeros
+        *reinterpret_cast<uint2*>(w.d + row * w.pitch + 2 * w.I + c) = make_uint2(0, 0);
       if (w.d_turned) {
         uint32_t* p = reinterpret_cast<uint32_t*>(tiles[0] + (m + i * TURN_ROWS) * TURN_PITCH + c);
         p[0] = dg.x, p[1] = dg.y;
@@ -108,8 +110,8 @@ __global__ __launch_bounds__(GRAD_THREADS) void gated_grad_kernel(GradArgs w) {
   });
   if (!w.d_turned) return;
   __syncthreads();
-  write_turned(tiles[0], w.d_turned + c0 * w.pitch, w.I - c0, m0, w.pitch);
-  write_turned(tiles[1], w.d_turned + (int64_t)(w.I + c0) * w.pitch, w.I - c0, m0, w.pitch);
+  write_turned(tiles[0], w.d_turned + c0 * w.pitch_turned, w.I - c0, m0, w.pitch_turned);
+  write_turned(tiles[1], w.d_turned + (int64_t)(w.I + c0) * w.pitch_turned, w.I - c0, m0, w.pitch_turned);
 }
 
 __global__ __launch_bounds__(GRAD_THREADS) void fill_zero_kernel(uint2* to, int64_t n) {
@@ -117,8 +119,8 @@ __global__ __launch_bounds__(GRAD_THREADS) void fill_zero_kernel(uint2* to, int6
     to[i] = make_uint2(0, 0);
 }
 
-// A row of D^T: the rows up to a whole slab of the product, the ones behind the last zeros.  D has as much room.
-int64_t turned_pitch(int64_t M) { return (M + TURN - 1) / TURN * TURN; }
+// A row of D or D^T: whole slabs of the products, zeros behind the last value.
+int64_t whole_slabs(int64_t n) { return (n + TURN - 1) / TURN * TURN; }
 
 int check_shape(const char* what, int64_t M, int64_t I, int64_t K) {
   if (M < 0 || I <= 0 || K <= 0 || M > INT32_MAX - TURN || I > INT32_MAX / 2 || K > INT32_MAX)
@@ -133,10 +135,10 @@ int check_shape(const char* what, int64_t M, int64_t I, int64_t K) {
 int64_t gated_backward_workspace(int64_t M, int64_t I, int64_t K, bool want_a, bool want_b) {
   if (int rc = check_shape("gated_gemm_bf16_nt_backward_workspace", M, I, K)) return rc;
   // D, D turned, and the partial sums of one product after the other
-  const int64_t pitch = turned_pitch(M);
-  const int64_t of_a = want_a && M ? gemm_bf16_nn_workspace(M, K, 2 * I) : 0;
-  const int64_t of_b = want_b && M ? gemm_bf16_nn_workspace(2 * I, K, pitch) : 0;
-  return 4 * I * ((want_a ? pitch : 0) + (want_b ? pitch : 0)) + std::max(of_a, of_b);
+  const int64_t pitch = whole_slabs(2 * I), pitch_turned = whole_slabs(M);
+  const int64_t of_a = want_a && M ? gemm_bf16_nn_workspace(M, K, pitch) : 0;
+  const int64_t of_b = want_b && M ? gemm_bf16_nn_workspace(2 * I, K, pitch_turned) : 0;
+  return 2 * ((want_a ? M * pitch : 0) + (want_b ? 2 * I * pitch_turned : 0)) + std::max(of_a, of_b);
 }
 
 int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad_out, int64_t ld_grad, const void* a,
@@ -146,7 +148,7 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   if (int rc = check_shape(what, M, I, K)) return rc;
   if (act < TW_ACT_SILU || act > TW_ACT_GELU_TANH)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, act);
-  if (K > GRAD_MAX_K || (grad_a && 2 * I > GRAD_MAX_K) || (grad_b && turned_pitch(M) > GRAD_MAX_K))
+  if (K > GRAD_MAX_K || (grad_a && 2 * I > GRAD_MAX_K) || (grad_b && whole_slabs(M) > GRAD_MAX_K))
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: K, 2 I and, for grad_b, the rows may be %lld at most", what,
                      (long long)GRAD_MAX_K);
   if (ld_grad < I || ld_grad % 4 != 0 || ld_both < 2 * I || ld_both % 4 != 0)
@@ -175,9 +177,9 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   GradArgs w = {};
   w.grad = static_cast<const uint16_t*>(grad_out);
   w.both = static_cast<const uint16_t*>(both);
-  w.pitch = turned_pitch(M);
-  if (grad_a) w.d = ws, ws += 2 * I * w.pitch;
-  if (grad_b) w.d_turned = ws, ws += 2 * I * w.pitch;
+  w.pitch = whole_slabs(2 * I), w.pitch_turned = whole_slabs(M);
+  if (grad_a) w.d = ws, ws += M * w.pitch;
+  if (grad_b) w.d_turned = ws, ws += 2 * I * w.pitch_turned;
   float* const sums = reinterpret_cast<float*>(ws);
   w.ld_grad = ld_grad, w.ld_both = ld_both;
   w.M = (int)M, w.I = (int)I, w.act = act;
@@ -187,8 +189,8 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   launch_kernel(gated_grad_kernel, dim3((unsigned)grid), dim3(GRAD_THREADS), 0, hs, w);
   if (int rc = finish_launch(what)) return rc;
   if (grad_a)
-    if (int rc = run_gemm_bf16_nn(grad_a, w.d, b, M, K, 2 * I, 2 * I, max_cus, sums, stream)) return rc;
-  if (grad_b) return run_gemm_bf16_nn(grad_b, w.d_turned, a, 2 * I, K, w.pitch, M, max_cus, sums, stream);
+    if (int rc = run_gemm_bf16_nn(grad_a, w.d, b, M, K, w.pitch, 2 * I, max_cus, sums, stream)) return rc;
+  if (grad_b) return run_gemm_bf16_nn(grad_b, w.d_turned, a, 2 * I, K, w.pitch_turned, M, max_cus, sums, stream);
   return TW_OK;
 }
 

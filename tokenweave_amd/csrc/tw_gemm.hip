@@ -198,6 +198,17 @@ struct GemmBatch {
   const uint16_t* bias[TW_MAX_PARTIALS];  // [N] bf16 or null: added to that product only
 };
 
+// How the gated and the "NN" tiles store: 8 bytes a lane, 16, or 16 that go through the L2 at once.  The last only where
+// rows begin on 64 bytes: a lane's group of four stores 64, and where those lie across two pieces of 64 memory gets parts
+// of each, which the L2 puts together if it may keep them.  [4352, 64] x [64, 7944]: 66.6 us through, 19.4 kept (what it
+// still holds then costs the next kernel 12); rows of 8192 go through in 19.7.
+enum StoreForm { kNarrowStores, kWideStores, kWideThrough };
+inline StoreForm store_form(const void* out, int64_t columns, int64_t ldc) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(out);
+  if (columns % 8 != 0 || ldc % 8 != 0 || begin % 16 != 0) return kNarrowStores;
+  return ldc % 32 == 0 && begin % 64 == 0 ? kWideThrough : kWideStores;
+}
+
 // The gated form (GATED) of both kernels below: b is [2 I, K], a gate row and an up row for each of the I columns of
 // out, out = act(a gate^T) * (a up^T).  A tile's rows of b are half gate and half up rows of the same columns, so both
 // sums of an element meet in one lane (tile kernel) or one thread (K-split kernel) as fp32 and the product is rounded
@@ -620,6 +631,13 @@ __device__ __forceinline__ void tile_loads(__amdgpu_buffer_rsrc_t da, __amdgpu_b
 
 constexpr int kStoreThrough = 19;  // nt sc0 sc1
 
+template <typename F>
+__device__ __forceinline__ void with_store_form(int form, F&& f) {
+  if (form == kWideThrough) f(std::integral_constant<StoreForm, kWideThrough>{});
+  else if (form == kWideStores) f(std::integral_constant<StoreForm, kWideStores>{});
+  else f(std::integral_constant<StoreForm, kNarrowStores>{});
+}
+
 // The wave's accumulators: row 16 i of `dc` at voffset + i * row_step.  WIDE: eight columns per
 // store, else four (rows that are only 8-byte aligned, or N % 8 != 0).
 template <int TM, int TN, bool WIDE, bool BIAS>
@@ -662,7 +680,7 @@ __device__ __forceinline__ float acc_read(float x) {
 
 // The gated form: tiles 4 p .. 4 p + 3 of a row of tiles are gate, up, gate, up of eight columns, 32 p + 8 quad and up.
 // Rows of 8 bytes' alignment or I % 8 != 0 (narrow) take two stores.
-template <int TM, int TN, bool WIDE, int ACT>
+template <int TM, int TN, StoreForm FORM, int ACT>
 __device__ __forceinline__ void tile_store_gated(const f32x4_t (&acc)[TM][TN], __amdgpu_buffer_rsrc_t dc,
                                                  uint32_t row_off, uint32_t row_step, int n, int N, int m, int M,
                                                  const GatedOut& gated) {
@@ -687,12 +705,12 @@ __device__ __forceinline__ void tile_store_gated(const f32x4_t (&acc)[TM][TN], _
         v[s] = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
       }
       const uint32_t off = row_off + (uint32_t)i * row_step + (uint32_t)p * 64u;
-      if (WIDE) {
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{v[0].x, v[0].y, v[1].x, v[1].y}, dc,
-                                               c < N ? off : TILE_OUT_OF_RANGE, 0, kStoreThrough);
+      if (FORM == kNarrowStores) {
+        __builtin_amdgcn_raw_buffer_store_b64(v[0], dc, c < N ? off : TILE_OUT_OF_RANGE, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b64(v[1], dc, c + 4 < N ? off + 8u : TILE_OUT_OF_RANGE, 0, 0);
       } else {
-        __builtin_amdgcn_raw_buffer_store_b64(v[0], dc, c < N ? off : TILE_OUT_OF_RANGE, 0, kStoreThrough);
-        __builtin_amdgcn_raw_buffer_store_b64(v[1], dc, c + 4 < N ? off + 8u : TILE_OUT_OF_RANGE, 0, kStoreThrough);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{v[0].x, v[0].y, v[1].x, v[1].y}, dc,
+                                               c < N ? off : TILE_OUT_OF_RANGE, 0, FORM == kWideThrough ? kStoreThrough : 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -929,9 +947,10 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
       const uint32_t row_off = (uint32_t)(row * (int)ldc + col) * 2u, row_step = (uint32_t)ldc * 32u;
       asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMA's result is written
       with_activation(gated.act, [&](auto act) {
-        if (wide_store)
-          tile_store_gated<TM, TN, true, act()>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
-        else tile_store_gated<TM, TN, false, act()>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
+        auto store = [&](auto form) {
+          tile_store_gated<TM, TN, form(), act()>(acc, dc, row_off, row_step, n0 + col, N, p.m0 + row, M, gated);
+        };
+        with_store_form(wide_store, store);
       });
       continue;
     }
@@ -1004,7 +1023,7 @@ __device__ __forceinline__ bf16x8_t nn_read(const lds_u8_t* p, int row_bytes) {
 // The wave's accumulators: lanes 16 q .. 16 q + 15 hold columns 4 q .. 4 q + 3 of every tile of columns.  Of a pair of
 // tiles, odd groups of lanes give their columns of the first to the even group before them and get that group's of
 // the second: eight adjacent columns each.  N % 8 == 0.
-template <int TM, int TN, bool WIDE>
+template <int TM, int TN, StoreForm FORM>
 __device__ __forceinline__ void nn_store(const f32x4_t (&acc)[TM][TN], __amdgpu_buffer_rsrc_t dc, uint32_t row_off,
                                              uint32_t row_step, int n, int N) {
 #pragma unroll
@@ -1016,11 +1035,12 @@ __device__ __forceinline__ void nn_store(const f32x4_t (&acc)[TM][TN], __amdgpu_
       const auto y = __builtin_amdgcn_permlane16_swap(tile_pack2(acc[i][j][2], acc[i][j][3]),
                                                       tile_pack2(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
       const uint32_t off = n + j * 16 < N ? row_off + (uint32_t)i * row_step + (uint32_t)j * 32u : TILE_OUT_OF_RANGE;
-      if (WIDE) {
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{x[0], y[0], x[1], y[1]}, dc, off, 0, kStoreThrough);
+      if (FORM == kNarrowStores) {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{x[0], y[0]}, dc, off, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{x[1], y[1]}, dc, off + 8u, 0, 0);
       } else {
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{x[0], y[0]}, dc, off, 0, kStoreThrough);
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{x[1], y[1]}, dc, off + 8u, 0, kStoreThrough);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{x[0], y[0], x[1], y[1]}, dc, off, 0,
+                                               FORM == kWideThrough ? kStoreThrough : 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -1064,14 +1084,14 @@ __device__ __forceinline__ void nn_phase(f32x4_t (&acc)[TM][TN], const bf16x8_t 
 
 #endif
 
-// rows: b's, at most K; a's columns behind as many are zeros.  TAIL: K % 64 != 0, a's chunks past K must arrive as zeros.
+// K: a's row, whole slabs.  rows: b's, at most K; a's columns behind as many are zeros.
 //
 // SPLIT: few tiles.  A tile's slabs are dealt out to `parts` workgroups, `per` each, whose fp32 sums go to sums[part][M][N];
 // nn_sum_kernel adds them in order.
-template <int TM, int TN, bool TAIL, bool SPLIT>
+template <int TM, int TN, bool SPLIT>
 __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nn_kernel(
     uint16_t* out, const uint16_t* a, const uint16_t* b, int M, int N, int K, int rows, int tiles_m, int tiles_n,
-    int wide_store, float* sums, int parts, int per) {
+    int form, float* sums, int parts, int per) {
 #ifdef __HIP_DEVICE_COMPILE__
   using S = TileShape<TM, TN>;
   static_assert(TN % 2 == 0, "whole groups of eight chunks a row");
@@ -1082,7 +1102,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1, r16 = lane & 15, quad = lane >> 4;
-  const int nk = (K + BK - 1) / BK, tail_chunks = TAIL ? (K % BK) / 8 : 8;
+  const int nk = K / BK;
   const int whole = tiles_m * tiles_n, num_tiles = SPLIT ? whole * parts : whole;
   auto tile_of = [&](int t) { return tile_place<TM, TN>(SPLIT ? t / parts : t, whole, tiles_m, tiles_n); };
   auto first_slab = [&](int t) { return SPLIT ? t % parts * per : 0; };
@@ -1101,13 +1121,11 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   lds_u8_t* const wa = lds_a + wave * LA * 1024;
   lds_u8_t* const wb = lds_b + wave * LB * 1024;
   uint32_t va[LA], vb[LB];
-  auto offsets = [&](int chunks) {
 #pragma unroll
-    for (int l = 0; l < LA; ++l) {
-      const int blk = wave * LA + l, c = (lane & 7) ^ (((blk & 1) << 2) | (lane >> 4));
-      va[l] = c < chunks ? (uint32_t)((blk * 8 + (lane >> 3)) * K + c * 8) * 2u : TILE_OUT_OF_RANGE;
-    }
-  };
+  for (int l = 0; l < LA; ++l) {
+    const int blk = wave * LA + l, c = (lane & 7) ^ (((blk & 1) << 2) | (lane >> 4));
+    va[l] = (uint32_t)((blk * 8 + (lane >> 3)) * K + c * 8) * 2u;
+  }
 #pragma unroll
   for (int l = 0; l < LB; ++l) {
     const int place = (wave * LB + l) * 64 + lane, row = place / (4 * TN);
@@ -1137,15 +1155,11 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     if (lk == l_end) {
       lt += gridDim.x;
       place();
-      if (TAIL) offsets(lk == nk - 1 ? tail_chunks : 8);
-    } else if (TAIL && lk == nk - 1) {
-      offsets(tail_chunks);
     }
     slab_of_b();
   };
   place();
   slab_of_b();
-  offsets(TAIL && lk == nk - 1 ? tail_chunks : 8);
 #pragma unroll
   for (int s = 0; s < D; ++s) {
 #pragma unroll
@@ -1208,8 +1222,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     const int col = wn * 16 * TN + (quad & 1) * 16 + (quad >> 1) * 8;
     const uint32_t row_off = (uint32_t)((wm * 16 * TM + r16) * N + col) * 2u, row_step = (uint32_t)N * 32u;
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMA's result is written
-    if (wide_store) nn_store<TM, TN, true>(acc, dc, row_off, row_step, p.n0 + col, N);
-    else nn_store<TM, TN, false>(acc, dc, row_off, row_step, p.n0 + col, N);
+    with_store_form(form, [&](auto f) { nn_store<TM, TN, f()>(acc, dc, row_off, row_step, p.n0 + col, N); });
   }
 #undef TW_NN_SLAB
 #undef TW_RING
@@ -1377,6 +1390,7 @@ static int launch_tile_kernel(const GemmBatch& batch, int count, int64_t M, int6
   int wide_store = (N % 8 == 0 && ldc % 8 == 0) ? 1 : 0;
   for (int p = 0; p < count; ++p)
     if (reinterpret_cast<uintptr_t>(batch.out[p]) & 15u) wide_store = 0;
+  if (GATED) wide_store = store_form(batch.out[0], N, ldc);
   launch_kernel(gemm_bf16_nt_tile_kernel<TM, TN, ROWS, GATED>, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs,
                 batch, count, (int)M, (int)N, (int)K, ldc, tiles_m, tiles_n, wide_store, gated);
   return TW_OK;
@@ -1497,23 +1511,24 @@ int64_t gemm_bf16_nn_workspace(int64_t M, int64_t N, int64_t K) {
   return s.parts > 1 ? 4 * s.parts * M * N : 0;
 }
 
-template <int TM, int TN, bool TAIL, bool SPLIT = false>
+template <int TM, int TN, bool SPLIT = false>
 static int launch_nn(uint16_t* out, const uint16_t* a, const uint16_t* b, int64_t M, int64_t N, int64_t K, int64_t rows,
                      int units, float* sums, const NnSplit& split, hipStream_t hs) {
   using S = TileShape<TM, TN>;
   static std::atomic<bool> lds_ok[kMaxDevices];
-  const auto kernel = gemm_bf16_nn_kernel<TM, TN, TAIL, SPLIT>;
+  const auto kernel = gemm_bf16_nn_kernel<TM, TN, SPLIT>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, S::LDS)) return rc;
   const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + S::BN - 1) / S::BN);
   const int64_t grid = std::min<int64_t>((int64_t)tiles_m * tiles_n * split.parts, units);
-  const int wide_store = reinterpret_cast<uintptr_t>(out) % 16 == 0;  // N is a multiple of 8
   launch_kernel(kernel, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, out, a, b, (int)M, (int)N, (int)K, (int)rows,
-                tiles_m, tiles_n, wide_store, sums, split.parts, split.per);
+                tiles_m, tiles_n, store_form(out, N, N), sums, split.parts, split.per);
   return TW_OK;
 }
 
-// out[M, N] = a[M, K] b[rows, N], everything contiguous, K and N multiples of 8, rows <= K, the last of them in the last
+// out[M, N] = a[M, K] b[rows, N], everything contiguous, K a multiple of 64, N of 8, rows <= K, the last of them in the last
 // slab of 64, and a's columns from `rows` on zeros; a 16-byte aligned, out and b 8; sums: gemm_bf16_nn_workspace bytes.
+// (Whole slabs are whole lines, each of which a unit requests once: [300, 7392] x [7392, 8192] 102 us with a's rows 7392
+// long, 61 with 7424; 256 rows 85 and 53.)
 int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t rows, int max_cus,
                      float* sums, void* stream) {
   const char* what = "gemm_bf16_nn";
@@ -1528,8 +1543,7 @@ int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t
   NnSplit split = nn_split(M, N, K);
   int rc = TW_OK;
   if (split.parts > 1) {
-    rc = K % BK == 0 ? launch_nn<2, 4, false, true>(o, x, y, M, N, K, rows, units, sums, split, hs)
-                     : launch_nn<2, 4, true, true>(o, x, y, M, N, K, rows, units, sums, split, hs);
+    rc = launch_nn<2, 4, true>(o, x, y, M, N, K, rows, units, sums, split, hs);
     if (rc) return rc;
     if ((rc = finish_launch(what))) return rc;
     launch_kernel(nn_sum_kernel, dim3((unsigned)((M * N / 4 + NN_SUM_THREADS - 1) / NN_SUM_THREADS)), dim3(NN_SUM_THREADS), 0,
@@ -1537,10 +1551,8 @@ int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t
     return finish_launch(what);
   }
   const TileChoice& t = pick_tile(M, N, 1, units);
-#define TW_NN_TILE(TM, TN, COST)                                                                       \
-  if (t.tm == TM && t.tn == TN)                                                                        \
-    rc = K % BK == 0 ? launch_nn<TM, TN, false>(o, x, y, M, N, K, rows, units, nullptr, split, hs)     \
-                     : launch_nn<TM, TN, true>(o, x, y, M, N, K, rows, units, nullptr, split, hs);
+#define TW_NN_TILE(TM, TN, COST) \
+  if (t.tm == TM && t.tn == TN) rc = launch_nn<TM, TN>(o, x, y, M, N, K, rows, units, nullptr, split, hs);
   TW_TILES(TW_NN_TILE)
 #undef TW_NN_TILE
   return rc ? rc : finish_launch(what);
