@@ -285,3 +285,22 @@ def test_a_run_captured(M):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(t, o) for t, o in zip((t1, mid, t2, out), want)), seed
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(129, 136, 144), (300, 8, 128), (1000, 1376, 272), (700, 7392, 400), (4096, 2048, 128),
+                                   (2458, 1440, 512), (2500, 7168, 128)])
+def test_outputs_that_begin_anywhere(M, N, K, dtype):
+    """Rows 8, 16 and 64 bytes into a buffer, as far apart as keeps that alignment: the same bits, and nothing beside them."""
+    x, sx, w, sw = operands(M, N, K)
+    plain = torch.empty((M, N), dtype=dtype, device="cuda")
+    ops.gemm_fp8_block_nt(plain, x, sx, w, sw)
+    want, off = R.block_product(x, sx, w, sw)
+    R.assert_within(plain, want, off + R.half(dtype) * want.abs() + (6e-8 if dtype == torch.float16 else 0), "plain")
+    for step in (4, 8, 32):
+        buf = torch.full((M + 2, (N + step - 1) // step * step + 2 * step), 777.0, dtype=dtype, device="cuda")
+        out = buf[1:1 + M, step:step + N]
+        ops.gemm_fp8_block_nt(out, x, sx, w, sw)
+        assert torch.equal(out, plain), step
+        out.fill_(777.0)
+        assert (buf == 777.0).all(), step

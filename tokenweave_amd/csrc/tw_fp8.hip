@@ -8,6 +8,7 @@
 
 #include "tw_activation.h"
 #include "tw_common.h"
+#include "tw_store.h"
 
 namespace tw {
 
@@ -172,6 +173,7 @@ void launch_quant(const QuantArgs& w, bool vec, int64_t grid, hipStream_t hs) {
 constexpr int ROWB = 128;
 [[maybe_unused]] constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
 constexpr int64_t BLOCK_MAX_K = 1 << 22;  // a tile's rows span at most 1 GiB
+constexpr int64_t BLOCK_WIDE_LDC = 1 << 22;  // 256 rows of the output, where they are stored 16 bytes a lane: 2 GiB
 
 constexpr int64_t BLOCK_MAX_SCALE_ROW = 1 << 20;  // 32-bit offsets of a tile's scales
 
@@ -181,6 +183,7 @@ struct BlockArgs {
   const float *a_scales, *b_scales;
   int64_t scale_row, scale_block, ldc;
   int M, N, K, half_out, tiles_m, tiles_n, cols;
+  int form;  // StoreForm, tile kernel
 };
 
 [[maybe_unused]] __device__ __forceinline__ uint32_t pack_out(float lo, float hi, int half_out) {
@@ -405,7 +408,8 @@ __global__ __launch_bounds__(SPLIT_THREADS) void gemm_fp8_block_split_kernel(Blo
 // slab three ahead, b's by a barrier of its own and 256 x 224 tiles 205 to 214 by board (2 300 TFLOP/s; 8192^3 of the
 // library with one scale a tensor 2 920).  In 256 x 256 tiles without the loads 211 of 253, without the multiply-adds 233,
 // without both 184: the matrix cores themselves, at the clock that the board's power limit leaves.
-// [1000, 3696] x [8192, 3696]^T 37 us: 256 tiles, a unit's 1.4 MB at its 50 GB/s.
+// [1000, 3696] x [8192, 3696]^T 35.3 us: 256 tiles, a unit's 1.4 MB at its 50 GB/s, and 5 us that a single slab takes as
+// well (8 bytes a lane and store: 39.2).
 constexpr int WIDE_THREADS = 512;
 template <int WM, int TM, int TN, int NA, int NB>
 struct WideShape {
@@ -608,20 +612,45 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
       }
       use_a = next_a, use_b = next_b, use_s = next_s;
     }
-    const int m = wm * 16 * TM + r16;
-    uint16_t* const to = w.out + (size_t)(m0 + m) * w.ldc + n0;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      if (j >= TN - S::LAG) add((TM - 1) * TN + j, first_scale, second_scale);
-      // a lane holds row r16 of each row of tiles, columns 8 quad + 0 .. 7 of a pair of column tiles
-      const int c = wn * 16 * TN + (TN % 2 && j == TN - 1 ? 16 * j + quad * 4 : (j >> 1) * 32 + quad * 8 + (j & 1) * 4);
+    for (int j = TN - S::LAG; j < TN; ++j) add((TM - 1) * TN + j, first_scale, second_scale);
+    // a lane holds row r16 of each row of tiles, columns 8 quad + 0 .. 7 of a pair of column tiles
+    const int m = wm * 16 * TM + r16, c0 = wn * 16 * TN;
+    auto four = [&](int i, int j) {
+      return u32x2_t{pack_out(acc[i][j][0], acc[i][j][1], w.half_out), pack_out(acc[i][j][2], acc[i][j][3], w.half_out)};
+    };
+    with_store_form(w.form, [&](auto form) {
+      uint16_t* const to = w.out + (size_t)(m0 + m) * w.ldc + n0;
+      const __amdgpu_buffer_rsrc_t dc = __builtin_amdgcn_make_buffer_rsrc(
+          w.out + (size_t)m0 * w.ldc + n0, 0, (uint32_t)rows * (uint32_t)w.ldc * 2u, 0x00020000);
+      constexpr int AUX = form() == kWideThrough ? kStoreThrough : 0;
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-        if (c < cols && m + 16 * i < rows)
-          *reinterpret_cast<uint2*>(to + (size_t)(16 * i) * w.ldc + c) = make_uint2(
-              pack_out(acc[i][j][0], acc[i][j][1], w.half_out), pack_out(acc[i][j][2], acc[i][j][3], w.half_out));
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next tile's slabs go where this one's were
+      for (int i = 0; i < TM; ++i) {
+        const uint32_t row = (uint32_t)(m + 16 * i) * (uint32_t)w.ldc * 2u;
+#pragma unroll
+        for (int j = 0; j + 1 < TN; j += 2) {
+          const int c = c0 + j * 16 + quad * 8;
+          const u32x2_t x = four(i, j), y = four(i, j + 1);
+          if (form() != kNarrowStores) {
+            __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{x.x, x.y, y.x, y.y}, dc, c < cols ? row + 2 * c : OUT_OF_RANGE, 0, AUX);
+          } else if (m + 16 * i < rows) {
+            if (c < cols) *reinterpret_cast<u32x2_t*>(to + (size_t)(16 * i) * w.ldc + c) = x;
+            if (c + 4 < cols) *reinterpret_cast<u32x2_t*>(to + (size_t)(16 * i) * w.ldc + c + 4) = y;
+          }
+        }
+        if (TN % 2) {
+          const int c = c0 + 16 * (TN - 1) + quad * 4;
+          const u32x2_t x = four(i, TN - 1);
+          if (form() != kNarrowStores)
+            __builtin_amdgcn_raw_buffer_store_b64(x, dc, c < cols ? row + 2 * c : OUT_OF_RANGE, 0, 0);
+          else if (m + 16 * i < rows && c < cols) *reinterpret_cast<u32x2_t*>(to + (size_t)(16 * i) * w.ldc + c) = x;
+        }
+      }
+    });
+    // The next tile's slabs go where this one's were: what is still on its way there has to arrive first, the stores
+    // behind it need not.
+    if (w.form == kNarrowStores) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(TM * ((TN + 1) / 2)) : "memory");
   }
 #endif
 }
@@ -662,7 +691,7 @@ int launch_split(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
 }
 
 template <int WM, int TM, int TN, int NA, int NB>
-int launch_wide(BlockArgs w, int max_cus, hipStream_t hs) {
+int launch_wide(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
   using S = WideShape<WM, TM, TN, NA, NB>;
   static std::atomic<bool> ok[2][kMaxDevices];
   const bool tail = w.K % GROUP != 0;
@@ -672,6 +701,10 @@ int launch_wide(BlockArgs w, int max_cus, hipStream_t hs) {
   w.tiles_m = (w.M + S::BM - 1) / S::BM;
   w.tiles_n = (w.N + S::BN - 1) / S::BN;
   int64_t grid = (int64_t)w.tiles_m * w.tiles_n;
+  // Through the L2 at once only where there is a tile a unit at most.  One: [1000, 3696] x [8192, 3696]^T 35.3 us, kept 37.5;
+  // two, the loads of the second beside the stores of the first: [4096, 8192] x [7168, 8192]^T 228, kept 208.
+  const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
+  if (w.form == kWideThrough && grid > units) w.form = kWideStores;
   if (max_cus > 0 && grid > max_cus) grid = max_cus;
   launch_kernel(kernel, dim3((unsigned)grid), dim3(WIDE_THREADS), S::LDS, hs, w);
   return TW_OK;
@@ -703,7 +736,7 @@ int launch_wide_for(const BlockArgs& w, int max_cus, int cus, hipStream_t hs) {
     if (cost < best_cost) best = &t, best_cost = cost;
   }
 #define TW_WIDE_LAUNCH(WM, TM, TN, NA, NB, COST) \
-  if (best->wm == WM && best->tm == TM && best->tn == TN) return launch_wide<WM, TM, TN, NA, NB>(w, max_cus, hs);
+  if (best->wm == WM && best->tm == TM && best->tn == TN) return launch_wide<WM, TM, TN, NA, NB>(w, max_cus, cus, hs);
   TW_WIDE_TILES(TW_WIDE_LAUNCH)
 #undef TW_WIDE_LAUNCH
   return set_error(TW_ERR_INVALID_ARGUMENT, "gemm_fp8_block_nt: no tile for %d rows", w.M);
@@ -773,6 +806,7 @@ int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64
   w.a_scales = a_scales, w.b_scales = b_scales;
   w.scale_row = scale_row, w.scale_block = scale_block, w.ldc = ldc;
   w.M = (int)M, w.N = (int)N, w.K = (int)K, w.half_out = dtype == TW_DTYPE_F16;
+  w.form = ldc > BLOCK_WIDE_LDC ? kNarrowStores : store_form(out, N, ldc);
   const hipStream_t hs = static_cast<hipStream_t>(stream);
   int cus = device_compute_units(), rc;
   if (cus <= 0) cus = 256;

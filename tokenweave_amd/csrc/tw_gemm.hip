@@ -32,6 +32,7 @@
 
 #include "tw_activation.h"
 #include "tw_common.h"
+#include "tw_store.h"
 
 namespace tw {
 
@@ -197,17 +198,6 @@ struct GemmBatch {
   const uint16_t* b[TW_MAX_PARTIALS];
   const uint16_t* bias[TW_MAX_PARTIALS];  // [N] bf16 or null: added to that product only
 };
-
-// How the gated and the "NN" tiles store: 8 bytes a lane, 16, or 16 that go through the L2 at once.  The last only where
-// rows begin on 64 bytes: a lane's group of four stores 64, and where those lie across two pieces of 64 memory gets parts
-// of each, which the L2 puts together if it may keep them.  [4352, 64] x [64, 7944]: 66.6 us through, 19.4 kept (what it
-// still holds then costs the next kernel 12); rows of 8192 go through in 19.7.
-enum StoreForm { kNarrowStores, kWideStores, kWideThrough };
-inline StoreForm store_form(const void* out, int64_t columns, int64_t ldc) {
-  const uintptr_t begin = reinterpret_cast<uintptr_t>(out);
-  if (columns % 8 != 0 || ldc % 8 != 0 || begin % 16 != 0) return kNarrowStores;
-  return ldc % 32 == 0 && begin % 64 == 0 ? kWideThrough : kWideStores;
-}
 
 // The gated form (GATED) of both kernels below: b is [2 I, K], a gate row and an up row for each of the I columns of
 // out, out = act(a gate^T) * (a up^T).  A tile's rows of b are half gate and half up rows of the same columns, so both
@@ -627,15 +617,6 @@ __device__ __forceinline__ void tile_loads(__amdgpu_buffer_rsrc_t da, __amdgpu_b
   for (int l = 0; l < S::LB; ++l)
     if ((S::B0 + l * S::B_STEP >= S::SLOTS) == (HALF == 1))
       __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(sb + l * 1024), 16, vb[l], koff, 0, 0);
-}
-
-constexpr int kStoreThrough = 19;  // nt sc0 sc1
-
-template <typename F>
-__device__ __forceinline__ void with_store_form(int form, F&& f) {
-  if (form == kWideThrough) f(std::integral_constant<StoreForm, kWideThrough>{});
-  else if (form == kWideStores) f(std::integral_constant<StoreForm, kWideStores>{});
-  else f(std::integral_constant<StoreForm, kNarrowStores>{});
 }
 
 // The wave's accumulators: row 16 i of `dc` at voffset + i * row_step.  WIDE: eight columns per
