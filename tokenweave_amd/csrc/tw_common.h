@@ -80,9 +80,14 @@ int run_gemm_bf16_nt_partials(void* const* outs, const void* const* as, const vo
 int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, int64_t M, int64_t I, int64_t K,
                            int64_t ldc, int64_t ld_both, int act, int max_cus, void* stream);
 
-// out[M, N] = a[M, K] b[rows, N]; rows <= K end in the last slab of 64, a's columns from `rows` on are zeros.
-int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t rows, int max_cus,
-                     float* sums, void* stream);
+// out[M, N] = a[M, K] b[rows, N], one or two of them; rows <= K end in the last slab of 64, a's columns from `rows` on are
+// zeros.
+struct NnOperands {
+  void* out;
+  const void *a, *b;
+  int64_t M, K, rows;
+};
+int run_gemm_bf16_nn(const NnOperands* products, int count, int64_t N, int max_cus, float* sums, void* stream);
 int64_t gemm_bf16_nn_workspace(int64_t M, int64_t N, int64_t K);  // bytes of `sums`
 
 int64_t gated_backward_workspace(int64_t M, int64_t I, int64_t K, bool want_a, bool want_b);

@@ -188,10 +188,11 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   if (grid > INT32_MAX) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too large", what);
   launch_kernel(gated_grad_kernel, dim3((unsigned)grid), dim3(GRAD_THREADS), 0, hs, w);
   if (int rc = finish_launch(what)) return rc;
-  if (grad_a)
-    if (int rc = run_gemm_bf16_nn(grad_a, w.d, b, M, K, w.pitch, 2 * I, max_cus, sums, stream)) return rc;
-  if (grad_b) return run_gemm_bf16_nn(grad_b, w.d_turned, a, 2 * I, K, w.pitch_turned, M, max_cus, sums, stream);
-  return TW_OK;
+  NnOperands products[2];
+  int count = 0;
+  if (grad_a) products[count++] = {grad_a, w.d, b, M, w.pitch, 2 * I};
+  if (grad_b) products[count++] = {grad_b, w.d_turned, a, 2 * I, w.pitch_turned, M};
+  return run_gemm_bf16_nn(products, count, K, max_cus, sums, stream);
 }
 
 }  // namespace tw

@@ -1069,13 +1069,26 @@ __device__ __forceinline__ void nn_phase(f32x4_t (&acc)[TM][TN], const bf16x8_t 
 //
 // SPLIT: few tiles.  A tile's slabs are dealt out to `parts` workgroups, `per` each, whose fp32 sums go to sums[part][M][N];
 // nn_sum_kernel adds them in order.
+//
+// A launch may be two products of the same columns, a tile a workgroup: workgroups from `tiles_first` on take `second`'s.
+struct NnProduct {
+  uint16_t* out;
+  const uint16_t *a, *b;
+  int M, K, rows, tiles_m, form;
+};
+
 template <int TM, int TN, bool SPLIT>
 __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nn_kernel(
-    uint16_t* out, const uint16_t* a, const uint16_t* b, int M, int N, int K, int rows, int tiles_m, int tiles_n,
-    int form, float* sums, int parts, int per) {
+    NnProduct first, NnProduct second, int tiles_first, int N, int tiles_n, float* sums, int parts, int per) {
 #ifdef __HIP_DEVICE_COMPILE__
   using S = TileShape<TM, TN>;
   static_assert(TN % 2 == 0, "whole groups of eight chunks a row");
+  const bool other = (int)blockIdx.x >= tiles_first;
+  uint16_t* const out = other ? second.out : first.out;
+  const uint16_t *const a = other ? second.a : first.a, *const b = other ? second.b : first.b;
+  const int M = other ? second.M : first.M, K = other ? second.K : first.K, rows = other ? second.rows : first.rows;
+  const int tiles_m = other ? second.tiles_m : first.tiles_m, form = other ? second.form : first.form;
+  const int t0 = (int)blockIdx.x - (other ? tiles_first : 0);
   constexpr int LA = S::LA, LB = S::LB, PA = S::PA, PB = S::PB, D = S::D;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_tile[];
   lds_u8_t* const lds_a = (lds_u8_t*)lds_tile;
@@ -1113,7 +1126,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     vb[l] = (uint32_t)row * (uint32_t)N * 2u + (uint32_t)(((place % (4 * TN)) ^ (2 * nn_key(TN, row))) << 4);
   }
   // Load cursor: slab lk, before l_end, of tile lt; past the last tile it stays at slab 0 of empty descriptors.
-  int lt = blockIdx.x, lk = 0, l_end = nk;
+  int lt = t0, lk = 0, l_end = nk;
   __amdgpu_buffer_rsrc_t da, db;
   TilePlace lp;
   auto place = [&]() {
@@ -1176,8 +1189,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     TW_RING(fill_a, PA, S::SA);                                                                                \
     TW_RING(fill_b, PB, S::SB);                                                                                \
   } while (0)
-  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-    TW_NN_SLAB(true, t != (int)blockIdx.x);
+  for (int t = t0; t < num_tiles; t += gridDim.x) {
+    TW_NN_SLAB(true, t != t0);
     const int slabs = slabs_of(first_slab(t));
     for (int kt = 1; kt < slabs; ++kt) TW_NN_SLAB(false, false);
     const TilePlace p = tile_of(t);
@@ -1492,51 +1505,91 @@ int64_t gemm_bf16_nn_workspace(int64_t M, int64_t N, int64_t K) {
   return s.parts > 1 ? 4 * s.parts * M * N : 0;
 }
 
+// One product, or two (`count`) with a tile a unit at most.
 template <int TM, int TN, bool SPLIT = false>
-static int launch_nn(uint16_t* out, const uint16_t* a, const uint16_t* b, int64_t M, int64_t N, int64_t K, int64_t rows,
-                     int units, float* sums, const NnSplit& split, hipStream_t hs) {
+static int launch_nn(const NnOperands* w, int count, int64_t N, int units, float* sums, const NnSplit& split, hipStream_t hs) {
   using S = TileShape<TM, TN>;
   static std::atomic<bool> lds_ok[kMaxDevices];
   const auto kernel = gemm_bf16_nn_kernel<TM, TN, SPLIT>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, S::LDS)) return rc;
-  const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + S::BN - 1) / S::BN);
-  const int64_t grid = std::min<int64_t>((int64_t)tiles_m * tiles_n * split.parts, units);
-  launch_kernel(kernel, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, out, a, b, (int)M, (int)N, (int)K, (int)rows,
-                tiles_m, tiles_n, store_form(out, N, N), sums, split.parts, split.per);
+  const int tiles_n = (int)((N + S::BN - 1) / S::BN);
+  NnProduct p[2] = {};
+  for (int i = 0; i < count; ++i)
+    p[i] = {static_cast<uint16_t*>(w[i].out), static_cast<const uint16_t*>(w[i].a), static_cast<const uint16_t*>(w[i].b),
+            (int)w[i].M, (int)w[i].K, (int)w[i].rows, (int)((w[i].M + S::BM - 1) / S::BM), store_form(w[i].out, N, N)};
+  const int64_t tiles = (int64_t)(p[0].tiles_m + p[1].tiles_m) * tiles_n * split.parts;
+  launch_kernel(kernel, dim3((unsigned)std::min<int64_t>(tiles, units)), dim3(TILE_THREADS), S::LDS, hs, p[0], p[1],
+                count > 1 ? p[0].tiles_m * tiles_n : INT32_MAX, (int)N, tiles_n, sums, split.parts, split.per);
   return TW_OK;
 }
 
-// out[M, N] = a[M, K] b[rows, N], everything contiguous, K a multiple of 64, N of 8, rows <= K, the last of them in the last
-// slab of 64, and a's columns from `rows` on zeros; a 16-byte aligned, out and b 8; sums: gemm_bf16_nn_workspace bytes.
-// (Whole slabs are whole lines, each of which a unit requests once: [300, 7392] x [7392, 8192] 102 us with a's rows 7392
-// long, 61 with 7424; 256 rows 85 and 53.)
-int run_gemm_bf16_nn(void* out, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t rows, int max_cus,
-                     float* sums, void* stream) {
-  const char* what = "gemm_bf16_nn";
-  if (K > TILE_MAX_K || N > TILE_MAX_LDC)  // 32-bit offsets of a tile's rows of a and out, of 64 rows of b
-    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: an inner dimension of %lld or rows of %lld values are too long", what,
-                     (long long)K, (long long)N);
-  const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
-  const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
-  uint16_t* const o = static_cast<uint16_t*>(out);
-  const uint16_t *const x = static_cast<const uint16_t*>(a), *const y = static_cast<const uint16_t*>(b);
-  const hipStream_t hs = static_cast<hipStream_t>(stream);
-  NnSplit split = nn_split(M, N, K);
-  int rc = TW_OK;
-  if (split.parts > 1) {
-    rc = launch_nn<2, 4, true>(o, x, y, M, N, K, rows, units, sums, split, hs);
-    if (rc) return rc;
-    if ((rc = finish_launch(what))) return rc;
-    launch_kernel(nn_sum_kernel, dim3((unsigned)((M * N / 4 + NN_SUM_THREADS - 1) / NN_SUM_THREADS)), dim3(NN_SUM_THREADS), 0,
-                  hs, o, sums, M * N, split.parts);
-    return finish_launch(what);
-  }
-  const TileChoice& t = pick_tile(M, N, 1, units);
+static int launch_nn_tile(const TileChoice& t, const NnOperands* w, int count, int64_t N, int units, hipStream_t hs) {
 #define TW_NN_TILE(TM, TN, COST) \
-  if (t.tm == TM && t.tn == TN) rc = launch_nn<TM, TN>(o, x, y, M, N, K, rows, units, nullptr, split, hs);
+  if (t.tm == TM && t.tn == TN) return launch_nn<TM, TN>(w, count, N, units, nullptr, {1, 0}, hs);
   TW_TILES(TW_NN_TILE)
 #undef TW_NN_TILE
-  return rc ? rc : finish_launch(what);
+  return set_error(TW_ERR_INVALID_ARGUMENT, "gemm_bf16_nn: no %d x %d tile", 32 * t.tm, 32 * t.tn);
+}
+
+// The tile with which two products take a unit a tile at most, if one launch of it takes less than the two of their own:
+// a round of 256 x 256 tiles takes 1.5 us a slab (kTiles has the others) and whatever its tile some 4.5 us more.
+static const TileChoice* pick_tile_of_two(const NnOperands* w, int64_t N, int units) {
+  constexpr double FIXED = 3.0;  // in slabs of 256 x 256
+  double apart = 0;
+  for (int i = 0; i < 2; ++i) {
+    const TileChoice& t = pick_tile(w[i].M, N, 1, units);
+    const int64_t tiles = ((w[i].M + 32 * t.tm - 1) / (32 * t.tm)) * ((N + 32 * t.tn - 1) / (32 * t.tn));
+    apart += (double)((tiles + units - 1) / units) * t.cost * (double)(w[i].K / BK) + FIXED;
+  }
+  const TileChoice* best = nullptr;
+  for (const TileChoice& t : kTiles) {
+    const int64_t bm = 32 * t.tm, bn = 32 * t.tn;
+    const int64_t tiles = ((w[0].M + bm - 1) / bm + (w[1].M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    const double cost = t.cost * (double)(std::max(w[0].K, w[1].K) / BK) + FIXED;
+    if (tiles <= units && cost < apart) best = &t, apart = cost;
+  }
+  return best;
+}
+
+// out[M, N] = a[M, K] b[rows, N] for `count` (one or two) products, everything contiguous, K a multiple of 64, N of 8, rows
+// <= K, the last of them in the last slab of 64, and a's columns from `rows` on zeros; a 16-byte aligned, out and b 8; sums:
+// the most bytes that gemm_bf16_nn_workspace says for one.
+// (Whole slabs are whole lines, each of which a unit requests once: [300, 7392] x [7392, 8192] 102 us with a's rows 7392
+// long, 61 with 7424; 256 rows 85 and 53.)
+//
+// Two small ones share a launch: [1001, 1408] x [1408, 1024] beside [1408, 1024] x [1024, 1024] 14.3 us, in launches of
+// their own 12.8 and 9.2; 300 rows 11.6, 12.6 and 5.2.
+int run_gemm_bf16_nn(const NnOperands* w, int count, int64_t N, int max_cus, float* sums, void* stream) {
+  const char* what = "gemm_bf16_nn";
+  for (int i = 0; i < count; ++i)
+    if (w[i].K > TILE_MAX_K || N > TILE_MAX_LDC)  // 32-bit offsets of a tile's rows of a and out, of 64 rows of b
+      return set_error(TW_ERR_INVALID_ARGUMENT, "%s: an inner dimension of %lld or rows of %lld values are too long", what,
+                       (long long)w[i].K, (long long)N);
+  const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
+  const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
+  const hipStream_t hs = static_cast<hipStream_t>(stream);
+  NnSplit split[2] = {};
+  for (int i = 0; i < count; ++i) split[i] = nn_split(w[i].M, N, w[i].K);
+  if (count == 2 && split[0].parts == 1 && split[1].parts == 1)
+    if (const TileChoice* t = pick_tile_of_two(w, N, units)) {
+      const int rc = launch_nn_tile(*t, w, 2, N, units, hs);
+      return rc ? rc : finish_launch(what);
+    }
+  for (int i = 0; i < count; ++i) {
+    int rc;
+    if (split[i].parts == 1) {
+      rc = launch_nn_tile(pick_tile(w[i].M, N, 1, units), w + i, 1, N, units, hs);
+    } else {
+      if ((rc = launch_nn<2, 4, true>(w + i, 1, N, units, sums, split[i], hs))) return rc;
+      if ((rc = finish_launch(what))) return rc;
+      const int64_t values = w[i].M * N;
+      launch_kernel(nn_sum_kernel, dim3((unsigned)((values / 4 + NN_SUM_THREADS - 1) / NN_SUM_THREADS)), dim3(NN_SUM_THREADS),
+                    0, hs, static_cast<uint16_t*>(w[i].out), sums, values, split[i].parts);
+    }
+    if (rc) return rc;
+    if ((rc = finish_launch(what))) return rc;
+  }
+  return TW_OK;
 }
 
 // act(a b[:I]^T) * (a b[I:]^T).
