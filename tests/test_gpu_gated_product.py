@@ -217,3 +217,28 @@ def test_what_a_workspace_held_does_not_matter(M, inner, K):
         if before:
             assert torch.equal(gx, before[0]) and torch.equal(gw, before[1])
         before = gx.clone(), gw.clone()
+
+
+@pytest.mark.parametrize("M,inner,K", [(129, 136, 72), (300, 8, 64), (257, 100, 72), (1001, 704, 264), (4096, 3584, 64),
+                                       (2458, 1376, 192), (64, 136, 72)])
+@pytest.mark.parametrize("kind", R.ACTIVATIONS)
+def test_outputs_that_begin_anywhere(M, inner, K, kind):
+    """out and gate_up 8, 16 and 64 bytes into a buffer, apart from one another: the same bits, and nothing beside them."""
+    x, w = make(M, inner, K)
+
+    def place(width, step):
+        buf = torch.full((M + 2, (width + step - 1) // step * step + 2 * step), 777.0, dtype=BF16, device="cuda")
+        return buf, buf[1:1 + M, step:step + width]
+
+    plain, both = (torch.empty((M, n), dtype=BF16, device="cuda") for n in (inner, 2 * inner))
+    ops.gated_gemm_bf16_nt(plain, x, w, kind, gate_up=both)
+    want, bound, products, off = R.gated(x, w, kind)
+    R.assert_within(plain, want, bound, "out")
+    R.assert_within(both, products, off, "gate_up")
+    for step, step_both in ((4, 32), (8, 8), (32, 4), (32, 8), (8, 32), (32, 32)):
+        buf, out = place(inner, step)
+        both_buf, kept = place(2 * inner, step_both)
+        ops.gated_gemm_bf16_nt(out, x, w, kind, gate_up=kept)
+        assert torch.equal(out, plain) and torch.equal(kept, both), (step, step_both)
+        out.fill_(777.0), kept.fill_(777.0)
+        assert (buf == 777.0).all() and (both_buf == 777.0).all(), (step, step_both)

@@ -205,7 +205,7 @@ struct GemmBatch {
 // once.  `both`, where given, also takes the two sums, rounded: [M][2 I], what the gradient needs.
 //
 // The product takes the time of the plain one over the same rows of b: [4096, 8192] x [7168, 8192]^T 337 us, plain 340
-// (1 430 TFLOP/s; the tile loop is the bound, see there), with `both` 348; one row 20.4 us (117 MB of weights at 5.7 TB/s),
+// (1 430 TFLOP/s; the tile loop is the bound, see there), 5 more with `both` (in pieces of 8 bytes 11); one row 20.4 us (117 MB of weights at 5.7 TB/s),
 // 61 rows x [7392, 8192]^T 29.7 (4.1 TB/s: what a unit has under way is shared with a).  The activation is known outside the
 // loops that apply it: chosen per value the same call took 361, and [1001, 1024] x [1408, 1024]^T 9.3 instead of 8.6.
 struct GatedOut {
@@ -660,7 +660,7 @@ __device__ __forceinline__ float acc_read(float x) {
 }
 
 // The gated form: tiles 4 p .. 4 p + 3 of a row of tiles are gate, up, gate, up of eight columns, 32 p + 8 quad and up.
-// Rows of 8 bytes' alignment or I % 8 != 0 (narrow) take two stores.
+// Rows of 8 bytes' alignment or I % 8 != 0 (narrow) take two stores.  gate_up's stay in the L2, the gradient reads them.
 template <int TM, int TN, StoreForm FORM, int ACT>
 __device__ __forceinline__ void tile_store_gated(const f32x4_t (&acc)[TM][TN], __amdgpu_buffer_rsrc_t dc,
                                                  uint32_t row_off, uint32_t row_step, int n, int N, int m, int M,
@@ -670,20 +670,32 @@ __device__ __forceinline__ void tile_store_gated(const f32x4_t (&acc)[TM][TN], _
 #pragma unroll
     for (int p = 0; p < TN / 4; ++p) {
       const int c = n + p * 32;
-      u32x2_t v[2];
+      u32x2_t v[2], gate[2], up[2];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float g[4], u[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) g[e] = acc_read(acc[i][4 * p + 2 * s][e]), u[e] = acc_read(acc[i][4 * p + 2 * s + 1][e]);
-        if (gated.both && m + 16 * i < M && c + 4 * s < N) {
-          uint16_t* to = gated.both + (size_t)(m + 16 * i) * gated.ld_both + c + 4 * s;
-          *reinterpret_cast<uint2*>(to) = make_uint2(pack2(g[0], g[1]), pack2(g[2], g[3]));
-          *reinterpret_cast<uint2*>(to + N) = make_uint2(pack2(u[0], u[1]), pack2(u[2], u[3]));
-        }
+        gate[s] = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])}, up[s] = u32x2_t{pack2(u[0], u[1]), pack2(u[2], u[3])};
 #pragma unroll
         for (int e = 0; e < 4; ++e) g[e] = activation<ACT>(g[e]) * u[e];
         v[s] = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+      }
+      if (gated.both && m + 16 * i < M) {
+        uint16_t* const to = gated.both + (size_t)(m + 16 * i) * gated.ld_both + c;
+        if (FORM != kNarrowStores) {
+          if (c < N) {
+            *reinterpret_cast<u32x4_t*>(to) = u32x4_t{gate[0].x, gate[0].y, gate[1].x, gate[1].y};
+            *reinterpret_cast<u32x4_t*>(to + N) = u32x4_t{up[0].x, up[0].y, up[1].x, up[1].y};
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            if (c + 4 * s < N) {
+              *reinterpret_cast<u32x2_t*>(to + 4 * s) = gate[s];
+              *reinterpret_cast<u32x2_t*>(to + N + 4 * s) = up[s];
+            }
+        }
       }
       const uint32_t off = row_off + (uint32_t)i * row_step + (uint32_t)p * 64u;
       if (FORM == kNarrowStores) {
@@ -1384,7 +1396,10 @@ static int launch_tile_kernel(const GemmBatch& batch, int count, int64_t M, int6
   int wide_store = (N % 8 == 0 && ldc % 8 == 0) ? 1 : 0;
   for (int p = 0; p < count; ++p)
     if (reinterpret_cast<uintptr_t>(batch.out[p]) & 15u) wide_store = 0;
-  if (GATED) wide_store = store_form(batch.out[0], N, ldc);
+  if constexpr (GATED) {
+    wide_store = store_form(batch.out[0], N, ldc);
+    if (gated.both && store_form(gated.both, N, gated.ld_both) == kNarrowStores) wide_store = kNarrowStores;
+  }
   launch_kernel(gemm_bf16_nt_tile_kernel<TM, TN, ROWS, GATED>, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs,
                 batch, count, (int)M, (int)N, (int)K, ldc, tiles_m, tiles_n, wide_store, gated);
   return TW_OK;
