@@ -242,3 +242,23 @@ def test_outputs_that_begin_anywhere(M, inner, K, kind):
         assert torch.equal(out, plain) and torch.equal(kept, both), (step, step_both)
         out.fill_(777.0), kept.fill_(777.0)
         assert (buf == 777.0).all() and (both_buf == 777.0).all(), (step, step_both)
+
+
+@pytest.mark.parametrize("M,inner,K", [(129, 100, 72), (1001, 704, 264), (1000, 1376, 520), (2458, 260, 1024), (4096, 512, 64),
+                                       (700, 2100, 136)])
+@pytest.mark.parametrize("max_cus", [None, 1, 7, 24, 100])
+def test_gradients_together_and_alone(M, inner, K, max_cus):
+    """Both gradients asked for at once, by whatever share of the units each then has, have the bits of either alone."""
+    x, w = make(M, inner, K)
+    both = torch.empty((M, 2 * inner), dtype=BF16, device="cuda")
+    ops.gated_gemm_bf16_nt(torch.empty((M, inner), dtype=BF16, device="cuda"), x, w, gate_up=both)
+    grad = torch.randn((M, inner), device="cuda").to(BF16)
+    alone = torch.empty_like(x), torch.empty_like(w)
+    ops.gated_gemm_bf16_nt_backward(alone[0], None, grad, x, w, both)
+    ops.gated_gemm_bf16_nt_backward(None, alone[1], grad, x, w, both)
+    want_x, bound_x, want_w, bound_w = R.gated_gradients(grad, x, w, both, "silu")
+    R.assert_within(alone[0], want_x, bound_x, "grad_x")
+    R.assert_within(alone[1], want_w, bound_w, "grad_w")
+    gx, gw = torch.full_like(x, 777.0), torch.full_like(w, 777.0)
+    ops.gated_gemm_bf16_nt_backward(gx, gw, grad, x, w, both, max_cus=max_cus)
+    assert torch.equal(gx, alone[0]) and torch.equal(gw, alone[1])

@@ -1082,7 +1082,8 @@ __device__ __forceinline__ void nn_phase(f32x4_t (&acc)[TM][TN], const bf16x8_t 
 // SPLIT: few tiles.  A tile's slabs are dealt out to `parts` workgroups, `per` each, whose fp32 sums go to sums[part][M][N];
 // nn_sum_kernel adds them in order.
 //
-// A launch may be two products of the same columns, a tile a workgroup: workgroups from `tiles_first` on take `second`'s.
+// A launch may be two products of the same columns, each with workgroups of its own: those from `groups_first` on take
+// `second`'s tiles.
 struct NnProduct {
   uint16_t* out;
   const uint16_t *a, *b;
@@ -1091,16 +1092,17 @@ struct NnProduct {
 
 template <int TM, int TN, bool SPLIT>
 __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nn_kernel(
-    NnProduct first, NnProduct second, int tiles_first, int N, int tiles_n, float* sums, int parts, int per) {
+    NnProduct first, NnProduct second, int groups_first, int N, int tiles_n, float* sums, int parts, int per) {
 #ifdef __HIP_DEVICE_COMPILE__
   using S = TileShape<TM, TN>;
   static_assert(TN % 2 == 0, "whole groups of eight chunks a row");
-  const bool other = (int)blockIdx.x >= tiles_first;
+  const bool other = (int)blockIdx.x >= groups_first;
   uint16_t* const out = other ? second.out : first.out;
   const uint16_t *const a = other ? second.a : first.a, *const b = other ? second.b : first.b;
   const int M = other ? second.M : first.M, K = other ? second.K : first.K, rows = other ? second.rows : first.rows;
   const int tiles_m = other ? second.tiles_m : first.tiles_m, form = other ? second.form : first.form;
-  const int t0 = (int)blockIdx.x - (other ? tiles_first : 0);
+  const int t0 = (int)blockIdx.x - (other ? groups_first : 0);
+  const int stride = other ? (int)gridDim.x - groups_first : min((int)gridDim.x, groups_first);
   constexpr int LA = S::LA, LB = S::LB, PA = S::PA, PB = S::PB, D = S::D;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_tile[];
   lds_u8_t* const lds_a = (lds_u8_t*)lds_tile;
@@ -1159,7 +1161,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   auto advance = [&]() {
     if (lt < num_tiles) ++lk;
     if (lk == l_end) {
-      lt += gridDim.x;
+      lt += stride;
       place();
     }
     slab_of_b();
@@ -1201,7 +1203,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
     TW_RING(fill_a, PA, S::SA);                                                                                \
     TW_RING(fill_b, PB, S::SB);                                                                                \
   } while (0)
-  for (int t = t0; t < num_tiles; t += gridDim.x) {
+  for (int t = t0; t < num_tiles; t += stride) {
     TW_NN_SLAB(true, t != t0);
     const int slabs = slabs_of(first_slab(t));
     for (int kt = 1; kt < slabs; ++kt) TW_NN_SLAB(false, false);
@@ -1520,9 +1522,10 @@ int64_t gemm_bf16_nn_workspace(int64_t M, int64_t N, int64_t K) {
   return s.parts > 1 ? 4 * s.parts * M * N : 0;
 }
 
-// One product, or two (`count`) with a tile a unit at most.
+// One product with groups[0] workgroups at most, or two with `groups` of their own.
 template <int TM, int TN, bool SPLIT = false>
-static int launch_nn(const NnOperands* w, int count, int64_t N, int units, float* sums, const NnSplit& split, hipStream_t hs) {
+static int launch_nn(const NnOperands* w, int count, const int* groups, int64_t N, float* sums, const NnSplit& split,
+                     hipStream_t hs) {
   using S = TileShape<TM, TN>;
   static std::atomic<bool> lds_ok[kMaxDevices];
   const auto kernel = gemm_bf16_nn_kernel<TM, TN, SPLIT>;
@@ -1532,36 +1535,46 @@ static int launch_nn(const NnOperands* w, int count, int64_t N, int units, float
   for (int i = 0; i < count; ++i)
     p[i] = {static_cast<uint16_t*>(w[i].out), static_cast<const uint16_t*>(w[i].a), static_cast<const uint16_t*>(w[i].b),
             (int)w[i].M, (int)w[i].K, (int)w[i].rows, (int)((w[i].M + S::BM - 1) / S::BM), store_form(w[i].out, N, N)};
-  const int64_t tiles = (int64_t)(p[0].tiles_m + p[1].tiles_m) * tiles_n * split.parts;
-  launch_kernel(kernel, dim3((unsigned)std::min<int64_t>(tiles, units)), dim3(TILE_THREADS), S::LDS, hs, p[0], p[1],
-                count > 1 ? p[0].tiles_m * tiles_n : INT32_MAX, (int)N, tiles_n, sums, split.parts, split.per);
+  const int grid = count > 1 ? groups[0] + groups[1]
+                             : (int)std::min<int64_t>((int64_t)p[0].tiles_m * tiles_n * split.parts, groups[0]);
+  launch_kernel(kernel, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, p[0], p[1], count > 1 ? groups[0] : INT32_MAX,
+                (int)N, tiles_n, sums, split.parts, split.per);
   return TW_OK;
 }
 
-static int launch_nn_tile(const TileChoice& t, const NnOperands* w, int count, int64_t N, int units, hipStream_t hs) {
+static int launch_nn_tile(const TileChoice& t, const NnOperands* w, int count, const int* groups, int64_t N, hipStream_t hs) {
 #define TW_NN_TILE(TM, TN, COST) \
-  if (t.tm == TM && t.tn == TN) return launch_nn<TM, TN>(w, count, N, units, nullptr, {1, 0}, hs);
+  if (t.tm == TM && t.tn == TN) return launch_nn<TM, TN>(w, count, groups, N, nullptr, {1, 0}, hs);
   TW_TILES(TW_NN_TILE)
 #undef TW_NN_TILE
   return set_error(TW_ERR_INVALID_ARGUMENT, "gemm_bf16_nn: no %d x %d tile", 32 * t.tm, 32 * t.tn);
 }
 
-// The tile with which two products take a unit a tile at most, if one launch of it takes less than the two of their own:
-// a round of 256 x 256 tiles takes 1.5 us a slab (kTiles has the others) and whatever its tile some 4.5 us more.
-static const TileChoice* pick_tile_of_two(const NnOperands* w, int64_t N, int units) {
+// The tile and the share of the units with which one launch of two products takes the least, if that is less than two
+// launches: kTiles' cost is a slab's, 1.5 us for 256 x 256, and a launch takes some 4.5 us whatever its tile.  A tile a unit
+// where there are enough units, else the shares are whole eights: an XCD then keeps its tiles.
+struct TileOfTwo { const TileChoice* tile; int groups[2]; };
+static TileOfTwo pick_tile_of_two(const NnOperands* w, int64_t N, int units) {
   constexpr double FIXED = 3.0;  // in slabs of 256 x 256
-  double apart = 0;
+  auto tiles_of = [&](int i, const TileChoice& t) {
+    return (int64_t)((w[i].M + 32 * t.tm - 1) / (32 * t.tm)) * ((N + 32 * t.tn - 1) / (32 * t.tn));
+  };
+  const int64_t slabs[2] = {w[0].K / BK, w[1].K / BK};
+  double least = FIXED;
   for (int i = 0; i < 2; ++i) {
     const TileChoice& t = pick_tile(w[i].M, N, 1, units);
-    const int64_t tiles = ((w[i].M + 32 * t.tm - 1) / (32 * t.tm)) * ((N + 32 * t.tn - 1) / (32 * t.tn));
-    apart += (double)((tiles + units - 1) / units) * t.cost * (double)(w[i].K / BK) + FIXED;
+    least += (double)((tiles_of(i, t) + units - 1) / units * slabs[i]) * t.cost;
   }
-  const TileChoice* best = nullptr;
+  TileOfTwo best = {};
   for (const TileChoice& t : kTiles) {
-    const int64_t bm = 32 * t.tm, bn = 32 * t.tn;
-    const int64_t tiles = ((w[0].M + bm - 1) / bm + (w[1].M + bm - 1) / bm) * ((N + bn - 1) / bn);
-    const double cost = t.cost * (double)(std::max(w[0].K, w[1].K) / BK) + FIXED;
-    if (tiles <= units && cost < apart) best = &t, apart = cost;
+    const int64_t tiles[2] = {tiles_of(0, t), tiles_of(1, t)};
+    auto consider = [&](int64_t x, int64_t y) {
+      const int64_t longest = std::max((tiles[0] + x - 1) / x * slabs[0], (tiles[1] + y - 1) / y * slabs[1]);
+      if (t.cost * (double)longest < least) best = {&t, {(int)x, (int)y}}, least = t.cost * (double)longest;
+    };
+    if (tiles[0] + tiles[1] <= units) consider(tiles[0], tiles[1]);
+    else
+      for (int x = 8; x < units; x += 8) consider(x, units - x);
   }
   return best;
 }
@@ -1572,8 +1585,10 @@ static const TileChoice* pick_tile_of_two(const NnOperands* w, int64_t N, int un
 // (Whole slabs are whole lines, each of which a unit requests once: [300, 7392] x [7392, 8192] 102 us with a's rows 7392
 // long, 61 with 7424; 256 rows 85 and 53.)
 //
-// Two small ones share a launch: [1001, 1408] x [1408, 1024] beside [1408, 1024] x [1024, 1024] 14.3 us, in launches of
-// their own 12.8 and 9.2; 300 rows 11.6, 12.6 and 5.2.
+// Two share a launch where that is less: [1001, 1408] x [1408, 1024] beside [1408, 1024] x [1024, 1024] 14.3 us, in launches
+// of their own 12.8 and 9.2; 300 rows 11.6, 12.6 and 5.2.  Large ones have a last round each that leaves units without a
+// tile: [4096, 7168] x [7168, 8192] beside [7168, 4096] x [4096, 8192], half of the units each, 4 and 7 rounds of 256 x 256
+// tiles, 785 us, by themselves 379 and 441.
 int run_gemm_bf16_nn(const NnOperands* w, int count, int64_t N, int max_cus, float* sums, void* stream) {
   const char* what = "gemm_bf16_nn";
   for (int i = 0; i < count; ++i)
@@ -1586,16 +1601,16 @@ int run_gemm_bf16_nn(const NnOperands* w, int count, int64_t N, int max_cus, flo
   NnSplit split[2] = {};
   for (int i = 0; i < count; ++i) split[i] = nn_split(w[i].M, N, w[i].K);
   if (count == 2 && split[0].parts == 1 && split[1].parts == 1)
-    if (const TileChoice* t = pick_tile_of_two(w, N, units)) {
-      const int rc = launch_nn_tile(*t, w, 2, N, units, hs);
+    if (const TileOfTwo two = pick_tile_of_two(w, N, units); two.tile) {
+      const int rc = launch_nn_tile(*two.tile, w, 2, two.groups, N, hs);
       return rc ? rc : finish_launch(what);
     }
   for (int i = 0; i < count; ++i) {
     int rc;
     if (split[i].parts == 1) {
-      rc = launch_nn_tile(pick_tile(w[i].M, N, 1, units), w + i, 1, N, units, hs);
+      rc = launch_nn_tile(pick_tile(w[i].M, N, 1, units), w + i, 1, &units, N, hs);
     } else {
-      if ((rc = launch_nn<2, 4, true>(w + i, 1, N, units, sums, split[i], hs))) return rc;
+      if ((rc = launch_nn<2, 4, true>(w + i, 1, &units, N, sums, split[i], hs))) return rc;
       if ((rc = finish_launch(what))) return rc;
       const int64_t values = w[i].M * N;
       launch_kernel(nn_sum_kernel, dim3((unsigned)((values / 4 + NN_SUM_THREADS - 1) / NN_SUM_THREADS)), dim3(NN_SUM_THREADS),
