@@ -427,8 +427,9 @@ TW_API int tw_gated_gemm_bf16_nt(void* out, void* gate_up, const void* a, const 
 /* Its gradients, with D = [grad_out * U * act'(G), grad_out * act(G)] rounded to bf16:
  *   grad_a[M, K] = D b,  grad_b[2 I, K] = D^T a     (either may be NULL; contiguous)
  * K and, for grad_a, 2 I and, for grad_b, M at most 2^21.
- * workspace: tw_gated_gemm_bf16_nt_backward_workspace() bytes, 256-byte aligned, contents of no
- * meaning before and after; calls that may run at the same time need one each. */
+ * workspace: tw_gated_gemm_bf16_nt_backward_workspace() bytes (asked with the same device current,
+ * for the gradients that are wanted), 256-byte aligned, contents of no meaning before and after;
+ * calls that may run at the same time need one each. */
 TW_API int64_t tw_gated_gemm_bf16_nt_backward_workspace(int64_t M, int64_t I, int64_t K, int want_a,
                                                         int want_b);
 TW_API int tw_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad_out,

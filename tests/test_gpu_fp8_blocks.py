@@ -304,3 +304,17 @@ def test_outputs_that_begin_anywhere(M, N, K, dtype):
         assert torch.equal(out, plain), step
         out.fill_(777.0)
         assert (buf == 777.0).all(), step
+
+
+@pytest.mark.parametrize("M", [130, 300])
+def test_rows_of_the_output_far_apart(M):
+    """Strides on both sides of what a 32-bit offset of a tile's rows reaches."""
+    x, sx, w, sw = operands(M, 40, 272)
+    plain = torch.empty((M, 40), dtype=torch.bfloat16, device="cuda")
+    ops.gemm_fp8_block_nt(plain, x, sx, w, sw)
+    for stride in (1 << 22, (1 << 22) + 64):
+        buf = torch.empty(M * stride, dtype=torch.bfloat16, device="cuda")
+        out = buf.as_strided((M, 48), (stride, 1))
+        out.fill_(777.0)
+        ops.gemm_fp8_block_nt(out[:, :40], x, sx, w, sw)
+        assert torch.equal(out[:, :40], plain) and (out[:, 40:] == 777.0).all(), stride
