@@ -419,10 +419,15 @@ TW_API int tw_kv4_attention(const tw_heads* out, const tw_heads* q, const void* 
  * fp32, the result rounded once.  b is one contiguous [2 I, K] (gate rows, then up rows), out has
  * rows of stride ldc.  gate_up, where not NULL, takes G and U, rounded, as [M, 2 I] (stride
  * ld_gate_up): what the gradient needs.  K % 8 == 0, K <= 2^24, I % 4 == 0, strides % 4 == 0; a, b
- * 16-byte, out, gate_up 8-byte aligned; max_cus as for tw_gemm_bf16_nt. */
+ * 16-byte, out, gate_up 8-byte aligned; max_cus as for tw_gemm_bf16_nt.
+ * workspace: tw_gated_gemm_bf16_nt_workspace() bytes (asked with the same device current; 0 for
+ * most sizes: fp32 sums where some hundred rows are divided along K), 256-byte aligned, contents of
+ * no meaning before and after; calls that may run at the same time need one each. */
+TW_API int64_t tw_gated_gemm_bf16_nt_workspace(int64_t M, int64_t I, int64_t K);
 TW_API int tw_gated_gemm_bf16_nt(void* out, void* gate_up, const void* a, const void* b, int64_t M,
                                  int64_t I, int64_t K, int64_t ldc, int64_t ld_gate_up,
-                                 int activation, int max_cus, void* stream);
+                                 int activation, int max_cus, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
 
 /* Its gradients, with D = [grad_out * U * act'(G), grad_out * act(G)] rounded to bf16:
  *   grad_a[M, K] = D b,  grad_b[2 I, K] = D^T a     (either may be NULL; contiguous)

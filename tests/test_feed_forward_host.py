@@ -11,8 +11,8 @@ AT = (ctypes.addressof(BUF) + 255) & ~255   # host memory: never read by these c
 BAD, ALIGN, DTYPE = _lib.TW_ERR_INVALID_ARGUMENT, _lib.TW_ERR_ALIGNMENT, _lib.TW_ERR_DTYPE
 
 
-def gated(out=AT, both=None, a=AT, b=AT, M=4, inner=8, K=16, ldc=8, ld_both=0, act=0):
-    return _lib.lib().tw_gated_gemm_bf16_nt(out, both, a, b, M, inner, K, ldc, ld_both, act, 0, None)
+def gated(out=AT, both=None, a=AT, b=AT, M=4, inner=8, K=16, ldc=8, ld_both=0, act=0, ws=None, size=0):
+    return _lib.lib().tw_gated_gemm_bf16_nt(out, both, a, b, M, inner, K, ldc, ld_both, act, 0, ws, size, None)
 
 
 def test_gated_product():
@@ -24,6 +24,20 @@ def test_gated_product():
     for call in (dict(inner=6), dict(K=12), dict(ldc=10), dict(a=AT + 8), dict(b=AT + 8), dict(out=AT + 4),
                  dict(both=AT + 4, ld_both=16)):
         assert gated(**call) == ALIGN, call
+
+
+def test_gated_product_divided_along_k():
+    size = _lib.lib().tw_gated_gemm_bf16_nt_workspace
+    # few rows, many, few slabs, many columns: nothing to add; else the fp32 sums of both products, of some parts
+    for M, inner, K in ((0, 8, 8192), (1, 748, 6904), (32, 748, 6904), (1025, 748, 6904), (300, 704, 440), (4096, 3584, 8192)):
+        assert size(M, inner, K) == 0, (M, inner, K)
+    for M, inner, K in ((96, 748, 6904), (160, 3584, 8192), (160, 748, 6904), (1000, 36, 2048)):
+        assert size(M, inner, K) >= 2 * 8 * M * inner and size(M, inner, K) % (8 * M * inner) == 0, (M, inner, K)
+    assert size(4, 6, 16) == ALIGN and size(-1, 8, 16) == BAD and size(4, 8, 0) == BAD
+    shape = dict(M=160, inner=748, K=6904, ldc=748)
+    need = size(160, 748, 6904)
+    assert gated(**shape) == BAD and gated(**shape, ws=AT, size=need - 1) == BAD
+    assert gated(**shape, ws=AT + 64, size=need) == ALIGN
 
 
 def backward(ga=AT, gb=AT, grad=AT, ld_grad=8, a=AT, b=AT, both=AT, ld_both=16, M=4, inner=8, K=16, act=0, ws=AT, size=None):

@@ -262,3 +262,58 @@ def test_gradients_together_and_alone(M, inner, K, max_cus):
     gx, gw = torch.full_like(x, 777.0), torch.full_like(w, 777.0)
     ops.gated_gemm_bf16_nt_backward(gx, gw, grad, x, w, both, max_cus=max_cus)
     assert torch.equal(gx, alone[0]) and torch.equal(gw, alone[1])
+
+
+@pytest.mark.parametrize("M,inner,K", [(33, 4, 8192), (64, 100, 6152), (96, 748, 6904), (129, 1376, 4096), (160, 748, 6904),
+                                       (160, 3584, 8192), (256, 2048, 6144), (300, 1376, 4096), (256, 3584, 8192), (300, 36, 2048),
+                                       (384, 3584, 8192), (512, 748, 6904), (1000, 36, 2048), (1024, 100, 4104)])
+@pytest.mark.parametrize("kind", R.ACTIVATIONS)
+def test_divided_along_k(M, inner, K, kind):
+    """Some hundred rows, whose inner dimension is dealt out: against 64 bits, under grid caps, from any workspace."""
+    from tokenweave_amd import _lib
+    L = _lib.lib()
+    size = L.tw_gated_gemm_bf16_nt_workspace(M, inner, K)
+    assert size > 0, "this size is not divided any more: the test needs another"
+    x, w, both, out = check_forward(M, inner, K, kind)
+    for max_cus in (1, 24, 100):
+        again, kept = torch.full_like(out, 777.0), torch.full_like(both, 777.0)
+        ops.gated_gemm_bf16_nt(again, x, w, kind, max_cus, gate_up=kept)
+        assert torch.equal(again, out) and torch.equal(kept, both), max_cus
+    space = torch.full((size // 4 + 64,), float("nan"), device="cuda")
+    again = torch.empty((M, inner), dtype=BF16, device="cuda")
+    _lib.check(L.tw_gated_gemm_bf16_nt(again.data_ptr(), None, x.data_ptr(), w.data_ptr(), M, inner, K, inner, 0,
+                                       R.ACTIVATIONS.index(kind), 0, space.data_ptr(), size,
+                                       torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(again, out) and torch.isnan(space[size // 4:]).all()
+
+
+def test_divided_along_k_captured():
+    """Two captured calls beside each other on two streams, replayed between eager ones."""
+    shapes = ((160, 748, 2048), (96, 748, 6904))
+    sets = []
+    for seed, (M, inner, K) in enumerate(shapes):
+        x, w = make(M, inner, K, seed)
+        sets.append((torch.empty((M, inner), dtype=BF16, device="cuda"), x, w))
+    for s in sets:
+        ops.gated_gemm_bf16_nt(*s)
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream() for _ in sets]
+    for s, stream in zip(sets, streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            ops.gated_gemm_bf16_nt(*s)
+    for turn in range(4):
+        wants = []
+        for seed, (s, (M, inner, K)) in enumerate(zip(sets, shapes)):
+            x, w = make(M, inner, K, 10 * turn + seed)
+            s[1].copy_(x), s[2].copy_(w)
+            ops.gated_gemm_bf16_nt(*s)
+            wants.append(s[0].clone())
+            s[0].fill_(777.0)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for s, want in zip(sets, wants):
+            assert torch.equal(s[0], want), turn

@@ -1031,10 +1031,15 @@ def gated_gemm_bf16_nt(out: torch.Tensor, a: torch.Tensor, b: torch.Tensor, acti
     M, inner, K = _check_gated(a, b)
     ldc = _check_rows("out", out, torch.bfloat16, a.device, (M, inner))
     ld_both = 0 if gate_up is None else _check_rows("gate_up", gate_up, torch.bfloat16, a.device, (M, 2 * inner))
+    L = _lib.lib()
     with _on_device(a):
-        _lib.check(_lib.lib().tw_gated_gemm_bf16_nt(
+        need = L.tw_gated_gemm_bf16_nt_workspace(M, inner, K)
+        if need < 0:
+            _lib.check(need)
+        ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
+        _lib.check(L.tw_gated_gemm_bf16_nt(
             out.data_ptr(), None if gate_up is None else gate_up.data_ptr(), a.data_ptr(), b.data_ptr(), M, inner, K,
-            ldc, ld_both, act, _cap(max_cus), _stream_ptr(a)))
+            ldc, ld_both, act, _cap(max_cus), None if ws is None else ws.data_ptr(), need, _stream_ptr(a)))
 
 
 def gated_gemm_bf16_nt_backward(grad_a: Optional[torch.Tensor], grad_b: Optional[torch.Tensor], grad_out: torch.Tensor,

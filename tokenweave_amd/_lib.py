@@ -77,7 +77,8 @@ PROTOTYPES = {
     "tw_kv4_attention_workspace": [_ci, _ci, _ci, _i64, _i64, _i64, _i64, _ci],
     "tw_kv4_attention": [_hp, _hp, _vp, _i64, _ci, _ci, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _ci, _f32, _i64,
                          _ci, _vp, _i64, _vp],
-    "tw_gated_gemm_bf16_nt": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _ci, _ci, _vp],
+    "tw_gated_gemm_bf16_nt_workspace": [_i64, _i64, _i64],
+    "tw_gated_gemm_bf16_nt": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _ci, _ci, _vp, _i64, _vp],
     "tw_gated_gemm_bf16_nt_backward_workspace": [_i64, _i64, _i64, _ci, _ci],
     "tw_gated_gemm_bf16_nt_backward": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _ci, _ci, _vp, _i64,
                                        _vp],
@@ -86,7 +87,7 @@ PROTOTYPES = {
 }
 # what an entry point returns where it is no status code
 RETURNS = {"tw_last_error": ctypes.c_char_p, "tw_kv4_attention_workspace": _i64,
-           "tw_gated_gemm_bf16_nt_backward_workspace": _i64}
+           "tw_gated_gemm_bf16_nt_workspace": _i64, "tw_gated_gemm_bf16_nt_backward_workspace": _i64}
 
 _lib = None
 

@@ -4,9 +4,13 @@
 
 extern "C" {
 
+int64_t tw_gated_gemm_bf16_nt_workspace(int64_t M, int64_t I, int64_t K) { return tw::gated_gemm_workspace(M, I, K); }
+
 int tw_gated_gemm_bf16_nt(void* out, void* gate_up, const void* a, const void* b, int64_t M, int64_t I, int64_t K,
-                          int64_t ldc, int64_t ld_gate_up, int activation, int max_cus, void* stream) {
-  return tw::run_gated_gemm_bf16_nt(out, gate_up, a, b, M, I, K, ldc, ld_gate_up, activation, max_cus, stream);
+                          int64_t ldc, int64_t ld_gate_up, int activation, int max_cus, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  return tw::run_gated_gemm_bf16_nt(out, gate_up, a, b, M, I, K, ldc, ld_gate_up, activation, max_cus, workspace,
+                                    workspace_bytes, stream);
 }
 
 int64_t tw_gated_gemm_bf16_nt_backward_workspace(int64_t M, int64_t I, int64_t K, int want_a, int want_b) {

@@ -78,7 +78,9 @@ int run_gemm_bf16_nt_partials(void* const* outs, const void* const* as, const vo
 
 // out[M, I] = act(a b[:I]^T) * (a b[I:]^T); both: null or [M, 2 I] for the two products.
 int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, int64_t M, int64_t I, int64_t K,
-                           int64_t ldc, int64_t ld_both, int act, int max_cus, void* stream);
+                           int64_t ldc, int64_t ld_both, int act, int max_cus, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+int64_t gated_gemm_workspace(int64_t M, int64_t I, int64_t K);
 
 // out[M, N] = a[M, K] b[rows, N], one or two of them; rows <= K end in the last slab of 64, a's columns from `rows` on are
 // zeros.

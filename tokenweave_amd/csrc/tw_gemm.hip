@@ -217,6 +217,16 @@ struct NotGated {};
 template <bool GATED>
 using GatedArg = std::conditional_t<GATED, GatedOut, NotGated>;
 
+// The tile kernel's slabs dealt out (SPLIT): `count` workgroups share a tile, `per` slabs each, and leave fp32 sums at
+// sums[part][M][N].
+struct SplitOut {
+  float* sums;
+  int per;
+};
+struct NotSplit {};
+template <bool SPLIT>
+using SplitArg = std::conditional_t<SPLIT, SplitOut, NotSplit>;
+
 // ---------------------------------------------------------------------------
 // K-split kernel: few rows (a decode step, a short prefill chunk).  The product is bound by
 // reading b once, so what counts is how many compute units stream it and how evenly.
@@ -760,11 +770,12 @@ __device__ __forceinline__ TilePlace tile_place(int t, int num_tiles, int tiles_
 // tile of columns and a wave's load have one kind, which has its own descriptor.  Row x of the panel is of column
 // 32 (x / 64) + 8 (x / 4 % 4) + 4 (x / 32 % 2) + x % 4 of the tile, so that a lane's accumulators are eight adjacent
 // columns of both.  The panel is swizzled as a's.
-template <int TM, int TN, TileRows ROWS, bool GATED = false>
+template <int TM, int TN, TileRows ROWS, bool GATED = false, bool SPLIT = false>
 __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THREADS) void gemm_bf16_nt_tile_kernel(
     GemmBatch batch, int count, int M, int N, int K, int64_t ldc, int tiles_m, int tiles_n, int wide_store,
-    GatedArg<GATED> gated) {
+    GatedArg<GATED> gated, SplitArg<SPLIT> split) {
 #ifdef __HIP_DEVICE_COMPILE__
+  static_assert(!SPLIT || (!GATED && ROWS != kLines), "plain sums of whole slabs");
   static_assert(!GATED || (TN % 4 == 0 && ROWS != kLines), "gate and up rows alternate in groups of 64");
   using S = TileShape<TM, TN, ROWS>;
   // after a tile: how many stores its first barrier does not wait for
@@ -830,20 +841,32 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
   // its loads ask memory for nothing.  (The hardware compares with the extent less the slab's offset,
   // which for an extent of 0 must not go below 0.)
   int lt = blockIdx.x, lk = 0;
+  // SPLIT: a "product" is a part, slabs `per * part` and up; l_end of them, K's last among them in the last part
+  int l_end = nl;
+  bool last_part = true;
+  auto slabs_of = [&](int part) {
+    if constexpr (SPLIT) return min(split.per, nk - part * split.per);
+    else return nk;
+  };
   __amdgpu_buffer_rsrc_t da, db, du;  // du: b's up rows
 #define TW_TILE_DESCRIPTORS()                                                                                \
   do {                                                                                                       \
     const bool in = lt < num_tiles;                                                                          \
     const TilePlace p = tile_place<TM, TN>(in ? lt : 0, num_tiles, tiles_m, tiles_n);                        \
-    const uint16_t* pa = batch.a[p.product] + (size_t)p.m0 * K;                                              \
-    const uint16_t* pb = batch.b[p.product] + (size_t)(GATED ? p.n0 / 2 : p.n0) * K;                         \
+    const uint16_t* pa = batch.a[SPLIT ? 0 : p.product] + (size_t)p.m0 * K;                                  \
+    const uint16_t* pb = batch.b[SPLIT ? 0 : p.product] + (size_t)(GATED ? p.n0 / 2 : p.n0) * K;             \
+    uint32_t skip = 0;  /* bytes of a row ahead of the part */                                               \
+    if constexpr (SPLIT) {                                                                                   \
+      l_end = slabs_of(p.product), last_part = p.product == count - 1;                                       \
+      skip = (uint32_t)(p.product * split.per) * 128u, pa += skip / 2, pb += skip / 2;                       \
+    }                                                                                                        \
     if (S::LINES) load_phase_a = line_phase(pa), load_phase_b = line_phase(pb);                              \
     da = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pa) - (int)AHEAD / 2, 0,                    \
-                                           in ? (uint32_t)min(M - p.m0, S::BM) * (uint32_t)K * 2u + AHEAD : 0u, \
+                                           in ? (uint32_t)min(M - p.m0, S::BM) * (uint32_t)K * 2u + AHEAD - skip : 0u, \
                                            0x00020000);                                                      \
     db = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pb) - (int)AHEAD / 2, 0,                    \
                                            in ? (uint32_t)(GATED ? min(N - p.n0 / 2, S::BN / 2)              \
-                                                                 : min(N - p.n0, S::BN)) * (uint32_t)K * 2u + AHEAD : 0u, \
+                                                                 : min(N - p.n0, S::BN)) * (uint32_t)K * 2u + AHEAD - skip : 0u, \
                                            0x00020000);                                                      \
     du = !GATED ? db : __builtin_amdgcn_make_buffer_rsrc(                                                    \
         const_cast<uint16_t*>(pb) + (size_t)N * K, 0,                                                        \
@@ -852,21 +875,21 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
 #define TW_TILE_ADVANCE()                                                                                    \
   do {                                                                                                       \
     if (lt < num_tiles) ++lk;                                                                                \
-    if (lk == nl) {                                                                                          \
+    if (lk == (SPLIT ? l_end : nl)) {                                                                        \
       lk = 0;                                                                                                \
       lt += gridDim.x;                                                                                       \
       TW_TILE_DESCRIPTORS();                                                                                 \
       if (S::LINES) TW_TILE_LINE_OFFSETS(0);                                                                 \
-      else if (ROWS == kPartialSlab) TW_TILE_OFFSETS(nk == 1 ? tail_chunks : 8);                             \
+      else if (ROWS == kPartialSlab) TW_TILE_OFFSETS((SPLIT ? l_end : nk) == 1 && last_part ? tail_chunks : 8); \
     } else if (S::LINES && (lk == 1 || lk >= nk - 1)) {                                                      \
       if (lt < num_tiles) TW_TILE_LINE_OFFSETS(lk);                                                          \
-    } else if (ROWS == kPartialSlab && lk == nk - 1) {                                                       \
+    } else if (ROWS == kPartialSlab && lk == (SPLIT ? l_end : nk) - 1 && last_part) {                        \
       TW_TILE_OFFSETS(tail_chunks);                                                                          \
     }                                                                                                        \
   } while (0)
   TW_TILE_DESCRIPTORS();
   if (S::LINES) TW_TILE_LINE_OFFSETS(0);
-  else TW_TILE_OFFSETS(nk == 1 ? tail_chunks : 8);
+  else TW_TILE_OFFSETS((SPLIT ? l_end : nk) == 1 && last_part ? tail_chunks : 8);
 #pragma unroll
   for (int s = 0; s < D; ++s) {
 #pragma unroll
@@ -930,9 +953,27 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
 
   for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
     TW_TILE_SLAB(true, !S::LINES && t != (int)blockIdx.x);
-    for (int kt = 1; kt < nk; ++kt) TW_TILE_SLAB(false, false);
+    const int slabs = SPLIT ? slabs_of(tile_place<TM, TN>(t, num_tiles, tiles_m, tiles_n).product) : nk;
+    for (int kt = 1; kt < slabs; ++kt) TW_TILE_SLAB(false, false);
 
     const TilePlace p = tile_place<TM, TN>(t, num_tiles, tiles_m, tiles_n);
+    if constexpr (SPLIT) {
+      const __amdgpu_buffer_rsrc_t ds = __builtin_amdgcn_make_buffer_rsrc(
+          split.sums + ((size_t)p.product * M + p.m0) * N + p.n0, 0, (uint32_t)min(M - p.m0, S::BM) * (uint32_t)N * 4u,
+          0x00020000);
+      const uint32_t row = (uint32_t)(wm * 16 * TM + r16) * (uint32_t)N;
+      asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMA's result is written
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int c = wn * 16 * TN + quad * 8 + (j >> 1) * 32 + (j & 1) * 4;
+          const f32x4_t v = {acc_read(acc[i][j][0]), acc_read(acc[i][j][1]), acc_read(acc[i][j][2]), acc_read(acc[i][j][3])};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), ds,
+                                                 p.n0 + c < N ? (row + (uint32_t)(16 * i * N + c)) * 4u : TILE_OUT_OF_RANGE, 0, 0);
+        }
+      continue;
+    }
     if constexpr (GATED) {
       const int n0 = p.n0 / 2, col = wn * 8 * TN + quad * 8, row = wm * 16 * TM + r16;
       const __amdgpu_buffer_rsrc_t dc = __builtin_amdgcn_make_buffer_rsrc(
@@ -1403,7 +1444,7 @@ static int launch_tile_kernel(const GemmBatch& batch, int count, int64_t M, int6
     if (gated.both && store_form(gated.both, N, gated.ld_both) == kNarrowStores) wide_store = kNarrowStores;
   }
   launch_kernel(gemm_bf16_nt_tile_kernel<TM, TN, ROWS, GATED>, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs,
-                batch, count, (int)M, (int)N, (int)K, ldc, tiles_m, tiles_n, wide_store, gated);
+                batch, count, (int)M, (int)N, (int)K, ldc, tiles_m, tiles_n, wide_store, gated, NotSplit{});
   return TW_OK;
 }
 
@@ -1622,6 +1663,145 @@ int run_gemm_bf16_nn(const NnOperands* w, int count, int64_t N, int max_cus, flo
   return TW_OK;
 }
 
+static int check_gemm_shape(const char* what, int64_t M, int64_t N, int64_t K, int64_t ldc) {
+  if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX || ldc < N)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad shape M=%lld N=%lld K=%lld ldc=%lld", what, (long long)M,
+                     (long long)N, (long long)K, (long long)ldc);
+  if (K % 8 != 0 || N % 4 != 0 || ldc % 4 != 0)
+    return set_error(TW_ERR_ALIGNMENT, "%s: needs K %% 8 == 0, N %% 4 == 0, ldc %% 4 == 0", what);
+  return TW_OK;
+}
+
+// A product of some hundred rows whose slabs are dealt out: larger tiles, of which a unit reads fewer lines, and units for
+// narrow products; the sums, in fp32, are added by another launch.
+//
+// All times in us: a slab of a 256 x 256 tile 1.6 where rows are not whole lines, else 1.4 where the last-level cache does
+// not keep three sets of weights, 1.1 where it does (the other tiles as kTiles has them), a launch of tiles 4.5 besides, the one that adds 4 and the sums' way to memory
+// and back; nothing reads b faster than memory gives it (of forms that this makes equal, the one with the shorter slabs).  Gated products, three sets
+// of weights in turn, us, undivided / by this rule: [160, 8192] x [7168, 8192]^T 52 / 43, 256 rows 57 / 50, 384 rows 64 / 59;
+// [160, 6144] x [4096, 6144]^T 29.5 / 18.1, 256: 30.5 / 22.7; [256, 4096] x [2752, 4096]^T 18.6 / 16.7; [96, 6904] x [1496,
+// 6904]^T 22.9 / 14.5, 160: 47.9 / 15.8, 512: 47.8 / 25.0; [64, 8192] x [896, 8192]^T 15.1 / 11.6.  It loses a twentieth at
+// [300, 8192] x [7168, 8192]^T (53.6 / 55.9).  Where it leaves a product whole dividing it was no gain or a loss: [512, 8192] x
+// [7168, 8192]^T 72 / 71, [256, 1024] x [1408, 1024]^T 7.6 / 9.9, [64, 8192] x [7168, 8192]^T 29 / 32.
+constexpr double SPLIT_LAUNCH_US = 4.5, SPLIT_JOIN_US = 4.0, SPLIT_SUMS_A_US = 6e6, SPLIT_BYTES_A_US = 5e6, SPLIT_SAVES_US = 1.5;
+static double split_slab_us(int64_t N, int64_t K) {
+  return K % BK != 0 ? 1.6 : 2.0 * (double)N * (double)K > KS_STREAM_BYTES ? 1.4 : 1.1;
+}
+constexpr int64_t SPLIT_MAX_ROWS = 1024, SPLIT_MIN_SLABS = 4;  // slabs of a part
+#define TW_SPLIT_TILES(X) X(2, 4) X(3, 4) X(4, 4) X(4, 8)
+struct TileSplit { int tm, tn, parts, per; };
+
+// The shape and the parts that take least, if that saves something against `undivided`; else parts is 1.  The rows, N and
+// K decide, no grid cap: the parts' sums differ in the order of the additions.
+static TileSplit pick_split(int64_t M, int64_t N, int64_t K, double undivided, int cus) {
+  const int64_t nk = (K + BK - 1) / BK;
+  TileSplit best = {0, 0, 1, (int)nk};
+  double least = undivided - SPLIT_SAVES_US;
+  const double slab_us = split_slab_us(N, K), from_memory = 2.0 * (double)N * (double)K / SPLIT_BYTES_A_US;
+  for (const TileChoice& t : kTiles) {
+    bool built = false;
+#define TW_SPLIT_BUILT(TM, TN) built = built || (t.tm == TM && t.tn == TN);
+    TW_SPLIT_TILES(TW_SPLIT_BUILT)
+#undef TW_SPLIT_BUILT
+    if (!built) continue;
+    const int64_t tiles = ((M + 32 * t.tm - 1) / (32 * t.tm)) * ((N + 32 * t.tn - 1) / (32 * t.tn));
+    for (int64_t parts = 2; parts * tiles <= cus && parts * SPLIT_MIN_SLABS <= nk; ++parts) {
+      const int64_t per = (nk + parts - 1) / parts;
+      const double sums = 8.0 * (double)parts * (double)M * (double)N / SPLIT_SUMS_A_US;
+      const double slabs = slab_us * t.cost * (double)per;
+      const double us = std::max(slabs, from_memory) + 0.1 * slabs + SPLIT_LAUNCH_US + SPLIT_JOIN_US + sums;
+      if (us < least) least = us, best = {t.tm, t.tn, (int)((nk + per - 1) / per), (int)per};
+    }
+  }
+  return best;
+}
+
+// Undivided, up to 128 rows: a row tile's and a column tile's rows at 65 GB/s a unit.
+static TileSplit gated_split(int64_t M, int64_t I, int64_t K) {
+  const int64_t N = 2 * I, nk = (K + BK - 1) / BK;
+  TileSplit whole = {0, 0, 1, (int)nk};
+  if (M <= 32 || M > SPLIT_MAX_ROWS || nk < 2 * SPLIT_MIN_SLABS || K > TILE_MAX_K || N > TILE_MAX_LDC) return whole;
+  int cus = device_compute_units();
+  if (cus <= 0) cus = 256;
+  double us;
+  if (M > 128) {
+    const TileChoice& t = pick_tile(M, N, 1, cus, true);
+    const int64_t tiles = ((M + 32 * t.tm - 1) / (32 * t.tm)) * ((N + 32 * t.tn - 1) / (32 * t.tn));
+    us = SPLIT_LAUNCH_US + split_slab_us(N, K) * t.cost * (double)((tiles + cus - 1) / cus * nk);
+  } else {
+    const KsForm f = ksplit_form(M, N, K, 1, 0, cus);
+    const KsTiles tiles = ksplit_tiles(M, I, 1, 8 * f.la, 16 * f.nt, cus);
+    us = 2.5 + (double)((tiles.m * tiles.n + cus - 1) / cus * (8 * f.la + 2 * tiles.cols)) * 2.0 * (double)K / 65e3;
+  }
+  return pick_split(M, N, K, us, cus);
+}
+
+int64_t gated_gemm_workspace(int64_t M, int64_t I, int64_t K) {
+  if (int rc = check_gemm_shape("gated_gemm_bf16_nt_workspace", M, I, K, I)) return rc;
+  const TileSplit s = gated_split(M, I, K);
+  return s.parts > 1 ? 8 * s.parts * M * I : 0;
+}
+
+template <int TM, int TN, TileRows ROWS>
+static int launch_split_tile(const GemmBatch& batch, int64_t M, int64_t N, int64_t K, int units, float* sums,
+                             const TileSplit& split, hipStream_t hs) {
+  using S = TileShape<TM, TN, ROWS>;
+  static std::atomic<bool> lds_ok[kMaxDevices];
+  const auto kernel = gemm_bf16_nt_tile_kernel<TM, TN, ROWS, false, true>;
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, S::LDS)) return rc;
+  const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + S::BN - 1) / S::BN);
+  const int64_t grid = std::min<int64_t>((int64_t)split.parts * tiles_m * tiles_n, units);
+  launch_kernel(kernel, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, batch, split.parts, (int)M, (int)N, (int)K, N,
+                tiles_m, tiles_n, 0, NotGated{}, SplitOut{sums, split.per});
+  return TW_OK;
+}
+
+// The parts' sums of both products, added in order, to out and, where it is given, gate_up; four columns a thread.
+constexpr int JOIN_THREADS = 256;
+__global__ __launch_bounds__(JOIN_THREADS) void gated_join_kernel(uint16_t* out, const float* sums, int M, int I, int parts,
+                                                                  int64_t ldc, GatedOut gated) {
+  const int across = I / 4;
+  const int64_t i = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x, row = i / across;
+  if (row >= M) return;
+  const int c = (int)(i - row * across) * 4;
+  const float* p = sums + row * 2 * I + c;
+  f32x4_t g = *reinterpret_cast<const f32x4_t*>(p), u = *reinterpret_cast<const f32x4_t*>(p + I);
+#pragma unroll 4
+  for (int x = 1; x < parts; ++x) {
+    p += (int64_t)M * 2 * I;
+    g += *reinterpret_cast<const f32x4_t*>(p), u += *reinterpret_cast<const f32x4_t*>(p + I);
+  }
+  if (gated.both) {
+    uint16_t* const to = gated.both + row * gated.ld_both + c;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(g.x, g.y), pack2(g.z, g.w));
+    *reinterpret_cast<uint2*>(to + I) = make_uint2(pack2(u.x, u.y), pack2(u.z, u.w));
+  }
+  with_activation(gated.act, [&](auto act) {
+    f32x4_t h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = activation<act()>(g[e]) * u[e];
+    *reinterpret_cast<uint2*>(out + row * ldc + c) = make_uint2(pack2(h.x, h.y), pack2(h.z, h.w));
+  });
+}
+
+static int launch_gated_split(const char* what, const GemmBatch& batch, int64_t M, int64_t I, int64_t K, int64_t ldc,
+                              int max_cus, const GatedOut& gated, float* sums, const TileSplit& split, hipStream_t hs) {
+  const int cus = device_compute_units() > 0 ? device_compute_units() : 256;
+  const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
+  int rc = TW_OK;
+#define TW_SPLIT_LAUNCH(TM, TN)                                                                             \
+  if (split.tm == TM && split.tn == TN)                                                                     \
+    rc = K % BK == 0 ? launch_split_tile<TM, TN, kWholeSlabs>(batch, M, 2 * I, K, units, sums, split, hs)   \
+                     : launch_split_tile<TM, TN, kPartialSlab>(batch, M, 2 * I, K, units, sums, split, hs);
+  TW_SPLIT_TILES(TW_SPLIT_LAUNCH)
+#undef TW_SPLIT_LAUNCH
+  if (rc) return rc;
+  if ((rc = finish_launch(what))) return rc;
+  launch_kernel(gated_join_kernel, dim3((unsigned)((M * (I / 4) + JOIN_THREADS - 1) / JOIN_THREADS)), dim3(JOIN_THREADS), 0,
+                hs, batch.out[0], sums, (int)M, (int)I, split.parts, ldc, gated);
+  return TW_OK;
+}
+
 // act(a b[:I]^T) * (a b[I:]^T).
 static int launch_gated_tile(const GemmBatch& batch, int64_t M, int64_t I, int64_t K, int64_t ldc, int max_cus,
                              const GatedOut& gated, hipStream_t hs) {
@@ -1637,15 +1817,6 @@ static int launch_gated_tile(const GemmBatch& batch, int64_t M, int64_t I, int64
   TW_TILES(TW_GATED_TILE)
 #undef TW_GATED_TILE
   return set_error(TW_ERR_INVALID_ARGUMENT, "gated_gemm_bf16_nt: no %d x %d tile", 32 * t.tm, 32 * t.tn);
-}
-
-static int check_gemm_shape(const char* what, int64_t M, int64_t N, int64_t K, int64_t ldc) {
-  if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX || ldc < N)
-    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad shape M=%lld N=%lld K=%lld ldc=%lld", what, (long long)M,
-                     (long long)N, (long long)K, (long long)ldc);
-  if (K % 8 != 0 || N % 4 != 0 || ldc % 4 != 0)
-    return set_error(TW_ERR_ALIGNMENT, "%s: needs K %% 8 == 0, N %% 4 == 0, ldc %% 4 == 0", what);
-  return TW_OK;
 }
 
 static int check_gemm_pointers(const char* what, const void* out, const void* a, const void* b,
@@ -1693,7 +1864,8 @@ int run_gemm_bf16_nt(void* out, const void* a, const void* b, const void* bias, 
 }
 
 int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, int64_t M, int64_t I, int64_t K,
-                           int64_t ldc, int64_t ld_both, int act, int max_cus, void* stream) {
+                           int64_t ldc, int64_t ld_both, int act, int max_cus, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
   const char* what = "gated_gemm_bf16_nt";
   if (I > INT32_MAX / 2) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld columns", what, (long long)I);
   if (int rc = check_gemm_shape(what, M, I, K, ldc)) return rc;
@@ -1712,8 +1884,19 @@ int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, 
   batch.b[0] = static_cast<const uint16_t*>(b);
   const GatedOut gated = {static_cast<uint16_t*>(both), ld_both, act};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
+  const TileSplit split = gated_split(M, I, K);
+  if (split.parts > 1) {
+    const int64_t need = 8 * split.parts * M * I;
+    if (!workspace || workspace_bytes < need)
+      return set_error(TW_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", what, (long long)need,
+                       (long long)(workspace ? workspace_bytes : 0));
+    if (reinterpret_cast<uintptr_t>(workspace) % 256)
+      return set_error(TW_ERR_ALIGNMENT, "%s: needs a 256-byte aligned workspace", what);
+  }
   int rc;
-  if (tile_kernel_fits(M, 2 * I, K, ldc))
+  if (split.parts > 1)
+    rc = launch_gated_split(what, batch, M, I, K, ldc, max_cus, gated, static_cast<float*>(workspace), split, hs);
+  else if (tile_kernel_fits(M, 2 * I, K, ldc))
     rc = launch_gated_tile(batch, M, I, K, ldc, max_cus, gated, hs);
   else
     rc = launch_ksplit_for<true>(batch, 1, M, I, K, ldc, max_cus, hs, gated);

@@ -629,8 +629,13 @@ void gated_gemm_bf16_nt(const Tensor& out, const Tensor& a, const Tensor& b, int
   const int64_t ldc = check_rows("out", out, at::kBFloat16, a.device(), s.M, s.I);
   const int64_t ld = gate_up ? check_rows("gate_up", *gate_up, at::kBFloat16, a.device(), s.M, 2 * s.I) : 0;
   Launch l(a);
+  const int64_t need = tw_gated_gemm_bf16_nt_workspace(s.M, s.I, s.K);
+  if (need < 0) check_rc((int)need);
+  Tensor ws;
+  if (need > 0) ws = at::detail::empty_cuda({need}, at::kByte, a.device(), std::nullopt);
   check_rc(tw_gated_gemm_bf16_nt(out.data_ptr(), gate_up ? gate_up->data_ptr() : nullptr, a.data_ptr(), b.data_ptr(),
-                                 s.M, s.I, s.K, ldc, ld, activation, (int)max_cus, l.stream));
+                                 s.M, s.I, s.K, ldc, ld, activation, (int)max_cus, need > 0 ? ws.data_ptr() : nullptr, need,
+                                 l.stream));
 }
 
 void gated_gemm_bf16_nt_backward(const Tensor* grad_a, const Tensor* grad_b, const Tensor& grad_out, const Tensor& a,
