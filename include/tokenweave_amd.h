@@ -460,11 +460,14 @@ TW_API int tw_quant_fp8_groups(void* out, float* scales, int64_t scale_row_strid
  * a [M, K] and b [N, K] e4m3fn codes, contiguous; a's scales at any strides (elements), b's
  * [ceil(N / 128), ceil(K / 128)] contiguous; sums in fp32, rounded once to dtype (TW_DTYPE_BF16 or
  * TW_DTYPE_F16), rows of out at stride ldc.  K % 16 == 0, K <= 2^22, N % 4 == 0, ldc % 4 == 0; a, b
- * 16-byte, out 8-byte aligned; max_cus as for tw_gemm_bf16_nt. */
+ * 16-byte, out 8-byte aligned; max_cus as for tw_gemm_bf16_nt.
+ * workspace: tw_gemm_fp8_block_nt_workspace() bytes, as for tw_gated_gemm_bf16_nt. */
+TW_API int64_t tw_gemm_fp8_block_nt_workspace(int64_t M, int64_t N, int64_t K);
 TW_API int tw_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales,
                                 int64_t scale_row_stride, int64_t scale_block_stride, const void* b,
                                 const float* b_scales, int64_t M, int64_t N, int64_t K, int64_t ldc,
-                                int dtype, int max_cus, void* stream);
+                                int dtype, int max_cus, void* workspace, int64_t workspace_bytes,
+                                void* stream);
 
 #ifdef __cplusplus
 }

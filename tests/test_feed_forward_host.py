@@ -80,8 +80,8 @@ def test_codes():
         assert quant(**call) == ALIGN, call
 
 
-def block(out=AT, a=AT, sa=AT, b=AT, sb=AT, M=4, N=8, K=32, ldc=8, dtype=0):
-    return _lib.lib().tw_gemm_fp8_block_nt(out, a, sa, 1, 4, b, sb, M, N, K, ldc, dtype, 0, None)
+def block(out=AT, a=AT, sa=AT, b=AT, sb=AT, M=4, N=8, K=32, ldc=8, dtype=0, ws=None, size=0):
+    return _lib.lib().tw_gemm_fp8_block_nt(out, a, sa, 1, 4, b, sb, M, N, K, ldc, dtype, 0, ws, size, None)
 
 
 def test_block_product():
@@ -93,6 +93,20 @@ def test_block_product():
     for call in (dict(N=6), dict(K=24), dict(ldc=10), dict(a=AT + 8), dict(b=AT + 8), dict(out=AT + 4), dict(sa=AT + 2),
                  dict(sb=AT + 2)):
         assert block(**call) == ALIGN, call
+
+
+def test_block_product_divided_along_k():
+    size = _lib.lib().tw_gemm_fp8_block_nt_workspace
+    for M, N, K in ((0, 1024, 8192), (1, 1024, 8192), (64, 1024, 8192), (1025, 1024, 8192), (300, 1024, 384), (1000, 8192, 3696),
+                    (96, 7168, 8192)):
+        assert size(M, N, K) == 0, (M, N, K)
+    for M, N, K in ((96, 1024, 8192), (200, 1024, 8192), (1000, 1024, 8192), (300, 100, 4112)):
+        assert size(M, N, K) >= 2 * 4 * M * N and size(M, N, K) % (4 * M * N) == 0, (M, N, K)
+    assert size(-1, 8, 16) == BAD and size(4, 0, 16) == BAD and size(4, 8, (1 << 22) + 16) == BAD
+    shape = dict(M=200, N=1024, K=8192, ldc=1024)
+    need = size(200, 1024, 8192)
+    assert block(**shape) == BAD and block(**shape, ws=AT, size=need - 1) == BAD
+    assert block(**shape, ws=AT + 64, size=need) == ALIGN
 
 
 def bf16(*shape):

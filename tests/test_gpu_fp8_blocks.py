@@ -318,3 +318,29 @@ def test_rows_of_the_output_far_apart(M):
         out.fill_(777.0)
         ops.gemm_fp8_block_nt(out[:, :40], x, sx, w, sw)
         assert torch.equal(out[:, :40], plain) and (out[:, 40:] == 777.0).all(), stride
+
+
+@pytest.mark.parametrize("M,N,K", [(65, 4, 8208), (96, 1024, 8192), (128, 1280, 8192), (129, 100, 4112), (200, 1024, 8192),
+                                   (257, 132, 6160), (300, 1024, 4096), (512, 768, 3600), (640, 700, 6144), (1000, 1024, 8192),
+                                   (1024, 520, 20000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_divided_along_k(M, N, K, dtype):
+    """Few columns and a long inner dimension: against 64 bits, under grid caps, from any workspace."""
+    from tokenweave_amd import _lib
+    L = _lib.lib()
+    size = L.tw_gemm_fp8_block_nt_workspace(M, N, K)
+    assert size > 0, "this size is not divided any more: the test needs another"
+    check_product(M, N, K, dtype, seed=M)
+    x, sx, w, sw = operands(M, N, K, M)
+    out = torch.empty((M, N), dtype=dtype, device="cuda")
+    ops.gemm_fp8_block_nt(out, x, sx, w, sw)
+    for max_cus in (1, 24, 100):
+        again = torch.full_like(out, 777.0)
+        ops.gemm_fp8_block_nt(again, x, sx, w, sw, max_cus)
+        assert torch.equal(again, out), max_cus
+    space = torch.full((size // 4 + 64,), float("nan"), device="cuda")
+    again = torch.empty_like(out)
+    _lib.check(L.tw_gemm_fp8_block_nt(again.data_ptr(), x.data_ptr(), sx.data_ptr(), sx.stride(0), sx.stride(1), w.data_ptr(),
+                                      sw.data_ptr(), M, N, K, N, ops._DTYPE_CODE[dtype], 0, space.data_ptr(), size,
+                                      torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(again, out) and torch.isnan(space[size // 4:]).all()

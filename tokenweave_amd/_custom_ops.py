@@ -1146,10 +1146,16 @@ def gemm_fp8_block_nt(out: torch.Tensor, a: torch.Tensor, a_scales: torch.Tensor
     _check_group_scales("a_scales", a_scales, dev, M, blocks)
     _check_group_scales("b_scales", b_scales, dev, -(-N // FP8_GROUP), blocks)
     _require(b_scales.is_contiguous(), "b_scales must be contiguous")
+    L = _lib.lib()
     with _on_device(a):
-        _lib.check(_lib.lib().tw_gemm_fp8_block_nt(
+        need = L.tw_gemm_fp8_block_nt_workspace(M, N, K)
+        if need < 0:
+            _lib.check(need)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(L.tw_gemm_fp8_block_nt(
             out.data_ptr(), a.data_ptr(), a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), b.data_ptr(),
-            b_scales.data_ptr(), M, N, K, ldc, _DTYPE_CODE[out.dtype], _cap(max_cus), _stream_ptr(a)))
+            b_scales.data_ptr(), M, N, K, ldc, _DTYPE_CODE[out.dtype], _cap(max_cus),
+            None if ws is None else ws.data_ptr(), need, _stream_ptr(a)))
 
 
 def num_compute_units(device=None) -> int:

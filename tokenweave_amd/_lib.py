@@ -83,11 +83,13 @@ PROTOTYPES = {
     "tw_gated_gemm_bf16_nt_backward": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _ci, _ci, _vp, _i64,
                                        _vp],
     "tw_quant_fp8_groups": [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _ci, _ci, _vp],
-    "tw_gemm_fp8_block_nt": [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _ci, _ci, _vp],
+    "tw_gemm_fp8_block_nt_workspace": [_i64, _i64, _i64],
+    "tw_gemm_fp8_block_nt": [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _ci, _ci, _vp, _i64, _vp],
 }
 # what an entry point returns where it is no status code
 RETURNS = {"tw_last_error": ctypes.c_char_p, "tw_kv4_attention_workspace": _i64,
-           "tw_gated_gemm_bf16_nt_workspace": _i64, "tw_gated_gemm_bf16_nt_backward_workspace": _i64}
+           "tw_gated_gemm_bf16_nt_workspace": _i64, "tw_gated_gemm_bf16_nt_backward_workspace": _i64,
+           "tw_gemm_fp8_block_nt_workspace": _i64}
 
 _lib = None
 

@@ -32,11 +32,14 @@ int tw_quant_fp8_groups(void* out, float* scales, int64_t scale_row_stride, int6
                                   activation, dtype, stream);
 }
 
+int64_t tw_gemm_fp8_block_nt_workspace(int64_t M, int64_t N, int64_t K) { return tw::gemm_fp8_block_workspace(M, N, K); }
+
 int tw_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64_t scale_row_stride,
                          int64_t scale_block_stride, const void* b, const float* b_scales, int64_t M, int64_t N,
-                         int64_t K, int64_t ldc, int dtype, int max_cus, void* stream) {
+                         int64_t K, int64_t ldc, int dtype, int max_cus, void* workspace, int64_t workspace_bytes,
+                         void* stream) {
   return tw::run_gemm_fp8_block_nt(out, a, a_scales, scale_row_stride, scale_block_stride, b, b_scales, M, N, K, ldc,
-                                   dtype, max_cus, stream);
+                                   dtype, max_cus, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -103,7 +103,8 @@ int run_quant_fp8_groups(void* out, float* scales, int64_t scale_row, int64_t sc
 
 int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64_t scale_row, int64_t scale_block,
                           const void* b, const float* b_scales, int64_t M, int64_t N, int64_t K, int64_t ldc, int dtype,
-                          int max_cus, void* stream);
+                          int max_cus, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t gemm_fp8_block_workspace(int64_t M, int64_t N, int64_t K);
 
 struct Kv4Pages;
 

@@ -184,6 +184,8 @@ struct BlockArgs {
   int64_t scale_row, scale_block, ldc;
   int M, N, K, half_out, tiles_m, tiles_n, cols;
   int form;  // StoreForm, tile kernel
+  float* sums;     // tile kernel, K divided: [parts][M][N], `per` slabs a part
+  int parts, per;
 };
 
 [[maybe_unused]] __device__ __forceinline__ uint32_t pack_out(float lo, float hi, int half_out) {
@@ -437,8 +439,9 @@ __device__ __forceinline__ uint32_t after(uint32_t at, uint32_t panel, int n) {
 }
 #endif
 
-// TAIL: the last slab is a partial one, whose chunks past K must arrive as zeros.
-template <int WM, int TM, int TN, int NA, int NB, bool TAIL>
+// TAIL: the last slab is a partial one, whose chunks past K must arrive as zeros.  SPLIT: `parts` workgroups share a tile's
+// slabs and leave fp32 sums, which block_join_kernel adds in order.
+template <int WM, int TM, int TN, int NA, int NB, bool TAIL, bool SPLIT>
 __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(BlockArgs w) {
 #ifdef __HIP_DEVICE_COMPILE__
   using S = WideShape<WM, TM, TN, NA, NB>;
@@ -478,11 +481,14 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
   const uint32_t past_a = TAIL && chunk_a >= tail_chunks ? OUT_OF_RANGE : 0u;  // of the last slab
   const uint32_t past_b = TAIL && chunk_b >= tail_chunks ? OUT_OF_RANGE : 0u;
 
-  const int num_tiles = w.tiles_m * w.tiles_n;
+  const int whole = w.tiles_m * w.tiles_n, num_tiles = SPLIT ? whole * w.parts : whole;
   for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
     int pid = t;
     const int per_xcd = num_tiles / 8;
     if (t < per_xcd * 8) pid = (t & 7) * per_xcd + (t >> 3);
+    // the part's slabs: `slabs` of them from `from` on
+    const int part_of = SPLIT ? pid / whole : 0, from = SPLIT ? part_of * w.per : 0, slabs = SPLIT ? min(w.per, nk - from) : nk;
+    pid -= part_of * whole;
     const int sweep = 4 * w.tiles_n, group = pid / sweep, first = group * 4, in_group = min(w.tiles_m - first, 4);
     const int m0 = (first + pid % sweep % in_group) * BM, n0 = pid % sweep / in_group * BN;
     const int rows = min(w.M - m0, BM), cols = min(w.N - n0, BN);
@@ -496,20 +502,20 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
     // Past the last slab loads bring that one again and fragments are read that nobody uses: branches cost more (a
     // second set of registers for b's fragments, and spills).
     auto load_a = [&](int l, int slab, uint32_t at, uint32_t at_s) {
-      const int k = min(slab, nk - 1);
+      const int k = from + min(slab, slabs - 1);
       if (l == LA) {
         load_scales(scales + k * w.scale_block, my_scale, base + S::AT_S + at_s + scale_part * 4);
         return;
       }
-      const uint32_t off = TAIL ? va[l] | (slab >= nk - 1 ? past_a : 0u) : va[l];
+      const uint32_t off = TAIL ? va[l] | (k == nk - 1 ? past_a : 0u) : va[l];
       __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_void_t*)(base + at + (wave + 8 * l) * 1024), 16, off,
                                                (uint32_t)k * ROWB, 0, 0);
     };
     auto load_b = [&](int l, int slab, uint32_t at) {
-      const uint32_t off = TAIL ? vb[l] | (slab >= nk - 1 ? past_b : 0u) : vb[l];
+      const int k = from + min(slab, slabs - 1);
+      const uint32_t off = TAIL ? vb[l] | (k == nk - 1 ? past_b : 0u) : vb[l];
       const uint32_t to = BN % 64 == 0 || (wave + 8 * l) * 8 < BN ? S::AT_B + at + (wave + 8 * l) * 1024 : S::AT_NONE;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(base + to), 16, off,
-                                               (uint32_t)min(slab, nk - 1) * ROWB, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_void_t*)(base + to), 16, off, (uint32_t)k * ROWB, 0, 0);
     };
     auto all_a = [&](int slab) {
 #pragma unroll
@@ -523,10 +529,10 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
     // keeps those of slab l of 64.
     constexpr bool TWO = GROUP % (16 * TN) != 0;
     const int col = n0 + wn * 16 * TN, most_block = (w.N - 1) / GROUP;
-    const float* const sb = w.b_scales + (int64_t)min(col / GROUP, most_block) * nk;
+    const float* const sb = w.b_scales + (int64_t)min(col / GROUP, most_block) * nk + from;
     const int64_t second = TWO && col / GROUP + 1 <= most_block ? nk : 0;
     const int border = GROUP - col % GROUP;  // columns of the first block
-    float sb0 = sb[min(lane, nk - 1)], sb1 = sb[min(lane, nk - 1) + second];
+    float sb0 = sb[min(lane, slabs - 1)], sb1 = sb[min(lane, slabs - 1) + second];
 
     f32x4_t acc[TM][TN], part[S::RING];
 #pragma unroll
@@ -566,10 +572,10 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
     float sa = *(lds_f32_t*)at_scale;
 #pragma unroll
     for (int j = 0; j < TN; ++j) fb[j] = fragment_b(j, 0);
-    for (int slab = 0; slab < nk; ++slab) {
+    for (int slab = 0; slab < slabs; ++slab) {
       if (slab && slab % 64 == 0) {
-        sb0 = sb[min(slab + lane, nk - 1)];
-        sb1 = sb[min(slab + lane, nk - 1) + second];
+        sb0 = sb[min(slab + lane, slabs - 1)];
+        sb1 = sb[min(slab + lane, slabs - 1) + second];
         asm volatile("" : "+v"(sb0), "+v"(sb1));  // waited for here: not in every slab, for all loads under way
       }
       const float s0 = lane_value(sb0, slab & 63), s1 = lane_value(sb1, slab & 63);
@@ -616,6 +622,20 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
     for (int j = TN - S::LAG; j < TN; ++j) add((TM - 1) * TN + j, first_scale, second_scale);
     // a lane holds row r16 of each row of tiles, columns 8 quad + 0 .. 7 of a pair of column tiles
     const int m = wm * 16 * TM + r16, c0 = wn * 16 * TN;
+    if constexpr (SPLIT) {
+      const __amdgpu_buffer_rsrc_t ds = __builtin_amdgcn_make_buffer_rsrc(
+          w.sums + ((size_t)part_of * w.M + m0) * w.N + n0, 0, (uint32_t)rows * (uint32_t)w.N * 4u, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int c = c0 + (TN % 2 && j == TN - 1 ? 16 * j + quad * 4 : (j >> 1) * 32 + quad * 8 + (j & 1) * 4);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[i][j]), ds,
+                                                 c < cols ? ((uint32_t)(m + 16 * i) * (uint32_t)w.N + c) * 4u : OUT_OF_RANGE, 0, 0);
+        }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next tile's slabs go where this one's were
+      continue;
+    }
     auto four = [&](int i, int j) {
       return u32x2_t{pack_out(acc[i][j][0], acc[i][j][1], w.half_out), pack_out(acc[i][j][2], acc[i][j][3], w.half_out)};
     };
@@ -690,17 +710,17 @@ int launch_split(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
   return TW_OK;
 }
 
-template <int WM, int TM, int TN, int NA, int NB>
+template <int WM, int TM, int TN, int NA, int NB, bool SPLIT = false>
 int launch_wide(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
   using S = WideShape<WM, TM, TN, NA, NB>;
   static std::atomic<bool> ok[2][kMaxDevices];
   const bool tail = w.K % GROUP != 0;
-  const auto kernel = tail ? gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, true>
-                           : gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, false>;
+  const auto kernel = tail ? gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, true, SPLIT>
+                           : gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, false, SPLIT>;
   if (int rc = allow_lds(kernel, ok[tail], S::LDS)) return rc;
   w.tiles_m = (w.M + S::BM - 1) / S::BM;
   w.tiles_n = (w.N + S::BN - 1) / S::BN;
-  int64_t grid = (int64_t)w.tiles_m * w.tiles_n;
+  int64_t grid = (int64_t)w.tiles_m * w.tiles_n * (SPLIT ? w.parts : 1);
   // Through the L2 at once only where there is a tile a unit at most.  One: [1000, 3696] x [8192, 3696]^T 35.3 us, kept 37.5;
   // two, the loads of the second beside the stores of the first: [4096, 8192] x [7168, 8192]^T 228, kept 208.
   const int units = max_cus > 0 && max_cus < cus ? max_cus : cus;
@@ -742,6 +762,82 @@ int launch_wide_for(const BlockArgs& w, int max_cus, int cus, hipStream_t hs) {
   return set_error(TW_ERR_INVALID_ARGUMENT, "gemm_fp8_block_nt: no tile for %d rows", w.M);
 }
 
+// K divided: for more than 64 rows, where columns are few and tiles leave units idle or the inner dimension is long.  All
+// times in us: a slab of a 256 x 224 tile 1.66 (the others as kWideTiles has them), 3 for a launch besides, 4 for the one that
+// adds the sums, and those to memory and back; nothing reads b faster than memory gives it.  Undivided, up to 128 rows, a
+// wave's slab takes 0.95, and a unit's lines come at 50 GB/s.  [M, 8192] x [1024, 8192]^T, undivided / by this rule: 96 rows 18.7
+// / 11.1, 200: 24.0 / 13.6, 512: 24.6 / 17.8, 1000: 25.0 / 20.9.  Left whole: [96, 8192] x [7168, 8192]^T (17.6; divided 16.3 and
+// the launch that adds), [1000, 3696] x [8192, 3696]^T, [341, 2048] x [768, 2048]^T (8.7, of which the launch and the first slab 4).
+constexpr double SPLIT_SLAB_US = 1.66, SPLIT_LAUNCH_US = 3.0, SPLIT_JOIN_US = 4.0, SPLIT_SUMS_A_US = 6e6, SPLIT_BYTES_A_US = 5e6,
+                 SPLIT_SAVES_US = 1.5;
+constexpr int64_t SPLIT_MAX_ROWS = 1024, SPLIT_MIN_SLABS = 2, SPLIT_MAX_N = 1 << 21;
+// 64 x 128, 128 x 128 and 128 x 256 of kWideTiles
+#define TW_BLOCK_SPLIT_TILES(X) X(2, 2, 2, 3, 3, 0.22) X(2, 4, 2, 3, 3, 0.37) X(2, 4, 4, 3, 3, 0.59)
+struct BlockSplit { int tm, tn, parts, per; };
+
+// The rows, N and K decide, no grid cap: the parts' sums differ in the order of the additions.
+BlockSplit block_split(int64_t M, int64_t N, int64_t K, int cus) {
+  const int64_t nk = (K + GROUP - 1) / GROUP;
+  BlockSplit best = {0, 0, 1, (int)nk};
+  if (M <= 64 || M > SPLIT_MAX_ROWS || N > SPLIT_MAX_N || nk < 2 * SPLIT_MIN_SLABS) return best;
+  double least = 1e300;
+  if (M > 128) {
+    for (const WideTile& t : kWideTiles) {
+      const int64_t bm = 16 * t.tm * t.wm, bn = 16 * t.tn * (8 / t.wm), tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);
+      least = std::min(least, SPLIT_LAUNCH_US + SPLIT_SLAB_US * t.cost * (double)((tiles + cus - 1) / cus * nk));
+    }
+  } else {
+    const int64_t rows = (M + 1) / 2, cols = std::min<int64_t>(64, (2 * N + cus - 1) / cus);
+    least = 2.5 + std::max(0.95 * (double)((nk + 3) / 4), (double)((rows + cols) * K) / 50e3);
+  }
+  least -= SPLIT_SAVES_US;
+  const double from_memory = (double)N * (double)K / SPLIT_BYTES_A_US;
+#define TW_BLOCK_SPLIT_COST(WM, TM, TN, NA, NB, COST)                                                                   \
+  {                                                                                                                    \
+    const int64_t bm = 16 * TM * WM, bn = 16 * TN * (8 / WM), tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);         \
+    for (int64_t parts = 2; parts * tiles <= cus && parts * SPLIT_MIN_SLABS <= nk; ++parts) {                          \
+      const int64_t per = (nk + parts - 1) / parts;                                                                    \
+      const double slabs = SPLIT_SLAB_US * COST * (double)per;                                                         \
+      const double us = std::max(slabs, from_memory) + 0.1 * slabs + SPLIT_LAUNCH_US + SPLIT_JOIN_US +                 \
+                        8.0 * (double)parts * (double)M * (double)N / SPLIT_SUMS_A_US;                                 \
+      if (us < least) least = us, best = {TM, TN, (int)((nk + per - 1) / per), (int)per};                              \
+    }                                                                                                                  \
+  }
+  TW_BLOCK_SPLIT_TILES(TW_BLOCK_SPLIT_COST)
+#undef TW_BLOCK_SPLIT_COST
+  return best;
+}
+
+constexpr int JOIN_THREADS = 256;
+__global__ __launch_bounds__(JOIN_THREADS) void block_join_kernel(BlockArgs w) {
+  const int across = w.N / 4;
+  const int64_t i = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x, row = i / across;
+  if (row >= w.M) return;
+  const int c = (int)(i - row * across) * 4;
+  const float* p = w.sums + row * w.N + c;
+  f32x4_t s = *reinterpret_cast<const f32x4_t*>(p);
+#pragma unroll 4
+  for (int x = 1; x < w.parts; ++x) {
+    p += (int64_t)w.M * w.N;
+    s += *reinterpret_cast<const f32x4_t*>(p);
+  }
+  *reinterpret_cast<uint2*>(w.out + row * w.ldc + c) = make_uint2(pack_out(s.x, s.y, w.half_out), pack_out(s.z, s.w, w.half_out));
+}
+
+int launch_block_split(const char* what, BlockArgs w, const BlockSplit& split, float* sums, int max_cus, int cus, hipStream_t hs) {
+  w.sums = sums, w.parts = split.parts, w.per = split.per;
+  int rc = TW_OK;
+#define TW_BLOCK_SPLIT_LAUNCH(WM, TM, TN, NA, NB, COST) \
+  if (split.tm == TM && split.tn == TN) rc = launch_wide<WM, TM, TN, NA, NB, true>(w, max_cus, cus, hs);
+  TW_BLOCK_SPLIT_TILES(TW_BLOCK_SPLIT_LAUNCH)
+#undef TW_BLOCK_SPLIT_LAUNCH
+  if (rc) return rc;
+  if ((rc = finish_launch(what))) return rc;
+  const int64_t groups = ((int64_t)w.M * (w.N / 4) + JOIN_THREADS - 1) / JOIN_THREADS;
+  launch_kernel(block_join_kernel, dim3((unsigned)groups), dim3(JOIN_THREADS), 0, hs, w);
+  return TW_OK;
+}
+
 }  // namespace
 
 int run_quant_fp8_groups(void* out, float* scales, int64_t scale_row, int64_t scale_group, const void* input,
@@ -777,9 +873,18 @@ int run_quant_fp8_groups(void* out, float* scales, int64_t scale_row, int64_t sc
   return finish_launch(what);
 }
 
+int64_t gemm_fp8_block_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > BLOCK_MAX_K)
+    return set_error(TW_ERR_INVALID_ARGUMENT, "gemm_fp8_block_nt_workspace: bad shape M=%lld N=%lld K=%lld", (long long)M,
+                     (long long)N, (long long)K);
+  const int cus = device_compute_units();
+  const BlockSplit s = block_split(M, N, K, cus > 0 ? cus : 256);
+  return s.parts > 1 ? 4 * s.parts * M * N : 0;
+}
+
 int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64_t scale_row, int64_t scale_block,
                           const void* b, const float* b_scales, int64_t M, int64_t N, int64_t K, int64_t ldc, int dtype,
-                          int max_cus, void* stream) {
+                          int max_cus, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "gemm_fp8_block_nt";
   if (M == 1) scale_row = 0;  // a single row's has no meaning
   if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > BLOCK_MAX_K || ldc < N)
@@ -810,7 +915,15 @@ int run_gemm_fp8_block_nt(void* out, const void* a, const float* a_scales, int64
   const hipStream_t hs = static_cast<hipStream_t>(stream);
   int cus = device_compute_units(), rc;
   if (cus <= 0) cus = 256;
-  if (M <= 8) rc = launch_split<1, 1, 3, 1>(w, max_cus, cus, hs);
+  const BlockSplit split = block_split(M, N, K, cus);
+  if (split.parts > 1) {
+    const int64_t need = 4 * split.parts * M * N;
+    if (!workspace || workspace_bytes < need)
+      return set_error(TW_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", what, (long long)need,
+                       (long long)(workspace ? workspace_bytes : 0));
+    if (misaligned(workspace, 256)) return set_error(TW_ERR_ALIGNMENT, "%s: needs a 256-byte aligned workspace", what);
+    rc = launch_block_split(what, w, split, static_cast<float*>(workspace), max_cus, cus, hs);
+  } else if (M <= 8) rc = launch_split<1, 1, 3, 1>(w, max_cus, cus, hs);
   else if (M <= 16) rc = launch_split<1, 1, 3, 2>(w, max_cus, cus, hs);
   else if (M <= 32) rc = launch_split<1, 1, 3, 4>(w, max_cus, cus, hs);
   else if (M <= 64) rc = launch_split<2, 1, 2, 8>(w, max_cus, cus, hs);

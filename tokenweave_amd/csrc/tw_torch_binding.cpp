@@ -700,10 +700,14 @@ void gemm_fp8_block_nt(const Tensor& out, const Tensor& a, const Tensor& a_scale
   check_group_scales("b_scales", b_scales, dev, (N + TW_FP8_GROUP - 1) / TW_FP8_GROUP, blocks);
   TORCH_CHECK(b_scales.is_contiguous(), "b_scales must be contiguous");
   Launch l(a);
+  const int64_t need = tw_gemm_fp8_block_nt_workspace(M, N, K);
+  if (need < 0) check_rc((int)need);
+  Tensor ws;
+  if (need > 0) ws = at::detail::empty_cuda({need}, at::kByte, dev, std::nullopt);
   check_rc(tw_gemm_fp8_block_nt(out.data_ptr(), a.data_ptr(), static_cast<const float*>(a_scales.data_ptr()),
                                 a_scales.stride(0), a_scales.stride(1), b.data_ptr(),
                                 static_cast<const float*>(b_scales.data_ptr()), M, N, K, ldc, code, (int)max_cus,
-                                l.stream));
+                                need > 0 ? ws.data_ptr() : nullptr, need, l.stream));
 }
 
 }  // namespace tw_torch
