@@ -162,6 +162,9 @@ class FeedForward(nn.Module):
     ``hidden_states`` and leaves the down projection's partial sum there, for the schedule to reduce.
     ``intermediate_size`` is the whole model's; ``gemm_cus`` is the compute-unit budget of the down projection.
 
+    The result takes its input's place in memory, so no gradient can be recorded: where grad mode is on and the rows or a
+    weight require one, the call raises.  `GatedLinear` is the projection with its gradient.
+
     ``to_fp8_blocks()`` turns both weights into e4m3 codes with a scale for each block of 128 x 128; a call is then
     codes of the rows, the merged projection, activation, product and codes in one pass, the down projection."""
 
@@ -182,6 +185,8 @@ class FeedForward(nn.Module):
         return self
 
     def forward(self, hidden_states: torch.Tensor, gemm_cus: Optional[int] = None) -> torch.Tensor:
+        ops._refuse_recording("FeedForward", "call it under torch.no_grad(), or train GatedLinear and a product of your own",
+                              hidden_states, self.gate_up.weight, self.down.weight)
         if not self.fp8:
             inner = self.gate_up(hidden_states)
             self.down(inner, hidden_states, is_tokenweave=True, gemm_cus=gemm_cus)
