@@ -33,3 +33,13 @@ def test_a_block_whose_gradient_is_wanted_is_refused(fp8):
         part.weight.requires_grad_(False)
     with pytest.raises(RuntimeError, match="GPU"):
         block(torch.randn(4, 64).to(BF16))
+
+
+@pytest.mark.parametrize("make", [lambda: tw.RowParallelLinear(64, 64, bias=False), lambda: tw.GatedLinear(64, 32)])
+def test_a_models_type_is_a_bf16_weights_whatever_stands_beside_it(make):
+    """`weight_scale` is any method's name for its scales: only e4m3 codes keep their type."""
+    for holder in (torch.nn.Parameter(torch.ones(1), requires_grad=False), torch.ones(1)):
+        layer = filled(make())
+        layer.weight_scale = holder
+        assert layer.half().weight.dtype == torch.float16
+        assert layer.weight_scale.dtype == (torch.float16 if isinstance(holder, torch.nn.Parameter) else torch.float32)

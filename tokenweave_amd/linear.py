@@ -54,14 +54,23 @@ def _is_unquantized(method: Any) -> bool:
             and "apply_inplace" not in method.__dict__)
 
 
+def _holds_codes(layer: nn.Module) -> bool:
+    """Whether the layer's weight is e4m3 codes."""
+    weight = layer._parameters.get("weight")
+    return weight is not None and weight.dtype == ops.FP8_DTYPE
+
+
 def _apply_beside_codes(layer: nn.Module, apply: Any, fn: Any, recurse: bool) -> nn.Module:
     """A model's type (`model.bfloat16()`) is not that of 8-bit codes and of their fp32 scales: they stay what they
     are, on the device they are moved to."""
-    held = {name: p.data for name, p in layer._parameters.items() if p is not None} if hasattr(layer, "weight_scale") else {}
+    held = {}
+    if _holds_codes(layer):
+        held = {name: layer._parameters[name].data for name in ("weight", "weight_scale")
+                if layer._parameters.get(name) is not None}
     apply(fn, recurse)
-    for name in ("weight", "weight_scale"):
-        if name in held and getattr(layer, name).dtype != held[name].dtype:
-            getattr(layer, name).data = held[name].to(getattr(layer, name).device)
+    for name, data in held.items():
+        if getattr(layer, name).dtype != data.dtype:
+            getattr(layer, name).data = data.to(getattr(layer, name).device)
     return layer
 
 
