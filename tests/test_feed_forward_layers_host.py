@@ -43,3 +43,43 @@ def test_a_models_type_is_a_bf16_weights_whatever_stands_beside_it(make):
         layer.weight_scale = holder
         assert layer.half().weight.dtype == torch.float16
         assert layer.weight_scale.dtype == (torch.float16 if isinstance(holder, torch.nn.Parameter) else torch.float32)
+
+
+def values(codes, scales):
+    N, K = codes.shape
+    return codes.double() * scales.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+
+
+@pytest.mark.parametrize("tp", [1, 2])
+def test_8_bit_weights_are_loaded(tp):
+    """A whole model's codes and scales: every rank's layers stand for its part of the whole weights."""
+    hidden, inner = 144, 512
+    gate, up, down = (tw.quantize_fp8_blocks(torch.randn(s)) for s in ((inner, hidden), (inner, hidden), (hidden, inner)))
+    n = inner // tp
+    for rank in range(tp):
+        block = filled(tw.FeedForward(hidden, inner, tp_rank=rank, tp_size=tp)).to_fp8_blocks()
+        for shard, (codes, scales) in enumerate((gate, up)):
+            block.gate_up.weight_loader(block.gate_up.weight, codes, shard)
+            block.gate_up.weight_loader(block.gate_up.weight_scale, scales, shard)
+        block.down.weight_loader(block.down.weight, down[0])
+        block.down.weight_loader(block.down.weight_scale, down[1])
+        rows = slice(rank * n, (rank + 1) * n)
+        want = torch.cat((values(*gate)[rows], values(*up)[rows]))
+        assert torch.equal(values(block.gate_up.weight, block.gate_up.weight_scale), want)
+        assert torch.equal(values(block.down.weight, block.down.weight_scale), values(*down)[:, rows])
+        # one rank's own, as a sharded checkpoint has them
+        block.down.weight_loader(block.down.weight_scale, block.down.weight_scale.data * 2)
+        assert torch.equal(values(block.down.weight, block.down.weight_scale), 2 * values(*down)[:, rows])
+
+
+def test_8_bit_weights_that_do_not_fit_are_refused():
+    block = filled(tw.FeedForward(64, 96)).to_fp8_blocks()
+    with pytest.raises(ValueError, match="holds 8-bit codes"):
+        block.gate_up.weight_loader(block.gate_up.weight, torch.zeros(96, 64, dtype=BF16), 0)
+    with pytest.raises(ValueError, match="holds 8-bit codes"):
+        block.down.weight_loader(block.down.weight, torch.zeros(64, 96, dtype=BF16))
+    with pytest.raises(ValueError, match="inside a block of 128"):      # the up rows begin inside the gate rows' last block
+        block.gate_up.weight_loader(block.gate_up.weight_scale, torch.ones(1, 1), 0)
+    block = filled(tw.FeedForward(64, 384, tp_rank=1, tp_size=2)).to_fp8_blocks()
+    with pytest.raises(ValueError, match="inside a block of 128"):
+        block.down.weight_loader(block.down.weight_scale, torch.ones(1, 3))

@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 from torch.nn.parameter import Parameter
 
 from . import _custom_ops as ops
-from .linear import RowParallelLinear, _apply_beside_codes
+from .linear import RowParallelLinear, _apply_beside_codes, _check_loaded, _holds_codes, _rank_blocks
 
 
 def _refuse_capture() -> None:
@@ -83,8 +83,12 @@ class GatedLinear(nn.Module):
         return _apply_beside_codes(self, super()._apply, fn, recurse)
 
     def weight_loader(self, param: Parameter, loaded_weight: torch.Tensor, shard_id: int) -> None:
-        """This rank's rows of a full gate (``shard_id`` 0) or up (1) weight."""
+        """This rank's rows of a full gate (``shard_id`` 0) or up (1) weight; of an 8-bit one the codes and, as ``param``
+        ``weight_scale``, the scales of its blocks."""
+        _check_loaded(self, param, loaded_weight)
         n = self.intermediate_size
+        if param is getattr(self, "weight_scale", None) and _holds_codes(self):
+            n = _rank_blocks(self, n)
         if loaded_weight.shape[0] != n:
             loaded_weight = loaded_weight.narrow(0, self.tp_rank * n, n)
         param.data.narrow(0, shard_id * n, n).copy_(loaded_weight)
@@ -116,7 +120,8 @@ def quantize_fp8_blocks(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tenso
 class Fp8BlockLinearMethod:
     """``quant_method`` of a linear layer whose weight is e4m3 codes with a scale for each block of 128 x 128
     (``layer.weight``, ``layer.weight_scale``): the input's rows are coded with a scale for 128 channels on the
-    way.  ``process_weights`` makes both from a layer's bf16 weight; a checkpoint that holds them is copied in."""
+    way.  ``process_weights`` makes both from a layer's bf16 weight; the layer's ``weight_loader`` then takes a
+    checkpoint's codes and scales instead."""
 
     @staticmethod
     def check(layer: nn.Module) -> None:

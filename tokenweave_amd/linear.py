@@ -74,6 +74,21 @@ def _apply_beside_codes(layer: nn.Module, apply: Any, fn: Any, recurse: bool) ->
     return layer
 
 
+def _rank_blocks(layer: nn.Module, size: int) -> int:
+    """How many blocks of an 8-bit weight's scales lie along a dimension of which the layer has `size`."""
+    if size % ops.FP8_GROUP:
+        raise ValueError(f"{size} channels of one rank's {type(layer).__name__} end inside a block of {ops.FP8_GROUP}, so it "
+                         "has no scales of its own among the whole weight's: load bf16 and code that")
+    return size // ops.FP8_GROUP
+
+
+def _check_loaded(layer: nn.Module, param: Parameter, loaded_weight: torch.Tensor) -> None:
+    """Values are no codes: copied into them they would stand for others, by scales that they do not have."""
+    if param is layer.weight and _holds_codes(layer) and loaded_weight.dtype != param.dtype:
+        raise ValueError(f"this {type(layer).__name__} holds 8-bit codes and was given {loaded_weight.dtype} values: load them "
+                         "before its weight is coded, or load codes and their scales")
+
+
 class RowParallelLinear(nn.Module):
     """Y = X A + b with A split along its first dimension (X along its last) over
     ``tp_size`` ranks; this module is rank ``tp_rank``'s share.  Constructor and
@@ -113,10 +128,15 @@ class RowParallelLinear(nn.Module):
 
     def weight_loader(self, param: Parameter, loaded_weight: torch.Tensor) -> None:
         """This rank's slice of a full weight along the input dimension; biases whole
-        (linear.py:1243-1277)."""
+        (linear.py:1243-1277).  Of an 8-bit weight the codes and, as ``param`` ``weight_scale``, the scales of
+        the whole weight's blocks."""
+        _check_loaded(self, param, loaded_weight)
         if param is self.weight and loaded_weight.shape[1] != self.input_size_per_partition:
             shard = self.input_size_per_partition
             loaded_weight = loaded_weight.narrow(1, self.tp_rank * shard, shard)
+        elif param is getattr(self, "weight_scale", None) and _holds_codes(self) and loaded_weight.shape != param.shape:
+            blocks = _rank_blocks(self, self.input_size_per_partition)
+            loaded_weight = loaded_weight.narrow(1, self.tp_rank * blocks, blocks)
         assert param.data.shape == loaded_weight.shape
         param.data.copy_(loaded_weight)
 
