@@ -83,3 +83,9 @@ def test_8_bit_weights_that_do_not_fit_are_refused():
     block = filled(tw.FeedForward(64, 384, tp_rank=1, tp_size=2)).to_fp8_blocks()
     with pytest.raises(ValueError, match="inside a block of 128"):
         block.down.weight_loader(block.down.weight_scale, torch.ones(1, 3))
+
+
+def test_an_8_bit_block_takes_any_leading_dimensions():
+    block = filled(tw.FeedForward(64, 96)).to_fp8_blocks()
+    with pytest.raises(RuntimeError, match="GPU"):      # no complaint about the shape
+        block(torch.zeros(2, 3, 64, dtype=BF16))

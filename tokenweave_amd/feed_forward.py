@@ -196,10 +196,10 @@ class FeedForward(nn.Module):
             inner = self.gate_up(hidden_states)
             self.down(inner, hidden_states, is_tokenweave=True, gemm_cus=gemm_cus)
             return hidden_states
-        x = hidden_states
-        codes, scales = _codes(x)
-        both = torch.empty((x.shape[0], self.gate_up.weight.shape[0]), dtype=x.dtype, device=x.device)
+        rows = hidden_states if hidden_states.dim() == 2 else hidden_states.view(-1, hidden_states.shape[-1])
+        codes, scales = _codes(rows)
+        both = torch.empty((rows.shape[0], self.gate_up.weight.shape[0]), dtype=rows.dtype, device=rows.device)
         ops.gemm_fp8_block_nt(both, codes, scales, self.gate_up.weight.data, self.gate_up.weight_scale.data)
         codes, scales = _codes(both, self.gate_up.activation)
-        ops.gemm_fp8_block_nt(x, codes, scales, self.down.weight.data, self.down.weight_scale.data, gemm_cus)
-        return x
+        ops.gemm_fp8_block_nt(rows, codes, scales, self.down.weight.data, self.down.weight_scale.data, gemm_cus)
+        return hidden_states
