@@ -89,3 +89,10 @@ def test_an_8_bit_block_takes_any_leading_dimensions():
     block = filled(tw.FeedForward(64, 96)).to_fp8_blocks()
     with pytest.raises(RuntimeError, match="GPU"):      # no complaint about the shape
         block(torch.zeros(2, 3, 64, dtype=BF16))
+
+
+def test_a_gated_projection_alone_has_no_8_bit_form():
+    layer = tw.GatedLinear(64, 32)
+    with pytest.raises(ValueError, match="to_fp8_blocks"):
+        tw.Fp8BlockLinearMethod().process_weights(layer)
+    assert layer.weight.dtype == BF16 and not hasattr(layer, "weight_scale")

@@ -131,6 +131,13 @@ class Fp8BlockLinearMethod:
                              f"of 4 output channels; this one is {tuple(layer.weight.shape)}")
 
     def process_weights(self, layer: nn.Module) -> None:
+        if isinstance(layer, GatedLinear):   # its activation is taken with the next projection's codes
+            raise ValueError("a GatedLinear has no 8-bit form of its own: FeedForward.to_fp8_blocks() codes it with the "
+                             "projection behind it")
+        self.code_weight(layer)
+
+    def code_weight(self, layer: nn.Module) -> None:
+        """``process_weights`` for a layer whose owner calls the products itself."""
         self.check(layer)
         codes, scales = quantize_fp8_blocks(layer.weight.data)
         layer.weight = Parameter(codes, requires_grad=False)
@@ -185,7 +192,7 @@ class FeedForward(nn.Module):
             method = Fp8BlockLinearMethod()
             method.check(self.gate_up), method.check(self.down)
             for layer in (self.gate_up, self.down):
-                method.process_weights(layer)
+                method.code_weight(layer)
             self.fp8 = True
         return self
 
