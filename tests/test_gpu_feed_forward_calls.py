@@ -1,5 +1,7 @@
 """Calls of the feed-forward half that the documentation allows: any leading dimensions, single rows of odd buffers, scales
 of any layout, grid caps, every tile shape that the rules may choose."""
+import ctypes
+
 import pytest
 import torch
 
@@ -29,3 +31,65 @@ def test_a_block_of_any_leading_dimensions(shape, fp8):
     want = block(x.view(-1, 256).clone())
     hidden = x.clone()
     assert block(hidden) is hidden and torch.equal(hidden.view(-1, 256), want)
+
+
+class KernelNode(ctypes.Structure):
+    """hipKernelNodeParams"""
+    _fields_ = [("block", ctypes.c_uint32 * 3), ("extra", ctypes.c_void_p), ("func", ctypes.c_void_p),
+                ("grid", ctypes.c_uint32 * 3), ("params", ctypes.c_void_p), ("lds", ctypes.c_uint32)]
+
+
+def grids(call):
+    """The workgroups of each kernel that a call launches, from the graph that captures it."""
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        call()
+    raw, count = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(0)
+    assert hip.hipGraphGetNodes(raw, None, ctypes.byref(count)) == 0
+    nodes = (ctypes.c_void_p * count.value)()
+    assert hip.hipGraphGetNodes(raw, nodes, ctypes.byref(count)) == 0
+    sizes = []
+    for node in nodes:
+        kind, params = ctypes.c_int(-1), KernelNode()
+        assert hip.hipGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0 and kind.value == 0
+        assert hip.hipGraphKernelNodeGetParams(ctypes.c_void_p(node), ctypes.byref(params)) == 0
+        sizes.append(params.grid[0] * params.grid[1] * params.grid[2])
+    return sizes
+
+
+@pytest.mark.parametrize("M,inner,K", [(5, 100, 72), (300, 36, 2048), (160, 748, 6904), (64, 2100, 264), (1001, 704, 1024), (0, 36, 72)])
+@pytest.mark.parametrize("cap", [1, 24, 100])
+def test_gated_calls_keep_their_cap(M, inner, K, cap):
+    """Every kernel of a capped call, the ones beside the products too, leaves the other units alone, and no bit
+    depends on the cap."""
+    x, w = (torch.randn(n, K, device=DEV).to(BF16) for n in (M, 2 * inner))
+    grad = torch.randn(M, inner, device=DEV).to(BF16)
+
+    def outputs():
+        return [torch.full(s, 777.0, dtype=BF16, device=DEV) for s in ((M, inner), (M, 2 * inner), (M, K), (2 * inner, K))]
+
+    def run(out, both, gx, gw, max_cus):
+        ops.gated_gemm_bf16_nt(out, x, w, "silu", max_cus, gate_up=both)
+        ops.gated_gemm_bf16_nt_backward(gx, gw, grad, x, w, both, "silu", max_cus)
+
+    want, got = outputs(), outputs()
+    run(*want, None), run(*got, cap)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    sizes = grids(lambda: run(*got, cap))
+    assert len(sizes) >= (1 if M == 0 else 3) and max(sizes) <= cap, sizes
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 700, 528), (96, 1024, 8192), (1000, 1024, 8192), (1000, 1376, 272)])
+@pytest.mark.parametrize("cap", [1, 24, 100])
+def test_8_bit_products_keep_their_cap(M, N, K, cap):
+    codes, scales = torch.empty((M, K), dtype=FP8, device=DEV), ops.fp8_group_scales(M, K)
+    ops.quant_fp8_groups(codes, scales, torch.randn(M, K, device=DEV))
+    w, sw = R.weight_codes(torch.randn(N, K, device=DEV))
+    want, got = (torch.full((M, N), 777.0, dtype=BF16, device=DEV) for _ in range(2))
+    ops.gemm_fp8_block_nt(want, codes, scales, w, sw)
+    ops.gemm_fp8_block_nt(got, codes, scales, w, sw, cap)
+    assert torch.equal(got, want)
+    sizes = grids(lambda: ops.gemm_fp8_block_nt(got, codes, scales, w, sw, cap))
+    assert sizes and max(sizes) <= cap, sizes

@@ -39,6 +39,11 @@ inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
       vals);
 }
 
+// The grid of a kernel that walks `groups` workgroups' work, under a caller's cap on workgroups (<= 0: none).
+inline dim3 capped_grid(int64_t groups, int max_cus) {
+  return dim3((unsigned)(max_cus > 0 && groups > max_cus ? max_cus : groups));
+}
+
 // TW_OK, or TW_ERR_LAUNCH with the runtime's message when the last launch_kernel failed.
 int finish_launch(const char* what);
 

@@ -811,17 +811,19 @@ BlockSplit block_split(int64_t M, int64_t N, int64_t K, int cus) {
 constexpr int JOIN_THREADS = 256;
 __global__ __launch_bounds__(JOIN_THREADS) void block_join_kernel(BlockArgs w) {
   const int across = w.N / 4;
-  const int64_t i = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x, row = i / across;
-  if (row >= w.M) return;
-  const int c = (int)(i - row * across) * 4;
-  const float* p = w.sums + row * w.N + c;
-  f32x4_t s = *reinterpret_cast<const f32x4_t*>(p);
+  const int64_t step = (int64_t)gridDim.x * JOIN_THREADS, n = (int64_t)w.M * across;
+  for (int64_t i = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x; i < n; i += step) {
+    const int64_t row = i / across;
+    const int c = (int)(i - row * across) * 4;
+    const float* p = w.sums + row * w.N + c;
+    f32x4_t s = *reinterpret_cast<const f32x4_t*>(p);
 #pragma unroll 4
-  for (int x = 1; x < w.parts; ++x) {
-    p += (int64_t)w.M * w.N;
-    s += *reinterpret_cast<const f32x4_t*>(p);
+    for (int x = 1; x < w.parts; ++x) {
+      p += (int64_t)w.M * w.N;
+      s += *reinterpret_cast<const f32x4_t*>(p);
+    }
+    *reinterpret_cast<uint2*>(w.out + row * w.ldc + c) = make_uint2(pack_out(s.x, s.y, w.half_out), pack_out(s.z, s.w, w.half_out));
   }
-  *reinterpret_cast<uint2*>(w.out + row * w.ldc + c) = make_uint2(pack_out(s.x, s.y, w.half_out), pack_out(s.z, s.w, w.half_out));
 }
 
 int launch_block_split(const char* what, BlockArgs w, const BlockSplit& split, float* sums, int max_cus, int cus, hipStream_t hs) {
@@ -834,7 +836,7 @@ int launch_block_split(const char* what, BlockArgs w, const BlockSplit& split, f
   if (rc) return rc;
   if ((rc = finish_launch(what))) return rc;
   const int64_t groups = ((int64_t)w.M * (w.N / 4) + JOIN_THREADS - 1) / JOIN_THREADS;
-  launch_kernel(block_join_kernel, dim3((unsigned)groups), dim3(JOIN_THREADS), 0, hs, w);
+  launch_kernel(block_join_kernel, capped_grid(groups, max_cus), dim3(JOIN_THREADS), 0, hs, w);
   return TW_OK;
 }
 

@@ -38,7 +38,7 @@ struct GradArgs {
   const uint16_t *grad, *both;
   uint16_t *d, *d_turned;  // null: not wanted
   int64_t ld_grad, ld_both, pitch, pitch_turned;
-  int M, I, across, act;
+  int M, I, across, tiles, act;
 };
 
 __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
@@ -62,56 +62,59 @@ __device__ __forceinline__ void write_turned(const uint16_t* tile, uint16_t* to,
 
 __global__ __launch_bounds__(GRAD_THREADS) void gated_grad_kernel(GradArgs w) {
   __shared__ __attribute__((aligned(16))) uint16_t tiles[2][TURN * TURN_PITCH];
-  const int c0 = blockIdx.x % w.across * TURN, m0 = blockIdx.x / w.across * TURN;
   const int m = threadIdx.x / (TURN / 4), c = threadIdx.x % (TURN / 4) * 4;
-  uint2 dh[TURN_STEPS], g2[TURN_STEPS], u2[TURN_STEPS];  // all under way before the first is used
-#pragma unroll
-  for (int i = 0; i < TURN_STEPS; ++i) {
-    const int row = m0 + m + i * TURN_ROWS;
-    dh[i] = g2[i] = u2[i] = make_uint2(0, 0);  // past the rows: zeros, which give zeros
-    if (row < w.M && c0 + c < w.I) {
-      const uint16_t* both = w.both + row * w.ld_both + c0 + c;
-      dh[i] = *reinterpret_cast<const uint2*>(w.grad + row * w.ld_grad + c0 + c);
-      g2[i] = *reinterpret_cast<const uint2*>(both);
-      u2[i] = *reinterpret_cast<const uint2*>(both + w.I);
-    }
-  }
-  with_activation(w.act, [&](auto act) {
+  for (int t = blockIdx.x; t < w.tiles; t += gridDim.x) {
+    const int c0 = t % w.across * TURN, m0 = t / w.across * TURN;
+    uint2 dh[TURN_STEPS], g2[TURN_STEPS], u2[TURN_STEPS];  // all under way before the first is used
 #pragma unroll
     for (int i = 0; i < TURN_STEPS; ++i) {
       const int row = m0 + m + i * TURN_ROWS;
-      const float h[4] = {low(dh[i].x), high(dh[i].x), low(dh[i].y), high(dh[i].y)};
-      const float gate[4] = {low(g2[i].x), high(g2[i].x), low(g2[i].y), high(g2[i].y)};
-      const float up[4] = {low(u2[i].x), high(u2[i].x), low(u2[i].y), high(u2[i].y)};
-      float x[4], y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float f, df;
-        activation_and_slope<act()>(gate[e], f, df);
-        x[e] = h[e] * up[e] * df;
-        y[e] = h[e] * f;
-      }
-      const uint2 dg = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
-      const uint2 du = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
-      if (w.d && row < w.M && c0 + c < w.I) {
-        uint16_t* d = w.d + row * w.pitch + c0 + c;
-        *reinterpret_cast<uint2*>(d) = dg;
-        *reinterpret_cast<uint2*>(d + w.I) = du;
-      }
-      if (w.d && row < w.M && c0 + TURN >= w.I && 2 * w.I + c < w.pitch)  // behind D's columns: zeros
-        *reinterpret_cast<uint2*>(w.d + row * w.pitch + 2 * w.I + c) = make_uint2(0, 0);
-      if (w.d_turned) {
-        uint32_t* p = reinterpret_cast<uint32_t*>(tiles[0] + (m + i * TURN_ROWS) * TURN_PITCH + c);
-        p[0] = dg.x, p[1] = dg.y;
-        p = reinterpret_cast<uint32_t*>(tiles[1] + (m + i * TURN_ROWS) * TURN_PITCH + c);
-        p[0] = du.x, p[1] = du.y;
+      dh[i] = g2[i] = u2[i] = make_uint2(0, 0);  // past the rows: zeros, which give zeros
+      if (row < w.M && c0 + c < w.I) {
+        const uint16_t* both = w.both + row * w.ld_both + c0 + c;
+        dh[i] = *reinterpret_cast<const uint2*>(w.grad + row * w.ld_grad + c0 + c);
+        g2[i] = *reinterpret_cast<const uint2*>(both);
+        u2[i] = *reinterpret_cast<const uint2*>(both + w.I);
       }
     }
-  });
-  if (!w.d_turned) return;
-  __syncthreads();
-  write_turned(tiles[0], w.d_turned + c0 * w.pitch_turned, w.I - c0, m0, w.pitch_turned);
-  write_turned(tiles[1], w.d_turned + (int64_t)(w.I + c0) * w.pitch_turned, w.I - c0, m0, w.pitch_turned);
+    with_activation(w.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < TURN_STEPS; ++i) {
+        const int row = m0 + m + i * TURN_ROWS;
+        const float h[4] = {low(dh[i].x), high(dh[i].x), low(dh[i].y), high(dh[i].y)};
+        const float gate[4] = {low(g2[i].x), high(g2[i].x), low(g2[i].y), high(g2[i].y)};
+        const float up[4] = {low(u2[i].x), high(u2[i].x), low(u2[i].y), high(u2[i].y)};
+        float x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float f, df;
+          activation_and_slope<act()>(gate[e], f, df);
+          x[e] = h[e] * up[e] * df;
+          y[e] = h[e] * f;
+        }
+        const uint2 dg = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+        const uint2 du = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+        if (w.d && row < w.M && c0 + c < w.I) {
+          uint16_t* d = w.d + row * w.pitch + c0 + c;
+          *reinterpret_cast<uint2*>(d) = dg;
+          *reinterpret_cast<uint2*>(d + w.I) = du;
+        }
+        if (w.d && row < w.M && c0 + TURN >= w.I && 2 * w.I + c < w.pitch)  // behind D's columns: zeros
+          *reinterpret_cast<uint2*>(w.d + row * w.pitch + 2 * w.I + c) = make_uint2(0, 0);
+        if (w.d_turned) {
+          uint32_t* p = reinterpret_cast<uint32_t*>(tiles[0] + (m + i * TURN_ROWS) * TURN_PITCH + c);
+          p[0] = dg.x, p[1] = dg.y;
+          p = reinterpret_cast<uint32_t*>(tiles[1] + (m + i * TURN_ROWS) * TURN_PITCH + c);
+          p[0] = du.x, p[1] = du.y;
+        }
+      }
+    });
+    if (!w.d_turned) continue;
+    __syncthreads();
+    write_turned(tiles[0], w.d_turned + c0 * w.pitch_turned, w.I - c0, m0, w.pitch_turned);
+    write_turned(tiles[1], w.d_turned + (int64_t)(w.I + c0) * w.pitch_turned, w.I - c0, m0, w.pitch_turned);
+    __syncthreads();  // the next tile's values go where these were
+  }
 }
 
 __global__ __launch_bounds__(GRAD_THREADS) void fill_zero_kernel(uint2* to, int64_t n) {
@@ -163,7 +166,7 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   if (M == 0) {  // a sum over no rows
     if (!grad_b) return TW_OK;
     const int64_t n = 2 * I * K / 4;
-    launch_kernel(fill_zero_kernel, dim3((unsigned)std::min<int64_t>(1024, (n + GRAD_THREADS - 1) / GRAD_THREADS)),
+    launch_kernel(fill_zero_kernel, capped_grid(std::min<int64_t>(1024, (n + GRAD_THREADS - 1) / GRAD_THREADS), max_cus),
                   dim3(GRAD_THREADS), 0, hs, static_cast<uint2*>(grad_b), n);
     return finish_launch(what);
   }
@@ -185,8 +188,9 @@ int run_gated_gemm_bf16_nt_backward(void* grad_a, void* grad_b, const void* grad
   w.M = (int)M, w.I = (int)I, w.act = act;
   w.across = (int)((I + TURN - 1) / TURN);
   const int64_t grid = (M + TURN - 1) / TURN * w.across;
-  if (grid > INT32_MAX) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too large", what);
-  launch_kernel(gated_grad_kernel, dim3((unsigned)grid), dim3(GRAD_THREADS), 0, hs, w);
+  if (grid > INT32_MAX / 2) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: too large", what);
+  w.tiles = (int)grid;
+  launch_kernel(gated_grad_kernel, capped_grid(grid, max_cus), dim3(GRAD_THREADS), 0, hs, w);
   if (int rc = finish_launch(what)) return rc;
   NnOperands products[2];
   int count = 0;

@@ -1281,11 +1281,12 @@ __global__ __attribute__((amdgpu_waves_per_eu(1, 1))) __launch_bounds__(TILE_THR
 constexpr int NN_SUM_THREADS = 256;
 // n: values of a part, a multiple of 8
 __global__ __launch_bounds__(NN_SUM_THREADS) void nn_sum_kernel(uint16_t* out, const float* sums, int64_t n, int parts) {
-  const int64_t i = ((int64_t)blockIdx.x * NN_SUM_THREADS + threadIdx.x) * 4;
-  if (i >= n) return;
-  f32x4_t s = *reinterpret_cast<const f32x4_t*>(sums + i);
-  for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4_t*>(sums + p * n + i);
-  *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
+  const int64_t step = (int64_t)gridDim.x * NN_SUM_THREADS * 4;
+  for (int64_t i = ((int64_t)blockIdx.x * NN_SUM_THREADS + threadIdx.x) * 4; i < n; i += step) {
+    f32x4_t s = *reinterpret_cast<const f32x4_t*>(sums + i);
+    for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4_t*>(sums + p * n + i);
+    *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
+  }
 }
 
 // More than 64 KiB of dynamic LDS must be allowed once per function and device.
@@ -1654,8 +1655,8 @@ int run_gemm_bf16_nn(const NnOperands* w, int count, int64_t N, int max_cus, flo
       if ((rc = launch_nn<2, 4, true>(w + i, 1, &units, N, sums, split[i], hs))) return rc;
       if ((rc = finish_launch(what))) return rc;
       const int64_t values = w[i].M * N;
-      launch_kernel(nn_sum_kernel, dim3((unsigned)((values / 4 + NN_SUM_THREADS - 1) / NN_SUM_THREADS)), dim3(NN_SUM_THREADS),
-                    0, hs, static_cast<uint16_t*>(w[i].out), sums, values, split[i].parts);
+      launch_kernel(nn_sum_kernel, capped_grid((values / 4 + NN_SUM_THREADS - 1) / NN_SUM_THREADS, max_cus),
+                    dim3(NN_SUM_THREADS), 0, hs, static_cast<uint16_t*>(w[i].out), sums, values, split[i].parts);
     }
     if (rc) return rc;
     if ((rc = finish_launch(what))) return rc;
@@ -1761,27 +1762,29 @@ constexpr int JOIN_THREADS = 256;
 __global__ __launch_bounds__(JOIN_THREADS) void gated_join_kernel(uint16_t* out, const float* sums, int M, int I, int parts,
                                                                   int64_t ldc, GatedOut gated) {
   const int across = I / 4;
-  const int64_t i = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x, row = i / across;
-  if (row >= M) return;
-  const int c = (int)(i - row * across) * 4;
-  const float* p = sums + row * 2 * I + c;
-  f32x4_t g = *reinterpret_cast<const f32x4_t*>(p), u = *reinterpret_cast<const f32x4_t*>(p + I);
+  const int64_t step = (int64_t)gridDim.x * JOIN_THREADS, n = (int64_t)M * across;
+  for (int64_t i = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x; i < n; i += step) {
+    const int64_t row = i / across;
+    const int c = (int)(i - row * across) * 4;
+    const float* p = sums + row * 2 * I + c;
+    f32x4_t g = *reinterpret_cast<const f32x4_t*>(p), u = *reinterpret_cast<const f32x4_t*>(p + I);
 #pragma unroll 4
-  for (int x = 1; x < parts; ++x) {
-    p += (int64_t)M * 2 * I;
-    g += *reinterpret_cast<const f32x4_t*>(p), u += *reinterpret_cast<const f32x4_t*>(p + I);
-  }
-  if (gated.both) {
-    uint16_t* const to = gated.both + row * gated.ld_both + c;
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(g.x, g.y), pack2(g.z, g.w));
-    *reinterpret_cast<uint2*>(to + I) = make_uint2(pack2(u.x, u.y), pack2(u.z, u.w));
-  }
-  with_activation(gated.act, [&](auto act) {
-    f32x4_t h;
+    for (int x = 1; x < parts; ++x) {
+      p += (int64_t)M * 2 * I;
+      g += *reinterpret_cast<const f32x4_t*>(p), u += *reinterpret_cast<const f32x4_t*>(p + I);
+    }
+    if (gated.both) {
+      uint16_t* const to = gated.both + row * gated.ld_both + c;
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack2(g.x, g.y), pack2(g.z, g.w));
+      *reinterpret_cast<uint2*>(to + I) = make_uint2(pack2(u.x, u.y), pack2(u.z, u.w));
+    }
+    with_activation(gated.act, [&](auto act) {
+      f32x4_t h;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = activation<act()>(g[e]) * u[e];
-    *reinterpret_cast<uint2*>(out + row * ldc + c) = make_uint2(pack2(h.x, h.y), pack2(h.z, h.w));
-  });
+      for (int e = 0; e < 4; ++e) h[e] = activation<act()>(g[e]) * u[e];
+      *reinterpret_cast<uint2*>(out + row * ldc + c) = make_uint2(pack2(h.x, h.y), pack2(h.z, h.w));
+    });
+  }
 }
 
 static int launch_gated_split(const char* what, const GemmBatch& batch, int64_t M, int64_t I, int64_t K, int64_t ldc,
@@ -1797,7 +1800,7 @@ static int launch_gated_split(const char* what, const GemmBatch& batch, int64_t 
 #undef TW_SPLIT_LAUNCH
   if (rc) return rc;
   if ((rc = finish_launch(what))) return rc;
-  launch_kernel(gated_join_kernel, dim3((unsigned)((M * (I / 4) + JOIN_THREADS - 1) / JOIN_THREADS)), dim3(JOIN_THREADS), 0,
+  launch_kernel(gated_join_kernel, capped_grid((M * (I / 4) + JOIN_THREADS - 1) / JOIN_THREADS, max_cus), dim3(JOIN_THREADS), 0,
                 hs, batch.out[0], sums, (int)M, (int)I, split.parts, ldc, gated);
   return TW_OK;
 }
