@@ -93,3 +93,34 @@ def test_8_bit_products_keep_their_cap(M, N, K, cap):
     assert torch.equal(got, want)
     sizes = grids(lambda: ops.gemm_fp8_block_nt(got, codes, scales, w, sw, cap))
     assert sizes and max(sizes) <= cap, sizes
+
+
+@pytest.mark.parametrize("route", ["direct", "ctypes"])
+def test_a_single_row_of_a_buffer_whose_rows_are_odd(route, monkeypatch):
+    """One row has no distance to another: its stride, which no alignment fits, is not looked at."""
+    if route == "ctypes":
+        monkeypatch.setattr(ops, "_fast", None)
+
+    def row(width, dtype=BF16):
+        return torch.zeros(3 * (width + 9), dtype=dtype, device=DEV).as_strided((1, width), (width + 9, 1))
+
+    x, w = torch.randn(1, 72, device=DEV).to(BF16), torch.randn(200, 72, device=DEV).to(BF16)
+    out, both, grad = row(100), row(200), row(100)
+    grad.copy_(torch.randn(1, 100))
+    ops.gated_gemm_bf16_nt(out, x, w, gate_up=both)
+    want, kept = torch.empty(1, 100, dtype=BF16, device=DEV), torch.empty(1, 200, dtype=BF16, device=DEV)
+    ops.gated_gemm_bf16_nt(want, x, w, gate_up=kept)
+    assert torch.equal(out, want) and torch.equal(both, kept)
+    gw, want_gw = torch.empty_like(w), torch.empty_like(w)
+    ops.gated_gemm_bf16_nt_backward(None, gw, grad, x, w, both)
+    ops.gated_gemm_bf16_nt_backward(None, want_gw, grad.clone(memory_format=torch.contiguous_format), x, w, kept)
+    assert torch.equal(gw, want_gw)
+    codes, scales = torch.empty(1, 272, dtype=FP8, device=DEV), ops.fp8_group_scales(1, 272)
+    x = row(272)
+    x.copy_(torch.randn(1, 272))
+    ops.quant_fp8_groups(codes, scales, x)
+    w, sw = R.weight_codes(torch.randn(260, 272, device=DEV))
+    out, want = row(260), torch.empty(1, 260, dtype=BF16, device=DEV)
+    ops.gemm_fp8_block_nt(out, codes, scales, w, sw)
+    ops.gemm_fp8_block_nt(want, codes, scales, w, sw)
+    assert torch.equal(out, want)

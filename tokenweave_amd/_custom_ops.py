@@ -999,7 +999,7 @@ def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.de
     rows, width = shape
     _require((t.stride(1) == 1 or width <= 1) and (rows <= 1 or t.stride(0) >= width),
              f"rows of {name} must be contiguous and apart; got stride {tuple(t.stride())}")
-    return t.stride(0) if rows > 1 else max(width, t.stride(0))
+    return t.stride(0) if rows > 1 else width   # (a single row's stride has no meaning)
 
 
 def _refuse_recording(op: str, instead: str, *tensors: Optional[torch.Tensor]) -> None:

@@ -606,7 +606,7 @@ static int64_t check_rows(const char* name, const Tensor& t, at::ScalarType dtyp
               rows, ", ", width, ")");
   TORCH_CHECK((t.stride(1) == 1 || width <= 1) && (rows <= 1 || t.stride(0) >= width), "rows of ", name,
               " must be contiguous and apart; got stride ", t.strides());
-  return rows > 1 ? t.stride(0) : std::max(width, t.stride(0));
+  return rows > 1 ? t.stride(0) : width;  // (a single row's stride has no meaning)
 }
 
 namespace {
