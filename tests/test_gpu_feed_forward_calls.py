@@ -124,3 +124,22 @@ def test_a_single_row_of_a_buffer_whose_rows_are_odd(route, monkeypatch):
     ops.gemm_fp8_block_nt(out, codes, scales, w, sw)
     ops.gemm_fp8_block_nt(want, codes, scales, w, sw)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("route", ["direct", "ctypes"])
+def test_scales_whose_rows_end_between_two_of_the_next(route, monkeypatch):
+    """Every second place of odd rows, and the same turned: no two scales share memory.  Where two do, the call raises."""
+    if route == "ctypes":
+        monkeypatch.setattr(ops, "_fast", None)
+    M, K, groups = 5, 400, 4
+    x, codes = torch.randn(M, K, device=DEV), torch.empty((M, K), dtype=FP8, device=DEV)
+    want = R.codes(x.double())[1]
+    for rows, columns, turn in ((M, groups, False), (groups, M, True)):
+        buf = torch.full((rows, 2 * columns - 1), -1.0, device=DEV)
+        scales = buf[:, ::2].t() if turn else buf[:, ::2]
+        ops.quant_fp8_groups(codes, scales, x)
+        assert torch.equal(scales, want) and (buf[:, 1::2] == -1.0).all()
+    base = torch.empty(64, device=DEV)
+    for strides in ((3, 1), (6, 2), (1, 4), (0, 1), (1, 0), (2, 2)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            ops.quant_fp8_groups(codes, base.as_strided((M, groups), strides), x)

@@ -1089,8 +1089,8 @@ def _check_group_scales(name: str, t: torch.Tensor, device: torch.device, rows: 
 
 def quant_fp8_groups(out: torch.Tensor, scales: torch.Tensor, input: torch.Tensor,
                      activation: Optional[str] = None) -> None:
-    """out [rows, K] (e4m3) and scales [rows, ceil(K / FP8_GROUP)] (fp32, any strides; `fp8_group_scales` makes the
-    usual layout) <- the rows of `input` [rows, K] in bf16, fp16 or fp32: of each group of 128 channels
+    """out [rows, K] (e4m3) and scales [rows, ceil(K / FP8_GROUP)] (fp32, rows or groups apart; `fp8_group_scales` makes
+    the usual layout) <- the rows of `input` [rows, K] in bf16, fp16 or fp32: of each group of 128 channels
     scale = max(largest magnitude, 1e-10) / 448 and code = the e4m3 value next to x / scale, ties to the even one.
     With `activation`, input is [rows, 2 K] and the rows are act(first half) * second half, taken in fp32 on the way
     (a gated block between its projections).  A group with an infinity or a NaN gives NaN codes."""
@@ -1114,7 +1114,7 @@ def quant_fp8_groups(out: torch.Tensor, scales: torch.Tensor, input: torch.Tenso
     _check_group_scales("scales", scales, dev, M, groups)
     s0, s1 = scales.stride()
     _require((M <= 1 or s0 > 0) and (groups <= 1 or s1 > 0) and
-             (M <= 1 or groups <= 1 or s0 >= groups * s1 or s1 >= M * s0),
+             (M <= 1 or groups <= 1 or s0 > (groups - 1) * s1 or s1 > (M - 1) * s0),
              f"scales must not share memory; got stride {tuple(scales.stride())}")
     with _on_device(input):
         _lib.check(_lib.lib().tw_quant_fp8_groups(out.data_ptr(), scales.data_ptr(), s0, s1, input.data_ptr(), ld, M, K,

@@ -679,7 +679,7 @@ void quant_fp8_groups(const Tensor& out, const Tensor& scales, const Tensor& inp
   check_group_scales("scales", scales, dev, M, groups);
   const int64_t s0 = scales.stride(0), s1 = scales.stride(1);
   TORCH_CHECK((M <= 1 || s0 > 0) && (groups <= 1 || s1 > 0) &&
-                  (M <= 1 || groups <= 1 || s0 >= groups * s1 || s1 >= M * s0),
+                  (M <= 1 || groups <= 1 || s0 > (groups - 1) * s1 || s1 > (M - 1) * s0),
               "scales must not share memory; got stride ", scales.strides());
   Launch l(input);
   check_rc(tw_quant_fp8_groups(out.data_ptr(), static_cast<float*>(scales.data_ptr()), s0, s1, input.data_ptr(), ld, M,
