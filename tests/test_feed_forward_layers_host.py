@@ -96,3 +96,12 @@ def test_a_gated_projection_alone_has_no_8_bit_form():
     with pytest.raises(ValueError, match="to_fp8_blocks"):
         tw.Fp8BlockLinearMethod().process_weights(layer)
     assert layer.weight.dtype == BF16 and not hasattr(layer, "weight_scale")
+
+
+def test_row_counts_next_to_32_bits_are_refused():
+    """Before anything is launched: a tile's last rows would be counted past them."""
+    from tokenweave_amd import _lib
+    L, at = _lib.lib(), 1 << 12
+    for M in (2 ** 31 - 1, 2 ** 31 - 16, 2 ** 31):
+        assert L.tw_quant_fp8_groups(at, at, 1, M, at, 8, M, 8, -1, 0, None) == _lib.TW_ERR_INVALID_ARGUMENT
+        assert L.tw_gated_gemm_bf16_nt(at, at, at, at, M, 4, 8, 4, 8, 0, 0, None, 0, None) == _lib.TW_ERR_INVALID_ARGUMENT

@@ -845,7 +845,7 @@ int launch_block_split(const char* what, BlockArgs w, const BlockSplit& split, f
 int run_quant_fp8_groups(void* out, float* scales, int64_t scale_row, int64_t scale_group, const void* input,
                          int64_t ld_in, int64_t M, int64_t K, int act, int dtype, void* stream) {
   const char* what = "quant_fp8_groups";
-  if (M < 0 || K <= 0 || M > INT32_MAX || K > INT32_MAX / 4)
+  if (M < 0 || K <= 0 || M > INT32_MAX - QUANT_ROWS || K > INT32_MAX / 4)  // (rows of a last group are counted past M)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: bad shape, %lld rows of %lld", what, (long long)M, (long long)K);
   if (act > TW_ACT_GELU_TANH) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, act);
   if (dtype != TW_DTYPE_BF16 && dtype != TW_DTYPE_F16 && dtype != TW_DTYPE_F32)

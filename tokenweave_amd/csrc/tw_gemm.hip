@@ -1871,6 +1871,8 @@ int run_gated_gemm_bf16_nt(void* out, void* both, const void* a, const void* b, 
                            void* stream) {
   const char* what = "gated_gemm_bf16_nt";
   if (I > INT32_MAX / 2) return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld columns", what, (long long)I);
+  if (M > INT32_MAX - 256)  // rows of a last tile are counted past M
+    return set_error(TW_ERR_INVALID_ARGUMENT, "%s: %lld rows", what, (long long)M);
   if (int rc = check_gemm_shape(what, M, I, K, ldc)) return rc;
   if (act < TW_ACT_SILU || act > TW_ACT_GELU_TANH)
     return set_error(TW_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, act);
