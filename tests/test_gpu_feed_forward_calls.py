@@ -143,3 +143,41 @@ def test_scales_whose_rows_end_between_two_of_the_next(route, monkeypatch):
     for strides in ((3, 1), (6, 2), (1, 4), (0, 1), (1, 0), (2, 2)):
         with pytest.raises(RuntimeError, match="share memory"):
             ops.quant_fp8_groups(codes, base.as_strided((M, groups), strides), x)
+
+
+@pytest.mark.parametrize("kind", R.ACTIVATIONS)
+def test_gradients_against_differences_of_the_64_bit_loss(kind):
+    """The derivative of the loss along directions near the gradient of each operand: central differences of the 64-bit
+    forward pass against the sum of gradient times direction, magnitudes included.
+
+    A gradient may be off by its own bound and by what the rounding of the kept products to bf16 does to it: G and U off by
+    `step` of themselves move U act'(G) by 1.13 |U| step + 0.8 |U| |G| step and act(G) by 1.13 |G| step (1.13 and 0.8: the
+    largest first and second derivatives of the three)."""
+    M, inner, K = 24, 60, 64
+    g = torch.Generator(device=DEV).manual_seed(5)
+    layer = filled(tw.GatedLinear(K, inner, kind), 6).requires_grad_()
+    x = torch.randn(M, K, generator=g, device=DEV).to(BF16).requires_grad_()
+    c = torch.randn(M, inner, generator=g, device=DEV).to(BF16)
+    layer(x).backward(c)
+    w = layer.weight.detach()
+    x64, w64 = x.detach().double(), w.double()
+    both = x64 @ w64.t()
+
+    def loss(x, w):
+        gate, up = (x @ w.t()).chunk(2, 1)
+        return float((R.act(gate, kind) * up * c.double()).sum())
+
+    _, bound_x, _, bound_w = R.gated_gradients(c, x.detach(), w, both.to(BF16), kind)
+    gate, up = both.abs().chunk(2, 1)
+    step = R.half(BF16)
+    off = c.double().abs().repeat(1, 2) * step * 1.02 * torch.cat((up * (1.13 + 0.8 * gate), 1.13 * gate), 1)
+    for grad, most, at in ((x.grad.double(), bound_x + off @ w64.abs(), lambda d: (x64 + d, w64)),
+                           (layer.weight.grad.double(), bound_w + off.t() @ x64.abs(), lambda d: (x64, w64 + d))):
+        # the bound means something: along the gradient the derivative is many times it
+        assert float((grad * grad).sum()) > 8 * float((most * grad.abs()).sum())
+        for _ in range(4):
+            d = grad * torch.rand(grad.shape, generator=g, device=DEV, dtype=torch.float64)
+            d, h = d / d.norm(), 1e-4
+            slope = (loss(*at(h * d)) - loss(*at(-h * d))) / (2 * h)
+            # 1e-4: h^2 / 6 of a third derivative of some 1e3, and 2^-48 of a loss of some 1e3 over h
+            assert abs(float((grad * d).sum()) - slope) <= float((most * d.abs()).sum()) + 1e-4
