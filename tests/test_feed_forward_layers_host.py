@@ -105,3 +105,21 @@ def test_row_counts_next_to_32_bits_are_refused():
     for M in (2 ** 31 - 1, 2 ** 31 - 16, 2 ** 31):
         assert L.tw_quant_fp8_groups(at, at, 1, M, at, 8, M, 8, -1, 0, None) == _lib.TW_ERR_INVALID_ARGUMENT
         assert L.tw_gated_gemm_bf16_nt(at, at, at, at, M, 4, 8, 4, 8, 0, 0, None, 0, None) == _lib.TW_ERR_INVALID_ARGUMENT
+
+
+def test_the_build_follows_its_makefiles_and_headers():
+    """How many jobs run is the caller's choice; flags and headers that change are compiled in."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+    def make(where, *args):
+        env = {k: v for k, v in os.environ.items() if k not in ("MAKEFLAGS", "MFLAGS", "MAKELEVEL")}
+        return subprocess.run(["make", "-C", os.path.join(root, where), *args], capture_output=True, text=True, env=env).stdout
+
+    csrc = os.path.join("tokenweave_amd", "csrc")
+    flags = [line for line in make(csrc, "-pn", "-j2", "lib").splitlines() if line.startswith("MAKEFLAGS")]
+    assert flags and not any("-j8" in line for line in flags), flags
+    assert make(csrc, "-n", "-W", "Makefile", "lib").count(" -c -o build/") == 9
+    for header in ("tw_activation.h", "tw_store.h"):
+        assert "tw_bench.hip" in make("benchlib", "-n", "-W", f"../tokenweave_amd/csrc/{header}")

@@ -97,7 +97,7 @@ _lib = None
 def build(verbose: bool = False) -> str:
     """Compile the HIP sources for gfx950 with hipcc (cross-compiles without a GPU)."""
     global _lib
-    proc = subprocess.run(["make", "-B", "-C", CSRC_DIR], stdout=subprocess.PIPE,
+    proc = subprocess.run(["make", "-B", "-j8", "-C", CSRC_DIR], stdout=subprocess.PIPE,
                           stderr=subprocess.STDOUT, text=True)
     if verbose or proc.returncode != 0:
         print(proc.stdout)
