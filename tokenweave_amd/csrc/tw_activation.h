@@ -13,6 +13,12 @@ namespace tw {
 constexpr float kTanhA = 0.7978845608028654f, kTanhB = 0.044715f;  // sqrt(2 / pi)
 
 // 1 / (1 + e^-x).  e^-x overflows to an infinity below -88.7, whose reciprocal is the zero it should be.
+//
+// By the exponential instruction on x log2 e, rounded to fp32: |x| 2^-24 of e^-x, where it counts beside 1; the tanh form's
+// argument, of x^3, and the exact one's x^2 are rounded likewise.  Against 64 bits, of the value, in units of 2^-24, for x
+// in [-1, 20] / [-5, -1] / [-10, -5]: silu 3.7 / 6.4 / 10, exact 4.9 / 24 / 88, tanh 4.9 / 47 / 230.  An exponent in two
+// floats would cost four instructions a value more for the first, some ten for the others; every caller rounds the
+// product with the up value to 8 bits, 4 or 3 of mantissa, at once, and the gelus below -5 are less than 1e-6 x.
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
 template <int ACT>

@@ -36,6 +36,10 @@ constexpr int GROUP = TW_FP8_GROUP;
 // A workgroup takes 16 rows of one group, its neighbours the next groups of the same rows: whole lines are read, and
 // the 16 scales leave together where the scales' rows are adjacent.  Bound by memory: act(gate) * up of [8192, 2 x 3584] in
 // bf16 31 us (148 MB, 4.8 TB/s); 1001 x 3696 in fp16 4.6 us, 32 x 8192 3.6: a launch and one trip to memory.
+//
+// K % 8 != 0, or rows that do not begin on 16 bytes (VEC = false): element by element, bound by the instructions of 2-byte
+// loads and 1-byte stores: 8192 x 7161 in bf16 114 us (1.6 TB/s; 7168 wide 41), fp32 146 (50), gated 8192 x 3581 95 (33),
+// 1001 x 3695 in fp16 10.0 (4.7), 32 x 8191 3.5.
 // ---------------------------------------------------------------------------
 constexpr int QUANT_THREADS = 256;
 constexpr int QUANT_ROWS = QUANT_THREADS / 16;
@@ -765,7 +769,7 @@ int launch_wide_for(const BlockArgs& w, int max_cus, int cus, hipStream_t hs) {
 // K divided: for more than 64 rows, where columns are few and tiles leave units idle or the inner dimension is long.  All
 // times in us: a slab of a 256 x 224 tile 1.66 (the others as kWideTiles has them), 3 for a launch besides, 4 for the one that
 // adds the sums, and those to memory and back; nothing reads b faster than memory gives it.  Undivided, up to 128 rows, a
-// wave's slab takes 0.95, and a unit's lines come at 50 GB/s.  [M, 8192] x [1024, 8192]^T, undivided / by this rule: 96 rows 18.7
+// wave's slab takes 0.95, and this kernel gets a unit's lines at 50 GB/s beside a launch of 2.5 us.  [M, 8192] x [1024, 8192]^T, undivided / by this rule: 96 rows 18.7
 // / 11.1, 200: 24.0 / 13.6, 512: 24.6 / 17.8, 1000: 25.0 / 20.9.  Left whole: [96, 8192] x [7168, 8192]^T (17.6; divided 16.3 and
 // the launch that adds), [1000, 3696] x [8192, 3696]^T, [341, 2048] x [768, 2048]^T (8.7, of which the launch and the first slab 4).
 constexpr double SPLIT_SLAB_US = 1.66, SPLIT_LAUNCH_US = 3.0, SPLIT_JOIN_US = 4.0, SPLIT_SUMS_A_US = 6e6, SPLIT_BYTES_A_US = 5e6,

@@ -9,9 +9,9 @@
 // matrix cores take it, and G and U were when they were kept: against 64 bits da and db of bf16 operands are off by
 // 0.29 % in the mean square, with neither rounding by 0.17 % (their own).
 //
-// 4096 rows, K = 8192, I = 3584: D and D^T 42 us (88 MB read, 117 written: 4.9 TB/s), da 341 and db 388 by themselves,
-// 696 in the launch that they share; with b and a turned beforehand as well, for the "NT" kernel, 104, 326 and 357, in a
-// workspace of 302 MB instead of 118.
+// 4096 rows, K = 8192, I = 3584, medians of 60: D and D^T 43 us (88 MB read, 117 written: 4.8 TB/s; one of them 30), da
+// 347 and db 380 by themselves, 704 in the launch that they share; with b and a turned beforehand as well, for the "NT"
+// kernel, 104, 326 and 357, in a workspace of 302 MB instead of 118.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -204,8 +204,9 @@ struct GemmBatch {
 // sums of an element meet in one lane (tile kernel) or one thread (K-split kernel) as fp32 and the product is rounded
 // once.  `both`, where given, also takes the two sums, rounded: [M][2 I], what the gradient needs.
 //
-// The product takes the time of the plain one over the same rows of b: [4096, 8192] x [7168, 8192]^T 337 us, plain 340
-// (1 430 TFLOP/s; the tile loop is the bound, see there), 5 more with `both` (in pieces of 8 bytes 11); one row 20.4 us (117 MB of weights at 5.7 TB/s),
+// The product takes the time of the plain one over the same rows of b: [4096, 8192] x [7168, 8192]^T 327 to 346 us by
+// board, plain 340 (1 430 TFLOP/s; the tile loop is the bound, see there), 5 to 12 more with `both` (in pieces of 8 bytes
+// 11 on a board where it is 5); one row 20.4 us (117 MB of weights at 5.8 TB/s),
 // 61 rows x [7392, 8192]^T 29.7 (4.1 TB/s: what a unit has under way is shared with a).  The activation is known outside the
 // loops that apply it: chosen per value the same call took 361, and [1001, 1024] x [1408, 1024]^T 9.3 instead of 8.6.
 struct GatedOut {
@@ -1630,7 +1631,7 @@ static TileOfTwo pick_tile_of_two(const NnOperands* w, int64_t N, int units) {
 // Two share a launch where that is less: [1001, 1408] x [1408, 1024] beside [1408, 1024] x [1024, 1024] 14.3 us, in launches
 // of their own 12.8 and 9.2; 300 rows 11.6, 12.6 and 5.2.  Large ones have a last round each that leaves units without a
 // tile: [4096, 7168] x [7168, 8192] beside [7168, 4096] x [4096, 8192], half of the units each, 4 and 7 rounds of 256 x 256
-// tiles, 785 us, by themselves 379 and 441.
+// tiles, 704 us (medians of 60), by themselves 347 and 380 (256 x 256 and 256 x 192).
 int run_gemm_bf16_nn(const NnOperands* w, int count, int64_t N, int max_cus, float* sums, void* stream) {
   const char* what = "gemm_bf16_nn";
   for (int i = 0; i < count; ++i)
@@ -1717,7 +1718,8 @@ static TileSplit pick_split(int64_t M, int64_t N, int64_t K, double undivided, i
   return best;
 }
 
-// Undivided, up to 128 rows: a row tile's and a column tile's rows at 65 GB/s a unit.
+// Undivided, up to 128 rows: a row tile's and a column tile's rows at 65 GB/s a unit beside a launch of 2.5 us (over the
+// whole launch of 61 rows of 8192 -> 3696, 29.6 us, the 1.6 MB of a unit are 53).
 static TileSplit gated_split(int64_t M, int64_t I, int64_t K) {
   const int64_t N = 2 * I, nk = (K + BK - 1) / BK;
   TileSplit whole = {0, 0, 1, (int)nk};
