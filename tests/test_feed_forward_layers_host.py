@@ -123,3 +123,12 @@ def test_the_build_follows_its_makefiles_and_headers():
     assert make(csrc, "-n", "-W", "Makefile", "lib").count(" -c -o build/") >= 9
     for header in ("tw_activation.h", "tw_store.h"):
         assert "tw_bench.hip" in make("benchlib", "-n", "-W", f"../tokenweave_amd/csrc/{header}")
+
+
+def test_weight_codes_and_scales_have_no_history():
+    """Of a weight in training: what the products take as constants, not tensors that want a gradient."""
+    w = torch.randn(130, 144).requires_grad_()
+    codes, scales = tw.quantize_fp8_blocks(w)
+    assert not codes.requires_grad and not scales.requires_grad
+    want = tw.quantize_fp8_blocks(w.detach())
+    assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])

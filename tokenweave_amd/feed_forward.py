@@ -101,6 +101,7 @@ class GatedLinear(nn.Module):
                 f"activation={self.activation}, tp_size={self.tp_size}")
 
 
+@torch.no_grad()
 def quantize_fp8_blocks(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """e4m3 codes of a [N, K] weight and the fp32 scales of its blocks of 128 x 128, [ceil(N / 128), ceil(K / 128)]:
     what `ops.gemm_fp8_block_nt` takes as its right operand.  (Plain torch: done once, when a model is loaded.)"""
