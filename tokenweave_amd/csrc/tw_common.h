@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <tuple>
 #include <utility>
 
@@ -37,6 +38,20 @@ inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
                                           lds_bytes, stream);
       },
       vals);
+}
+
+// More than 64 KiB of dynamic LDS must be allowed once per function and device; `ok`: one flag a device, the function's own.
+constexpr int kMaxDevices = 64;
+inline int allow_lds(const char* what, const void* kernel, std::atomic<bool>* ok, int bytes) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices)
+    return set_error(TW_ERR_LAUNCH, "%s: no current device", what);
+  if (!ok[dev].load(std::memory_order_acquire)) {
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+      return set_error(TW_ERR_LAUNCH, "%s: the device refused %d bytes of LDS", what, bytes);
+    ok[dev].store(true, std::memory_order_release);
+  }
+  return TW_OK;
 }
 
 // The grid of a kernel that walks `groups` workgroups' work, under a caller's cap on workgroups (<= 0: none).

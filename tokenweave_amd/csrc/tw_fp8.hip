@@ -432,7 +432,7 @@ struct WideShape {
   static constexpr int SPACE_EARLY = (TM - 2) * TN / LB / 2 < 1 ? 1 : (TM - 2) * TN / LB / 2;
   static constexpr int TOTAL = TM * TN, LAG = TN < 3 ? TN : 3, RING = 4;  // results in registers
   static_assert(TOTAL % RING == 0 && LAG < RING, "an instruction's results have one place in every slab");
-  static_assert(TM % 2 == 0 && BM % 64 == 0 && LDS <= 160 * 1024 && NA >= NB && (NA == NB || NA == 3), "shape");
+  static_assert(TM % 2 == 0 && BM % 64 == 0 && LDS <= 160 * 1024 && NA == 3 && NB >= 2 && NB <= 3, "shape");
   static_assert(EARLY ? TM > 2 && NB == 2 && (LATE - 1) * SPACE_LATE < 2 * TN && (LB - 1) * SPACE_EARLY < (TM - 2) * TN
                       : (LATE - 1) * SPACE_LATE < TM * TN, "every load has a place");
 };
@@ -556,11 +556,7 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
     };
 
     // as the loop would have left it
-    if (NA == 3) {
-      all_a(0), all_b(0), all_a(1), all_b(1);
-    } else {
-      all_b(0), all_a(0), all_b(1);
-    }
+    all_a(0), all_b(0), all_a(1), all_b(1);
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::PENDING) : "memory");
     uint32_t use_a = 0, use_b = 0, use_s = 0;           // of the slab at work
     uint32_t fill_a = (NA - 1) * PA, fill_s = (NA - 1) * BM * 4, fill_b = (NB - 1) * PB;
@@ -679,29 +675,12 @@ __global__ __launch_bounds__(WIDE_THREADS, 2) void gemm_fp8_block_tile_kernel(Bl
 #endif
 }
 
-constexpr int kMaxDevices = 64;
-
-// More than 64 KiB of dynamic LDS must be allowed once per function and device.
-template <typename Kernel>
-int allow_lds(Kernel kernel, std::atomic<bool>* ok, int bytes) {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices)
-    return set_error(TW_ERR_LAUNCH, "gemm_fp8_block_nt: no current device");
-  if (!ok[dev].load(std::memory_order_acquire)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
-        hipSuccess)
-      return set_error(TW_ERR_LAUNCH, "gemm_fp8_block_nt: the device refused %d bytes of LDS", bytes);
-    ok[dev].store(true, std::memory_order_release);
-  }
-  return TW_OK;
-}
-
 template <int MT, int NT, int STAGES, int LA>
 int launch_split(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
   constexpr int LDS = split_lds(MT, NT, STAGES);
   static std::atomic<bool> ok[kMaxDevices];
   const auto kernel = gemm_fp8_block_split_kernel<MT, NT, STAGES, LA>;
-  if (int rc = allow_lds(kernel, ok, LDS)) return rc;
+  if (int rc = allow_lds("gemm_fp8_block_nt", reinterpret_cast<const void*>(kernel), ok, LDS)) return rc;
   // tiles just wide enough for a whole number of workgroups per compute unit
   w.tiles_m = (w.M + 8 * LA - 1) / (8 * LA);
   const int64_t full = (w.N + 32 * NT - 1) / (32 * NT), rounds = (w.tiles_m * full + cus - 1) / cus;
@@ -721,7 +700,7 @@ int launch_wide(BlockArgs w, int max_cus, int cus, hipStream_t hs) {
   const bool tail = w.K % GROUP != 0;
   const auto kernel = tail ? gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, true, SPLIT>
                            : gemm_fp8_block_tile_kernel<WM, TM, TN, NA, NB, false, SPLIT>;
-  if (int rc = allow_lds(kernel, ok[tail], S::LDS)) return rc;
+  if (int rc = allow_lds("gemm_fp8_block_nt", reinterpret_cast<const void*>(kernel), ok[tail], S::LDS)) return rc;
   w.tiles_m = (w.M + S::BM - 1) / S::BM;
   w.tiles_n = (w.N + S::BN - 1) / S::BN;
   int64_t grid = (int64_t)w.tiles_m * w.tiles_n * (SPLIT ? w.parts : 1);

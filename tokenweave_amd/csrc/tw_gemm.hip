@@ -1290,20 +1290,6 @@ __global__ __launch_bounds__(NN_SUM_THREADS) void nn_sum_kernel(uint16_t* out, c
   }
 }
 
-// More than 64 KiB of dynamic LDS must be allowed once per function and device.
-static int allow_lds(const void* kernel, std::atomic<bool>* ok, int max_devices, int bytes) {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= max_devices)
-    return set_error(TW_ERR_LAUNCH, "gemm_bf16_nt: no current device");
-  if (!ok[dev].load(std::memory_order_acquire)) {
-    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
-      return set_error(TW_ERR_LAUNCH, "gemm_bf16_nt: the device refused %d bytes of LDS", bytes);
-    ok[dev].store(true, std::memory_order_release);
-  }
-  return TW_OK;
-}
-constexpr int kMaxDevices = 64;
-
 // A K-split launch's tiles: as few rounds of one workgroup per unit as full-width tiles need, and then tiles no
 // wider than that many rounds require, so that every unit streams its share of b.  The rounds are the whole batch's:
 // with those of one product alone its tiles were up to `count` times too narrow, us: two products [32, 1024] x [2048,
@@ -1324,7 +1310,7 @@ static int launch_ksplit(const GemmBatch& batch, int count, int64_t M, int64_t N
   constexpr int LDS = ks_lds_bytes(MT, NT, STAGES);
   static std::atomic<bool> lds_ok[kMaxDevices];
   const auto kernel = gemm_bf16_nt_ksplit_kernel<MT, NT, STAGES, LA, BAUX, TAIL, GATED>;
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, LDS)) return rc;
+  if (int rc = allow_lds("bf16 product", reinterpret_cast<const void*>(kernel), lds_ok, LDS)) return rc;
   const KsTiles tiles = ksplit_tiles(M, N, count, 8 * LA, GATED ? 16 * NT : 32 * NT, cus);
   int64_t grid = count * tiles.m * tiles.n;
   if (max_cus > 0 && grid > max_cus) grid = max_cus;
@@ -1428,7 +1414,7 @@ static int launch_tile_kernel(const GemmBatch& batch, int count, int64_t M, int6
                        int max_cus, hipStream_t hs, GatedArg<GATED> gated = {}) {
   using S = TileShape<TM, TN, ROWS>;
   static std::atomic<bool> lds_ok[kMaxDevices];
-  if (int rc = allow_lds(reinterpret_cast<const void*>(gemm_bf16_nt_tile_kernel<TM, TN, ROWS, GATED>), lds_ok, kMaxDevices,
+  if (int rc = allow_lds("bf16 product", reinterpret_cast<const void*>(gemm_bf16_nt_tile_kernel<TM, TN, ROWS, GATED>), lds_ok,
                          S::LDS))
     return rc;
   constexpr int COLS = GATED ? S::BN / 2 : S::BN;
@@ -1572,7 +1558,7 @@ static int launch_nn(const NnOperands* w, int count, const int* groups, int64_t 
   using S = TileShape<TM, TN>;
   static std::atomic<bool> lds_ok[kMaxDevices];
   const auto kernel = gemm_bf16_nn_kernel<TM, TN, SPLIT>;
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, S::LDS)) return rc;
+  if (int rc = allow_lds("bf16 product", reinterpret_cast<const void*>(kernel), lds_ok, S::LDS)) return rc;
   const int tiles_n = (int)((N + S::BN - 1) / S::BN);
   NnProduct p[2] = {};
   for (int i = 0; i < count; ++i)
@@ -1751,7 +1737,7 @@ static int launch_split_tile(const GemmBatch& batch, int64_t M, int64_t N, int64
   using S = TileShape<TM, TN, ROWS>;
   static std::atomic<bool> lds_ok[kMaxDevices];
   const auto kernel = gemm_bf16_nt_tile_kernel<TM, TN, ROWS, false, true>;
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds_ok, kMaxDevices, S::LDS)) return rc;
+  if (int rc = allow_lds("bf16 product", reinterpret_cast<const void*>(kernel), lds_ok, S::LDS)) return rc;
   const int tiles_m = (int)((M + S::BM - 1) / S::BM), tiles_n = (int)((N + S::BN - 1) / S::BN);
   const int64_t grid = std::min<int64_t>((int64_t)split.parts * tiles_m * tiles_n, units);
   launch_kernel(kernel, dim3((unsigned)grid), dim3(TILE_THREADS), S::LDS, hs, batch, split.parts, (int)M, (int)N, (int)K, N,
