@@ -132,3 +132,10 @@ def test_weight_codes_and_scales_have_no_history():
     assert not codes.requires_grad and not scales.requires_grad
     want = tw.quantize_fp8_blocks(w.detach())
     assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
+
+
+def test_an_e4m3_weight_without_scales_is_a_weight_like_others():
+    """A type that a layer was made with, not codes of another weight: it follows the model's and takes any values."""
+    layer = tw.RowParallelLinear(64, 64, bias=False, params_dtype=FP8)
+    layer.weight_loader(layer.weight, torch.ones(64, 64, dtype=BF16))
+    assert (layer.weight.float() == 1).all() and layer.half().weight.dtype == torch.float16

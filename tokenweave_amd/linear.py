@@ -55,9 +55,9 @@ def _is_unquantized(method: Any) -> bool:
 
 
 def _holds_codes(layer: nn.Module) -> bool:
-    """Whether the layer's weight is e4m3 codes."""
+    """Whether the layer's weight is e4m3 codes that have scales."""
     weight = layer._parameters.get("weight")
-    return weight is not None and weight.dtype == ops.FP8_DTYPE
+    return weight is not None and weight.dtype == ops.FP8_DTYPE and hasattr(layer, "weight_scale")
 
 
 def _apply_beside_codes(layer: nn.Module, apply: Any, fn: Any, recurse: bool) -> nn.Module:
